@@ -219,6 +219,95 @@ int lss_read_status(const void* workspace, uint32_t* flags_out, void* stream);
  * lss_sample on this workspace into host memory paths_out[B]. */
 int lss_read_row_paths(const void* workspace, int B, int32_t* paths_out, void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * The decode step around the sampler: the 4-bit vocabulary projection that makes the logits, the
+ * block tables and slot maps of a paged key/value cache, its 8-bit form, and the attention that
+ * reads it.  LocalStrm runs these as eager torch code (src/kernels/quantization.py,
+ * src/memory/block_manager.py, src/kernels/paged_attention.py); the formats below are this
+ * library's own.  All pointers are device pointers, all calls are asynchronous on `stream`.
+ * ------------------------------------------------------------------------------------------ */
+
+/* y[r, n] = sum_k x[r, k] * (code[n, k] - 8) * scale[n, k / group], sums in f32, one rounding to
+ * y's type.  Meant for the few rows of a decode step (the matrix is read once for up to eight rows).
+ *   x        [rows] x [x_stride elements], dtype LSS_DTYPE_*; K a multiple of 32
+ *   packed   uint8 [N][K / 2], column 2i in the low four bits of byte i, 2i + 1 in the high ones;
+ *            16-byte aligned
+ *   scales   [N][K / group], dtype LSS_DTYPE_BF16 or LSS_DTYPE_F16, 4-byte aligned;
+ *            group: 32, 64 or a multiple of 128 that divides K
+ *   y        [rows] x [y_stride elements], dtype LSS_DTYPE_*
+ * LSS_ERR_UNSUPPORTED when one row of x does not fit the shared memory of an SM (K beyond 49,152 for
+ * 16-bit x, 16,384 for f32). */
+int lss_int4_matvec(const void* x, int x_dtype, int rows, int K, int64_t x_stride, const uint8_t* packed,
+                    const void* scales, int scale_dtype, int N, int group, void* y, int y_dtype,
+                    int64_t y_stride, void* stream);
+
+/* Block tables.  A row (request) of `lens[b]` tokens holds the blocks table[b][0 ..
+ * ceil(lens[b] / block_size)); free blocks lie on a stack, free_blocks[0 .. n_free), whose top is
+ * taken first.  num_blocks is the length of free_blocks and the number of blocks of the cache.
+ *
+ * lss_block_plan gives every row a place for its new_lens[b] tokens (0 and less: none), rows in
+ * order.  A row is granted all of its tokens or none: none if they end behind `capacity` in the
+ * step's token order, behind the table's width, or if the blocks that it and the rows before it
+ * need (refused ones of this last kind among them, so that no later row overtakes) exceed the free list.
+ * The step's tokens lie row after row, starts[b] the first one of row b (granted or not).
+ *   table       int32 [B] x [table_stride], width entries used; entries of new blocks are written
+ *   slots       int64 [capacity]: block * block_size + offset of each token; -1 for tokens of refused
+ *               rows, of blocks outside [0, num_blocks), and behind the last token
+ *   positions   int32 [capacity]: the token's position in its row; 0 behind the last token
+ *   starts      int32 [B + 1], at most capacity
+ *   granted     int32 [B]: new_lens[b] or 0
+ *   lens_out    int32 [B]: lens + granted; may be `lens` itself
+ *   n_free_out  int32 [1]; may be `n_free` itself
+ * lss_block_release returns the blocks of the rows with codes[b] != 0 (lss_stop_check's codes) to
+ * the free list, in row and block order, and sets their lengths to 0.
+ * Both: B at most LSS_BLOCK_MAX_ROWS; n_free is taken as within [0, num_blocks]. */
+#define LSS_BLOCK_MAX_ROWS 16384
+int lss_block_plan(int32_t* table, int64_t table_stride, int width, const int32_t* lens,
+                   const int32_t* new_lens, int B, int block_size, const int32_t* free_blocks,
+                   int num_blocks, const int32_t* n_free, int capacity, int64_t* slots,
+                   int32_t* positions, int32_t* starts, int32_t* granted, int32_t* lens_out,
+                   int32_t* n_free_out, void* stream);
+int lss_block_release(const int32_t* table, int64_t table_stride, int width, const int32_t* lens,
+                      const int32_t* codes, int B, int block_size, int32_t* free_blocks,
+                      int num_blocks, const int32_t* n_free, int32_t* lens_out, int32_t* n_free_out,
+                      void* stream);
+
+/* The 8-bit cache: k_cache, v_cache e4m3 [num_blocks][heads][block_size][dim], 16-byte aligned;
+ * k_scale, v_scale f32 [num_blocks][heads], positive: a value is code * scale of its block and head.
+ * block_size 16, 32, 64, 128 or 256.
+ *
+ * lss_kv_append writes the step's keys and values (k, v: [T tokens][heads][dim], innermost stride 1,
+ * the other strides in elements): row b's tokens starts[b] .. starts[b] + granted[b] become its
+ * positions lens[b] - granted[b] .. lens[b] - 1 (lens: after the step, as lss_block_plan leaves
+ * them).  The scale of a block that this call begins is the smallest power of two (at least 2^-126)
+ * with which the finite new values fit e4m3 (448); that of a block that already holds tokens is the
+ * larger of this one and its own, and where it grows the tokens held are rounded again.  Rounding is
+ * to nearest even; infinities saturate, NaN stays.  A block that is written belongs to one row.
+ * dim a multiple of 8.  Rows whose numbers do not fit (granted > lens, tokens outside [0, T), lens
+ * beyond the table) and blocks outside [0, num_blocks) are passed over. */
+int lss_kv_append(const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v,
+                  int64_t v_token_stride, int64_t v_head_stride, int dtype, int T, int heads, int dim,
+                  uint8_t* k_cache, uint8_t* v_cache, float* k_scale, float* v_scale, int num_blocks,
+                  int block_size, const int32_t* table, int64_t table_stride, int width,
+                  const int32_t* starts, const int32_t* granted, const int32_t* lens, int B, void* stream);
+
+/* Softmax attention of the step's queries over that cache: query i of row b (token starts[b] + i of
+ * q, [T][q_heads][dim], bf16 or f16, innermost stride 1) is position lens[b] - granted[b] + i and sees
+ * the row's positions up to its own; query head h reads key head h / (q_heads / heads).
+ * dim 64, 128 or 256.  `scale` multiplies the products.  lse (f32 [T][q_heads], natural log of the
+ * sum) may be NULL.  Queries that see nothing (all of their blocks outside [0, num_blocks)) give 0
+ * and -inf; tokens of no granted row are left as they were in out and lse.
+ * workspace: lss_attend_workspace_bytes(dim) bytes, 16-byte aligned, of this call alone until it is
+ * done. */
+size_t lss_attend_workspace_bytes(int dim);
+int lss_attend(const void* q, int64_t q_token_stride, int64_t q_head_stride, int dtype, int T,
+               int q_heads, int heads, int dim, const uint8_t* k_cache, const uint8_t* v_cache,
+               const float* k_scale, const float* v_scale, int num_blocks, int block_size,
+               const int32_t* table, int64_t table_stride, int width, const int32_t* starts,
+               const int32_t* granted, const int32_t* lens, int B, float scale, void* out,
+               int64_t out_token_stride, int64_t out_head_stride, float* lse, void* workspace,
+               size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -7,7 +7,7 @@ from __future__ import annotations
 import ctypes
 import os
 import re
-from ctypes import c_char_p, c_int, c_int64, c_size_t, c_uint32, c_void_p
+from ctypes import c_char_p, c_float, c_int, c_int64, c_size_t, c_uint32, c_void_p
 
 from . import build as _build
 
@@ -64,6 +64,20 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.lss_argmax.argtypes = [P, c_int, c_int, c_int, c_int64, P, P]
     lib.lss_stop_check.restype = c_int
     lib.lss_stop_check.argtypes = [P, c_int, P, P, P, P, P]
+    lib.lss_int4_matvec.restype = c_int
+    lib.lss_int4_matvec.argtypes = [P, c_int, c_int, c_int, c_int64, P, P, c_int, c_int, c_int, P, c_int, c_int64, P]
+    lib.lss_block_plan.restype = c_int
+    lib.lss_block_plan.argtypes = [P, c_int64, c_int, P, P, c_int, c_int, P, c_int, P, c_int, P, P, P, P, P, P, P]
+    lib.lss_block_release.restype = c_int
+    lib.lss_block_release.argtypes = [P, c_int64, c_int, P, P, c_int, c_int, P, c_int, P, P, P, P]
+    lib.lss_kv_append.restype = c_int
+    lib.lss_kv_append.argtypes = [P, c_int64, c_int64, P, c_int64, c_int64, c_int, c_int, c_int, c_int, P, P, P, P,
+                                  c_int, c_int, P, c_int64, c_int, P, P, P, c_int, P]
+    lib.lss_attend_workspace_bytes.restype = c_size_t
+    lib.lss_attend_workspace_bytes.argtypes = [c_int]
+    lib.lss_attend.restype = c_int
+    lib.lss_attend.argtypes = [P, c_int64, c_int64, c_int, c_int, c_int, c_int, c_int, P, P, P, P, c_int, c_int,
+                               P, c_int64, c_int, P, P, P, c_int, c_float, P, c_int64, c_int64, P, P, c_size_t, P]
     lib.lss_read_status.restype = c_int
     lib.lss_read_status.argtypes = [P, ctypes.POINTER(c_uint32), P]
     lib.lss_read_row_paths.restype = c_int

@@ -1,0 +1,361 @@
+// lss_decode.cu — C ABI of the decode-step operators around the sampler: 4-bit products, block
+// tables, the 8-bit key/value cache and its attention.
+#include <algorithm>
+#include <mutex>
+
+#include "lss_attend.cuh"
+#include "lss_blocks.cuh"
+#include "lss_int4.cuh"
+#include "lss_kvcache.cuh"
+
+using namespace lss;
+
+static constexpr int MAX_DEV = 64;
+
+static int device_index() {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= MAX_DEV) dev = 0;
+  return dev;
+}
+
+static std::mutex g_mu;
+
+static int sm_count(int dev) {
+  static int n[MAX_DEV] = {};
+  std::lock_guard<std::mutex> lock(g_mu);
+  if (n[dev] == 0 && (cudaDeviceGetAttribute(&n[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n[dev] < 1)) {
+    cudaGetLastError();
+    n[dev] = 0;
+    return 148;
+  }
+  return n[dev];
+}
+
+// Raises a kernel's dynamic shared memory limit, once per device and size.
+struct SmemSet {
+  int bytes[MAX_DEV] = {};
+};
+template <class K>
+static cudaError_t allow_smem(K kern, SmemSet& set, int dev, int bytes) {
+  std::lock_guard<std::mutex> lock(g_mu);
+  if (bytes <= set.bytes[dev]) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) set.bytes[dev] = bytes;
+  return e;
+}
+
+template <class... KA, class... A>
+static cudaError_t launch(void (*kern)(KA...), unsigned grid, unsigned block, size_t smem, int cluster, bool pdl,
+                          cudaStream_t st, A... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid, 1, 1);
+  cfg.blockDim = dim3(block, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  int na = 0;
+  if (cluster > 1) {
+    at[na].id = cudaLaunchAttributeClusterDimension;
+    at[na].val.clusterDim.x = (unsigned)cluster;
+    at[na].val.clusterDim.y = 1;
+    at[na].val.clusterDim.z = 1;
+    ++na;
+  }
+  if (pdl) {
+    at[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[na].val.programmaticStreamSerializationAllowed = 1;
+    ++na;
+  }
+  cfg.attrs = at;
+  cfg.numAttrs = (unsigned)na;
+  return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+
+static int status_of(cudaError_t e) {
+  if (e == cudaSuccess) return LSS_OK;
+  cudaGetLastError();
+  return LSS_ERR_CUDA;
+}
+
+static bool aligned_to(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+static bool known_dtype(int d) { return d == LSS_DTYPE_F32 || d == LSS_DTYPE_BF16 || d == LSS_DTYPE_F16; }
+static bool block_size_ok(int bs) { return bs == 16 || bs == 32 || bs == 64 || bs == 128 || bs == 256; }
+static int log2_of(int v) {
+  int s = 0;
+  while ((1 << s) < v) ++s;
+  return s;
+}
+static int cluster_for(int64_t ctas, int most) {
+  int c = 1;
+  while (c < most && c < ctas) c <<= 1;
+  return c;
+}
+
+// ---------------------------------------------------------------- block tables
+static bool table_ok(const void* table, int64_t stride, int width, int B, int bs, int num_blocks) {
+  return (table || B == 0) && width >= 1 && stride >= width && B >= 0 && bs >= 1 && num_blocks >= 1 &&
+         (int64_t)width * bs <= (1 << 30);
+}
+
+// ---------------------------------------------------------------- attention
+static constexpr int AT_CAP_CTAS = 160;  // CTAs that the workspace has room for
+
+template <int D>
+static size_t attend_bytes() {
+  const size_t workers = (size_t)AT_CAP_CTAS * AtCfg<D>::NW;
+  return workers * sizeof(int4) + workers * 2 * (48 + 16 * D) * sizeof(float);
+}
+
+template <int D, int DT>
+static cudaError_t launch_attend(AttendArgs a, void* ws, cudaStream_t st) {
+  static SmemSet set;
+  const int dev = device_index();
+  constexpr int NW = AtCfg<D>::NW;
+  constexpr int smem = NW * AtCfg<D>::ST * (32 * D + 16);
+  cudaError_t e = allow_smem(lss_attend_kernel<D, DT>, set, dev, smem);
+  if (e != cudaSuccess) return e;
+  const int ctas = std::min(sm_count(dev), AT_CAP_CTAS);
+  a.meta = reinterpret_cast<int4*>(ws);
+  a.part = reinterpret_cast<float*>(a.meta + (size_t)ctas * NW);
+  e = launch(lss_attend_kernel<D, DT>, (unsigned)ctas, NW * 32, smem, 1, false, st, a);
+  if (e != cudaSuccess) return e;
+  return launch(lss_attend_join_kernel<D, DT>, (unsigned)(ctas * NW), 256, 0, 1, true, st, a);
+}
+
+template <int D>
+static cudaError_t launch_attend_dt(int dtype, const AttendArgs& a, void* ws, cudaStream_t st) {
+  return dtype == LSS_DTYPE_BF16 ? launch_attend<D, LSS_DTYPE_BF16>(a, ws, st) : launch_attend<D, LSS_DTYPE_F16>(a, ws, st);
+}
+
+// ---------------------------------------------------------------- 4-bit products
+static constexpr int I4_SMEM = 227 * 1024;
+
+template <int DT, int SPG>
+static cudaError_t launch_int4(const Int4Args& a, cudaStream_t st, bool& fits) {
+  static SmemSet set;
+  const int dev = device_index(), sms = sm_count(dev);
+  constexpr int planes = DT == LSS_DTYPE_F32 ? 3 : 1;
+  constexpr int fixed = I4_NW * I4_ST * (1024 + 64 * (4 / SPG)) + I4_NW * 2 * 128 * 4;
+  const int NB = (a.N + 15) / 16, KB = (a.K + I4_KB - 1) / I4_KB;
+  // CTAs per row block range: the split with the fewest units in the fullest CTA.  A cluster's
+  // exchange costs about as much as 16 units, and its row blocks' sums take 16 KB at most.
+  int ks = 1, nclusters = std::min(NB, sms);
+  int64_t best = INT64_MAX;
+  for (int k = 1; k <= 8 && k <= KB; k <<= 1) {
+    const int nc = std::min(NB, std::max(1, sms / k));
+    const int nrb = (NB + nc - 1) / nc;
+    if (k > 1 && nrb > 32) continue;
+    const int64_t cost = (int64_t)nrb * ((KB + k - 1) / k) + (k > 1 ? 16 : 0);
+    if (cost < best) {
+      best = cost;
+      ks = k;
+      nclusters = nc;
+    }
+  }
+  auto room = [&](int k) {  // rows of x that fit
+    const int nc = std::min(NB, std::max(1, sms / k));
+    const int left = I4_SMEM - fixed - (k > 1 ? (NB + nc - 1) / nc * 512 : 0);
+    return left / (((KB + k - 1) / k) * I4_KB * 2 * planes);
+  };
+  fits = room(ks) >= 1;
+  if (!fits) return cudaSuccess;
+  const int most = std::min(I4_ROWS, room(ks));
+  for (int r0 = 0; r0 < a.rows; r0 += most) {
+    const int rows = std::min(most, a.rows - r0);
+    const int smem = fixed + (ks > 1 ? (NB + nclusters - 1) / nclusters * 512 : 0) + rows * ((KB + ks - 1) / ks) * I4_KB * 2 * planes;
+    cudaError_t e = allow_smem(lss_int4_kernel<DT, SPG>, set, dev, smem);
+    if (e != cudaSuccess) return e;
+    e = launch(lss_int4_kernel<DT, SPG>, (unsigned)(nclusters * ks), I4_NT, smem, ks, false, st, a, r0, rows, ks);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
+}
+
+template <int DT>
+static cudaError_t launch_int4_group(const Int4Args& a, cudaStream_t st, bool& fits) {
+  if (a.group == 32) return launch_int4<DT, 1>(a, st, fits);
+  if (a.group == 64) return launch_int4<DT, 2>(a, st, fits);
+  return launch_int4<DT, 4>(a, st, fits);
+}
+
+extern "C" {
+
+int lss_int4_matvec(const void* x, int x_dtype, int rows, int K, int64_t x_stride, const uint8_t* packed,
+                    const void* scales, int scale_dtype, int N, int group, void* y, int y_dtype,
+                    int64_t y_stride, void* stream) {
+  if (rows < 0 || N < 1 || K < 32 || K % 32 != 0 || x_stride < K || y_stride < N) return LSS_ERR_INVALID_ARG;
+  if (!known_dtype(x_dtype) || !known_dtype(y_dtype)) return LSS_ERR_INVALID_ARG;
+  if (scale_dtype != LSS_DTYPE_BF16 && scale_dtype != LSS_DTYPE_F16) return LSS_ERR_INVALID_ARG;
+  if ((group != 32 && group != 64 && (group < 128 || group % 128 != 0)) || K % group != 0) return LSS_ERR_INVALID_ARG;
+  if (rows == 0) return LSS_OK;
+  if (!x || !packed || !scales || !y || !aligned_to(packed, 16) || !aligned_to(scales, 4)) return LSS_ERR_INVALID_ARG;
+  Int4Args a{};
+  a.x = x;
+  a.x_stride = x_stride;
+  a.rows = rows;
+  a.K = K;
+  a.N = N;
+  a.packed = packed;
+  a.scales = reinterpret_cast<const uint16_t*>(scales);
+  a.group = group;
+  a.scale_bf16 = scale_dtype == LSS_DTYPE_BF16;
+  a.y = y;
+  a.y_dtype = y_dtype;
+  a.y_stride = y_stride;
+  a.x_aligned = aligned_to(x, 16) && x_stride % 8 == 0;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  bool fits = true;
+  cudaError_t e;
+  switch (x_dtype) {
+    case LSS_DTYPE_F32: e = launch_int4_group<LSS_DTYPE_F32>(a, st, fits); break;
+    case LSS_DTYPE_BF16: e = launch_int4_group<LSS_DTYPE_BF16>(a, st, fits); break;
+    default: e = launch_int4_group<LSS_DTYPE_F16>(a, st, fits); break;
+  }
+  if (!fits) return LSS_ERR_UNSUPPORTED;
+  return status_of(e);
+}
+
+int lss_block_plan(int32_t* table, int64_t table_stride, int width, const int32_t* lens,
+                   const int32_t* new_lens, int B, int block_size, const int32_t* free_blocks, int num_blocks,
+                   const int32_t* n_free, int capacity, int64_t* slots, int32_t* positions, int32_t* starts,
+                   int32_t* granted, int32_t* lens_out, int32_t* n_free_out, void* stream) {
+  if (!table_ok(table, table_stride, width, B, block_size, num_blocks) || capacity < 0) return LSS_ERR_INVALID_ARG;
+  if (B > LSS_BLOCK_MAX_ROWS) return LSS_ERR_UNSUPPORTED;
+  if (!free_blocks || !n_free || !starts || !n_free_out) return LSS_ERR_INVALID_ARG;
+  if (B > 0 && (!lens || !new_lens || !granted || !lens_out)) return LSS_ERR_INVALID_ARG;
+  if (capacity > 0 && (!slots || !positions)) return LSS_ERR_INVALID_ARG;
+  PlanArgs a{table, table_stride, width, lens, new_lens, B, block_size, num_blocks, capacity, free_blocks,
+             n_free, slots, positions, starts, granted, lens_out, n_free_out};
+  static SmemSet set;
+  const int dev = device_index(), smem = 8 * B;
+  if (smem > 40 * 1024) {
+    const cudaError_t e = allow_smem(lss_plan_kernel, set, dev, smem);
+    if (e != cudaSuccess) return status_of(e);
+  }
+  const int ctas = cluster_for(((int64_t)capacity + BL_NT - 1) / BL_NT, BL_MAXCL);
+  return status_of(launch(lss_plan_kernel, (unsigned)ctas, BL_NT, (size_t)smem, ctas, false,
+                          reinterpret_cast<cudaStream_t>(stream), a));
+}
+
+int lss_block_release(const int32_t* table, int64_t table_stride, int width, const int32_t* lens,
+                      const int32_t* codes, int B, int block_size, int32_t* free_blocks, int num_blocks,
+                      const int32_t* n_free, int32_t* lens_out, int32_t* n_free_out, void* stream) {
+  if (!table_ok(table, table_stride, width, B, block_size, num_blocks)) return LSS_ERR_INVALID_ARG;
+  if (B > LSS_BLOCK_MAX_ROWS) return LSS_ERR_UNSUPPORTED;
+  if (!free_blocks || !n_free || !n_free_out) return LSS_ERR_INVALID_ARG;
+  if (B > 0 && (!lens || !codes || !lens_out)) return LSS_ERR_INVALID_ARG;
+  ReleaseArgs a{table, table_stride, width, lens, codes, B, block_size, num_blocks, free_blocks, n_free, lens_out, n_free_out};
+  static SmemSet set;
+  const int dev = device_index(), smem = 4 * B;
+  if (smem > 40 * 1024) {
+    const cudaError_t e = allow_smem(lss_release_kernel, set, dev, smem);
+    if (e != cudaSuccess) return status_of(e);
+  }
+  const int ctas = cluster_for((B + 31) / 32, BL_MAXCL);
+  return status_of(launch(lss_release_kernel, (unsigned)ctas, BL_NT, (size_t)smem, ctas, false,
+                          reinterpret_cast<cudaStream_t>(stream), a));
+}
+
+int lss_kv_append(const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v,
+                  int64_t v_token_stride, int64_t v_head_stride, int dtype, int T, int heads, int dim,
+                  uint8_t* k_cache, uint8_t* v_cache, float* k_scale, float* v_scale, int num_blocks,
+                  int block_size, const int32_t* table, int64_t table_stride, int width, const int32_t* starts,
+                  const int32_t* granted, const int32_t* lens, int B, void* stream) {
+  if (!known_dtype(dtype) || T < 0 || heads < 1 || dim < 8 || dim % 8 != 0 || !block_size_ok(block_size))
+    return LSS_ERR_INVALID_ARG;
+  if (k_token_stride < 0 || k_head_stride < 0 || v_token_stride < 0 || v_head_stride < 0) return LSS_ERR_INVALID_ARG;
+  if (!table_ok(table, table_stride, width, B, block_size, num_blocks)) return LSS_ERR_INVALID_ARG;
+  if (B > LSS_BLOCK_MAX_ROWS || heads > 65536 || dim > 65536) return LSS_ERR_UNSUPPORTED;
+  if (B == 0 || T == 0) return LSS_OK;
+  if (!k || !v || !k_cache || !v_cache || !k_scale || !v_scale || !starts || !granted || !lens)
+    return LSS_ERR_INVALID_ARG;
+  if (!aligned_to(k_cache, 16) || !aligned_to(v_cache, 16)) return LSS_ERR_INVALID_ARG;
+  AppendArgs a{k, v, k_token_stride, k_head_stride, v_token_stride, v_head_stride, k_cache, v_cache, k_scale,
+               v_scale, num_blocks, heads, block_size, dim, table, table_stride, width, starts, granted, lens, B, T, 0};
+  const int per16 = dtype == LSS_DTYPE_F32 ? 4 : 8;  // values in 16 bytes
+  a.aligned = aligned_to(k, 16) && aligned_to(v, 16) && k_token_stride % per16 == 0 && k_head_stride % per16 == 0 &&
+              v_token_stride % per16 == 0 && v_head_stride % per16 == 0;
+  // Blocks that a step can write: one per token at most, and two more per row than its tokens fill.
+  const int64_t blocks = std::min((int64_t)T, (int64_t)T / block_size + 2 * (int64_t)B);
+  const int64_t items = blocks * 2 * heads;
+  static SmemSet sets[3];
+  const int dev = device_index(), smem = 4 * B;
+  const int64_t ctas = std::max((int64_t)1, std::min((items + KV_NT / 32 - 1) / (KV_NT / 32), (int64_t)sm_count(dev) * 8));
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  auto go = [&](auto kern, SmemSet& set) {
+    if (smem > 40 * 1024) {
+      const cudaError_t e = allow_smem(kern, set, dev, smem);
+      if (e != cudaSuccess) return e;
+    }
+    return launch(kern, (unsigned)ctas, KV_NT, (size_t)smem, 1, false, st, a);
+  };
+  switch (dtype) {
+    case LSS_DTYPE_F32: return status_of(go(lss_append_kernel<LSS_DTYPE_F32>, sets[0]));
+    case LSS_DTYPE_BF16: return status_of(go(lss_append_kernel<LSS_DTYPE_BF16>, sets[1]));
+    default: return status_of(go(lss_append_kernel<LSS_DTYPE_F16>, sets[2]));
+  }
+}
+
+size_t lss_attend_workspace_bytes(int dim) {
+  switch (dim) {
+    case 64: return attend_bytes<64>();
+    case 128: return attend_bytes<128>();
+    case 256: return attend_bytes<256>();
+    default: return 0;
+  }
+}
+
+int lss_attend(const void* q, int64_t q_token_stride, int64_t q_head_stride, int dtype, int T, int q_heads,
+               int heads, int dim, const uint8_t* k_cache, const uint8_t* v_cache, const float* k_scale,
+               const float* v_scale, int num_blocks, int block_size, const int32_t* table, int64_t table_stride,
+               int width, const int32_t* starts, const int32_t* granted, const int32_t* lens, int B, float scale,
+               void* out, int64_t out_token_stride, int64_t out_head_stride, float* lse, void* workspace,
+               size_t workspace_bytes, void* stream) {
+  if ((dtype != LSS_DTYPE_BF16 && dtype != LSS_DTYPE_F16) || T < 0 || heads < 1 || q_heads < heads ||
+      q_heads % heads != 0 || !block_size_ok(block_size))
+    return LSS_ERR_INVALID_ARG;
+  if (q_token_stride < 0 || q_head_stride < 0 || out_token_stride < 0 || out_head_stride < dim) return LSS_ERR_INVALID_ARG;
+  if (!table_ok(table, table_stride, width, B, block_size, num_blocks)) return LSS_ERR_INVALID_ARG;
+  if (dim != 64 && dim != 128 && dim != 256) return LSS_ERR_UNSUPPORTED;
+  if (heads > 65536 || (int64_t)T * q_heads > (1 << 30)) return LSS_ERR_UNSUPPORTED;
+  if (B == 0 || T == 0) return LSS_OK;
+  if (!q || !out || !k_cache || !v_cache || !k_scale || !v_scale || !starts || !granted || !lens)
+    return LSS_ERR_INVALID_ARG;
+  if (!aligned_to(k_cache, 16) || !aligned_to(v_cache, 16)) return LSS_ERR_INVALID_ARG;
+  if (!workspace || workspace_bytes < lss_attend_workspace_bytes(dim) || !aligned_to(workspace, 16)) return LSS_ERR_WORKSPACE;
+  AttendArgs a{};
+  a.q = q;
+  a.q_st = q_token_stride;
+  a.q_sh = q_head_stride;
+  a.out = out;
+  a.o_st = out_token_stride;
+  a.o_sh = out_head_stride;
+  a.lse = lse;
+  a.kc = k_cache;
+  a.vc = v_cache;
+  a.ks = k_scale;
+  a.vs = v_scale;
+  a.num_blocks = num_blocks;
+  a.heads = heads;
+  a.per = q_heads / heads;
+  a.bs_shift = log2_of(block_size);
+  a.table = table;
+  a.table_stride = table_stride;
+  a.width = width;
+  a.starts = starts;
+  a.granted = granted;
+  a.lens = lens;
+  a.B = B;
+  a.T = T;
+  a.scale = scale * LOG2E;
+  a.aligned = aligned_to(q, 16) && aligned_to(out, 16) && q_token_stride % 8 == 0 && q_head_stride % 8 == 0 &&
+              out_token_stride % 8 == 0 && out_head_stride % 8 == 0;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  switch (dim) {
+    case 64: return status_of(launch_attend_dt<64>(dtype, a, workspace, st));
+    case 128: return status_of(launch_attend_dt<128>(dtype, a, workspace, st));
+    default: return status_of(launch_attend_dt<256>(dtype, a, workspace, st));
+  }
+}
+
+}  // extern "C"

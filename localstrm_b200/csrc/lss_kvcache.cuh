@@ -1,0 +1,232 @@
+// lss_kvcache.cuh — write of a step's keys and values into a paged cache of 8-bit values (e4m3)
+// with one scale per block and key head.
+#pragma once
+
+#include "lss_common.cuh"
+
+namespace lss {
+
+constexpr int KV_NT = 256;
+constexpr int KV_HOLD = 8;      // groups of eight values that a lane keeps between its two passes
+constexpr float E4M3_MAX = 448.0f;
+
+struct AppendArgs {
+  const void* k;
+  const void* v;
+  int64_t k_st, k_sh, v_st, v_sh;  // strides in elements: token, head
+  uint8_t* kc;                     // [num_blocks][heads][block_size][dim]
+  uint8_t* vc;
+  float* ks;                       // [num_blocks][heads]
+  float* vs;
+  int num_blocks, heads, block_size, dim;
+  const int32_t* table;
+  int64_t table_stride;
+  int width;
+  const int32_t* starts;
+  const int32_t* granted;
+  const int32_t* lens;
+  int B, T;
+  int aligned;                     // every group of eight values starts on a 16-byte boundary
+};
+
+template <int DT>
+__device__ __forceinline__ float kv_widen(const void* p, int64_t i) {
+  if (DT == LSS_DTYPE_F32) return reinterpret_cast<const float*>(p)[i];
+  if (DT == LSS_DTYPE_BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
+  return __half2float(reinterpret_cast<const __half*>(p)[i]);
+}
+
+// Eight consecutive values as loaded: 16 bytes of 16-bit values or 32 of f32.
+template <int DT>
+struct Vec8 {
+  uint4 w[DT == LSS_DTYPE_F32 ? 2 : 1];
+  __device__ __forceinline__ void load(const void* p, int64_t i, bool aligned) {
+    if (DT == LSS_DTYPE_F32) {
+      const float* f = reinterpret_cast<const float*>(p) + i;
+      if (aligned) {
+        w[0] = __ldg(reinterpret_cast<const uint4*>(f));
+        w[DT == LSS_DTYPE_F32 ? 1 : 0] = __ldg(reinterpret_cast<const uint4*>(f) + 1);
+      } else {
+        uint32_t* u = reinterpret_cast<uint32_t*>(w);
+#pragma unroll
+        for (int q = 0; q < (DT == LSS_DTYPE_F32 ? 8 : 0); ++q) u[q] = __float_as_uint(f[q]);
+      }
+    } else {
+      const uint16_t* h = reinterpret_cast<const uint16_t*>(p) + i;
+      if (aligned) {
+        w[0] = __ldg(reinterpret_cast<const uint4*>(h));
+      } else {
+        uint32_t* u = reinterpret_cast<uint32_t*>(w);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) u[q] = (uint32_t)h[2 * q] | ((uint32_t)h[2 * q + 1] << 16);
+      }
+    }
+  }
+  __device__ __forceinline__ float get(int q) const {  // q a constant after unrolling
+    const uint32_t* u = reinterpret_cast<const uint32_t*>(w);
+    if (DT == LSS_DTYPE_F32) return __uint_as_float(u[DT == LSS_DTYPE_F32 ? q : 0]);
+    const uint16_t b = (uint16_t)(u[q >> 1] >> ((q & 1) * 16));
+    if (DT == LSS_DTYPE_BF16) return __uint_as_float((uint32_t)b << 16);
+    return __half2float(__ushort_as_half(b));
+  }
+};
+
+// Two f32 values to e4m3, to nearest even; beyond +-448 (infinities among them) saturates, NaN stays.
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ __half2 e4m3x2_to_half2(uint16_t v) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(v));
+  return *reinterpret_cast<__half2*>(&r);
+}
+
+// Smallest power of two s with amax <= 448 s, at least 2^-126 (448 = 1.75 * 2^8).
+__device__ __forceinline__ float e4m3_scale(float amax) {
+  const uint32_t u = __float_as_uint(amax);
+  int e = (int)(u >> 23) - 127 - 8 + ((u & 0x7fffffu) > 0x600000u);
+  e = max(e, -126);
+  return __uint_as_float((uint32_t)(e + 127) << 23);
+}
+
+// Rows of [0, n) found by their inclusive sums: the first whose sum exceeds u.
+__device__ __forceinline__ int row_of(const int32_t* upto, int n, int u) {
+  int lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (upto[mid] > u) hi = mid; else lo = mid + 1;
+  }
+  return lo;
+}
+
+// A block that this call writes is one unit: the tokens of its row that fall into it, for one head,
+// of K or V, by one warp, so that the scale of (block, head) has one writer and no atomics.
+// Pass one takes the largest finite magnitude of the new values; the scale becomes
+//   s = max(s_old, 2^e),  e the smallest with amax <= 448 * 2^e,
+// where s_old counts only if the block keeps tokens of earlier steps; kept values are re-rounded
+// (code * s_old / s) where the scale grew.  Powers of two make every division exact, so a value is
+// rounded once when it is written and once more for each growth of its block's scale, by at most half
+// a step of e4m3 each (2^-4 relative; below 2^-6 s the step is 2^-9 s).
+// Bound by HBM for prompts and by its chain of dependent loads (lengths, table, scale, values) for
+// single tokens.
+template <int DT>
+__global__ void __launch_bounds__(KV_NT) lss_append_kernel(AppendArgs a) {
+  extern __shared__ int32_t kv_sm[];
+  int32_t* upto = kv_sm;  // [B] inclusive sums of the blocks that the rows write
+  __shared__ int scr[KV_NT / 32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int bs = a.block_size, D = a.dim;
+  const int64_t room = (int64_t)a.width * bs;
+  int units = 0;
+  for (int r0 = 0; r0 < a.B; r0 += KV_NT) {
+    const int r = r0 + tid;
+    int n = 0;
+    if (r < a.B) {
+      const int g = a.granted[r], len = a.lens[r];
+      if (g > 0 && g <= len && len <= room && a.starts[r] >= 0 && (int64_t)a.starts[r] + g <= a.T)
+        n = (len - 1) / bs - (len - g) / bs + 1;
+    }
+    int x = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    __syncthreads();
+    if (lane == 31) scr[warp] = x;
+    __syncthreads();
+    int before = 0, tot = 0;
+#pragma unroll
+    for (int i = 0; i < KV_NT / 32; ++i) {
+      if (i < warp) before += scr[i];
+      tot += scr[i];
+    }
+    if (r < a.B) upto[r] = units + before + x;
+    units += tot;
+  }
+  __syncthreads();
+
+  const int per = 2 * a.heads;
+  const int64_t items = (int64_t)units * per;
+  for (int64_t it = (int64_t)blockIdx.x * (KV_NT / 32) + warp; it < items; it += (int64_t)gridDim.x * (KV_NT / 32)) {
+    const int u = (int)(it / per), which = (int)(it - (int64_t)u * per);
+    const int head = which >> 1;
+    const bool is_v = which & 1;
+    const int r = row_of(upto, a.B, u);
+    const int len = a.lens[r], old = len - a.granted[r];
+    const int j = old / bs + u - (r > 0 ? upto[r - 1] : 0);
+    const int lo = max(old, j * bs) - j * bs, hi = min(len - j * bs, bs);  // new tokens: offsets [lo, hi)
+    const int page = a.table[r * a.table_stride + j];
+    if (page < 0 || page >= a.num_blocks) continue;
+    const void* x = is_v ? a.v : a.k;
+    const int64_t st = is_v ? a.v_st : a.k_st, sh = is_v ? a.v_sh : a.k_sh;
+    const int64_t src = (int64_t)(a.starts[r] + j * bs + lo - old) * st + head * sh;
+    const int64_t ph = (int64_t)page * a.heads + head;
+    uint8_t* dst = (is_v ? a.vc : a.kc) + ph * bs * D;
+    float* sp = (is_v ? a.vs : a.ks) + ph;
+    const float was = lo > 0 ? *sp : 0.0f;
+    const int d8 = D >> 3, n = (hi - lo) * d8;
+    Vec8<DT> keep[KV_HOLD];
+    float amax = 0.0f;
+    auto finite_max = [&](const Vec8<DT>& w) {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const float f = fabsf(w.get(q));
+        if (f <= FLT_MAX) amax = fmaxf(amax, f);
+      }
+    };
+#pragma unroll
+    for (int i = 0; i < KV_HOLD; ++i) {
+      const int e = lane + 32 * i;
+      if (e < n) keep[i].load(x, src + (int64_t)(e / d8) * st + (e % d8) * 8, a.aligned);
+    }
+#pragma unroll
+    for (int i = 0; i < KV_HOLD; ++i)
+      if (lane + 32 * i < n) finite_max(keep[i]);
+    for (int e = lane + 32 * KV_HOLD; e < n; e += 32) {
+      Vec8<DT> w;
+      w.load(x, src + (int64_t)(e / d8) * st + (e % d8) * 8, a.aligned);
+      finite_max(w);
+    }
+    amax = warp_allreduce(amax, [](float p, float q) { return fmaxf(p, q); });
+    const float s = fmaxf(was, e4m3_scale(amax));
+    const bool pow2 = (__float_as_uint(s) & 0x7fffffu) == 0u;
+    const float inv = __frcp_rn(s);
+    auto store = [&](const Vec8<DT>& w, int e) {
+      float f[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) f[q] = pow2 ? w.get(q) * inv : __fdiv_rn(w.get(q), s);
+      uint2 o;
+      o.x = e4m3x2(f[0], f[1]) | (e4m3x2(f[2], f[3]) << 16);
+      o.y = e4m3x2(f[4], f[5]) | (e4m3x2(f[6], f[7]) << 16);
+      *reinterpret_cast<uint2*>(dst + (int64_t)lo * D + (int64_t)e * 8) = o;
+    };
+#pragma unroll
+    for (int i = 0; i < KV_HOLD; ++i)
+      if (lane + 32 * i < n) store(keep[i], lane + 32 * i);
+    for (int e = lane + 32 * KV_HOLD; e < n; e += 32) {
+      Vec8<DT> w;
+      w.load(x, src + (int64_t)(e / d8) * st + (e % d8) * 8, a.aligned);
+      store(w, e);
+    }
+    if (lo > 0 && s != was) {  // kept tokens, rounded again to the larger step
+      const float ratio = __fdiv_rn(was, s);
+      for (int e = lane; e < lo * d8; e += 32) {
+        uint2* at = reinterpret_cast<uint2*>(dst + (int64_t)e * 8);
+        uint2 c = *at;
+        uint32_t in[4] = {c.x & 0xffffu, c.x >> 16, c.y & 0xffffu, c.y >> 16}, out[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float2 f = __half22float2(e4m3x2_to_half2((uint16_t)in[q]));
+          out[q] = e4m3x2(f.x * ratio, f.y * ratio);
+        }
+        *at = make_uint2(out[0] | (out[1] << 16), out[2] | (out[3] << 16));
+      }
+    }
+    if (lane == 0 && !(s == was)) *sp = s;
+  }
+}
+
+}  // namespace lss

@@ -1,0 +1,129 @@
+"""CPU-only checks of the decode-step operators: refusals of the C entries before any device work,
+and the plain forms that the GPU tests compare with."""
+import pytest
+import torch
+
+import localstrm_b200 as lb
+from localstrm_b200 import _lib
+from tests import decode_util as U
+
+OK, INVALID, WORKSPACE, UNSUPPORTED = 0, 1, 2, 4
+
+
+def int4(**kw):
+    a = dict(x=16, xd=1, rows=1, K=64, xs=64, packed=16, scales=16, sd=2, N=4, group=32, y=16, yd=0, ys=4, stream=None)
+    a.update(kw)
+    return _lib.load().lss_int4_matvec(*a.values())
+
+
+def test_int4_refusals():
+    assert int4(rows=0) == OK
+    for bad in (dict(rows=-1), dict(K=48), dict(K=0), dict(N=0), dict(xs=63), dict(ys=3), dict(xd=3), dict(yd=-1), dict(sd=0),
+                dict(group=16), dict(group=96), dict(group=128), dict(K=320, xs=320, group=128), dict(x=None), dict(packed=None),
+                dict(packed=8), dict(scales=18), dict(scales=None), dict(y=None)):
+        assert int4(**bad) == INVALID, bad
+
+
+def plan(fn="lss_block_plan", **kw):
+    a = dict(table=16, ts=4, width=4, lens=16, new=16, B=1, bs=16, free=16, blocks=8, n_free=16, cap=4, slots=16, pos=16, starts=16,
+             granted=16, lens_out=16, n_free_out=16, stream=None)
+    if fn == "lss_block_release":
+        for k in ("cap", "slots", "pos", "starts", "granted"):
+            del a[k]
+    a.update(kw)
+    return getattr(_lib.load(), fn)(*a.values())
+
+
+@pytest.mark.parametrize("fn", ["lss_block_plan", "lss_block_release"])
+def test_block_refusals(fn):
+    for bad in (dict(table=None), dict(ts=3), dict(width=0), dict(B=-1), dict(bs=0), dict(blocks=0), dict(lens=None), dict(new=None),
+                dict(free=None), dict(n_free=None), dict(lens_out=None), dict(n_free_out=None), dict(width=1 << 20, ts=1 << 20, bs=2048)):
+        assert plan(fn, **bad) == INVALID, bad
+    assert plan(fn, B=16385) == UNSUPPORTED
+    if fn == "lss_block_plan":
+        for bad in (dict(cap=-1), dict(slots=None), dict(pos=None), dict(starts=None), dict(granted=None)):
+            assert plan(fn, **bad) == INVALID, bad
+
+
+def append(**kw):
+    a = dict(k=16, kt=128, kh=64, v=16, vt=128, vh=64, dt=1, T=2, heads=2, dim=64, kc=16, vc=16, ks=16, vs=16, blocks=8, bs=16, table=16,
+             ts=4, width=4, starts=16, granted=16, lens=16, B=1, stream=None)
+    a.update(kw)
+    return _lib.load().lss_kv_append(*a.values())
+
+
+def test_append_refusals():
+    assert append(T=0) == OK and append(B=0) == OK
+    for bad in (dict(dt=5), dict(T=-1), dict(heads=0), dict(dim=60), dict(dim=0), dict(bs=24), dict(bs=512), dict(bs=8), dict(kt=-1),
+                dict(vh=-64), dict(table=None), dict(ts=3), dict(blocks=0), dict(k=None), dict(v=None), dict(kc=None), dict(vc=24),
+                dict(ks=None), dict(vs=None), dict(starts=None), dict(granted=None), dict(lens=None)):
+        assert append(**bad) == INVALID, bad
+    assert append(B=16385) == UNSUPPORTED
+
+
+def attend(**kw):
+    a = dict(q=16, qt=256, qh=64, dt=1, T=2, hq=4, heads=2, dim=64, kc=16, vc=16, ks=16, vs=16, blocks=8, bs=16, table=16, ts=4, width=4,
+             starts=16, granted=16, lens=16, B=1, scale=0.1, out=16, ot=256, oh=64, lse=None, ws=16, wsb=1 << 30, stream=None)
+    a.update(kw)
+    return _lib.load().lss_attend(*a.values())
+
+
+def test_attend_refusals():
+    lib = _lib.load()
+    assert attend(T=0) == OK and attend(B=0) == OK
+    for bad in (dict(dt=0), dict(dt=7), dict(T=-1), dict(heads=0), dict(hq=1), dict(hq=5), dict(bs=20), dict(qt=-1), dict(oh=63),
+                dict(table=None), dict(width=5), dict(q=None), dict(out=None), dict(kc=8), dict(vs=None), dict(starts=None), dict(lens=None)):
+        assert attend(**bad) == INVALID, bad
+    assert attend(dim=96, oh=96) == UNSUPPORTED and attend(T=1 << 29) == UNSUPPORTED
+    assert attend(ws=None) == WORKSPACE and attend(ws=24) == WORKSPACE
+    assert attend(wsb=lib.lss_attend_workspace_bytes(64) - 1) == WORKSPACE
+    assert 0 < lib.lss_attend_workspace_bytes(64) < lib.lss_attend_workspace_bytes(256) and lib.lss_attend_workspace_bytes(80) == 0
+
+
+def test_cpu_tensors_fail_loudly():
+    i = lambda *v: torch.tensor(v, dtype=torch.int32)
+    w = lb.Int4Weight.quantize(torch.randn(8, 64), group=32)
+    with pytest.raises(RuntimeError):
+        lb.int4_matvec(torch.zeros(1, 64), w)
+    with pytest.raises(RuntimeError):
+        lb.sample_hidden(torch.zeros(1, 64), w, [])
+    table = i(0, 1).view(1, 2)
+    with pytest.raises(RuntimeError):
+        lb.plan_blocks(table, i(3), i(1), i(1, 2), i(2), 16, 4)
+    with pytest.raises(RuntimeError):
+        lb.release_blocks(table, i(3), i(1), i(1, 2), i(2), 16)
+    cache = lb.KVCache8.empty(4, 1, 16, 64, device="cpu")
+    p = lb.StepPlan(i(0, 1), i(1), i(1))
+    with pytest.raises(RuntimeError):
+        lb.append_kv(cache, torch.zeros(1, 1, 64), torch.zeros(1, 1, 64), table, p)
+    with pytest.raises(RuntimeError):
+        lb.attend(torch.zeros(1, 1, 64).half(), cache, table, p)
+
+
+def test_quantize_round_trip():
+    w = torch.randn(33, 128, generator=torch.Generator().manual_seed(0))
+    w[5] = 0
+    for group in (32, 64, 128):
+        for dt, eps in ((torch.float16, 2.0 ** -11), (torch.bfloat16, 2.0 ** -8)):
+            q = lb.Int4Weight.quantize(w, group, dt)
+            assert q.shape == (33, 128) and q.group == group and q.packed.shape == (33, 64)
+            step = q.scales.float().repeat_interleave(group, 1)
+            # half a step, and where the scale was rounded down the largest values end at code 7
+            assert bool(((q.dequantize() - w).abs() <= step * (0.5 + 7 * 2 * eps) + 1e-30).all())
+    assert bool((q.dequantize()[5] == 0).all())
+    with pytest.raises(ValueError):
+        lb.Int4Weight.quantize(w, group=48)
+    with pytest.raises(ValueError):
+        lb.Int4Weight.quantize(torch.randn(4, 40), group=40)
+
+
+def test_plain_forms_on_known_values():
+    # a row that needs a block, one that needs none, one that the free list does not hold any more, an idle one
+    want, table = U.plan_reference([[7, -1], [3, -1], [4, -1], [5, -1]], [16, 3, 16, 9], [1, 2, 1, 0], [2, 6, 0, 0, 0, 0, 0, 0], 1, 16, 5)
+    assert want == dict(slots=[2 * 16, 51, 52, -1, -1], positions=[16, 3, 4, 16, 0], starts=[0, 1, 3, 4, 4], granted=[1, 2, 0, 0],
+                        lens=[17, 5, 16, 9], n_free=[0])
+    assert table == [[7, 2], [3, -1], [4, -1], [5, -1]]
+    assert U.scale_for(448.0) == 1.0 and U.scale_for(448.1) == 2.0 and U.scale_for(0.0) == 2.0 ** -126 and U.scale_for(7.0) == 2.0 ** -6
+    x = torch.tensor([0.0, 1.0625, 1.1875, 448.0, 500.0, 2.0 ** -9, 2.0 ** -10, 3 * 2.0 ** -10, -17.0], dtype=torch.float64)
+    assert U.to_e4m3(x).tolist() == [0.0, 1.0, 1.25, 448.0, 448.0, 2.0 ** -9, 0.0, 2.0 ** -8, -16.0]
+    assert torch.equal(U.to_e4m3(x), x.clamp(-448, 448).float().to(torch.float8_e4m3fn).double())

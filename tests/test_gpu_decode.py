@@ -1,0 +1,560 @@
+"""The decode-step operators on the GPU against plain 64-bit forms."""
+import math
+
+import pytest
+import torch
+
+import localstrm_b200 as lb
+from localstrm_b200 import sampling as S
+from tests import decode_util as U
+
+pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not torch.cuda.is_available(), reason="needs a CUDA device")]
+DEV = torch.device("cuda", 0)
+E4M3 = torch.float8_e4m3fn
+DTYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+
+
+def gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def ints(v):
+    return torch.tensor(v, dtype=torch.int32, device=DEV)
+
+
+# ------------------------------------------------------------------------------- 4-bit products
+def int4_case(rows, n, k, group, seed, scale_dtype=torch.float16):
+    g = gen(seed)
+    packed = torch.randint(0, 256, (n, k // 2), dtype=torch.uint8, generator=g, device=DEV)
+    scales = (0.02 * torch.exp(torch.randn(n, k // group, generator=g, device=DEV))).to(scale_dtype)
+    x = torch.randn(rows, k, generator=g, device=DEV)
+    return lb.Int4Weight(packed, scales), x
+
+
+def int4_check(y, x, w):
+    """Products of the 16-bit operands are exact in f32; what rounds is the running f32 sums of K / 16
+    tensor steps (twice 2^-24 each, they may truncate), the sum over the groups, and the result."""
+    wd = torch.stack([w.packed & 15, w.packed >> 4], -1).reshape(w.packed.shape[0], -1).double() - 8
+    wd = wd * w.scales.double().repeat_interleave(w.group, 1)
+    want, size = x.double() @ wd.t(), x.double().abs() @ wd.abs().t()
+    k = x.shape[-1]
+    tol = (3 * k / 16 + 2 * k / w.group + 8) * 2.0 ** -23 * size + torch.finfo(y.dtype).eps / 2 * want.abs() + 2.0 ** -24 * (y.dtype == torch.float16)
+    off = (y.double() - want).abs()
+    assert bool((off <= tol).all()), float((off - tol).max())
+
+
+@pytest.mark.parametrize("rows,n,k,group", [
+    (1, 1, 32, 32), (1, 17, 64, 64), (2, 16, 128, 128), (3, 2057, 896, 64), (8, 33, 160, 32), (9, 515, 256, 256),
+    (5, 4099, 1120, 32), (17, 130, 8192, 128), (33, 1000, 512, 128), (64, 771, 4096, 128), (65, 96, 384, 384),
+    (1, 151936, 896, 128), (8, 20000, 640, 128)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_int4_sizes(rows, n, k, group, dtype):
+    w, x = int4_case(rows, n, k, group, seed=rows * 1000 + n, scale_dtype=torch.bfloat16 if n % 2 else torch.float16)
+    x = x.to(DTYPES[dtype])
+    int4_check(lb.int4_matvec(x, w), x, w)
+    y = lb.int4_matvec(x, w, out_dtype=torch.float32)
+    int4_check(y, x, w)
+    assert torch.equal(y, lb.int4_matvec(x, w, out_dtype=torch.float32))  # the same sums in the same order
+
+
+def test_int4_layouts_and_values():
+    w, x = int4_case(6, 301, 256, 64, seed=3)
+    wide = torch.zeros(6, 700, device=DEV)
+    for off in (0, 3):  # a slice of a wider tensor, 16-byte aligned rows and not
+        for dt in DTYPES.values():
+            xs = wide.to(dt)
+            xs[:, off: off + 256] = x.to(dt)
+            int4_check(lb.int4_matvec(xs[:, off: off + 256], w), xs[:, off: off + 256], w)
+    xt = x.t().contiguous().t()
+    int4_check(lb.int4_matvec(xt, w), xt, w)
+    out = torch.full((6, 400), 7.0, device=DEV)
+    lb.int4_matvec(x, w, out=out[:, 50:351])
+    int4_check(out[:, 50:351], x, w)
+    assert bool((out[:, :50] == 7).all()) and bool((out[:, 351:] == 7).all())
+    int4_check(lb.int4_matvec(x[2], w)[None], x[2:3], w)
+    assert lb.int4_matvec(x[:0], w).shape == (0, 301)
+    # f32 values of all magnitudes (their three bf16 parts are exact down to 2^-126), bf16 up to its end
+    big = x * torch.exp2(torch.randint(-60, 60, (1, 256), generator=gen(5), device=DEV).float())
+    int4_check(lb.int4_matvec(big, w), big, w)
+    # what is not finite stays in its row
+    x[1, 7], x[3, 9] = math.nan, math.inf
+    y = lb.int4_matvec(x, w)
+    int4_check(y[[0, 2, 4, 5]], x[[0, 2, 4, 5]], w)
+    assert bool(y[1].isnan().all()) and not bool(y[3].isfinite().any())
+
+
+def test_int4_quantize_and_sample_hidden():
+    w = torch.randn(777, 256, generator=gen(9), device=DEV)
+    q = lb.Int4Weight.quantize(w, group=64)
+    step = q.scales.float().repeat_interleave(64, 1)
+    # half a step; the f16 rounding of the scale shifts the largest value (code 7) by 7 * 2^-11 of one
+    assert bool(((q.dequantize() - w).abs() <= step * (0.5 + 7 * 2.0 ** -10)).all())
+    h = torch.randn(5, 256, generator=gen(10), device=DEV)
+    logits = lb.int4_matvec(h, q)
+    u = torch.rand(5, generator=gen(11), device=DEV)
+    params = [S.SamplingParams(temperature=t, top_k=20, top_p=0.9, repetition_penalty=1.1) for t in (0.0, 0.5, 0.8, 1.0, 1.3)]
+    past = [[1, 2, 3], None, [5, 5], [], [700]]
+    got = lb.sample_hidden(h, q, params, past, uniforms=u)
+    assert torch.equal(got, S.sample_batch(logits, params, past, uniforms=u))
+    assert got[0] == logits[0].argmax()
+
+
+# --------------------------------------------------------------------------------- block tables
+def plan_case(rows, bs, hi_ctx, hi_new, spare, seed, width_cut=0):
+    g = torch.Generator().manual_seed(seed)
+    lens = torch.randint(0, hi_ctx + 1, (rows,), generator=g).tolist()
+    new = torch.randint(-1, hi_new + 1, (rows,), generator=g).tolist()
+    width = max(1, -(-(hi_ctx + hi_new) // bs) - width_cut)
+    held = [min(-(-n // bs), width) for n in lens]
+    blocks = sum(held) + spare
+    ids = torch.randperm(blocks, generator=g).tolist()
+    table, at = [], 0
+    for n in held:
+        table.append(ids[at: at + n] + [-1] * (width - n))
+        at += n
+    return table, lens, new, ids[at:] + [0] * at, len(ids) - at
+
+
+@pytest.mark.parametrize("rows,bs,hi_ctx,hi_new,spare,cut,pad", [
+    (1, 16, 0, 1, 1, 0, 0), (1, 1, 5, 3, 9, 0, 2), (7, 16, 40, 5, 3, 0, 5), (64, 32, 300, 1, 64, 0, 0),
+    (1000, 16, 200, 33, 900, 1, 3), (1024, 7, 100, 9, 400, 0, -500), (1025, 128, 4000, 60, 300, 2, 1), (4099, 16, 50, 40, 9000, 0, 11)])
+def test_plan_matches_row_by_row(rows, bs, hi_ctx, hi_new, spare, cut, pad):
+    table, lens, new, free, n_free = plan_case(rows, bs, hi_ctx, hi_new, spare, seed=rows + bs, width_cut=cut)
+    capacity = max(0, sum(max(n, 0) for n in new) + pad)
+    want, table_after = U.plan_reference(table, lens, new, free, n_free, bs, capacity)
+    t, ln, nf = ints(table), ints(lens), ints([n_free])
+    p = lb.plan_blocks(t, ln, ints(new), ints(free), nf, bs, capacity)
+    for name, v in want.items():
+        assert getattr(p, name).tolist() == v, name
+    assert t.tolist() == table_after and ln.tolist() == lens and nf.tolist() == [n_free]
+    # in place, in a wider table
+    wide = torch.full((rows, len(table[0]) + 5), -7, dtype=torch.int32, device=DEV)
+    wide[:, : len(table[0])] = ints(table)
+    p = lb.plan_blocks(wide[:, : len(table[0])], ln, ints(new), ints(free), nf, bs, capacity, lens_out=ln, n_free_out=nf)
+    for name, v in want.items():
+        assert getattr(p, name).tolist() == v, name
+    assert wide[:, : len(table[0])].tolist() == table_after and bool((wide[:, len(table[0]):] == -7).all())
+    assert ln.tolist() == want["lens"]
+
+
+def test_plan_odd_inputs():
+    # no rows; no room; lengths and counts that make no sense; ids outside the cache
+    p = lb.plan_blocks(torch.empty(0, 4, dtype=torch.int32, device=DEV), ints([]), ints([]), ints([3, 4]), ints([2]), 16, 5)
+    assert p.slots.tolist() == [-1] * 5 and p.starts.tolist() == [0] and p.n_free.tolist() == [2]
+    table = [[9, -1], [1, -1], [5, 0], [2, -1]]
+    for n_free, cap in ((3, 30), (99, 30), (-5, 30), (3, 0)):
+        args = ([-4, 3, 2147483647, 16], [2, 2, 5, 2], [0, 77, 2, 1, 0, 0], n_free, 16, cap)
+        want, after = U.plan_reference(table, *args)
+        t = ints(table)
+        p = lb.plan_blocks(t, ints(args[0]), ints(args[1]), ints(args[2]), ints([n_free]), 16, cap)
+        assert p.granted.tolist() == want["granted"] and p.slots.tolist() == want["slots"] and t.tolist() == after
+        assert p.n_free.tolist() == want["n_free"] and p.starts.tolist() == want["starts"]
+
+
+@pytest.mark.parametrize("rows,bs,hi", [(1, 16, 0), (5, 16, 100), (1000, 32, 700), (3000, 4, 60)])
+def test_release_then_plan_again(rows, bs, hi):
+    table, lens, _, free, n_free = plan_case(rows, bs, hi, 1, 10, seed=rows)
+    g = torch.Generator().manual_seed(rows + 1)
+    codes = torch.randint(0, 3, (rows,), generator=g).tolist()
+    want, left = list(free), n_free
+    for b in range(rows):
+        if codes[b]:
+            for j in range(min(-(-lens[b] // bs), len(table[b]))):
+                want[left] = table[b][j]
+                left += 1
+    t, ln, f, nf = ints(table), ints(lens), ints(free), ints([n_free])
+    after, n_after = lb.release_blocks(t, ln, ints(codes), f, nf, bs)
+    assert f.tolist() == want and n_after.tolist() == [left]
+    assert after.tolist() == [0 if c else n for c, n in zip(codes, lens)] and ln.tolist() == lens and nf.tolist() == [n_free]
+    # in place, and once more: the rows hold nothing now
+    lb.release_blocks(t, ln, ints(codes), f, nf, bs, lens_out=ln, n_free_out=nf)
+    lb.release_blocks(t, ln, ints(codes), f, nf, bs, lens_out=ln, n_free_out=nf)
+    assert f.tolist() == want and nf.tolist() == [left] and ln.tolist() == after.tolist()
+    # a block list that is full already stays as it is
+    full = ints([len(free)])
+    _, n_full = lb.release_blocks(t, ints(lens), ints([1] * rows), f, full, bs)
+    assert f.tolist() == want and n_full.tolist() == [len(free)]
+
+
+# ---------------------------------------------------------------------------- 8-bit cache: write
+def check_append(k, v, rows, heads, bs, dim, seed, out_of=None):
+    table, t, starts, granted, lens, blocks = rows
+    cache = lb.KVCache8(*U.random_cache(blocks, heads, bs, dim, seed))
+    want = [(c.double(), s.double()) for c, s in ((cache.k, cache.k_scale), (cache.v, cache.v_scale))]
+    for x, (c, s) in zip((k, v), want):
+        U.append_reference(c, s, x, table, starts.tolist(), granted.tolist(), lens.tolist())
+    lb.append_kv(cache, k, v, t, lb.StepPlan(starts, granted, lens))
+    for name, (c, s) in zip("kv", want):
+        assert torch.equal(getattr(cache, name + "_scale").double(), s), name
+        assert torch.equal(getattr(cache, name).double().nan_to_num(999.0), c.nan_to_num(999.0)), name
+    return cache
+
+
+@pytest.mark.parametrize("ctx,new,heads,bs,dim", [
+    ([0], [1], 1, 16, 64), ([15, 16, 17, 0], [1, 1, 1, 1], 2, 16, 128), ([3, 0, 31], [60, 16, 1], 3, 32, 64),
+    ([100, 7], [0, 130], 2, 64, 256), ([0, 5, 250], [256, 300, 7], 1, 128, 128), ([1], [700], 1, 256, 64), ([2, 9], [5, 40], 5, 16, 8)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_append_matches_block_by_block(ctx, new, heads, bs, dim, dtype):
+    g = gen(sum(ctx) + dim)
+    spread = torch.exp(1.5 * torch.randn(sum(new), heads, 1, generator=g, device=DEV))
+    k, v = ((torch.randn(sum(new), heads, dim, generator=g, device=DEV) * spread).to(DTYPES[dtype]) for _ in range(2))
+    check_append(k, v, U.make_rows(ctx, new, bs, seed=dim), heads, bs, dim, seed=bs)
+
+
+def test_append_values_and_layouts():
+    rows = U.make_rows([5, 0, 40], [7, 33, 1], 16)
+    g = gen(1)
+    # one fused projection: keys and values are slices of it, 16-byte aligned rows and not
+    for off in (0, 1):
+        for dt in DTYPES.values():
+            fused = torch.randn(41, 900, generator=g, device=DEV).to(dt)
+            k, v = (fused[:, off + a: off + a + 256].view(41, 2, 128) for a in (128, 384))
+            check_append(k, v, rows, 2, 16, 128, seed=2)
+    # heads that share one value (stride 0), tokens inside heads, an inner stride that is not 1
+    x = torch.randn(41, 1, 64, generator=g, device=DEV)
+    check_append(x.expand(41, 4, 64), x.expand(41, 4, 64) * 3, rows, 4, 16, 64, seed=3)
+    y = torch.randn(4, 41, 64, generator=g, device=DEV).transpose(0, 1)
+    check_append(y, y.flip(0), rows, 4, 16, 64, seed=4)
+    z = torch.randn(41, 64, 4, generator=g, device=DEV).transpose(1, 2)
+    check_append(z, z, rows, 4, 16, 64, seed=5)
+    # zeros, the smallest and largest numbers, exact powers and borders of the scale, not finite ones
+    s = torch.randn(41, 2, 64, generator=g, device=DEV)
+    s[0] = 0
+    s[7:] = s[7:] * 2.0 ** -130
+    check_append(s, -s, rows, 2, 16, 64, seed=6)
+    s = torch.zeros(41, 2, 64, device=DEV)
+    s[:, 0, 0], s[:, 1, 1] = 448.0 * 4, 449.0
+    s[:, 0, 1] = 3.0e38
+    check_append(s, torch.full_like(s, 1.75), rows, 2, 16, 64, seed=7)
+    s = torch.randn(41, 2, 64, generator=g, device=DEV)
+    s[3, 0, 5], s[9, 1, 6], s[20, 0, 7] = math.nan, math.inf, -math.inf
+    check_append(s, s, rows, 2, 16, 64, seed=8)
+    check_append(torch.full_like(s, math.nan), torch.full_like(s, math.inf), rows, 2, 16, 64, seed=9)
+
+
+def test_append_passes_over_what_does_not_fit():
+    table, t, starts, granted, lens, blocks = U.make_rows([5, 0, 40, 3], [7, 33, 1, 2], 16)
+    k = torch.randn(43, 2, 64, generator=gen(2), device=DEV)
+    # a refused row, a row of fewer tokens than granted, one behind the table, blocks outside the cache
+    for g2, l2, edit in (([0, 33, 1, 2], None, None), ([7, 34, 1, 2], [12, 33, 41, 5], None), (None, [12, 33, 4100, 5], None),
+                         (None, None, (1, 1, -1)), (None, None, (1, 0, blocks)), (None, None, (2, 2, 2 ** 31 - 1))):
+        tb = [list(r) for r in table]
+        if edit:
+            tb[edit[0]][edit[1]] = edit[2]
+        rows = (tb, ints(tb), starts, ints(g2) if g2 else granted, ints(l2) if l2 else lens, blocks)
+        check_append(k, -k, rows, 2, 16, 64, seed=10)
+    check_append(k[:20], k[:20], (table, t, starts, granted, lens, blocks), 2, 16, 64, seed=11)  # tokens missing
+    # a second step on the first one's blocks, the scale growing and not
+    cache = lb.KVCache8.empty(8, 2, 16, 64)
+    t2 = ints([[6, 3, 1]])
+    ref = [torch.zeros(8, 2, 16, 64, dtype=torch.float64, device=DEV), torch.ones(8, 2, dtype=torch.float64, device=DEV)]
+    for step, (old, n, size) in enumerate(((0, 5, 1.0), (5, 1, 30.0), (6, 1, 0.01), (7, 20, 500.0), (27, 1, 1.0))):
+        x = torch.randn(n, 2, 64, generator=gen(30 + step), device=DEV) * size
+        U.append_reference(ref[0], ref[1], x, [[6, 3, 1]], [0], [n], [old + n])
+        lb.append_kv(cache, x, -x, t2, lb.StepPlan(ints([0, n]), ints([n]), ints([old + n])))
+        assert torch.equal(cache.k.double(), ref[0]) and torch.equal(cache.k_scale.double(), ref[1])
+        assert torch.equal(cache.v.double(), -ref[0])
+
+
+# ------------------------------------------------------------------------------------ attention
+def check_attend(q, cache, rows, scale=None, out=None):
+    """The products with e4m3 codes are exact, the softmax sum is f32: what rounds is the weights to
+    f16 (2^-11 each, so 2^-11 of the sum of |weight * value|), scores and exponentials in f32 (held to a
+    quarter of that for the scores of these inputs, below 2^6), and the result."""
+    table, t, starts, granted, lens, blocks = rows
+    dim = q.shape[2]
+    sc = dim ** -0.5 if scale is None else scale
+    lse = torch.full(q.shape[:2], 77.0, device=DEV)
+    y = torch.full(q.shape, 77.0, dtype=q.dtype, device=DEV) if out is None else out
+    lb.attend(q, cache, t, lb.StepPlan(starts, granted, lens), scale=scale, out=y, lse_out=lse)
+    want, mag, wl = U.attend_reference(q, cache.k, cache.v, cache.k_scale, cache.v_scale, table, starts.tolist(), granted.tolist(), lens.tolist(), sc)
+    idle = wl.isnan() & (lse == 77)
+    tol = 1.25 * 2.0 ** -11 * mag + torch.finfo(q.dtype).eps / 2 * want.abs() + (2.0 ** -24 if q.dtype == torch.float16 else 0)
+    off = (y.double() - want).abs()
+    ok = (off <= tol) | (want.isnan() & (y.isnan() | idle[..., None]))
+    assert bool(ok.all()), (float((off - tol).nan_to_num(0).max()), ok.logical_not().nonzero()[:5].tolist())
+    assert bool((y[idle] == 77).all()) if out is None else True
+    near = ((lse.double() - wl).abs() <= 2.0 ** -16 * (1 + wl.abs())) | (lse == wl) | wl.isnan()
+    assert bool(near.all())
+    return y, lse
+
+
+@pytest.mark.parametrize("ctx,new,heads,per,bs,dim", [
+    ([0], [1], 1, 1, 16, 64), ([15, 16, 17, 0], [1, 1, 1, 1], 2, 7, 16, 64), ([300, 2, 1111], [1, 1, 1], 2, 4, 32, 128),
+    ([0, 900], [1, 1], 1, 16, 64, 256), ([70, 0, 5, 33], [5, 40, 1, 16], 2, 3, 16, 128), ([5000], [1], 1, 8, 128, 128),
+    ([10, 300], [130, 77], 2, 4, 256, 64), ([3, 0, 100, 50], [0, 2, 0, 9], 1, 32, 16, 256), ([40], [200], 1, 1, 16, 128)])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_attend_sizes(ctx, new, heads, per, bs, dim, dtype):
+    rows = U.make_rows(ctx, new, bs, seed=dim)
+    cache = lb.KVCache8(*U.random_cache(rows[-1], heads, bs, dim, seed=per))
+    q = torch.randn(sum(new) + 2, heads * per, dim, generator=gen(dim), device=DEV).to(DTYPES[dtype])
+    y, lse = check_attend(q, cache, rows)
+    y2, lse2 = check_attend(q, cache, rows)
+    assert torch.equal(y, y2) or bool(y.isnan().any())
+    assert torch.equal(lse, lse2)
+
+
+def test_attend_many_rows():
+    ctx = [(i * 37) % 90 for i in range(1300)]
+    new = [1 if i % 5 else 0 for i in range(1300)]
+    rows = U.make_rows(ctx, new, 16)
+    cache = lb.KVCache8(*U.random_cache(rows[-1], 1, 16, 64))
+    q = torch.randn(sum(new), 2, 64, generator=gen(1), device=DEV).half()
+    check_attend(q, cache, rows)
+
+
+def test_attend_layouts_and_scales():
+    rows = U.make_rows([100, 33], [1, 20], 16)
+    cache = lb.KVCache8(*U.random_cache(rows[-1], 2, 16, 128))
+    for off in (0, 1):  # queries as a slice of a fused projection, 16-byte aligned and not; an output of its own strides
+        for dt in (torch.bfloat16, torch.float16):
+            fused = torch.randn(21, 1400, generator=gen(2), device=DEV).to(dt)
+            q = fused[:, off: off + 768].view(21, 6, 128)
+            check_attend(q, cache, rows)
+            out = torch.zeros(21, 6, 150, dtype=dt, device=DEV)
+            check_attend(q, cache, rows, scale=0.3, out=out[:, :, off: off + 128])
+            assert bool((out[:, :, off + 128:] == 0).all())
+    q = torch.randn(6, 21, 128, generator=gen(3), device=DEV).half().transpose(0, 1)
+    check_attend(q, cache, rows, scale=0.0)
+    check_attend(q, cache, rows, scale=-0.05)
+    # large queries (bf16 reaches far beyond f16), tiny ones, rows of zeros
+    q = torch.randn(21, 6, 128, generator=gen(4), device=DEV).bfloat16()
+    check_attend(q * 2.0 ** 100, cache, rows, scale=2.0 ** -104)
+    check_attend(q * 2.0 ** -100, cache, rows, scale=2.0 ** 96)
+    check_attend(q * 0, cache, rows)
+    # scales of the blocks that differ by far, that are no powers of two, blocks of zeros
+    cache.k_scale.mul_(torch.rand(cache.k_scale.shape, generator=gen(5), device=DEV) + 0.5)
+    cache.v_scale.mul_(torch.exp2(torch.randint(-30, 30, cache.v_scale.shape, generator=gen(6), device=DEV).float()) * 1.3)
+    check_attend(q, cache, rows)
+    cache.v.view(torch.uint8)[::2] = 0
+    cache.v_scale[::2] = 2.0 ** -126
+    check_attend(q, cache, rows)
+
+
+def test_attend_small_weights_are_not_lost():
+    """One token far above 60,000 others: together they hold a good part of the sum."""
+    n, dim = 60000, 64
+    rows = U.make_rows([n - 1], [1], 32)
+    k = torch.zeros(rows[-1], 1, 32, dim, device=DEV)
+    k[rows[0][0][0], 0, 0, 0] = 14.0
+    v = torch.randn(rows[-1], 1, 32, dim, generator=gen(1), device=DEV) * 0.1 + 2.0
+    one = torch.ones(rows[-1], 1, device=DEV)
+    cache = lb.KVCache8(k.to(E4M3), v.to(E4M3), one, one.clone())
+    q = torch.zeros(1, 1, dim, dtype=torch.float16, device=DEV)
+    q[0, 0, 0] = 1.0
+    for scale in (0.5, 0.8, 1.2):
+        check_attend(q, cache, rows, scale=scale)
+
+
+def test_attend_masked_places_and_bad_blocks():
+    table, t, starts, granted, lens, blocks = U.make_rows([20, 37, 9], [1, 30, 1], 16)
+    k, v, ks, vs = U.random_cache(blocks, 1, 16, 64, seed=3)
+    nan, q = 0x7F, torch.randn(32, 4, 64, generator=gen(7), device=DEV).bfloat16()
+    for name, x in (("k", k), ("v", v)):
+        for b, ln in enumerate(lens.tolist()):  # behind each row's end, in its last block
+            if ln % 16:
+                x.view(torch.uint8)[table[b][ln // 16], :, ln % 16:] = nan
+    cache = lb.KVCache8(k, v, ks, vs)
+    y, _ = check_attend(q, cache, (table, t, starts, granted, lens, blocks))
+    assert bool(y.isfinite().all())
+    # a NaN that later queries of the same row see and earlier ones do not
+    v.view(torch.uint8)[table[1][50 // 16], 0, 50 % 16, 5] = nan
+    y, _ = check_attend(q, cache, (table, t, starts, granted, lens, blocks))
+    seen = (torch.arange(37, 67, device=DEV) >= 50)
+    assert torch.equal(y[1:31, 0, 5].isnan(), seen) and not bool(y[1:31, 0, 4].isnan().any())
+    v.view(torch.uint8)[table[1][50 // 16], 0, 50 % 16, 5] = 0
+    k.view(torch.uint8)[table[1][44 // 16], 0, 44 % 16, 5] = nan
+    y, _ = check_attend(q, cache, (table, t, starts, granted, lens, blocks))
+    assert torch.equal(y[1:31, 0, 0].isnan(), torch.arange(37, 67, device=DEV) >= 44)
+    k.view(torch.uint8)[table[1][44 // 16], 0, 44 % 16, 5] = 0
+    # blocks outside the cache are not seen: some, and all of a row
+    for edits in ([(1, 0, -1)], [(1, 1, blocks), (2, 0, -9)], [(0, 0, -1), (0, 1, 2 ** 31 - 1)]):
+        tb = [list(r) for r in table]
+        for b, j, p in edits:
+            tb[b][j] = p
+        check_attend(q, cache, (tb, ints(tb), starts, granted, lens, blocks))
+    # rows whose numbers do not fit are left out
+    check_attend(q, cache, (table, t, starts, ints([1, 30, 11]), lens, blocks))
+    check_attend(q, cache, (table, t, starts, granted, ints([21, 9999, 10]), blocks))
+    check_attend(q[:10], cache, (table, t, starts, granted, lens, blocks))
+
+
+def test_attend_far_blocks():
+    """Blocks whose values lie behind 2^31 bytes of the cache."""
+    blocks, heads, bs, dim = 40000, 8, 64, 128
+    cache = lb.KVCache8(*(torch.zeros(blocks, heads, bs, dim, dtype=torch.uint8, device=DEV).view(E4M3) for _ in range(2)),
+                        torch.ones(blocks, heads, device=DEV), torch.ones(blocks, heads, device=DEV))
+    pages = [39999, 5, 39000, 33000, 20001]
+    x, y = (torch.randn(300, heads, dim, generator=gen(i), device=DEV).bfloat16() for i in (1, 2))
+    t, plan = ints([pages]), lb.StepPlan(ints([0, 300]), ints([300]), ints([300]))
+    lb.append_kv(cache, x, y, t, plan)
+    q = torch.randn(300, heads, dim, generator=gen(3), device=DEV).bfloat16()
+    got = lb.attend(q, cache, t, plan)
+    small = lb.KVCache8.empty(5, heads, bs, dim)
+    t2 = ints([[0, 1, 2, 3, 4]])
+    lb.append_kv(small, x, y, t2, plan)
+    assert torch.equal(got, lb.attend(q, small, t2, plan))
+    for i, p in enumerate(pages):
+        n = min(64, 300 - 64 * i)  # what lies behind the tokens of a block is nobody's
+        assert torch.equal(cache.k[p, :, :n].view(torch.uint8), small.k[i, :, :n].view(torch.uint8))
+
+
+# ---------------------------------------------------------------------------------- run together
+class Loop:
+    """A decode loop of one attention layer between two 4-bit projections, all state on the device."""
+
+    def __init__(self, rows=6, blocks=40, bs=16, heads=2, per=3, dim=64, vocab=500, hidden=128):
+        g = gen(77)
+        r = lambda *s: torch.randn(*s, generator=g, device=DEV)
+        self.rows, self.bs, self.heads, self.per, self.dim, self.width = rows, bs, heads, per, dim, 8
+        self.embed = r(vocab, hidden)
+        self.qkv = lb.Int4Weight.quantize(r((heads * (per + 2)) * dim, hidden) / 8, 32)
+        self.proj = lb.Int4Weight.quantize(r(hidden, heads * per * dim) / 8, 64)
+        self.head = lb.Int4Weight.quantize(r(vocab, hidden), 128)
+        self.cache = lb.KVCache8.empty(blocks, heads, bs, dim)
+        self.table = torch.full((rows, self.width), -1, dtype=torch.int32, device=DEV)
+        self.lens, self.free, self.n_free = ints([0] * rows), torch.arange(blocks, dtype=torch.int32, device=DEV), ints([blocks])
+        self.new = ints([5, 1, 17, 0, 3, 1])
+        self.tokens = torch.randint(0, vocab, (32,), generator=g, device=DEV)
+        self.prm = S.RowParams.from_params([S.SamplingParams(temperature=0.0)] * rows, DEV)
+        self.u = torch.rand(rows, generator=g, device=DEV)
+
+    def step(self, capacity):
+        plan = lb.plan_blocks(self.table, self.lens, self.new, self.free, self.n_free, self.bs, capacity, lens_out=self.lens, n_free_out=self.n_free)
+        x = self.embed[self.tokens[:capacity]].bfloat16()
+        hq, hk = self.heads * self.per, self.heads
+        qkv = lb.int4_matvec(x, self.qkv).view(capacity, hq + 2 * hk, self.dim)
+        lb.append_kv(self.cache, qkv[:, hq: hq + hk], qkv[:, hq + hk:], self.table, plan)
+        o = torch.zeros(capacity, hq, self.dim, dtype=x.dtype, device=DEV)
+        lse = torch.zeros(capacity, hq, device=DEV)
+        lb.attend(qkv[:, :hq], self.cache, self.table, plan, out=o, lse_out=lse)
+        h = x + lb.int4_matvec(o.view(capacity, -1), self.proj)
+        last = (plan.starts[1:] - 1).clamp(min=0)
+        tok = lb.sample_hidden(h[last.long()], self.head, self.prm, uniforms=self.u)
+        return plan, qkv, o, h, last, tok
+
+
+def test_decode_loop_against_64_bits():
+    m = Loop()
+    plan, qkv, o, h, last, tok = m.step(27)
+    hq, hk = m.heads * m.per, m.heads
+    # what the step did, in 64 bits from its own rounded intermediate values
+    table = m.table.tolist()
+    k, ks = torch.zeros(m.cache.k.shape, dtype=torch.float64, device=DEV), torch.ones(m.cache.k_scale.shape, dtype=torch.float64, device=DEV)
+    U.append_reference(k, ks, qkv[:, hq: hq + hk], table, plan.starts.tolist(), plan.granted.tolist(), plan.lens.tolist())
+    assert torch.equal(m.cache.k.double(), k) and torch.equal(m.cache.k_scale.double(), ks)
+    want, mag, _ = U.attend_reference(qkv[:, :hq], m.cache.k, m.cache.v, m.cache.k_scale, m.cache.v_scale, table, plan.starts.tolist(), plan.granted.tolist(), plan.lens.tolist(), m.dim ** -0.5)
+    off = (o.double() - want).abs()
+    assert bool((off <= 1.25 * 2.0 ** -11 * mag + 2.0 ** -8 * want.abs()).all())
+    logits = h[last.long()].double() @ m.head.dequantize().double().t()
+    best = logits.topk(2, -1).values
+    sure = best[:, 0] - best[:, 1] > 1e-3 * best.abs().amax(-1)
+    assert bool((tok.long() == logits.argmax(-1))[sure].all()) and int(sure.sum()) >= 4
+    # stop some rows, give their blocks back, decode on
+    codes = S.check_stop_batch(tok, None, [[int(tok[0])], [], [int(tok[2])], [], [], []])
+    held = {p for b in range(m.rows) for p in table[b][: -(-int(plan.lens[b]) // m.bs)]}
+    lb.release_blocks(m.table, m.lens, codes, m.free, m.n_free, m.bs, lens_out=m.lens, n_free_out=m.n_free)
+    assert [int(c) for c in codes[:2]] == [S.STOP_TOKEN, S.STOP_NONE] and m.lens[0] == 0 and m.lens[2] == 0
+    left = set(m.free[: int(m.n_free)].tolist())
+    live = {p for b in (1, 3, 4, 5) for p in table[b][: -(-int(m.lens[b]) // m.bs)]}
+    assert len(left) == int(m.n_free) and left | live == set(range(40)) and not left & live and held >= live
+
+
+def test_decode_loop_captured_and_replayed():
+    """The captured step against eager ones, several steps on: state in place, no host reads."""
+    eager, graph = Loop(), Loop()
+    for m in (eager, graph):
+        m.step(27)
+        m.new.fill_(1)
+    tokens = eager.tokens.clone()
+
+    def step(m):
+        plan, _, o, h, _, tok = m.step(6)
+        m.tokens[:6] = tok.long()
+        codes = (tok % 7 == 0).int()
+        lb.release_blocks(m.table, m.lens, codes, m.free, m.n_free, m.bs, lens_out=m.lens, n_free_out=m.n_free)
+        return tok, o, plan.slots
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    g = torch.cuda.CUDAGraph()
+    keep = [t.clone() for t in (graph.tokens, graph.table, graph.lens, graph.free, graph.n_free)]
+    with torch.cuda.stream(side):
+        with torch.cuda.graph(g, stream=side):
+            got = step(graph)
+    torch.cuda.current_stream().wait_stream(side)
+    for t, was in zip((graph.tokens, graph.table, graph.lens, graph.free, graph.n_free), keep):
+        assert torch.equal(t, was)  # capturing ran nothing
+    for _ in range(25):
+        want = step(eager)
+        g.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+    for name in ("table", "lens", "free", "n_free"):
+        assert torch.equal(getattr(eager, name), getattr(graph, name)), name
+    assert torch.equal(eager.cache.k.view(torch.uint8), graph.cache.k.view(torch.uint8)) and tokens.numel() == 32
+
+
+def test_two_streams_at_once():
+    rows = U.make_rows([3000, 77], [1, 1], 16)
+    cache = lb.KVCache8(*U.random_cache(rows[-1], 2, 16, 128))
+    w, x = int4_case(2, 3001, 512, 64, seed=1)
+    qs = [torch.randn(2, 8, 128, generator=gen(i), device=DEV).half() for i in range(2)]
+    plan = lb.StepPlan(*rows[2:5])
+    want = [(lb.attend(q, cache, rows[1], plan), lb.int4_matvec(x, w)) for q in qs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in qs]
+    got = []
+    for _ in range(20):
+        got = []
+        for q, s in zip(qs, streams):
+            with torch.cuda.stream(s):
+                got.append((lb.attend(q, cache, rows[1], plan), lb.int4_matvec(x, w)))
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+# -------------------------------------------------------------------------------------- refusals
+def test_refusals():
+    w, x = int4_case(2, 20, 64, 32, seed=1)
+    bad = lambda exc, f, *a, **k: pytest.raises(exc, f, *a, **k)
+    bad(RuntimeError, lb.int4_matvec, x.cpu(), w)
+    bad(ValueError, lb.int4_matvec, x[:, :32], w)
+    bad(TypeError, lb.int4_matvec, x.double(), w)
+    bad(TypeError, lb.int4_matvec, x, w, out_dtype=torch.int32)
+    bad(ValueError, lb.int4_matvec, x, lb.Int4Weight(w.packed[:, ::2], w.scales))
+    bad(ValueError, lb.int4_matvec, x, lb.Int4Weight(w.packed, w.scales.float()))
+    bad(ValueError, lb.int4_matvec, x, lb.Int4Weight(w.packed, w.scales[:10]))
+    bad(ValueError, lb.int4_matvec, x, lb.Int4Weight(w.packed.cpu(), w.scales))
+    bad(ValueError, lb.int4_matvec, x, w, out=torch.empty(2, 21, device=DEV))
+    bad(lb.SamplerError, lb.int4_matvec, torch.zeros(1, 96, device=DEV), lb.Int4Weight(torch.zeros(4, 48, dtype=torch.uint8, device=DEV), torch.zeros(4, 1, device=DEV).half()))
+    rows = U.make_rows([5], [2], 16)
+    cache, plan = lb.KVCache8(*U.random_cache(rows[-1], 2, 16, 64)), lb.StepPlan(*rows[2:5])
+    k = torch.zeros(2, 2, 64, device=DEV)
+    q = torch.zeros(2, 4, 64, device=DEV).half()
+    bad(ValueError, lb.append_kv, cache, k[:, :1], k, rows[1], plan)
+    bad(TypeError, lb.append_kv, cache, k.double(), k.double(), rows[1], plan)
+    bad(ValueError, lb.append_kv, cache, k, k, rows[1].long(), plan)
+    bad(ValueError, lb.append_kv, cache, k, k, rows[1], lb.StepPlan(rows[2][:1], *rows[3:5]))
+    bad(ValueError, lb.append_kv, lb.KVCache8(cache.k, cache.v, cache.k_scale, cache.v_scale.double()), k, k, rows[1], plan)
+    bad(TypeError, lb.attend, q.float(), cache, rows[1], plan)
+    bad(ValueError, lb.attend, q[:, :3], cache, rows[1], plan)
+    bad(ValueError, lb.attend, q, cache, rows[1], plan, out=torch.empty(2, 4, 64, device=DEV))
+    bad(ValueError, lb.attend, q, cache, rows[1], plan, lse_out=torch.empty(4, 2, device=DEV))
+    odd = lb.KVCache8(*U.random_cache(rows[-1], 2, 16, 96))
+    bad(lb.SamplerError, lb.attend, torch.zeros(2, 4, 96, device=DEV).half(), odd, rows[1], plan)
+    odd = lb.KVCache8(*U.random_cache(rows[-1], 2, 24, 64))
+    bad(lb.SamplerError, lb.attend, q, odd, rows[1], plan)
+    bad(lb.SamplerError, lb.append_kv, odd, k, k, rows[1], plan)
+    args = (ints([[0, 1]]), ints([3]), ints([1]), ints([1, 2]), ints([2]))
+    bad(ValueError, lb.plan_blocks, *args, 16, -1)
+    bad(lb.SamplerError, lb.plan_blocks, *args, 0, 4)
+    bad(ValueError, lb.plan_blocks, args[0], args[1].long(), *args[2:], 16, 4)
+    bad(ValueError, lb.plan_blocks, args[0], args[1], args[2], args[3], ints([1, 1]), 16, 4)
+    bad(ValueError, lb.release_blocks, args[0], args[1], ints([1, 1]), args[3], args[4], 16)
+    bad(RuntimeError, lb.plan_blocks, args[0].cpu(), *args[1:], 16, 4)
+    # no tokens, no rows
+    lb.append_kv(cache, k[:0], k[:0], rows[1], plan)
+    assert lb.attend(q[:0], cache, rows[1], plan).shape == (0, 4, 64)
