@@ -179,6 +179,10 @@ __device__ __forceinline__ void fence_cluster() { asm volatile("fence.acq_rel.cl
 __device__ __forceinline__ void cp_async4(void* smem_dst, const void* gmem_src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(saddr(smem_dst)), "l"(gmem_src) : "memory");
 }
+// 16-byte asynchronous global -> shared copy past the L1 cache.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 __device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 // Waits until at most N of this thread's most recent cp.async groups are still pending.

@@ -100,31 +100,46 @@ static bool table_ok(const void* table, int64_t stride, int width, int B, int bs
 // ---------------------------------------------------------------- attention
 static constexpr int AT_CAP_CTAS = 160;  // CTAs that the workspace has room for
 
-template <int D>
+template <int D, int NQ>
 static size_t attend_bytes() {
-  const size_t workers = (size_t)AT_CAP_CTAS * AtCfg<D>::NW;
-  return workers * sizeof(int4) + workers * 2 * (48 + 16 * D) * sizeof(float);
+  const size_t workers = (size_t)AT_CAP_CTAS * AtCfg<D, NQ>::NW;
+  return workers * (sizeof(int4) + 2 * at_piece(D, NQ) * sizeof(float));
 }
 
-template <int D, int DT>
+template <int D, int DT, int NQ>
 static cudaError_t launch_attend(AttendArgs a, void* ws, cudaStream_t st) {
   static SmemSet set;
   const int dev = device_index();
-  constexpr int NW = AtCfg<D>::NW;
-  constexpr int smem = NW * AtCfg<D>::ST * (32 * D + 16);
-  cudaError_t e = allow_smem(lss_attend_kernel<D, DT>, set, dev, smem);
+  constexpr int NW = AtCfg<D, NQ>::NW;
+  constexpr int smem = NW * AtCfg<D, NQ>::ST * (32 * D + 16);
+  cudaError_t e = allow_smem(lss_attend_kernel<D, DT, NQ>, set, dev, smem);
   if (e != cudaSuccess) return e;
-  const int ctas = std::min(sm_count(dev), AT_CAP_CTAS);
+  // No more warps than there can be units.
+  const int64_t groups = a.B + (int64_t)a.T * a.per / (8 * NQ) + 1;
+  const int64_t units = groups * a.heads * ((((int64_t)a.width << a.bs_shift) + 15) >> 4);
+  const int ctas = (int)std::min((int64_t)std::min(sm_count(dev), AT_CAP_CTAS), (units + NW - 1) / NW);
   a.meta = reinterpret_cast<int4*>(ws);
   a.part = reinterpret_cast<float*>(a.meta + (size_t)ctas * NW);
-  e = launch(lss_attend_kernel<D, DT>, (unsigned)ctas, NW * 32, smem, 1, false, st, a);
+  e = launch(lss_attend_kernel<D, DT, NQ>, (unsigned)ctas, NW * 32, smem, 1, false, st, a);
   if (e != cudaSuccess) return e;
-  return launch(lss_attend_join_kernel<D, DT>, (unsigned)(ctas * NW), 256, 0, 1, true, st, a);
+  return launch(lss_attend_join_kernel<D, DT, NQ>, (unsigned)(ctas * NW), 256, 0, 1, true, st, a);
+}
+
+// Query rows per group: as many as a key head's rows fill on the average (a batch of single tokens:
+// the query heads of a key head).
+template <int D, int DT>
+static cudaError_t launch_attend_rows(const AttendArgs& a, void* ws, cudaStream_t st) {
+  const int64_t rows = (int64_t)a.per * ((a.T + (int64_t)a.B - 1) / a.B);
+  if (rows <= 8) return launch_attend<D, DT, 1>(a, ws, st);
+  if constexpr (D < 256) {
+    if (rows > 16) return launch_attend<D, DT, 4>(a, ws, st);
+  }
+  return launch_attend<D, DT, 2>(a, ws, st);
 }
 
 template <int D>
 static cudaError_t launch_attend_dt(int dtype, const AttendArgs& a, void* ws, cudaStream_t st) {
-  return dtype == LSS_DTYPE_BF16 ? launch_attend<D, LSS_DTYPE_BF16>(a, ws, st) : launch_attend<D, LSS_DTYPE_F16>(a, ws, st);
+  return dtype == LSS_DTYPE_BF16 ? launch_attend_rows<D, LSS_DTYPE_BF16>(a, ws, st) : launch_attend_rows<D, LSS_DTYPE_F16>(a, ws, st);
 }
 
 // ---------------------------------------------------------------- 4-bit products
@@ -135,17 +150,17 @@ static cudaError_t launch_int4(const Int4Args& a, cudaStream_t st, bool& fits) {
   static SmemSet set;
   const int dev = device_index(), sms = sm_count(dev);
   constexpr int planes = DT == LSS_DTYPE_F32 ? 3 : 1;
-  constexpr int fixed = I4_NW * I4_ST * (1024 + 64 * (4 / SPG)) + I4_NW * 2 * 128 * 4;
-  const int NB = (a.N + 15) / 16, KB = (a.K + I4_KB - 1) / I4_KB;
+  constexpr int fixed = I4_NW * I4_ST * (I4_RB * I4_KB / 2) + I4_NW * 2 * I4_SUMS * 4;
+  const int NB = (a.N + I4_RB - 1) / I4_RB, KB = (a.K + I4_KB - 1) / I4_KB;
   // CTAs per row block range: the split with the fewest units in the fullest CTA.  A cluster's
-  // exchange costs about as much as 16 units, and its row blocks' sums take 16 KB at most.
+  // exchange costs about as much as 8 units, and its row blocks' sums take 16 KB at most.
   int ks = 1, nclusters = std::min(NB, sms);
   int64_t best = INT64_MAX;
   for (int k = 1; k <= 8 && k <= KB; k <<= 1) {
     const int nc = std::min(NB, std::max(1, sms / k));
     const int nrb = (NB + nc - 1) / nc;
-    if (k > 1 && nrb > 32) continue;
-    const int64_t cost = (int64_t)nrb * ((KB + k - 1) / k) + (k > 1 ? 16 : 0);
+    if (k > 1 && nrb > 16) continue;
+    const int64_t cost = (int64_t)nrb * ((KB + k - 1) / k) + (k > 1 ? 8 : 0);
     if (cost < best) {
       best = cost;
       ks = k;
@@ -154,7 +169,7 @@ static cudaError_t launch_int4(const Int4Args& a, cudaStream_t st, bool& fits) {
   }
   auto room = [&](int k) {  // rows of x that fit
     const int nc = std::min(NB, std::max(1, sms / k));
-    const int left = I4_SMEM - fixed - (k > 1 ? (NB + nc - 1) / nc * 512 : 0);
+    const int left = I4_SMEM - fixed - (k > 1 ? (NB + nc - 1) / nc * I4_SUMS * 4 : 0);
     return left / (((KB + k - 1) / k) * I4_KB * 2 * planes);
   };
   fits = room(ks) >= 1;
@@ -162,7 +177,7 @@ static cudaError_t launch_int4(const Int4Args& a, cudaStream_t st, bool& fits) {
   const int most = std::min(I4_ROWS, room(ks));
   for (int r0 = 0; r0 < a.rows; r0 += most) {
     const int rows = std::min(most, a.rows - r0);
-    const int smem = fixed + (ks > 1 ? (NB + nclusters - 1) / nclusters * 512 : 0) + rows * ((KB + ks - 1) / ks) * I4_KB * 2 * planes;
+    const int smem = fixed + (ks > 1 ? (NB + nclusters - 1) / nclusters * I4_SUMS * 4 : 0) + rows * ((KB + ks - 1) / ks) * I4_KB * 2 * planes;
     cudaError_t e = allow_smem(lss_int4_kernel<DT, SPG>, set, dev, smem);
     if (e != cudaSuccess) return e;
     e = launch(lss_int4_kernel<DT, SPG>, (unsigned)(nclusters * ks), I4_NT, smem, ks, false, st, a, r0, rows, ks);
@@ -271,36 +286,46 @@ int lss_kv_append(const void* k, int64_t k_token_stride, int64_t k_head_stride, 
     return LSS_ERR_INVALID_ARG;
   if (!aligned_to(k_cache, 16) || !aligned_to(v_cache, 16)) return LSS_ERR_INVALID_ARG;
   AppendArgs a{k, v, k_token_stride, k_head_stride, v_token_stride, v_head_stride, k_cache, v_cache, k_scale,
-               v_scale, num_blocks, heads, block_size, dim, table, table_stride, width, starts, granted, lens, B, T, 0};
+               v_scale, num_blocks, heads, log2_of(block_size), dim, table, table_stride, width, starts, granted, lens, B, T, 0};
   const int per16 = dtype == LSS_DTYPE_F32 ? 4 : 8;  // values in 16 bytes
   a.aligned = aligned_to(k, 16) && aligned_to(v, 16) && k_token_stride % per16 == 0 && k_head_stride % per16 == 0 &&
               v_token_stride % per16 == 0 && v_head_stride % per16 == 0;
   // Blocks that a step can write: one per token at most, and two more per row than its tokens fill.
   const int64_t blocks = std::min((int64_t)T, (int64_t)T / block_size + 2 * (int64_t)B);
   const int64_t items = blocks * 2 * heads;
-  static SmemSet sets[3];
   const int dev = device_index(), smem = 4 * B;
-  const int64_t ctas = std::max((int64_t)1, std::min((items + KV_NT / 32 - 1) / (KV_NT / 32), (int64_t)sm_count(dev) * 8));
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  auto go = [&](auto kern, SmemSet& set) {
+  auto go = [&](auto kern, SmemSet& set, int team) {
     if (smem > 40 * 1024) {
       const cudaError_t e = allow_smem(kern, set, dev, smem);
       if (e != cudaSuccess) return e;
     }
+    const int teams = KV_NT / 32 / team;
+    const int64_t ctas = std::max((int64_t)1, std::min((items + teams - 1) / teams, (int64_t)sm_count(dev) * 3));
     return launch(kern, (unsigned)ctas, KV_NT, (size_t)smem, 1, false, st, a);
   };
+  static SmemSet sets[9];
+  // Warps per unit: as many as its values fill on the average (2048 a warp).
+  const int64_t values = (int64_t)T * dim / blocks;
+  const int team = values > 4096 ? 4 : values > 2048 + 512 ? 2 : 1;
+  auto by_team = [&](auto k1, auto k2, auto k4, int at) {
+    return status_of(team == 4 ? go(k4, sets[at + 2], 4) : team == 2 ? go(k2, sets[at + 1], 2) : go(k1, sets[at], 1));
+  };
   switch (dtype) {
-    case LSS_DTYPE_F32: return status_of(go(lss_append_kernel<LSS_DTYPE_F32>, sets[0]));
-    case LSS_DTYPE_BF16: return status_of(go(lss_append_kernel<LSS_DTYPE_BF16>, sets[1]));
-    default: return status_of(go(lss_append_kernel<LSS_DTYPE_F16>, sets[2]));
+    case LSS_DTYPE_F32:
+      return by_team(lss_append_kernel<LSS_DTYPE_F32, 1>, lss_append_kernel<LSS_DTYPE_F32, 2>, lss_append_kernel<LSS_DTYPE_F32, 4>, 0);
+    case LSS_DTYPE_BF16:
+      return by_team(lss_append_kernel<LSS_DTYPE_BF16, 1>, lss_append_kernel<LSS_DTYPE_BF16, 2>, lss_append_kernel<LSS_DTYPE_BF16, 4>, 3);
+    default:
+      return by_team(lss_append_kernel<LSS_DTYPE_F16, 1>, lss_append_kernel<LSS_DTYPE_F16, 2>, lss_append_kernel<LSS_DTYPE_F16, 4>, 6);
   }
 }
 
 size_t lss_attend_workspace_bytes(int dim) {
   switch (dim) {
-    case 64: return attend_bytes<64>();
-    case 128: return attend_bytes<128>();
-    case 256: return attend_bytes<256>();
+    case 64: return std::max({attend_bytes<64, 1>(), attend_bytes<64, 2>(), attend_bytes<64, 4>()});
+    case 128: return std::max({attend_bytes<128, 1>(), attend_bytes<128, 2>(), attend_bytes<128, 4>()});
+    case 256: return std::max(attend_bytes<256, 1>(), attend_bytes<256, 2>());
     default: return 0;
   }
 }

@@ -21,9 +21,17 @@ __all__ = ["Int4Weight", "int4_matvec", "sample_hidden"]
 _CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
+_HERE = contextlib.nullcontext()
+
+
 def _on(dev: torch.device):
     """The device that the library launches on, where it is not the current one."""
-    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+    return _HERE if dev.index == torch._C._cuda_getDevice() else torch.cuda.device(dev)
+
+
+def _stream(dev: torch.device) -> int:
+    """torch's current stream on ``dev`` as a cudaStream_t."""
+    return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
 @dataclass
@@ -103,7 +111,7 @@ def int4_matvec(x: torch.Tensor, weight: Int4Weight, out_dtype: Optional[torch.d
         _lib.check("lss_int4_matvec", lib.lss_int4_matvec(
             x2.data_ptr(), _CODES[x.dtype], rows, k, max(x2.stride(0), k), packed.data_ptr(), scales.data_ptr(),
             _CODES[scales.dtype], n, k // groups, out.data_ptr(), _CODES[out_dtype],
-            max(out.stride(0), n) if out.dim() == 2 else n, torch.cuda.current_stream(dev).cuda_stream))
+            max(out.stride(0), n) if out.dim() == 2 else n, _stream(dev)))
     return out
 
 

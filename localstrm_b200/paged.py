@@ -15,7 +15,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .head import _CODES, _on
+from .head import _CODES, _on, _stream
 
 __all__ = ["StepPlan", "KVCache8", "plan_blocks", "release_blocks", "append_kv", "attend"]
 
@@ -90,9 +90,9 @@ def _stride0(t: torch.Tensor) -> int:
     return max(t.stride(0), t.shape[1])  # one row: its stride says nothing
 
 
-def _out(name: str, t: Optional[torch.Tensor], n: int, dev: torch.device) -> torch.Tensor:
+def _out(name: str, t: Optional[torch.Tensor], new: torch.Tensor, n: int, dev: torch.device) -> torch.Tensor:
     if t is None:
-        return torch.empty(n, dtype=torch.int32, device=dev)
+        return new
     _ints(name, t, n, dev)
     return t
 
@@ -116,9 +116,10 @@ def plan_blocks(block_table: torch.Tensor, lens: torch.Tensor, new_lens: torch.T
     _ints("n_free", n_free, 1, dev)
     if capacity < 0 or free_blocks.numel() < 1:
         raise ValueError("capacity must not be negative, free_blocks not empty")
-    lens_out, n_free_out = _out("lens_out", lens_out, B, dev), _out("n_free_out", n_free_out, 1, dev)
-    i32 = torch.empty(capacity + 2 * B + 1, dtype=torch.int32, device=dev)
-    positions, granted, starts = i32[:capacity], i32[capacity:capacity + B], i32[capacity + B:]
+    # One allocation for the int32 results.
+    positions, granted, starts, new_state, new_free = torch.empty(capacity + 3 * B + 2, dtype=torch.int32, device=dev).split_with_sizes(
+        (capacity, B, B + 1, B, 1))
+    lens_out, n_free_out = _out("lens_out", lens_out, new_state, B, dev), _out("n_free_out", n_free_out, new_free, 1, dev)
     slots = torch.empty(capacity, dtype=torch.int64, device=dev)
     lib = _lib.load()
     with _on(dev):
@@ -126,7 +127,7 @@ def plan_blocks(block_table: torch.Tensor, lens: torch.Tensor, new_lens: torch.T
             block_table.data_ptr(), _stride0(block_table), width, lens.data_ptr(), new_lens.data_ptr(), B, block_size,
             free_blocks.data_ptr(), free_blocks.numel(), n_free.data_ptr(), capacity, slots.data_ptr(), positions.data_ptr(),
             starts.data_ptr(), granted.data_ptr(), lens_out.data_ptr(), n_free_out.data_ptr(),
-            torch.cuda.current_stream(dev).cuda_stream))
+            _stream(dev)))
     return StepPlan(starts, granted, lens_out, slots, positions, n_free_out)
 
 
@@ -143,13 +144,14 @@ def release_blocks(block_table: torch.Tensor, lens: torch.Tensor, codes: torch.T
     _ints("n_free", n_free, 1, dev)
     if free_blocks.numel() < 1:
         raise ValueError("free_blocks must not be empty")
-    lens_out, n_free_out = _out("lens_out", lens_out, B, dev), _out("n_free_out", n_free_out, 1, dev)
+    new_state, new_free = torch.empty(B + 1, dtype=torch.int32, device=dev).split_with_sizes((B, 1))
+    lens_out, n_free_out = _out("lens_out", lens_out, new_state, B, dev), _out("n_free_out", n_free_out, new_free, 1, dev)
     lib = _lib.load()
     with _on(dev):
         _lib.check("lss_block_release", lib.lss_block_release(
             block_table.data_ptr(), _stride0(block_table), width, lens.data_ptr(), codes.data_ptr(), B, block_size,
             free_blocks.data_ptr(), free_blocks.numel(), n_free.data_ptr(), lens_out.data_ptr(), n_free_out.data_ptr(),
-            torch.cuda.current_stream(dev).cuda_stream))
+            _stream(dev)))
     return lens_out, n_free_out
 
 
@@ -181,7 +183,7 @@ def append_kv(cache: KVCache8, k: torch.Tensor, v: torch.Tensor, block_table: to
             k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), _CODES[k.dtype], k.shape[0], heads,
             dim, cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), blocks, bs,
             block_table.data_ptr(), _stride0(block_table), width, plan.starts.data_ptr(), plan.granted.data_ptr(),
-            plan.lens.data_ptr(), B, torch.cuda.current_stream(dev).cuda_stream))
+            plan.lens.data_ptr(), B, _stream(dev)))
 
 
 def attend(q: torch.Tensor, cache: KVCache8, block_table: torch.Tensor, plan: StepPlan, scale: Optional[float] = None,
@@ -219,5 +221,5 @@ def attend(q: torch.Tensor, cache: KVCache8, block_table: torch.Tensor, plan: St
             _stride0(block_table), width, plan.starts.data_ptr(), plan.granted.data_ptr(), plan.lens.data_ptr(), B,
             float(scale if scale is not None else dim ** -0.5), out.data_ptr(), out.stride(0), out.stride(1),
             lse_out.data_ptr() if lse_out is not None else None, ws.data_ptr(), ws.numel(),
-            torch.cuda.current_stream(dev).cuda_stream))
+            _stream(dev)))
     return out
