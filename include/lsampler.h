@@ -228,18 +228,22 @@ int lss_read_row_paths(const void* workspace, int B, int32_t* paths_out, void* s
  * ------------------------------------------------------------------------------------------ */
 
 /* y[r, n] = sum_k x[r, k] * (code[n, k] - 8) * scale[n, k / group], sums in f32, one rounding to
- * y's type.  Meant for the few rows of a decode step (the matrix is read once for up to eight rows).
+ * y's type.  Meant for the rows of a decode step: the matrix is read once for up to 64 of them.
  *   x        [rows] x [x_stride elements], dtype LSS_DTYPE_*; K a multiple of 32
  *   packed   uint8 [N][K / 2], column 2i in the low four bits of byte i, 2i + 1 in the high ones;
  *            16-byte aligned
  *   scales   [N][K / group], dtype LSS_DTYPE_BF16 or LSS_DTYPE_F16, 4-byte aligned;
  *            group: 32, 64 or a multiple of 128 that divides K
  *   y        [rows] x [y_stride elements], dtype LSS_DTYPE_*
- * LSS_ERR_UNSUPPORTED when one row of x does not fit the shared memory of an SM (K beyond 49,152 for
- * 16-bit x, 16,384 for f32). */
+ *   workspace  lss_int4_workspace_bytes(rows, K, x_dtype, N) bytes (0 for up to eight rows: NULL will do),
+ *              16-byte aligned, of this call alone until it is done
+ * LSS_ERR_UNSUPPORTED for up to eight rows when one row of x does not fit the shared memory of an SM (K
+ * beyond 49,152 for 16-bit x, 16,384 for f32).  A wait inside the kernel for more than eight rows that gives
+ * up after about a second leaves NaN in y. */
+size_t lss_int4_workspace_bytes(int rows, int K, int x_dtype, int N);
 int lss_int4_matvec(const void* x, int x_dtype, int rows, int K, int64_t x_stride, const uint8_t* packed,
                     const void* scales, int scale_dtype, int N, int group, void* y, int y_dtype,
-                    int64_t y_stride, void* stream);
+                    int64_t y_stride, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Block tables.  A row (request) of `lens[b]` tokens holds the blocks table[b][0 ..
  * ceil(lens[b] / block_size)); free blocks lie on a stack, free_blocks[0 .. n_free), whose top is

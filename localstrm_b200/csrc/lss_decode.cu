@@ -5,7 +5,7 @@
 
 #include "lss_attend.cuh"
 #include "lss_blocks.cuh"
-#include "lss_int4.cuh"
+#include "lss_int4_tc.cuh"
 #include "lss_kvcache.cuh"
 
 using namespace lss;
@@ -186,18 +186,81 @@ static cudaError_t launch_int4(const Int4Args& a, cudaStream_t st, bool& fits) {
   return cudaSuccess;
 }
 
+// Nine rows and more: the tensor-memory kernel, 64 rows of x at a time.
+struct TcPlan {
+  int blocks, ks;  // row blocks (teams) and column slices: teams on all SMs first, then slices
+  size_t xop, part;
+};
+static TcPlan tc_plan(int rows, int N, int K, int x_dtype, int sms) {
+  TcPlan p;
+  const int NB = (N + T4_RB - 1) / T4_RB, KB = (K + I4_KB - 1) / I4_KB;
+  p.blocks = std::min(T4_TEAMS, (NB + sms - 1) / sms);
+  const int ctas = (NB + p.blocks - 1) / p.blocks;
+  p.ks = std::max(1, std::min(KB, sms / ctas));
+  const int most = std::min(rows, 64);
+  p.xop = (size_t)KB * (x_dtype == LSS_DTYPE_F32 ? 3 : 1) * 64 * 256;
+  p.part = p.ks > 1 ? (size_t)p.ks * most * N * sizeof(float) : 0;
+  return p;
+}
+
+template <int DT, int SPG, int NR>
+static cudaError_t launch_int4_tc(const Int4Args& a, int row0, int rows, const TcPlan& p, unsigned char* ws, cudaStream_t st) {
+  static SmemSet set;
+  constexpr int planes = DT == LSS_DTYPE_F32 ? 3 : 1;
+  constexpr int smem = 1024 + (planes == 1 ? 4 : 2) * planes * NR * 256 + T4_NW * T4_ST * (32 * I4_KB / 2);
+  cudaError_t e = allow_smem(lss_int4_tc_kernel<DT, SPG, NR>, set, device_index(), smem);
+  if (e != cudaSuccess) return e;
+  const int NB = (a.N + T4_RB - 1) / T4_RB, KB = (a.K + I4_KB - 1) / I4_KB;
+  Int4TcArgs t{a, ws, reinterpret_cast<float*>(ws + p.xop), row0, rows, p.ks, p.blocks};
+  e = launch(lss_int4_operand_kernel<DT, NR>, (unsigned)((KB * NR * 16 + 255) / 256), 256, 0, 1, false, st, a, row0, rows, ws);
+  if (e != cudaSuccess) return e;
+  e = launch(lss_int4_tc_kernel<DT, SPG, NR>, (unsigned)((NB + p.blocks - 1) / p.blocks * p.ks), T4_NT, smem, 1, true, st, t);
+  if (e != cudaSuccess || p.ks == 1) return e;
+  return launch(lss_int4_sum_kernel, (unsigned)(((int64_t)rows * a.N + 255) / 256), 256, 0, 1, false, st, t);
+}
+
+template <int DT, int SPG>
+static cudaError_t launch_int4_rows(const Int4Args& a, void* ws, size_t ws_bytes, cudaStream_t st, int& status) {
+  if (a.rows <= I4_ROWS) {
+    bool fits = true;
+    const cudaError_t e = launch_int4<DT, SPG>(a, st, fits);
+    if (!fits) status = LSS_ERR_UNSUPPORTED;
+    return e;
+  }
+  const TcPlan p = tc_plan(a.rows, a.N, a.K, DT, sm_count(device_index()));
+  if (!ws || ws_bytes < p.xop + p.part || !aligned_to(ws, 16)) {
+    status = LSS_ERR_WORKSPACE;
+    return cudaSuccess;
+  }
+  unsigned char* w = reinterpret_cast<unsigned char*>(ws);
+  for (int r0 = 0; r0 < a.rows; r0 += 64) {
+    const int rows = std::min(64, a.rows - r0);
+    const cudaError_t e = rows <= 16   ? launch_int4_tc<DT, SPG, 16>(a, r0, rows, p, w, st)
+                          : rows <= 32 ? launch_int4_tc<DT, SPG, 32>(a, r0, rows, p, w, st)
+                                       : launch_int4_tc<DT, SPG, 64>(a, r0, rows, p, w, st);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
+}
+
 template <int DT>
-static cudaError_t launch_int4_group(const Int4Args& a, cudaStream_t st, bool& fits) {
-  if (a.group == 32) return launch_int4<DT, 1>(a, st, fits);
-  if (a.group == 64) return launch_int4<DT, 2>(a, st, fits);
-  return launch_int4<DT, 4>(a, st, fits);
+static cudaError_t launch_int4_group(const Int4Args& a, void* ws, size_t ws_bytes, cudaStream_t st, int& status) {
+  if (a.group == 32) return launch_int4_rows<DT, 1>(a, ws, ws_bytes, st, status);
+  if (a.group == 64) return launch_int4_rows<DT, 2>(a, ws, ws_bytes, st, status);
+  return launch_int4_rows<DT, 4>(a, ws, ws_bytes, st, status);
 }
 
 extern "C" {
 
+size_t lss_int4_workspace_bytes(int rows, int K, int x_dtype, int N) {
+  if (rows <= I4_ROWS || K < 1 || N < 1) return 0;
+  const TcPlan p = tc_plan(rows, N, K, x_dtype, sm_count(device_index()));
+  return p.xop + p.part;
+}
+
 int lss_int4_matvec(const void* x, int x_dtype, int rows, int K, int64_t x_stride, const uint8_t* packed,
                     const void* scales, int scale_dtype, int N, int group, void* y, int y_dtype,
-                    int64_t y_stride, void* stream) {
+                    int64_t y_stride, void* workspace, size_t workspace_bytes, void* stream) {
   if (rows < 0 || N < 1 || K < 32 || K % 32 != 0 || x_stride < K || y_stride < N) return LSS_ERR_INVALID_ARG;
   if (!known_dtype(x_dtype) || !known_dtype(y_dtype)) return LSS_ERR_INVALID_ARG;
   if (scale_dtype != LSS_DTYPE_BF16 && scale_dtype != LSS_DTYPE_F16) return LSS_ERR_INVALID_ARG;
@@ -219,15 +282,14 @@ int lss_int4_matvec(const void* x, int x_dtype, int rows, int K, int64_t x_strid
   a.y_stride = y_stride;
   a.x_aligned = aligned_to(x, 16) && x_stride % 8 == 0;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  bool fits = true;
+  int status = LSS_OK;
   cudaError_t e;
   switch (x_dtype) {
-    case LSS_DTYPE_F32: e = launch_int4_group<LSS_DTYPE_F32>(a, st, fits); break;
-    case LSS_DTYPE_BF16: e = launch_int4_group<LSS_DTYPE_BF16>(a, st, fits); break;
-    default: e = launch_int4_group<LSS_DTYPE_F16>(a, st, fits); break;
+    case LSS_DTYPE_F32: e = launch_int4_group<LSS_DTYPE_F32>(a, workspace, workspace_bytes, st, status); break;
+    case LSS_DTYPE_BF16: e = launch_int4_group<LSS_DTYPE_BF16>(a, workspace, workspace_bytes, st, status); break;
+    default: e = launch_int4_group<LSS_DTYPE_F16>(a, workspace, workspace_bytes, st, status); break;
   }
-  if (!fits) return LSS_ERR_UNSUPPORTED;
-  return status_of(e);
+  return e != cudaSuccess ? status_of(e) : status;
 }
 
 int lss_block_plan(int32_t* table, int64_t table_stride, int width, const int32_t* lens,

@@ -110,64 +110,69 @@ __device__ __forceinline__ void i4_store(const Int4Args& a, int row, int n, floa
   else reinterpret_cast<__half*>(a.y)[at] = __float2half_rn(v);
 }
 
+// Eight values of x (row r, columns k .. k + 7) as operand words in the order of int4_unpack's pairs; zero
+// where `in` is false.  f32 values become P = 3 planes of bf16 that add up to them exactly (8 + 8 + 8
+// bits, truncated).
+template <int DT, int P>
+__device__ __forceinline__ void i4_octet(const Int4Args& a, int r, int k, bool in, uint32_t (&out)[P][4]) {
+  constexpr int ord[8] = {0, 4, 1, 5, 2, 6, 3, 7};
+  const int64_t at = (int64_t)r * a.x_stride + k;
+  if constexpr (DT == LSS_DTYPE_F32) {
+    float f[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = in ? reinterpret_cast<const float*>(a.x)[at + e] : 0.0f;
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      uint16_t h[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        h[e] = (uint16_t)(__float_as_uint(f[e]) >> 16);
+        // An infinity leaves no rest; a NaN whose payload lies in the low half stays one.
+        if (f[e] != f[e]) h[e] |= 0x40;
+        const float rest = f[e] - __uint_as_float((uint32_t)h[e] << 16);
+        f[e] = fabsf(f[e]) <= FLT_MAX ? rest : 0.0f;
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) out[p][e] = (uint32_t)h[ord[2 * e]] | ((uint32_t)h[ord[2 * e + 1]] << 16);
+    }
+  } else {
+    uint16_t h[8];
+    const uint16_t* src = reinterpret_cast<const uint16_t*>(a.x) + at;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) h[e] = 0;
+    if (in) {  // K is a multiple of 32
+      if (a.x_aligned) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(src));
+        const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) h[e] = (uint16_t)(u[e >> 1] >> ((e & 1) * 16));
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) h[e] = src[e];
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) out[0][e] = (uint32_t)h[ord[2 * e]] | ((uint32_t)h[ord[2 * e + 1]] << 16);
+  }
+}
+
 // Stages columns [k0, k0 + kn) of `rows` rows of x in shared memory as matrix operands.  The 8 columns
 // that lane c of a row multiplies in step j of a unit (a 32-bit word of codes) are number
 // 4 SPG (j / SPG) + SPG c + j % SPG of the unit's 16: a lane's words of one group are neighbours, and a
-// step stays inside a group.  They lie at [unit][j][row][c], 16 bytes in the order of int4_unpack's pairs.
-// f32 values become three planes of bf16 that add up to them exactly (8 + 8 + 8 bits, truncated).
+// step stays inside a group.  They lie at [plane][unit][j][row][c], 16 bytes each.
 template <int DT, int SPG>
 __device__ __forceinline__ void i4_stage_x(const Int4Args& a, int row0, int rows, int k0, int kn, unsigned char* xs) {
   constexpr int P = DT == LSS_DTYPE_F32 ? 3 : 1;
   const int groups = kn >> 3;  // kn is a multiple of 128; columns from K on are zero
+  const int plane = (kn >> 5) * rows * 64;
   for (int i = threadIdx.x; i < rows * groups; i += blockDim.x) {
     const int r = i / groups, q = i - r * groups, k = k0 + q * 8;
-    const int64_t at = (int64_t)(row0 + r) * a.x_stride + k;
     const int o = q & 15, gq = o / (4 * SPG), c = (o % (4 * SPG)) / SPG, j = gq * SPG + o % SPG;
     unsigned char* dst = xs + (((q >> 4) * 4 + j) * rows + r) * 64 + c * 16;
-    constexpr int ord[8] = {0, 4, 1, 5, 2, 6, 3, 7};
-    if (DT == LSS_DTYPE_F32) {
-      float f[8];
+    uint32_t out[P][4];
+    i4_octet<DT, P>(a, row0 + r, k, k < a.K, out);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] = k < a.K ? reinterpret_cast<const float*>(a.x)[at + e] : 0.0f;
-      const int plane = (kn >> 5) * rows * 64;
-#pragma unroll
-      for (int p = 0; p < P; ++p) {
-        uint16_t h[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          h[e] = (uint16_t)(__float_as_uint(f[e]) >> 16);
-          // An infinity leaves no rest; a NaN whose payload lies in the low half stays one.
-          if (f[e] != f[e]) h[e] |= 0x40;
-          const float rest = f[e] - __uint_as_float((uint32_t)h[e] << 16);
-          f[e] = fabsf(f[e]) <= FLT_MAX ? rest : 0.0f;
-        }
-        uint32_t o[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = (uint32_t)h[ord[2 * e]] | ((uint32_t)h[ord[2 * e + 1]] << 16);
-        *reinterpret_cast<uint4*>(dst + p * plane) = make_uint4(o[0], o[1], o[2], o[3]);
-      }
-    } else {
-      uint16_t h[8];
-      const uint16_t* src = reinterpret_cast<const uint16_t*>(a.x) + at;
-      if (k < a.K) {  // K is a multiple of 32
-        if (a.x_aligned) {
-          const uint4 v = __ldg(reinterpret_cast<const uint4*>(src));
-          const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-          for (int e = 0; e < 8; ++e) h[e] = (uint16_t)(u[e >> 1] >> ((e & 1) * 16));
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) h[e] = src[e];
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) h[e] = 0;
-      }
-      uint32_t o[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = (uint32_t)h[ord[2 * e]] | ((uint32_t)h[ord[2 * e + 1]] << 16);
-      *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
-    }
+    for (int p = 0; p < P; ++p) *reinterpret_cast<uint4*>(dst + p * plane) = make_uint4(out[p][0], out[p][1], out[p][2], out[p][3]);
   }
 }
 

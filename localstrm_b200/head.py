@@ -14,7 +14,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .sampling import _DT, _require_cuda, sample_batch
+from .sampling import _require_cuda, sample_batch
 
 __all__ = ["Int4Weight", "int4_matvec", "sample_hidden"]
 
@@ -24,14 +24,14 @@ _CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _HERE = contextlib.nullcontext()
 
 
-def _on(dev: torch.device):
+def _on(device: int):
     """The device that the library launches on, where it is not the current one."""
-    return _HERE if dev.index == torch._C._cuda_getDevice() else torch.cuda.device(dev)
+    return _HERE if device == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
-def _stream(dev: torch.device) -> int:
-    """torch's current stream on ``dev`` as a cudaStream_t."""
-    return torch._C._cuda_getCurrentRawStream(dev.index)
+def _stream(device: int) -> int:
+    """torch's current stream on a device as a cudaStream_t."""
+    return torch._C._cuda_getCurrentRawStream(device)
 
 
 @dataclass
@@ -75,43 +75,58 @@ class Int4Weight:
 def int4_matvec(x: torch.Tensor, weight: Int4Weight, out_dtype: Optional[torch.dtype] = None,
                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``x @ W.T`` for ``x [rows, K]`` or ``[K]`` (f32, bf16 or f16), sums in f32, one rounding to
-    ``out_dtype`` (default: x's).  One pass over the matrix serves eight rows."""
+    ``out_dtype`` (default: x's).  One pass over the matrix serves 64 rows."""
     _require_cuda(x)
     packed, scales = weight.packed, weight.scales
-    if x.dim() not in (1, 2):
+    shape, dev = x.shape, x.get_device()
+    if len(shape) not in (1, 2):
         raise ValueError("x must be [K] or [rows, K]")
-    dev = x.device
-    if packed.device != dev or scales.device != dev:
-        raise ValueError(f"weight on {packed.device} / {scales.device}, x on {dev}")
-    if packed.dtype != torch.uint8 or packed.dim() != 2 or not packed.is_contiguous():
+    if packed.get_device() != dev or scales.get_device() != dev:
+        raise ValueError(f"weight on {packed.device} / {scales.device}, x on {x.device}")
+    if packed.dtype is not torch.uint8 or packed.dim() != 2 or not packed.is_contiguous():
         raise ValueError("packed: expected a contiguous uint8 tensor [N, K / 2]")
-    if scales.dtype not in (torch.float16, torch.bfloat16) or scales.dim() != 2 or not scales.is_contiguous() \
-            or scales.shape[0] != packed.shape[0]:
+    n, half = packed.shape
+    k, scale_code = 2 * half, _CODES.get(scales.dtype, 0)
+    if scale_code == 0 or scales.dim() != 2 or not scales.is_contiguous() or scales.shape[0] != n:
         raise ValueError("scales: expected a contiguous float16 or bfloat16 tensor [N, K / group]")
-    n, k, groups = packed.shape[0], 2 * packed.shape[1], scales.shape[1]
-    if x.shape[-1] != k:
-        raise ValueError(f"x has {x.shape[-1]} columns, the weight {k}")
+    groups = scales.shape[1]
+    if shape[-1] != k:
+        raise ValueError(f"x has {shape[-1]} columns, the weight {k}")
     if n < 1 or groups < 1 or k % groups:
         raise ValueError(f"{groups} groups do not divide {k} columns")
-    out_dtype = out_dtype or (out.dtype if out is not None else x.dtype)
-    if x.dtype not in _DT or out_dtype not in _DT:
+    if out_dtype is None:
+        out_dtype = x.dtype if out is None else out.dtype
+    if x.dtype not in _CODES or out_dtype not in _CODES:
         raise TypeError(f"unsupported dtypes {x.dtype} -> {out_dtype}")
-    x2 = x if x.dim() == 2 else x.unsqueeze(0)
-    rows = x2.shape[0]
-    if x2.stride(1) != 1 or (rows > 1 and x2.stride(0) < k):
-        x2 = x2.contiguous()
-    want = (n,) if x.dim() == 1 else (rows, n)
+    if len(shape) == 1:
+        rows, x_stride, want = 1, k, (n,)
+        if x.stride(0) != 1:
+            x = x.contiguous()
+    else:
+        rows, want = shape[0], (shape[0], n)
+        x_stride, inner = x.stride()
+        if inner != 1 or (rows > 1 and x_stride < k):
+            x = x.contiguous()
+            x_stride = k
+        x_stride = max(x_stride, k)  # one row: its stride says nothing
+    y_stride = n
     if out is None:
-        out = torch.empty(want, dtype=out_dtype, device=dev)
-    elif tuple(out.shape) != want or out.dtype != out_dtype or out.device != dev or out.stride(-1) != 1 \
-            or (out.dim() == 2 and rows > 1 and out.stride(0) < n):
-        raise ValueError(f"out: expected {out_dtype} {list(want)} on {dev} with rows of stride 1")
+        out = torch.empty(want, dtype=out_dtype, device=x.device)
+    else:
+        if tuple(out.shape) != want or out.dtype is not out_dtype or out.get_device() != dev or out.stride(-1) != 1 \
+                or (rows > 1 and out.stride(0) < n):
+            raise ValueError(f"out: expected {out_dtype} {list(want)} on {x.device} with rows of stride 1")
+        if len(want) == 2:
+            y_stride = max(out.stride(0), n)
     lib = _lib.load()
     with _on(dev):
+        ws, size = None, 0
+        if rows > 8:  # from torch's allocator for every call: other streams and captured calls have their own
+            size = lib.lss_int4_workspace_bytes(rows, k, _CODES[x.dtype], n)
+            ws = torch.empty(size, dtype=torch.uint8, device=x.device)
         _lib.check("lss_int4_matvec", lib.lss_int4_matvec(
-            x2.data_ptr(), _CODES[x.dtype], rows, k, max(x2.stride(0), k), packed.data_ptr(), scales.data_ptr(),
-            _CODES[scales.dtype], n, k // groups, out.data_ptr(), _CODES[out_dtype],
-            max(out.stride(0), n) if out.dim() == 2 else n, _stream(dev)))
+            x.data_ptr(), _CODES[x.dtype], rows, k, x_stride, packed.data_ptr(), scales.data_ptr(), scale_code, n, k // groups,
+            out.data_ptr(), _CODES[out_dtype], y_stride, None if ws is None else ws.data_ptr(), size, _stream(dev)))
     return out
 
 

@@ -53,48 +53,44 @@ class KVCache8:
         scales = lambda: torch.ones(num_blocks, heads, dtype=torch.float32, device=device)
         return cls(values(), values(), scales(), scales())
 
-    def check(self, device: torch.device) -> Tuple[int, int, int, int]:
-        """(num_blocks, heads, block_size, dim); raises where a tensor is not what the kernels read."""
-        shape = self.k.shape
-        if self.k.dim() != 4:
+    def check(self, device: int) -> torch.Size:
+        """[num_blocks, heads, block_size, dim]; raises where a tensor is not what the kernels read on
+        this CUDA device."""
+        k, v, ks, vs = self.k, self.v, self.k_scale, self.v_scale
+        shape = k.shape
+        if len(shape) != 4:
             raise ValueError("cache: k must be [num_blocks, heads, block_size, dim]")
-        for name, t in (("k", self.k), ("v", self.v)):
-            if t.shape != shape or t.dtype != torch.float8_e4m3fn or t.device != device or not t.is_contiguous():
-                raise ValueError(f"cache: {name} must be a contiguous float8_e4m3fn {list(shape)} on {device}")
-        for name, t in (("k_scale", self.k_scale), ("v_scale", self.v_scale)):
-            if t.shape != shape[:2] or t.dtype != torch.float32 or t.device != device or not t.is_contiguous():
-                raise ValueError(f"cache: {name} must be a contiguous float32 {list(shape[:2])} on {device}")
-        return tuple(shape)
+        for name, t in (("k", k), ("v", v)):
+            if t.dtype is not _E4M3 or t.get_device() != device or not t.is_contiguous() or t.shape != shape:
+                raise ValueError(f"cache: {name} must be a contiguous float8_e4m3fn {list(shape)} on cuda:{device}")
+        for name, t in (("k_scale", ks), ("v_scale", vs)):
+            if t.dtype is not _F32 or t.get_device() != device or not t.is_contiguous() or t.dim() != 2 \
+                    or t.shape[0] != shape[0] or t.shape[1] != shape[1]:
+                raise ValueError(f"cache: {name} must be a contiguous float32 {list(shape[:2])} on cuda:{device}")
+        return shape
 
 
-def _cuda(name: str, t: torch.Tensor) -> torch.device:
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
-        raise RuntimeError(f"{name}: a CUDA tensor is needed (no CPU fallback)")
-    return t.device
+_I32, _F32, _E4M3 = torch.int32, torch.float32, torch.float8_e4m3fn
 
 
-def _ints(name: str, t: torch.Tensor, n: int, dev: torch.device) -> None:
-    if t.dtype != torch.int32 or t.numel() != n or t.device != dev or not t.is_contiguous():
-        raise ValueError(f"{name}: expected a contiguous int32 tensor of {n} entries on {dev}")
+def _ints(name: str, t: torch.Tensor, n: int, device: int) -> int:
+    """The address of a contiguous int32 tensor of n entries on this device; raises for any other."""
+    if t.dtype is not _I32 or t.numel() != n or t.get_device() != device or not t.is_contiguous():
+        raise ValueError(f"{name}: expected a contiguous int32 tensor of {n} entries on cuda:{device}")
+    return t.data_ptr()
 
 
-def _table(table: torch.Tensor) -> Tuple[torch.device, int, int]:
-    dev = _cuda("block_table", table)
-    if table.dtype != torch.int32 or table.dim() != 2 or table.shape[1] < 1 or table.stride(1) != 1 \
-            or (table.shape[0] > 1 and table.stride(0) < table.shape[1]):
+def _table(table: torch.Tensor) -> Tuple[int, int, int, int]:
+    """(device, rows, width, row stride) of a block table."""
+    if not isinstance(table, torch.Tensor) or not table.is_cuda:
+        raise RuntimeError("block_table: a CUDA tensor is needed (no CPU fallback)")
+    if table.dtype is not _I32 or table.dim() != 2:
+        raise ValueError("block_table: expected int32 [B, width]")
+    B, width = table.shape
+    stride, inner = table.stride()
+    if width < 1 or inner != 1 or (B > 1 and stride < width):
         raise ValueError("block_table: expected int32 [B, width >= 1] with rows of stride 1")
-    return dev, table.shape[0], table.shape[1]
-
-
-def _stride0(t: torch.Tensor) -> int:
-    return max(t.stride(0), t.shape[1])  # one row: its stride says nothing
-
-
-def _out(name: str, t: Optional[torch.Tensor], new: torch.Tensor, n: int, dev: torch.device) -> torch.Tensor:
-    if t is None:
-        return new
-    _ints(name, t, n, dev)
-    return t
+    return table.get_device(), B, width, max(stride, width)  # one row: its stride says nothing
 
 
 def plan_blocks(block_table: torch.Tensor, lens: torch.Tensor, new_lens: torch.Tensor, free_blocks: torch.Tensor,
@@ -109,25 +105,23 @@ def plan_blocks(block_table: torch.Tensor, lens: torch.Tensor, new_lens: torch.T
     blocks are written into the table.  ``lens_out`` / ``n_free_out`` may be ``lens`` / ``n_free``
     (state updated in place, as a captured step needs it); otherwise both inputs are left as they are.
     """
-    dev, B, width = _table(block_table)
-    _ints("lens", lens, B, dev)
-    _ints("new_lens", new_lens, B, dev)
-    _ints("free_blocks", free_blocks, free_blocks.numel(), dev)
-    _ints("n_free", n_free, 1, dev)
-    if capacity < 0 or free_blocks.numel() < 1:
+    dev, B, width, stride = _table(block_table)
+    lens_at, new_at = _ints("lens", lens, B, dev), _ints("new_lens", new_lens, B, dev)
+    blocks = free_blocks.numel()
+    free_at, n_free_at = _ints("free_blocks", free_blocks, blocks, dev), _ints("n_free", n_free, 1, dev)
+    if capacity < 0 or blocks < 1:
         raise ValueError("capacity must not be negative, free_blocks not empty")
     # One allocation for the int32 results.
-    positions, granted, starts, new_state, new_free = torch.empty(capacity + 3 * B + 2, dtype=torch.int32, device=dev).split_with_sizes(
-        (capacity, B, B + 1, B, 1))
-    lens_out, n_free_out = _out("lens_out", lens_out, new_state, B, dev), _out("n_free_out", n_free_out, new_free, 1, dev)
-    slots = torch.empty(capacity, dtype=torch.int64, device=dev)
+    positions, granted, starts, new_state, new_free = torch.empty(
+        capacity + 3 * B + 2, dtype=_I32, device=block_table.device).split_with_sizes((capacity, B, B + 1, B, 1))
+    lens_out, n_free_out = new_state if lens_out is None else lens_out, new_free if n_free_out is None else n_free_out
+    slots = torch.empty(capacity, dtype=torch.int64, device=block_table.device)
     lib = _lib.load()
     with _on(dev):
         _lib.check("lss_block_plan", lib.lss_block_plan(
-            block_table.data_ptr(), _stride0(block_table), width, lens.data_ptr(), new_lens.data_ptr(), B, block_size,
-            free_blocks.data_ptr(), free_blocks.numel(), n_free.data_ptr(), capacity, slots.data_ptr(), positions.data_ptr(),
-            starts.data_ptr(), granted.data_ptr(), lens_out.data_ptr(), n_free_out.data_ptr(),
-            _stream(dev)))
+            block_table.data_ptr(), stride, width, lens_at, new_at, B, block_size, free_at, blocks, n_free_at, capacity,
+            slots.data_ptr(), positions.data_ptr(), starts.data_ptr(), granted.data_ptr(), _ints("lens_out", lens_out, B, dev),
+            _ints("n_free_out", n_free_out, 1, dev), _stream(dev)))
     return StepPlan(starts, granted, lens_out, slots, positions, n_free_out)
 
 
@@ -137,28 +131,22 @@ def release_blocks(block_table: torch.Tensor, lens: torch.Tensor, codes: torch.T
     """Returns the blocks of the rows with a non-zero code (``check_stop_batch``'s) to ``free_blocks``, in
     row and block order; their lengths become 0.  Gives ``(lens, n_free)`` afterwards; ``lens_out`` and
     ``n_free_out`` as for ``plan_blocks``.  Blocks that rows share must be released once."""
-    dev, B, width = _table(block_table)
-    _ints("lens", lens, B, dev)
-    _ints("codes", codes, B, dev)
-    _ints("free_blocks", free_blocks, free_blocks.numel(), dev)
-    _ints("n_free", n_free, 1, dev)
-    if free_blocks.numel() < 1:
+    dev, B, width, stride = _table(block_table)
+    lens_at, codes_at = _ints("lens", lens, B, dev), _ints("codes", codes, B, dev)
+    blocks = free_blocks.numel()
+    free_at, n_free_at = _ints("free_blocks", free_blocks, blocks, dev), _ints("n_free", n_free, 1, dev)
+    if blocks < 1:
         raise ValueError("free_blocks must not be empty")
-    new_state, new_free = torch.empty(B + 1, dtype=torch.int32, device=dev).split_with_sizes((B, 1))
-    lens_out, n_free_out = _out("lens_out", lens_out, new_state, B, dev), _out("n_free_out", n_free_out, new_free, 1, dev)
+    if lens_out is None:
+        lens_out = torch.empty(B, dtype=_I32, device=block_table.device)
+    if n_free_out is None:
+        n_free_out = torch.empty(1, dtype=_I32, device=block_table.device)
     lib = _lib.load()
     with _on(dev):
         _lib.check("lss_block_release", lib.lss_block_release(
-            block_table.data_ptr(), _stride0(block_table), width, lens.data_ptr(), codes.data_ptr(), B, block_size,
-            free_blocks.data_ptr(), free_blocks.numel(), n_free.data_ptr(), lens_out.data_ptr(), n_free_out.data_ptr(),
-            _stream(dev)))
+            block_table.data_ptr(), stride, width, lens_at, codes_at, B, block_size, free_at, blocks, n_free_at,
+            _ints("lens_out", lens_out, B, dev), _ints("n_free_out", n_free_out, 1, dev), _stream(dev)))
     return lens_out, n_free_out
-
-
-def _plan(plan: StepPlan, B: int, dev: torch.device) -> None:
-    _ints("plan.starts", plan.starts, B + 1, dev)
-    _ints("plan.granted", plan.granted, B, dev)
-    _ints("plan.lens", plan.lens, B, dev)
 
 
 def append_kv(cache: KVCache8, k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor, plan: StepPlan) -> None:
@@ -168,22 +156,28 @@ def append_kv(cache: KVCache8, k: torch.Tensor, v: torch.Tensor, block_table: to
     A block's scale is the smallest power of two with which its finite values fit e4m3; where tokens
     of this step make it grow, the tokens that the block already holds are rounded again.  Tokens of
     refused rows are passed over.  A block that is written must belong to one row."""
-    dev, B, width = _table(block_table)
+    dev, B, width, stride = _table(block_table)
     blocks, heads, bs, dim = cache.check(dev)
-    _plan(plan, B, dev)
-    if k.dim() != 3 or k.shape != v.shape or k.shape[1:] != (heads, dim) or k.dtype != v.dtype or k.device != dev or v.device != dev:
-        raise ValueError(f"k, v: expected [T, {heads}, {dim}] of one dtype on {dev}")
-    if k.dtype not in _CODES:
-        raise TypeError(f"unsupported dtype {k.dtype}")
-    k = k if k.stride(2) == 1 else k.contiguous()
-    v = v if v.stride(2) == 1 else v.contiguous()
+    shape, dtype = k.shape, k.dtype
+    if len(shape) != 3 or shape[1] != heads or shape[2] != dim or shape != v.shape or dtype is not v.dtype \
+            or k.get_device() != dev or v.get_device() != dev:
+        raise ValueError(f"k, v: expected [T, {heads}, {dim}] of one dtype on cuda:{dev}")
+    if dtype not in _CODES:
+        raise TypeError(f"unsupported dtype {dtype}")
+    ks, vs = k.stride(), v.stride()
+    if ks[2] != 1:
+        k = k.contiguous()
+        ks = k.stride()
+    if vs[2] != 1:
+        v = v.contiguous()
+        vs = v.stride()
     lib = _lib.load()
     with _on(dev):
         _lib.check("lss_kv_append", lib.lss_kv_append(
-            k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), _CODES[k.dtype], k.shape[0], heads,
-            dim, cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), blocks, bs,
-            block_table.data_ptr(), _stride0(block_table), width, plan.starts.data_ptr(), plan.granted.data_ptr(),
-            plan.lens.data_ptr(), B, _stream(dev)))
+            k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], _CODES[dtype], shape[0], heads, dim, cache.k.data_ptr(),
+            cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), blocks, bs, block_table.data_ptr(), stride,
+            width, _ints("plan.starts", plan.starts, B + 1, dev), _ints("plan.granted", plan.granted, B, dev),
+            _ints("plan.lens", plan.lens, B, dev), B, _stream(dev)))
 
 
 def attend(q: torch.Tensor, cache: KVCache8, block_table: torch.Tensor, plan: StepPlan, scale: Optional[float] = None,
@@ -195,31 +189,42 @@ def attend(q: torch.Tensor, cache: KVCache8, block_table: torch.Tensor, plan: St
     first).  ``scale`` defaults to ``dim ** -0.5``; ``lse_out`` (float32 ``[T, q_heads]``) receives the natural
     log of the softmax sums.  Tokens of refused rows, and those behind the last row, are left as they
     are in ``out`` and ``lse_out`` (in a fresh ``out``: undefined)."""
-    dev, B, width = _table(block_table)
+    dev, B, width, stride = _table(block_table)
     blocks, heads, bs, dim = cache.check(dev)
-    _plan(plan, B, dev)
-    if q.dim() != 3 or q.shape[2] != dim or q.shape[1] < heads or q.shape[1] % heads or q.device != dev:
-        raise ValueError(f"q: expected [T, a multiple of {heads}, {dim}] on {dev}")
-    if q.dtype not in (torch.bfloat16, torch.float16):
-        raise TypeError(f"unsupported dtype {q.dtype}")
-    q = q if q.stride(2) == 1 else q.contiguous()
+    shape, dtype = q.shape, q.dtype
+    if len(shape) != 3 or shape[2] != dim or shape[1] < heads or shape[1] % heads or q.get_device() != dev:
+        raise ValueError(f"q: expected [T, a multiple of {heads}, {dim}] on cuda:{dev}")
+    if dtype is not torch.bfloat16 and dtype is not torch.float16:
+        raise TypeError(f"unsupported dtype {dtype}")
+    qs = q.stride()
+    if qs[2] != 1:
+        q = q.contiguous()
+        qs = q.stride()
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or out.stride(2) != 1 \
-            or out.stride(1) < dim or out.stride(0) < out.stride(1):
-        raise ValueError(f"out: expected {q.dtype} {list(q.shape)} on {dev}, rows of stride 1 that do not overlap")
-    if lse_out is not None and (lse_out.dtype != torch.float32 or lse_out.shape != q.shape[:2] or lse_out.device != dev
+        out = torch.empty(shape, dtype=dtype, device=block_table.device)
+        os = out.stride()
+    else:
+        os = out.stride()
+        if out.shape != shape or out.dtype is not dtype or out.get_device() != dev or os[2] != 1 or os[1] < dim \
+                or os[0] < (shape[1] - 1) * os[1] + dim:
+            raise ValueError(f"out: expected {dtype} {list(shape)} on cuda:{dev}, rows of stride 1 that do not overlap")
+    if lse_out is not None and (lse_out.dtype is not _F32 or lse_out.shape != shape[:2] or lse_out.get_device() != dev
                                 or not lse_out.is_contiguous()):
-        raise ValueError(f"lse_out: expected a contiguous float32 {list(q.shape[:2])} on {dev}")
+        raise ValueError(f"lse_out: expected a contiguous float32 {list(shape[:2])} on cuda:{dev}")
     lib = _lib.load()
     with _on(dev):
         # From torch's allocator for every call: calls on other streams, and captured ones, have their own.
-        ws = torch.empty(int(lib.lss_attend_workspace_bytes(dim)), dtype=torch.uint8, device=dev)
+        size = _WORKSPACE.get(dim)
+        if size is None:
+            size = _WORKSPACE[dim] = int(lib.lss_attend_workspace_bytes(dim))
+        ws = torch.empty(size, dtype=torch.uint8, device=block_table.device)
         _lib.check("lss_attend", lib.lss_attend(
-            q.data_ptr(), q.stride(0), q.stride(1), _CODES[q.dtype], q.shape[0], q.shape[1], heads, dim, cache.k.data_ptr(),
-            cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), blocks, bs, block_table.data_ptr(),
-            _stride0(block_table), width, plan.starts.data_ptr(), plan.granted.data_ptr(), plan.lens.data_ptr(), B,
-            float(scale if scale is not None else dim ** -0.5), out.data_ptr(), out.stride(0), out.stride(1),
-            lse_out.data_ptr() if lse_out is not None else None, ws.data_ptr(), ws.numel(),
-            _stream(dev)))
+            q.data_ptr(), qs[0], qs[1], _CODES[dtype], shape[0], shape[1], heads, dim, cache.k.data_ptr(), cache.v.data_ptr(),
+            cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), blocks, bs, block_table.data_ptr(), stride, width,
+            _ints("plan.starts", plan.starts, B + 1, dev), _ints("plan.granted", plan.granted, B, dev),
+            _ints("plan.lens", plan.lens, B, dev), B, dim ** -0.5 if scale is None else scale, out.data_ptr(), os[0], os[1],
+            None if lse_out is None else lse_out.data_ptr(), ws.data_ptr(), size, _stream(dev)))
     return out
+
+
+_WORKSPACE = {}  # bytes that the attention needs, by head dimension

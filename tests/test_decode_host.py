@@ -11,7 +11,7 @@ OK, INVALID, WORKSPACE, UNSUPPORTED = 0, 1, 2, 4
 
 
 def int4(**kw):
-    a = dict(x=16, xd=1, rows=1, K=64, xs=64, packed=16, scales=16, sd=2, N=4, group=32, y=16, yd=0, ys=4, stream=None)
+    a = dict(x=16, xd=1, rows=1, K=64, xs=64, packed=16, scales=16, sd=2, N=4, group=32, y=16, yd=0, ys=4, ws=None, wsb=0, stream=None)
     a.update(kw)
     return _lib.load().lss_int4_matvec(*a.values())
 
@@ -22,6 +22,12 @@ def test_int4_refusals():
                 dict(group=16), dict(group=96), dict(group=128), dict(K=320, xs=320, group=128), dict(x=None), dict(packed=None),
                 dict(packed=8), dict(scales=18), dict(scales=None), dict(y=None)):
         assert int4(**bad) == INVALID, bad
+    lib = _lib.load()
+    assert lib.lss_int4_workspace_bytes(8, 64, 1, 4) == 0
+    need = lib.lss_int4_workspace_bytes(9, 64, 1, 4)
+    assert 0 < need < lib.lss_int4_workspace_bytes(9, 64, 0, 4)
+    for bad in (dict(rows=9), dict(rows=9, ws=16, wsb=need - 1), dict(rows=9, ws=8, wsb=need)):
+        assert int4(**bad) == WORKSPACE, bad
 
 
 def plan(fn="lss_block_plan", **kw):
