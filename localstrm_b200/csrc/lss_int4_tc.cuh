@@ -48,10 +48,11 @@ __device__ __forceinline__ void tc_ld16(uint32_t at, uint32_t (&r)[16]) {
       : "memory");
 }
 // D (+)= A B with A in tensor memory and B in shared memory; one thread issues it.
-__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, bool add) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+      "{\n .reg .pred p;\n .reg .b64 b;\n mov.b64 b, {%2, %3};\n setp.ne.b32 p, %5, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n}\n" ::"r"(d),
+      "r"(a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"((uint32_t)add)
       : "memory");
 }
 // Arrives on `bar` when the products issued so far by this thread are done.
@@ -59,25 +60,33 @@ __device__ __forceinline__ void tc_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(saddr(bar)) : "memory");
 }
 // Shared-memory operand whose rows are 128-byte lines (64 16-bit columns) in 8-line groups, pieces of
-// 16 bytes permuted inside a line by the line number (the 128-byte swizzle).
-__device__ __forceinline__ uint64_t tc_desc128(uint32_t addr) {
-  return (uint64_t)((addr >> 4) & 0x3fffu) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
+// 16 bytes permuted inside a line by the line number (the 128-byte swizzle): the two halves of its
+// descriptor.  The lower one counts the address in 16 bytes.
+__device__ __forceinline__ uint32_t tc_desc_lo(uint32_t addr) { return ((addr >> 4) & 0x3fffu) | (1u << 16); }
+constexpr uint32_t TC_DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);
 // 16-bit operands, f32 sums, both operands along columns; M = 128.
 __device__ __forceinline__ constexpr uint32_t tc_idesc(bool bf16, int n) {
   return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
 }
-// Bounded wait; once one has given up anywhere in the CTA, all others give up at once.
+// Bounded wait; once one has given up anywhere in the CTA, all others give up at once.  The thread
+// sleeps until the phase completes (asking again and again would take the widening's issue slots).
 __device__ __forceinline__ bool tc_wait(uint64_t* bar, uint32_t parity, volatile int* failed) {
+  if (mbar_try_wait(bar, parity)) return true;
   const long long t0 = clock64();
-  while (!mbar_try_wait(bar, parity)) {
+  for (;;) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(saddr(bar)), "r"(parity), "r"(100000u)
+        : "memory");
+    if (ok) return true;
     if (*failed) return false;
     if (clock64() - t0 > T4_WAIT) {
       *failed = 1;
       return false;
     }
   }
-  return true;
 }
 
 // Writes x as the operand that the product kernel copies: [unit of 128 columns][plane][half][NR rows][128
@@ -205,7 +214,8 @@ __global__ void __launch_bounds__(T4_NT, 1) lss_int4_tc_kernel(Int4TcArgs t) {
   // Unit u's copy waits for unit u - XS of all teams; the thread that issues it asks one unit late, so that its
   // own team is not held up by the slowest one.
   int xu = 0;
-  if (tid == 0)
+  const bool fetches = tid == 96;  // team 0's last warp: its first one issues products
+  if (fetches)
     for (; xu < min(XS, nu); ++xu) fetch_x(xu);
 
   float acc[NR];
@@ -254,13 +264,13 @@ __global__ void __launch_bounds__(T4_NT, 1) lss_int4_tc_kernel(Int4TcArgs t) {
           tc_after_sync();
           const bool ok = g0 > 0 || tc_wait(&xfull[b], (u / XS) & 1, &failed);
           if (ok && !*(volatile int*)&failed) {
-            const uint32_t x0 = saddr(xs) + b * XB;
+            const uint32_t x0 = tc_desc_lo(saddr(xs) + b * XB);
 #pragma unroll
             for (int s = g0 * 2 * SPG; s < (g0 + GR) * 2 * SPG; ++s)
 #pragma unroll
               for (int p = 0; p < P; ++p)
-                tc_mma_ts(d_at + (s / (2 * SPG) - g0) * NR, a_at + 8 * s, tc_desc128(x0 + (p * 2 + (s >> 2)) * NR * 128 + (s & 3) * 32), idesc,
-                          s % (2 * SPG) != 0 || p > 0);
+                tc_mma_ts(d_at + (s / (2 * SPG) - g0) * NR, a_at + 8 * s, x0 + ((p * 2 + (s >> 2)) * NR * 128 + (s & 3) * 32) / 16, TC_DESC_HI,
+                          idesc, s % (2 * SPG) != 0 || p > 0);
             tc_commit(&done[team]);
             if (g0 + GR >= SPU) tc_commit(&xempty[b]);
           }
@@ -279,7 +289,7 @@ __global__ void __launch_bounds__(T4_NT, 1) lss_int4_tc_kernel(Int4TcArgs t) {
             for (int e = 0; e < 16; ++e) acc[i + e] = fmaf(sc[g0 + q], __uint_as_float(d[e]), acc[i + e]);
           }
       }
-      if (tid == 0 && u > 0 && xu < nu) {  // the place of unit u - 1
+      if (fetches && u > 0 && xu < nu) {  // the place of unit u - 1
         if (tc_wait(&xempty[xu % XS], ((xu / XS) - 1) & 1, &failed)) fetch_x(xu);
         ++xu;
       }
