@@ -3,7 +3,7 @@
 #include <algorithm>
 #include <mutex>
 
-#include "lss_attend.cuh"
+#include "lss_attend_tc.cuh"
 #include "lss_blocks.cuh"
 #include "lss_int4_tc.cuh"
 #include "lss_kvcache.cuh"
@@ -125,6 +125,16 @@ static cudaError_t launch_attend(AttendArgs a, void* ws, cudaStream_t st) {
   return launch(lss_attend_join_kernel<D, DT, NQ>, (unsigned)(ctas * NW), 256, 0, 1, true, st, a);
 }
 
+template <int D, int DT>
+static cudaError_t launch_attend_tc(const AttendArgs& a, cudaStream_t st) {
+  static SmemSet set;
+  const int dev = device_index();
+  constexpr int smem = 1024 + 6 * 128 * D * 2;
+  const cudaError_t e = allow_smem(lss_attend_tc_kernel<D, DT>, set, dev, smem);
+  if (e != cudaSuccess) return e;
+  return launch(lss_attend_tc_kernel<D, DT>, (unsigned)sm_count(dev), PA_NT, smem, 1, false, st, a);
+}
+
 // Query rows per group: as many as a key head's rows fill on the average (a batch of single tokens:
 // the query heads of a key head).
 template <int D, int DT>
@@ -132,6 +142,7 @@ static cudaError_t launch_attend_rows(const AttendArgs& a, void* ws, cudaStream_
   const int64_t rows = (int64_t)a.per * ((a.T + (int64_t)a.B - 1) / a.B);
   if (rows <= 8) return launch_attend<D, DT, 1>(a, ws, st);
   if constexpr (D < 256) {
+    if (rows >= 128 && (int64_t)a.heads * a.per * a.T >= (int64_t)PA_ROWS * sm_count(device_index()) / 4) return launch_attend_tc<D, DT>(a, st);
     if (rows > 16) return launch_attend<D, DT, 4>(a, ws, st);
   }
   return launch_attend<D, DT, 2>(a, ws, st);

@@ -102,7 +102,9 @@ def attend_reference(q, k, v, ks, vs, table, starts, granted, lens, scale):
                 top = z.amax(-1, keepdim=True)
                 p = torch.where(seen, torch.exp(z - torch.where(top == -math.inf, 0.0, top)), 0.0)
                 tot = p.sum(-1, keepdim=True)
-                for i in range(g):  # only what a query sees enters its sum
+                if bool(vv.isfinite().all()):
+                    out[s0: s0 + g, r], mag[s0: s0 + g, r] = ((p @ x) / torch.where(tot == 0, 1.0, tot) for x in (vv, vv.abs()))
+                for i in range(0 if bool(vv.isfinite().all()) else g):  # only what a query sees enters its sum
                     w = p[i][seen[i]] / tot[i]
                     out[s0 + i, r] = (w[:, None] * vv[seen[i]]).sum(0) if tot[i] != 0 else 0.0
                     mag[s0 + i, r] = (w[:, None] * vv[seen[i]].abs()).sum(0) if tot[i] != 0 else 0.0
