@@ -2,6 +2,8 @@
 // on the fifth-generation tensor cores (tcgen05, sums in tensor memory).
 #pragma once
 
+#include <type_traits>
+
 #include "lss_attend.cuh"
 #include "lss_int4_tc.cuh"
 
@@ -20,16 +22,10 @@ __device__ __forceinline__ void tc_mma_ss(uint32_t d, uint32_t a_lo, uint32_t a_
       "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"((uint32_t)add)
       : "memory");
 }
-__device__ __forceinline__ void tc_ld32(uint32_t at, uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,"
-      "%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]),
-        "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]),
-        "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(at)
-      : "memory");
+__device__ __forceinline__ void tc_st8(uint32_t at, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
 }
 
 // Where 16 bytes (8 values) `q` of row `r` lie in an operand of 128 rows: panels of 64 columns, a
@@ -63,7 +59,7 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
   __shared__ __align__(8) uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sfull[2], pready[2], ofull[2], qready;
   __shared__ uint32_t tmem_base;
   __shared__ int failed;
-  __shared__ float sks[4][8], slv[4][8];   // scales of the tile's 16-token parts (ks < 0: not seen), log2 of those of V
+  __shared__ float2 sscale[4][8];          // scales of the tile's 16-token parts: of K (< 0: not seen), log2 of that of V
   __shared__ int nan_from[D];              // first position with a NaN among the values of a column
   __shared__ int scr[PA_NT / 32];
   __shared__ int4 found;
@@ -96,7 +92,9 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
 
   uint32_t tiles = 0;       // K/V tiles of earlier groups
   uint32_t scount[2] = {0, 0}, groups = 0;
-  for (int item0 = blockIdx.x;; item0 += gridDim.x) {
+  // Groups in rounds of the grid's size, every second round the other way round: later rows tend to have less.
+  for (int round = 0;; ++round) {
+    const int item0 = round * (int)gridDim.x + (round & 1 ? (int)(gridDim.x - 1 - blockIdx.x) : (int)blockIdx.x);
     // ---- which row, key head and group: rows' groups counted up by all threads
     int rest = item0, row = -1;
     for (int r0 = 0; r0 < a.B && row < 0; r0 += PA_NT) {
@@ -133,7 +131,7 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
         rest -= tot;
       }
     }
-    if (row < 0) break;
+    if (row < 0) break;  // places of later rounds lie further behind
     const AtRow rw = at_row<PA_ROWS / 8>(a, row);
     // Later groups see more: they come first.
     const int head = rest % a.heads, mt = rw.mt - 1 - rest / a.heads;
@@ -216,40 +214,33 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
           ++scount[q];
           tc_after_sync();
           const int slot = (int)((tiles + j) & 3), pos = j * PA_KT;
-          float f[8], lv[8];
-          bool hidden = false;
+          const float2* sc = sscale[slot];
+          bool masked = pos + PA_KT > see_warp;
 #pragma unroll
-          for (int g = 0; g < 8; ++g) {
-            const float k = sks[slot][g];
-            hidden |= k < 0.0f;
-            f[g] = k < 0.0f ? -1.0f : fq * k;
-            lv[g] = slv[slot][g];
-          }
-          const bool masked = hidden || pos + PA_KT > see_warp;
-          // Largest score, and largest weight of V.
-          float top = -INFINITY, topw = -INFINITY;
+          for (int g = 0; g < 8; ++g) masked |= sc[g].x < 0.0f;
+          // Largest score, and largest weight of V.  Sixteen columns at a time, the next ones on their way.
+          float top = -INFINITY, topw = -INFINITY, least = INFINITY;
+          auto maxima = [&](auto mask_c) {
+            constexpr bool with_mask = decltype(mask_c)::value;
+            uint32_t x[2][16];
+            tc_ld16(s_at[q] + lanes, x[0]);
 #pragma unroll
-          for (int h = 0; h < 4; ++h) {
-            uint32_t x[32];
-            tc_ld32(s_at[q] + lanes + 32 * h, x);
-            tc_wait_ld();
-#pragma unroll
-            for (int g = 0; g < 2; ++g) {
+            for (int g = 0; g < 8; ++g) {
+              tc_wait_ld();
+              if (g < 7) tc_ld16(s_at[q] + lanes + 16 * (g + 1), x[(g + 1) & 1]);
+              const float2 k = sc[g];
               float t = -INFINITY;
-              if (masked) {
 #pragma unroll
-                for (int e = 0; e < 16; ++e)
-                  if (pos + 32 * h + 16 * g + e < limit) t = fmaxf(t, __uint_as_float(x[16 * g + e]));
-                if (f[2 * h + g] < 0.0f) t = -INFINITY;  // a part that is not seen
-              } else {
-#pragma unroll
-                for (int e = 0; e < 16; ++e) t = fmaxf(t, __uint_as_float(x[16 * g + e]));
-              }
-              t = t == -INFINITY ? t : t * f[2 * h + g];
+              for (int e = 0; e < 16; ++e)
+                if (!with_mask || pos + 16 * g + e < limit) t = fmaxf(t, __uint_as_float(x[g & 1][e]));
+              if (with_mask && (k.x < 0.0f || t == -INFINITY)) continue;
+              t *= fq * k.x;
               top = fmaxf(top, t);
-              topw = fmaxf(topw, t + lv[2 * h + g]);
+              topw = fmaxf(topw, t + k.y);
+              least = fminf(least, k.y);
             }
-          }
+          };
+          if (masked) maxima(std::true_type{}); else maxima(std::false_type{});
           if (__any_sync(0xffffffffu, top > m + AT_SLACK || topw > w + AT_SLACK)) {
             const float mn = fmaxf(m, top), wn = fmaxf(w, topw);
             l *= ex2(m - (mn == -INFINITY ? 0.0f : mn));
@@ -269,29 +260,47 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
             }
           }
           const float mu = m == -INFINITY ? 0.0f : m, wu = w == -INFINITY ? 0.0f : w;
+          // A token's weight of V is 2^z, z = s + log2(v scale) - W + 10; its share p = 2^(s - m) of the softmax
+          // differs by a factor of its part, so that one exponential does for both: p = 2^z 2^(-shift).  Where the factor
+          // is far from 1 (a block of zeros has the scale 2^-126) p would be lost: then p itself is taken.
+          const bool apart = __any_sync(0xffffffffu, mu + least - wu + AT_BIAS < -60.0f);
+          auto weights = [&](auto mask_c, auto share_c) {
+            constexpr bool with_mask = decltype(mask_c)::value, by_share = decltype(share_c)::value;
+            uint32_t x[2][16];
+            tc_ld16(s_at[q] + lanes, x[0]);
 #pragma unroll
-          for (int h = 0; h < 4; ++h) {
-            uint32_t x[32], p[16];
-            tc_ld32(s_at[q] + lanes + 32 * h, x);
-            tc_wait_ld();
-#pragma unroll
-            for (int g = 0; g < 2; ++g) {
-              const float fg = f[2 * h + g], gain = ex2(fminf(mu + lv[2 * h + g] - wu + AT_BIAS, 126.0f));
+            for (int g = 0; g < 8; ++g) {
+              tc_wait_ld();
+              if (g < 7) tc_ld16(s_at[q] + lanes + 16 * (g + 1), x[(g + 1) & 1]);
+              const float2 k = sc[g];
+              const float fg = fq * k.x, shift = fminf(mu + k.y - wu + AT_BIAS, 126.0f);
+              const float add = by_share ? -mu : k.y - wu + AT_BIAS, gain = by_share ? ex2(shift) : 0.0f;
+              uint32_t p[8];
+              float part = 0.0f;
 #pragma unroll
               for (int e = 0; e < 16; e += 2) {
-                float y0 = fmaf(__uint_as_float(x[16 * g + e]), fg, -mu), y1 = fmaf(__uint_as_float(x[16 * g + e + 1]), fg, -mu);
-                if (masked) {
-                  if (fg < 0.0f || pos + 32 * h + 16 * g + e >= limit) y0 = -INFINITY;
-                  if (fg < 0.0f || pos + 32 * h + 16 * g + e + 1 >= limit) y1 = -INFINITY;
+                float y0 = fmaf(__uint_as_float(x[g & 1][e]), fg, add), y1 = fmaf(__uint_as_float(x[g & 1][e + 1]), fg, add);
+                if (with_mask) {
+                  if (k.x < 0.0f || pos + 16 * g + e >= limit) y0 = -INFINITY;
+                  if (k.x < 0.0f || pos + 16 * g + e + 1 >= limit) y1 = -INFINITY;
                 }
-                const float p0 = ex2(y0), p1 = ex2(y1);
-                l += p0 + p1;
-                const __half2 v = __floats2half2_rn(p0 * gain, p1 * gain);
-                p[8 * g + e / 2] = *reinterpret_cast<const uint32_t*>(&v);
+                float p0 = ex2(y0), p1 = ex2(y1);
+                part += p0 + p1;
+                if (by_share) {
+                  p0 *= gain;
+                  p1 *= gain;
+                }
+                const __half2 v = __floats2half2_rn(p0, p1);
+                p[e / 2] = *reinterpret_cast<const uint32_t*>(&v);
               }
+              if (by_share) l += part;
+              else if (!with_mask || part != 0.0f) l = fmaf(part, ex2(-shift), l);
+              tc_st8(s_at[q] + lanes + 8 * g, p);  // over scores that have been read
             }
-            tc_st16(s_at[q] + lanes + 16 * h, p);  // over scores that have been read
-          }
+          };
+          if (masked) weights(std::true_type{}, std::true_type{});
+          else if (apart) weights(std::false_type{}, std::true_type{});
+          else weights(std::false_type{}, std::false_type{});
           tc_wait_st();
           tc_before_sync();
           __syncwarp();
@@ -387,8 +396,7 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
           widen(kr[i], ksm + st * OPB, p / (D / 16), p % (D / 16));
         }
         if (ct < 8) {
-          sks[n & 3][ct] = ksn;
-          slv[n & 3][ct] = lvn;
+          sscale[n & 3][ct] = make_float2(ksn, lvn);
         }
         fence_proxy_async();
         __syncwarp();
@@ -400,8 +408,8 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
           uint32_t u[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
           uint32_t any = 0;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) any |= __vcmpeq4(u[e] & 0x7f7f7f7fu, 0x7f7f7f7fu);
-          if (any) {
+          for (int e = 0; e < 4; ++e) any |= (u[e] & 0x7f7f7f7fu) + 0x01010101u;  // a byte of 0x7f carries into its sign
+          if (any & 0x80808080u) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const uint32_t nan = __vcmpeq4(u[e] & 0x7f7f7f7fu, 0x7f7f7f7fu);
