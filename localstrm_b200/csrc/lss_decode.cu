@@ -125,14 +125,24 @@ static cudaError_t launch_attend(AttendArgs a, void* ws, cudaStream_t st) {
   return launch(lss_attend_join_kernel<D, DT, NQ>, (unsigned)(ctas * NW), 256, 0, 1, true, st, a);
 }
 
+template <int D>
+static size_t attend_tc_bytes() {
+  return (size_t)AT_CAP_CTAS * (sizeof(int4) + 2 * pa_piece(D) * sizeof(float));
+}
+
 template <int D, int DT>
-static cudaError_t launch_attend_tc(const AttendArgs& a, cudaStream_t st) {
+static cudaError_t launch_attend_tc(AttendArgs a, void* ws, cudaStream_t st) {
   static SmemSet set;
   const int dev = device_index();
   constexpr int smem = 1024 + 6 * 128 * D * 2;
-  const cudaError_t e = allow_smem(lss_attend_tc_kernel<D, DT>, set, dev, smem);
+  cudaError_t e = allow_smem(lss_attend_tc_kernel<D, DT>, set, dev, smem);
   if (e != cudaSuccess) return e;
-  return launch(lss_attend_tc_kernel<D, DT>, (unsigned)sm_count(dev), PA_NT, smem, 1, false, st, a);
+  const int ctas = std::min(sm_count(dev), AT_CAP_CTAS);
+  a.meta = reinterpret_cast<int4*>(ws);
+  a.part = reinterpret_cast<float*>(a.meta + AT_CAP_CTAS);
+  e = launch(lss_attend_tc_kernel<D, DT>, (unsigned)ctas, PA_NT, smem, 1, false, st, a);
+  if (e != cudaSuccess) return e;
+  return launch(lss_attend_tc_join_kernel<D, DT>, (unsigned)(ctas * (PA_ROWS / 32)), 256, 0, 1, true, st, a);
 }
 
 // Query rows per group: as many as a key head's rows fill on the average (a batch of single tokens:
@@ -142,7 +152,7 @@ static cudaError_t launch_attend_rows(const AttendArgs& a, void* ws, cudaStream_
   const int64_t rows = (int64_t)a.per * ((a.T + (int64_t)a.B - 1) / a.B);
   if (rows <= 8) return launch_attend<D, DT, 1>(a, ws, st);
   if constexpr (D < 256) {
-    if (rows >= 128 && (int64_t)a.heads * a.per * a.T >= (int64_t)PA_ROWS * sm_count(device_index()) / 4) return launch_attend_tc<D, DT>(a, st);
+    if (rows >= 128 && (int64_t)a.heads * a.per * a.T >= (int64_t)PA_ROWS * sm_count(device_index()) / 4) return launch_attend_tc<D, DT>(a, ws, st);
     if (rows > 16) return launch_attend<D, DT, 4>(a, ws, st);
   }
   return launch_attend<D, DT, 2>(a, ws, st);
@@ -396,8 +406,8 @@ int lss_kv_append(const void* k, int64_t k_token_stride, int64_t k_head_stride, 
 
 size_t lss_attend_workspace_bytes(int dim) {
   switch (dim) {
-    case 64: return std::max({attend_bytes<64, 1>(), attend_bytes<64, 2>(), attend_bytes<64, 4>()});
-    case 128: return std::max({attend_bytes<128, 1>(), attend_bytes<128, 2>(), attend_bytes<128, 4>()});
+    case 64: return std::max({attend_bytes<64, 1>(), attend_bytes<64, 2>(), attend_bytes<64, 4>(), attend_tc_bytes<64>()});
+    case 128: return std::max({attend_bytes<128, 1>(), attend_bytes<128, 2>(), attend_bytes<128, 4>(), attend_tc_bytes<128>()});
     case 256: return std::max(attend_bytes<256, 1>(), attend_bytes<256, 2>());
     default: return 0;
   }

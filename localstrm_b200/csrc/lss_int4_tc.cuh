@@ -55,6 +55,14 @@ __device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint32_t b_lo,
       "r"(a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"((uint32_t)add)
       : "memory");
 }
+// True for one thread of a warp whose lanes are all here.  Products are issued under it, by a warp that
+// otherwise stays together, so that their operands are known to be the same for all lanes: under
+// `lane == 0` every tcgen05.mma took 60 to 125 cycles to issue.
+__device__ __forceinline__ bool tc_elect() {
+  uint32_t one;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(one));
+  return one != 0;
+}
 // Arrives on `bar` when the products issued so far by this thread are done.
 __device__ __forceinline__ void tc_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(saddr(bar)) : "memory");
@@ -260,10 +268,11 @@ __global__ void __launch_bounds__(T4_NT, 1) lss_int4_tc_kernel(Int4TcArgs t) {
       for (int g0 = 0; g0 < SPU; g0 += GR) {
         tc_before_sync();
         asm volatile("bar.sync %0, 128;" ::"r"(1 + team) : "memory");
-        if (quarter == 0 && lane == 0) {
+        if (quarter == 0) {
           tc_after_sync();
-          const bool ok = g0 > 0 || tc_wait(&xfull[b], (u / XS) & 1, &failed);
-          if (ok && !*(volatile int*)&failed) {
+          if (g0 == 0) tc_wait(&xfull[b], (u / XS) & 1, &failed);
+          __syncwarp();
+          if (tc_elect() && !*(volatile int*)&failed) {
             const uint32_t x0 = tc_desc_lo(saddr(xs) + b * XB);
 #pragma unroll
             for (int s = g0 * 2 * SPG; s < (g0 + GR) * 2 * SPG; ++s)
