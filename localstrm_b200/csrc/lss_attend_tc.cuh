@@ -12,7 +12,7 @@ namespace lss {
 constexpr int PA_ROWS = 256;   // query rows of a group: two tiles of 128
 constexpr int PA_KT = 128;     // tokens of a tile of keys and values
 constexpr int PA_HT = 64;      // tokens that a softmax step takes: half a tile
-constexpr int PA_CONV = 8;     // warps that widen keys and values
+constexpr int PA_CONV = 7;     // warps that widen keys and values (16 in all: 128 registers a thread)
 constexpr int PA_NT = (8 + PA_CONV + 1) * 32;
 
 // D (+)= A B, both operands in shared memory.
@@ -75,7 +75,7 @@ __device__ __forceinline__ uint32_t pa_place(int r, int q) {
 // Two tiles of 128 rows have a warpgroup each, a thread per row, and take 64 tokens a step: while it takes the
 // softmax of a step's scores, the next step's are under way.  Scores S = Q K^T (two places of 128 x 64, f32) lie in
 // tensor memory, the weights take their place as f16, the sums O stay there for the whole group.  Keys and
-// values come as e4m3 and are widened to f16 by eight warps into two stages of shared memory, once for
+// values come as e4m3 and are widened to f16 by seven warps into two stages of shared memory, once for
 // 256 rows (exact; 16 rows at a time, the widening is what bounds lss_attend_kernel here).
 // Scales and the power of two of a query row act as in lss_attend_kernel; the weight of V is
 // p 2^(m + log2(v scale) - W + 10) from the softmax's own p, one exponential per score.  Both running
@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
   constexpr int CH = D / 8;                // 16-byte pieces of a row in f16
   constexpr int OPB = 128 * D * 2;         // bytes of a 128-row operand
   constexpr int PIECES = PA_KT * D / 16;   // 16-byte pieces of a tile in e4m3
-  constexpr int PER_T = PIECES / (PA_CONV * 32);
+  constexpr int PER_T = (PIECES + PA_CONV * 32 - 1) / (PA_CONV * 32);
   constexpr uint32_t NOWHERE = 0x7fffffff;
   extern __shared__ __align__(1024) unsigned char pa_dyn[];
   __shared__ __align__(8) uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sfull[2][2], pready[2][2], pvdone[2], ofull[2], qready;
@@ -281,21 +281,21 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
           bool masked = at + PA_HT > see_warp;
 #pragma unroll
           for (int g = 0; g < 4; ++g) masked |= sc[g].x < 0.0f;
-          // Largest score, and largest weight of V.  Sixteen columns at a time, the next ones on their way.
+          uint32_t x[4][16];
+#pragma unroll
+          for (int g = 0; g < 4; ++g) tc_ld16(s_here + 16 * g, x[g]);
+          tc_wait_ld();
+          // Largest score, and largest weight of V.
           float top = -INFINITY, topw = -INFINITY, least = INFINITY;
           auto maxima = [&](auto mask_c) {
             constexpr bool with_mask = decltype(mask_c)::value;
-            uint32_t x[2][16];
-            tc_ld16(s_here, x[0]);
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-              tc_wait_ld();
-              if (g < 3) tc_ld16(s_here + 16 * (g + 1), x[(g + 1) & 1]);
               const float2 k = sc[g];
               float t = -INFINITY;
 #pragma unroll
               for (int e = 0; e < 16; ++e)
-                if (!with_mask || at + 16 * g + e < limit) t = fmaxf(t, __uint_as_float(x[g & 1][e]));
+                if (!with_mask || at + 16 * g + e < limit) t = fmaxf(t, __uint_as_float(x[g][e]));
               if (with_mask && (k.x < 0.0f || t == -INFINITY)) continue;
               t *= fq * k.x;
               top = fmaxf(top, t);
@@ -331,12 +331,8 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
           const bool apart = __any_sync(0xffffffffu, mu + least - wu + AT_BIAS < -60.0f);
           auto weights = [&](auto mask_c, auto share_c) {
             constexpr bool with_mask = decltype(mask_c)::value, by_share = decltype(share_c)::value;
-            uint32_t x[2][16];
-            tc_ld16(s_here, x[0]);
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-              tc_wait_ld();
-              if (g < 3) tc_ld16(s_here + 16 * (g + 1), x[(g + 1) & 1]);
               const float2 k = sc[g];
               const float fg = fq * k.x, shift = fminf(mu + k.y - wu + AT_BIAS, 126.0f);
               const float add = by_share ? -mu : k.y - wu + AT_BIAS, gain = by_share ? ex2(shift) : 0.0f;
@@ -344,7 +340,7 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
               float part = 0.0f;
 #pragma unroll
               for (int e = 0; e < 16; e += 2) {
-                float y0 = fmaf(__uint_as_float(x[g & 1][e]), fg, add), y1 = fmaf(__uint_as_float(x[g & 1][e + 1]), fg, add);
+                float y0 = fmaf(__uint_as_float(x[g][e]), fg, add), y1 = fmaf(__uint_as_float(x[g][e + 1]), fg, add);
                 if (with_mask) {
                   if (k.x < 0.0f || at + 16 * g + e >= limit) y0 = -INFINITY;
                   if (k.x < 0.0f || at + 16 * g + e + 1 >= limit) y1 = -INFINITY;
@@ -440,32 +436,39 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
       const int32_t* trow = a.table + row * a.table_stride;
       const int bsm = (1 << a.bs_shift) - 1;
       uint4 kr[PER_T], vr[PER_T];
+      int ids[PER_T], ids_next[PER_T], part_id = -1, part_next = -1;
       float ksn = 0.0f, lvn = 0.0f;
-      auto fetch = [&](int j) {
+      // Block ids of the thread's pieces of tile j (-1: not seen), a tile ahead of their use; then keys with the
+      // scales, and values, each as soon as the registers of the tile before are free.
+      auto locate = [&](int j) {
+        auto id = [&](int t) {
+          const int page = t < see_last && j < tile1 ? __ldg(trow + (t >> a.bs_shift)) : -1;
+          return (unsigned)page < (unsigned)a.num_blocks ? page : -1;
+        };
+#pragma unroll
+        for (int i = 0; i < PER_T; ++i) {
+          const int p = ct + i * PA_CONV * 32;
+          ids_next[i] = p < PIECES ? id(j * PA_KT + p / (D / 16)) : -1;
+        }
+        if (ct < 8) part_next = id(j * PA_KT + ct * 16);
+      };
+      auto advance = [&]() {
+#pragma unroll
+        for (int i = 0; i < PER_T; ++i) ids[i] = ids_next[i];
+        part_id = part_next;
+      };
+      auto fetch = [&](const uint8_t* from, uint4 (&to)[PER_T], int j) {
 #pragma unroll
         for (int i = 0; i < PER_T; ++i) {
           const int p = ct + i * PA_CONV * 32, t = j * PA_KT + p / (D / 16), cc = p % (D / 16);
-          kr[i] = vr[i] = make_uint4(0, 0, 0, 0);
-          if (t < see_last) {
-            const int page = trow[t >> a.bs_shift];
-            if ((unsigned)page < (unsigned)a.num_blocks) {
-              const int64_t at = ((((int64_t)page * a.heads + head) << a.bs_shift) + (t & bsm)) * D + cc * 16;
-              kr[i] = __ldg(reinterpret_cast<const uint4*>(a.kc + at));
-              vr[i] = __ldg(reinterpret_cast<const uint4*>(a.vc + at));
-            }
-          }
+          to[i] = ids[i] >= 0 ? __ldg(reinterpret_cast<const uint4*>(from + (((int64_t)ids[i] * a.heads + head) << a.bs_shift) * D + (t & bsm) * D + cc * 16))
+                              : make_uint4(0, 0, 0, 0);
         }
+      };
+      auto fetch_scales = [&]() {
         if (ct < 8) {
-          const int t = j * PA_KT + ct * 16;
-          ksn = -1.0f;
-          lvn = -INFINITY;
-          if (t < see_last) {
-            const int page = trow[t >> a.bs_shift];
-            if ((unsigned)page < (unsigned)a.num_blocks) {
-              ksn = __ldg(a.ks + (int64_t)page * a.heads + head);
-              lvn = lg2(__ldg(a.vs + (int64_t)page * a.heads + head));
-            }
-          }
+          ksn = part_id >= 0 ? __ldg(a.ks + (int64_t)part_id * a.heads + head) : -1.0f;
+          lvn = part_id >= 0 ? lg2(__ldg(a.vs + (int64_t)part_id * a.heads + head)) : -INFINITY;
         }
       };
       auto widen = [&](const uint4& v, unsigned char* to, int t, int cc) {
@@ -477,14 +480,19 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
         *reinterpret_cast<uint4*>(to + pa_place(t, 2 * cc + swap)) = swap ? hi : lo;
         *reinterpret_cast<uint4*>(to + pa_place(t, 2 * cc + !swap)) = swap ? lo : hi;
       };
-      fetch(tile0);
+      locate(tile0);
+      advance();
+      locate(tile0 + 1);
+      fetch(a.kc, kr, tile0);
+      fetch_scales();
+      fetch(a.vc, vr, tile0);
       for (int j = tile0; j < tile1; ++j) {
         const uint32_t n = tiles + j - tile0, st = n & 1;
         if (n >= 2) tc_wait(&kempty[st], ((n >> 1) - 1) & 1, &failed);
 #pragma unroll
         for (int i = 0; i < PER_T; ++i) {
           const int p = ct + i * PA_CONV * 32;
-          widen(kr[i], ksm + st * OPB, p / (D / 16), p % (D / 16));
+          if (p < PIECES) widen(kr[i], ksm + st * OPB, p / (D / 16), p % (D / 16));
         }
         if (ct < 8) {
           sscale[n & 3][ct] = make_float2(ksn, lvn);
@@ -492,6 +500,12 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
         fence_proxy_async();
         __syncwarp();
         if (lane == 0) mbar_arrive_local(&kfull[st]);
+        advance();
+        if (j + 1 < tile1) {
+          fetch(a.kc, kr, j + 1);
+          fetch_scales();
+          locate(j + 2);
+        }
         if (n >= 2) tc_wait(&vempty[st], ((n >> 1) - 1) & 1, &failed);
 #pragma unroll
         for (int i = 0; i < PER_T; ++i) {
@@ -510,9 +524,9 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
               u[e] &= ~nan;
             }
           }
-          widen(make_uint4(u[0], u[1], u[2], u[3]), vsm + st * OPB, t, cc);
+          if (p < PIECES) widen(make_uint4(u[0], u[1], u[2], u[3]), vsm + st * OPB, t, cc);
         }
-        if (j + 1 < tile1) fetch(j + 1);
+        if (j + 1 < tile1) fetch(a.vc, vr, j + 1);
         fence_proxy_async();
         __syncwarp();
         if (lane == 0) mbar_arrive_local(&vfull[st]);
