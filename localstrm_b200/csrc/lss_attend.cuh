@@ -47,6 +47,7 @@ struct AttendArgs {
   int B, T;
   float scale;         // softmax scale times log2(e)
   int aligned;         // q and out rows start on 16-byte boundaries
+  int fused;           // the grid is one cluster, which joins its own pieces
   int4* meta;          // [workers]: row, group, pieces (0: nothing to join)
   float* part;         // [workers][2][at_piece]: a warp's first piece, its last one
 };
@@ -195,6 +196,23 @@ __device__ __forceinline__ void at_join(const AttendArgs& a, PieceAt piece_at, i
   }
 }
 
+// The group that `worker` joins: its pieces are the last one of the warp before, then the first ones of this
+// warp and those after it.  Inside a CTA they are added up already, in the place of the first of them; so what
+// counts is the one before, the first warp of each CTA that follows, and the last warp, whose first piece may
+// stand alone.
+template <int D, int DT, int NQ>
+__device__ __forceinline__ void at_join_cut(const AttendArgs& a, int64_t worker, const int4& me, int t0, int nth) {
+  constexpr int NW = AtCfg<D, NQ>::NW;
+  constexpr int64_t PS = at_piece(D, NQ);
+  const int64_t end = worker + me.z - 2, cta = (worker + NW - 1) / NW;
+  const int ctas = end >= cta * NW ? (int)(end / NW - cta) + 1 : 0;
+  const bool extra = end % NW != 0;
+  at_join<D, DT, NQ>(a, [&](int i) {
+    const int64_t at = i == 0 ? (worker - 1) * 2 + 1 : i <= ctas ? (cta + i - 1) * NW * 2 : end * 2;
+    return a.part + at * PS;
+  }, 1 + ctas + extra, true, nullptr, me.x, me.y, t0, nth);
+}
+
 // o = sum_t p_t v_t,  p = softmax_t(c q . k_t) over the tokens t up to the query's own position.
 //
 // Work: for each row and key head, the queries that share it (`per` heads times the row's new
@@ -202,7 +220,8 @@ __device__ __forceinline__ void at_join(const AttendArgs& a, PieceAt piece_at, i
 // cut into equal ranges, one per warp, whatever the lengths are: every warp streams its own tiles
 // through its own copy ring and keeps its own running softmax, with no barrier between warps.
 // Ranges that end inside a group leave pieces: those of the CTA's warps are added up in shared memory,
-// those of several CTAs by lss_attend_join_kernel, always in order.
+// those of several CTAs by lss_attend_join_kernel, always in order; where the work fits one cluster
+// (`fused`), behind a cluster barrier instead, which saves a launch.
 //
 // Arithmetic: with keys and values as the 16-row operand of mma.m16n8k16 (f16 operands, f32 sums),
 // S^T = K Q^T and O^T = V^T P^T need no padding for 8 query rows, and the weights turn from result to
@@ -721,7 +740,16 @@ __global__ void __launch_bounds__(AtCfg<D, NQ>::NW * 32, 1) lss_attend_kernel(At
     }
     w0 = w1;
   }
-  if (lane == 0) a.meta[worker] = join;
+  if (a.fused) {
+    __threadfence();
+    cg::this_cluster().sync();
+    if (lane == 0) w_last[warp] = join;
+    __syncthreads();
+    for (int i = 0; i < NW; ++i)
+      if (w_last[i].z > 0) at_join_cut<D, DT, NQ>(a, first_w + i, w_last[i], tid, NTH);
+  } else if (lane == 0) {
+    a.meta[worker] = join;
+  }
 }
 
 // Adds up the pieces of the groups that were cut between CTAs: one CTA per warp of the first kernel,
@@ -729,21 +757,8 @@ __global__ void __launch_bounds__(AtCfg<D, NQ>::NW * 32, 1) lss_attend_kernel(At
 template <int D, int DT, int NQ>
 __global__ void __launch_bounds__(256) lss_attend_join_kernel(AttendArgs a) {
   pdl_wait();
-  const int64_t worker = blockIdx.x;
-  const int4 me = a.meta[worker];
-  if (me.z == 0) return;
-  // The pieces: the last one of the warp before, then the first ones of this warp and those after it.
-  // Inside a CTA they are added up already, in the place of the first of them; so what counts is the one
-  // before, the first warp of each CTA that follows, and the last warp, whose first piece may stand alone.
-  constexpr int NW = AtCfg<D, NQ>::NW;
-  constexpr int64_t PS = at_piece(D, NQ);
-  const int64_t end = worker + me.z - 2, cta = (worker + NW - 1) / NW;
-  const int ctas = end >= cta * NW ? (int)(end / NW - cta) + 1 : 0;
-  const bool extra = end % NW != 0;
-  at_join<D, DT, NQ>(a, [&](int i) {
-    const int64_t at = i == 0 ? (worker - 1) * 2 + 1 : i <= ctas ? (cta + i - 1) * NW * 2 : end * 2;
-    return a.part + at * PS;
-  }, 1 + ctas + extra, true, nullptr, me.x, me.y, threadIdx.x, 256);
+  const int4 me = a.meta[blockIdx.x];
+  if (me.z > 0) at_join_cut<D, DT, NQ>(a, blockIdx.x, me, threadIdx.x, 256);
 }
 
 }  // namespace lss

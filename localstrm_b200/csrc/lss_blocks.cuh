@@ -49,7 +49,8 @@ struct PlanArgs {
   int32_t* n_free_out;  // [1], may be n_free
 };
 
-__device__ __forceinline__ int64_t blocks_of(int64_t tokens, int bs) { return (tokens + bs - 1) / bs; }
+// Blocks of 0 <= tokens <= 2^30 (a table's width): a 32-bit division.
+__device__ __forceinline__ int blocks_of(int tokens, int bs) { return (int)((unsigned)(tokens + bs - 1) / (unsigned)bs); }
 
 // One step's plan.  With new = max(new_lens, 0), upto the inclusive sums of new and
 // need = ceil((len + new) / bs) - ceil(len / bs) for the rows whose tokens fit (the capacity and
@@ -58,17 +59,18 @@ __device__ __forceinline__ int64_t blocks_of(int64_t tokens, int bs) { return (t
 // free_blocks[n_free - 1 - k].
 //
 // The work is a few hundred kilobytes at most: what bounds it is the chain load lengths -> two
-// block-wide sums -> a search and two dependent loads per token, not bytes.  So it is one launch of
-// one cluster: every CTA takes the sums of all rows by itself (cheaper than passing them on through
-// memory and a second launch), each fills its share of the tokens, and one cluster barrier behind
-// the last read of the lengths lets rank 0 write the new state in place.
+// block-wide sums -> a search and two dependent loads per token, not bytes.  So it is one launch: every CTA
+// takes the sums of all rows by itself (cheaper than passing them on through memory and a second
+// launch), and each fills its share of the tokens.  Where the new state is written in place the CTAs are one
+// cluster, with a barrier between the last read of the lengths and their update; else there are as many as the
+// tokens need (65,000 tokens of 1,000 rows: eight CTAs issue for 14 us, 64 for 5).
 __global__ void __launch_bounds__(BL_NT) lss_plan_kernel(PlanArgs a) {
   extern __shared__ int32_t bl_sm[];
   int32_t* upto = bl_sm;          // [B] inclusive sums of the new tokens, at most INT_MAX
   int32_t* taken = bl_sm + a.B;   // [B] blocks taken by the rows before, -1: not granted
   __shared__ int64_t scr[32];
   cg::cluster_group cl = cg::this_cluster();
-  const int rank = (int)cl.block_rank(), nct = (int)cl.num_blocks(), tid = threadIdx.x;
+  const int rank = blockIdx.x, nct = gridDim.x, tid = threadIdx.x;
   const int bs = a.block_size;
   const int nfree = min(max(a.n_free[0], 0), a.num_blocks);
   int64_t base_tok = 0, base_need = 0;
@@ -82,7 +84,7 @@ __global__ void __launch_bounds__(BL_NT) lss_plan_kernel(PlanArgs a) {
     const int64_t first = base_tok + bl_scan(nw, scr, tot);
     base_tok += tot;
     const bool fits = nw > 0 && len >= 0 && first + nw <= a.capacity && len + nw <= (int64_t)a.width * bs;
-    const int64_t need = fits ? blocks_of(len + nw, bs) - blocks_of(len, bs) : 0;
+    const int64_t need = fits ? blocks_of((int)(len + nw), bs) - blocks_of((int)len, bs) : 0;
     const int64_t before = base_need + bl_scan(need, scr, tot);
     base_need += tot;
     const bool ok = fits && (need == 0 || before + need <= nfree);
@@ -106,35 +108,55 @@ __global__ void __launch_bounds__(BL_NT) lss_plan_kernel(PlanArgs a) {
   used = __reduce_max_sync(0xffffffffu, (int)scr[tid & 31]);
 
   const int total = (int)min(base_tok, (int64_t)a.capacity);
-  for (int64_t t = (int64_t)rank * BL_NT + tid; t < a.capacity; t += (int64_t)nct * BL_NT) {
-    int64_t slot = -1;
-    int pos = 0;
-    if (t < total) {
-      int lo = 0, hi = a.B - 1;  // first row whose sum exceeds t
+  // Four tokens a thread at a time: their searches and loads run side by side.
+  constexpr int TOK = 4;
+  const int64_t stride = (int64_t)nct * BL_NT;
+  for (int64_t t0 = (int64_t)rank * BL_NT + tid; t0 < a.capacity; t0 += TOK * stride) {
+    int row[TOK], page[TOK], pos[TOK], off[TOK];
+    int32_t* entry[TOK];
+    bool fresh[TOK];
+#pragma unroll
+    for (int i = 0; i < TOK; ++i) {
+      const int64_t t = t0 + i * stride;
+      int lo = 0, hi = t < total ? a.B - 1 : 0;  // first row whose sum exceeds t
       while (lo < hi) {
         const int mid = (lo + hi) >> 1;
         if (upto[mid] > t) hi = mid; else lo = mid + 1;
       }
-      const int r = lo, len = a.lens[r], tk = taken[r];
-      const int64_t p = (int64_t)len + t - (r > 0 ? upto[r - 1] : 0);
-      pos = (int)p;
-      if (tk >= 0) {
-        const int j = (int)(p / bs), off = (int)(p - (int64_t)j * bs), held = (int)blocks_of(len, bs);
-        int32_t* entry = a.table + r * a.table_stride + j;
-        int page;
-        if (j < held) {
-          page = *entry;
-        } else {
-          page = a.free_blocks[nfree - 1 - (tk + j - held)];
-          if (off == 0) *entry = page;  // a block taken now starts with a token of this step
+      row[i] = t < total ? lo : -1;
+    }
+#pragma unroll
+    for (int i = 0; i < TOK; ++i) {
+      const int r = row[i];
+      pos[i] = off[i] = 0;
+      page[i] = -1;
+      entry[i] = nullptr;
+      fresh[i] = false;
+      if (r >= 0) {
+        const int len = a.lens[r], tk = taken[r];
+        const int64_t p = (int64_t)len + t0 + i * stride - (r > 0 ? upto[r - 1] : 0);
+        pos[i] = (int)p;
+        if (tk >= 0) {
+          const int j = (int)((unsigned)p / (unsigned)bs), held = blocks_of(len, bs);
+          off[i] = (int)p - j * bs;
+          entry[i] = a.table + r * a.table_stride + j;
+          fresh[i] = j >= held;
+          page[i] = fresh[i] ? a.free_blocks[nfree - 1 - (tk + j - held)] : *entry[i];
         }
-        if (page >= 0 && page < a.num_blocks) slot = (int64_t)page * bs + off;
       }
     }
-    a.slots[t] = slot;
-    a.positions[t] = pos;
+#pragma unroll
+    for (int i = 0; i < TOK; ++i) {
+      const int64_t t = t0 + i * stride;
+      if (t < a.capacity) {
+        if (fresh[i] && off[i] == 0) *entry[i] = page[i];  // a block taken now starts with a token of this step
+        a.slots[t] = page[i] >= 0 && page[i] < a.num_blocks ? (int64_t)page[i] * bs + off[i] : -1;
+        a.positions[t] = pos[i];
+      }
+    }
   }
-  // Every CTA has read the lengths and the free count: rank 0 may write over them.
+  // In place, the grid is one cluster: every CTA has read the lengths and the free count, the first one may
+  // write over them.
   cl.sync();
   if (rank == 0) {
     for (int r = tid; r < a.B; r += BL_NT) {
@@ -174,7 +196,7 @@ __global__ void __launch_bounds__(BL_NT) lss_release_kernel(ReleaseArgs a) {
     const int r = r0 + tid;
     int64_t n = 0;
     if (r < a.B && a.codes[r] != 0)
-      n = blocks_of(min(max((int64_t)a.lens[r], (int64_t)0), (int64_t)a.width * bs), bs);
+      n = blocks_of(min(max(a.lens[r], 0), a.width * bs), bs);
     int64_t tot;
     const int64_t first = base + bl_scan(n, scr, tot);
     base += tot;
@@ -184,9 +206,15 @@ __global__ void __launch_bounds__(BL_NT) lss_release_kernel(ReleaseArgs a) {
   const int lane = tid & 31;
   for (int r = rank * (BL_NT / 32) + (tid >> 5); r < a.B; r += nct * (BL_NT / 32)) {
     const int first = r > 0 ? upto[r - 1] : 0, n = upto[r] - first;
-    for (int j = lane; j < n; j += 32) {
-      const int64_t at = (int64_t)nfree + first + j;
-      if (at < a.num_blocks) a.free_blocks[at] = a.table[r * a.table_stride + j];
+    for (int j0 = lane; j0 < n; j0 += 32 * 8) {  // eight loads on their way before the first store
+      int32_t ids[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ids[i] = j0 + 32 * i < n ? a.table[r * a.table_stride + j0 + 32 * i] : 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int64_t at = (int64_t)nfree + first + j0 + 32 * i;
+        if (j0 + 32 * i < n && at < a.num_blocks) a.free_blocks[at] = ids[i];
+      }
     }
   }
   cl.sync();

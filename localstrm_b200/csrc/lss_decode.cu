@@ -120,6 +120,13 @@ static cudaError_t launch_attend(AttendArgs a, void* ws, cudaStream_t st) {
   const int ctas = (int)std::min((int64_t)std::min(sm_count(dev), AT_CAP_CTAS), (units + NW - 1) / NW);
   a.meta = reinterpret_cast<int4*>(ws);
   a.part = reinterpret_cast<float*>(a.meta + (size_t)ctas * NW);
+  // Two tiles a warp and less on eight SMs: one launch (a call for one short request 20.6 -> 17.5 us on the host); with
+  // more tiles eight SMs' share of the bandwidth would cost more than the second launch.
+  a.fused = units <= 8 * NW * 2;
+  if (a.fused) {
+    const int size = ctas <= 1 ? 1 : ctas <= 2 ? 2 : ctas <= 4 ? 4 : 8;
+    return launch(lss_attend_kernel<D, DT, NQ>, (unsigned)size, NW * 32, smem, size, false, st, a);
+  }
   e = launch(lss_attend_kernel<D, DT, NQ>, (unsigned)ctas, NW * 32, smem, 1, false, st, a);
   if (e != cudaSuccess) return e;
   return launch(lss_attend_join_kernel<D, DT, NQ>, (unsigned)(ctas * NW), 256, 0, 1, true, st, a);
@@ -330,8 +337,10 @@ int lss_block_plan(int32_t* table, int64_t table_stride, int width, const int32_
     const cudaError_t e = allow_smem(lss_plan_kernel, set, dev, smem);
     if (e != cudaSuccess) return status_of(e);
   }
-  const int ctas = cluster_for(((int64_t)capacity + BL_NT - 1) / BL_NT, BL_MAXCL);
-  return status_of(launch(lss_plan_kernel, (unsigned)ctas, BL_NT, (size_t)smem, ctas, false,
+  const int64_t want = ((int64_t)capacity + BL_NT - 1) / BL_NT;
+  const bool in_place = n_free_out == n_free || (lens_out < lens + B && lens < lens_out + B);
+  const int ctas = in_place ? cluster_for(want, BL_MAXCL) : (int)std::max((int64_t)1, std::min(want, (int64_t)sm_count(dev)));
+  return status_of(launch(lss_plan_kernel, (unsigned)ctas, BL_NT, (size_t)smem, in_place ? ctas : 1, false,
                           reinterpret_cast<cudaStream_t>(stream), a));
 }
 
