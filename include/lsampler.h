@@ -232,8 +232,8 @@ int lss_read_row_paths(const void* workspace, int B, int32_t* paths_out, void* s
  *   x        [rows] x [x_stride elements], dtype LSS_DTYPE_*; K a multiple of 32
  *   packed   uint8 [N][K / 2], column 2i in the low four bits of byte i, 2i + 1 in the high ones;
  *            16-byte aligned
- *   scales   [N][K / group], dtype LSS_DTYPE_BF16 or LSS_DTYPE_F16, 4-byte aligned;
- *            group: 32, 64 or a multiple of 128 that divides K
+ *   scales   [N][K / group], dtype LSS_DTYPE_BF16 or LSS_DTYPE_F16; group: 32, 64 or a multiple of 128
+ *            that divides K
  *   y        [rows] x [y_stride elements], dtype LSS_DTYPE_*
  *   workspace  lss_int4_workspace_bytes(rows, K, x_dtype, N) bytes (0 for up to eight rows: NULL will do),
  *              16-byte aligned, of this call alone until it is done

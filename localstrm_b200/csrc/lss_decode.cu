@@ -294,7 +294,7 @@ int lss_int4_matvec(const void* x, int x_dtype, int rows, int K, int64_t x_strid
   if (scale_dtype != LSS_DTYPE_BF16 && scale_dtype != LSS_DTYPE_F16) return LSS_ERR_INVALID_ARG;
   if ((group != 32 && group != 64 && (group < 128 || group % 128 != 0)) || K % group != 0) return LSS_ERR_INVALID_ARG;
   if (rows == 0) return LSS_OK;
-  if (!x || !packed || !scales || !y || !aligned_to(packed, 16) || !aligned_to(scales, 4)) return LSS_ERR_INVALID_ARG;
+  if (!x || !packed || !scales || !y || !aligned_to(packed, 16) || !aligned_to(scales, 2)) return LSS_ERR_INVALID_ARG;
   Int4Args a{};
   a.x = x;
   a.x_stride = x_stride;

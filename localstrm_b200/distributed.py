@@ -164,3 +164,11 @@ class VocabShardSampler:
         gathered = torch.empty(world * B * self.rec_bytes, dtype=torch.uint8, device=rec.device)
         dist.all_gather_into_tensor(gathered, rec, group=self.group)
         return self._merge(gathered, world, B, self.K, V_total, temperature, top_p, uniforms)
+
+    def sample_hidden(self, hidden, head, offset: int, V_total: int, temperature, top_p, uniforms,
+                      **row_params) -> torch.Tensor:
+        """``sample`` from the hidden states ``[B, K]``: this rank's columns of the vocabulary projection are
+        the rows of ``head`` (an ``Int4Weight``), its f32 logits never leave the GPU."""
+        from .head import int4_matvec
+        return self.sample(int4_matvec(hidden, head, out_dtype=torch.float32), offset, V_total, temperature,
+                           top_p, uniforms, **row_params)

@@ -57,8 +57,8 @@ class Int4Weight:
     def quantize(cls, weight: torch.Tensor, group: int = 128, scale_dtype: torch.dtype = torch.float16) -> "Int4Weight":
         """The nearest codes -7 .. 7 for the scale ``max |w| / 7`` of each group (done once, where
         the weights lie)."""
-        if weight.dim() != 2 or weight.shape[1] % 32 or group < 32 or weight.shape[1] % group:
-            raise ValueError(f"weight: expected [N, K] with K a multiple of 32 and of the group {group}")
+        if weight.dim() != 2 or (group not in (32, 64) and (group < 128 or group % 128)) or weight.shape[1] % group:
+            raise ValueError(f"weight: expected [N, K], K a multiple of the group {group}: 32, 64 or a multiple of 128")
         n, k = weight.shape
         w = weight.float().view(n, k // group, group)
         scales = (w.abs().amax(-1) / 7.0).to(scale_dtype)

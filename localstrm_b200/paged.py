@@ -206,7 +206,7 @@ def attend(q: torch.Tensor, cache: KVCache8, block_table: torch.Tensor, plan: St
     else:
         os = out.stride()
         if out.shape != shape or out.dtype is not dtype or out.get_device() != dev or os[2] != 1 or os[1] < dim \
-                or os[0] < (shape[1] - 1) * os[1] + dim:
+                or (shape[0] > 1 and os[0] < (shape[1] - 1) * os[1] + dim):
             raise ValueError(f"out: expected {dtype} {list(shape)} on cuda:{dev}, rows of stride 1 that do not overlap")
     if lse_out is not None and (lse_out.dtype is not _F32 or lse_out.shape != shape[:2] or lse_out.get_device() != dev
                                 or not lse_out.is_contiguous()):

@@ -20,7 +20,7 @@ def test_int4_refusals():
     assert int4(rows=0) == OK
     for bad in (dict(rows=-1), dict(K=48), dict(K=0), dict(N=0), dict(xs=63), dict(ys=3), dict(xd=3), dict(yd=-1), dict(sd=0),
                 dict(group=16), dict(group=96), dict(group=128), dict(K=320, xs=320, group=128), dict(x=None), dict(packed=None),
-                dict(packed=8), dict(scales=18), dict(scales=None), dict(y=None)):
+                dict(packed=8), dict(scales=17), dict(scales=None), dict(y=None)):
         assert int4(**bad) == INVALID, bad
     lib = _lib.load()
     assert lib.lss_int4_workspace_bytes(8, 64, 1, 4) == 0
@@ -117,8 +117,9 @@ def test_quantize_round_trip():
             # half a step, and where the scale was rounded down the largest values end at code 7
             assert bool(((q.dequantize() - w).abs() <= step * (0.5 + 7 * 2 * eps) + 1e-30).all())
     assert bool((q.dequantize()[5] == 0).all())
-    with pytest.raises(ValueError):
-        lb.Int4Weight.quantize(w, group=48)
+    for group in (48, 16, 96, 192):
+        with pytest.raises(ValueError):
+            lb.Int4Weight.quantize(torch.randn(4, 192), group=group)
     with pytest.raises(ValueError):
         lb.Int4Weight.quantize(torch.randn(4, 40), group=40)
 

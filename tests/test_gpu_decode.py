@@ -99,6 +99,57 @@ def test_int4_quantize_and_sample_hidden():
     assert got[0] == logits[0].argmax()
 
 
+def test_int4_row_slices_and_vocabulary_shards(monkeypatch):
+    """Rows of a matrix by themselves (their scales may start on any 16-bit boundary), and the projection in
+    front of the vocabulary-sharded sampler."""
+    from localstrm_b200 import distributed as D
+    w, x = int4_case(3, 700, 96, 32, seed=21)
+    whole = lb.int4_matvec(x, w)
+    for a, b in ((1, 350), (351, 700)):
+        assert torch.equal(lb.int4_matvec(x, lb.Int4Weight(w.packed[a:b], w.scales[a:b])), whole[:, a:b])
+    # one rank that holds the whole vocabulary: its all-gather is a copy
+    held = []
+    monkeypatch.setattr(D, "_world", lambda group: (1, 0))
+    monkeypatch.setattr(D.dist, "all_gather_into_tensor", lambda out, rec, group=None: (held.append(rec.clone()), out.copy_(rec)))
+    head = lb.Int4Weight.quantize(torch.randn(2000, 128, generator=gen(22), device=DEV), 128)
+    h = torch.randn(4, 128, generator=gen(23), device=DEV)
+    temp, top_p, u = (torch.full((4,), v, device=DEV) for v in (0.8, 0.9, 0.37))
+    s = D.VocabShardSampler(DEV, K=64)
+    got = s.sample_hidden(h, head, 0, 2000, temp, top_p, u, top_k=[64] * 4)
+    logits = lb.int4_matvec(h, head)
+    assert torch.equal(got, s.sample(logits, 0, 2000, temp, top_p, u)) and torch.equal(held[0], held[1])
+    prm = [S.SamplingParams(temperature=0.8, top_k=64, top_p=0.9)] * 4
+    assert torch.equal(got, S.sample_batch(logits, prm, uniforms=u))
+    with pytest.raises(ValueError):
+        s.sample_hidden(h, head, 0, 2000, temp, top_p, u, top_k=[3] * 4)
+
+
+def test_attend_in_place_and_at_once():
+    """The output over the queries; two captured steps that share everything but the workspace."""
+    for ctx, new in (([700, 30, 0], [1, 1, 1]), ([9000], [1]), ([100, 0, 700], [900, 513, 300])):
+        rows = U.make_rows(ctx, new, 16)
+        cache = lb.KVCache8(*U.random_cache(rows[-1], 8, 16, 128))
+        q = torch.randn(sum(new), 32, 128, generator=gen(1), device=DEV).bfloat16()
+        plan = lb.StepPlan(*rows[2:5])
+        want = lb.attend(q, cache, rows[1], plan)
+        own = q.clone()
+        lb.attend(own, cache, rows[1], plan, out=own)
+        assert torch.equal(own, want)
+        graphs, outs = [], []
+        for _ in range(2):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                outs.append(lb.attend(q, cache, rows[1], plan))
+            graphs.append(g)
+        streams = [torch.cuda.Stream() for _ in graphs]
+        for _ in range(5):
+            for g, s in zip(graphs, streams):
+                with torch.cuda.stream(s):
+                    g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, want) for o in outs)
+
+
 # --------------------------------------------------------------------------------- block tables
 def plan_case(rows, bs, hi_ctx, hi_new, spare, seed, width_cut=0):
     g = torch.Generator().manual_seed(seed)
