@@ -58,7 +58,7 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -632,8 +632,7 @@ __global__ void __launch_bounds__(AtCfg<D, NQ>::NW * 32, 1) lss_attend_kernel(At
             for (int nq = 0; nq < NQ; ++nq) mma_f16(o[p * SP + 2 * i + q][nq], va, pb[nq][0], pb[nq][1]);
           }
       }
-      __syncwarp();
-    }
+    }  // the next tile's __syncwarp lets its place be written again
     asm volatile("cp.async.wait_all;" ::: "memory");
 
 #pragma unroll
