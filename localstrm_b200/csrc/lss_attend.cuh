@@ -12,18 +12,21 @@ constexpr float AT_BIAS = 10.0f, AT_SLACK = 5.0f;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
 
-// Shape of the kernel for a head dimension and query rows per group (8 NQ): warps per CTA (one CTA per
-// SM), stages of the copy ring per warp.  Registers set the warps (queries and sums take 6 NQ D / 16 of
-// them), the shared memory the stages.
-template <int D, int NQ> struct AtCfg;
-template <> struct AtCfg<64, 1> { static constexpr int NW = 16, ST = 6; };
-template <> struct AtCfg<64, 2> { static constexpr int NW = 16, ST = 6; };
-template <> struct AtCfg<64, 4> { static constexpr int NW = 12, ST = 8; };
-template <> struct AtCfg<128, 1> { static constexpr int NW = 16, ST = 3; };
-template <> struct AtCfg<128, 2> { static constexpr int NW = 12, ST = 4; };
-template <> struct AtCfg<128, 4> { static constexpr int NW = 8, ST = 6; };
-template <> struct AtCfg<256, 1> { static constexpr int NW = 8, ST = 3; };
-template <> struct AtCfg<256, 2> { static constexpr int NW = 8, ST = 3; };
+// Shape of the kernel for a head dimension, query rows per group (8 NQ) and tiles a step (TP): warps per
+// CTA (one CTA per SM), stages of the copy ring per warp.  Registers set the warps (queries and sums take
+// 6 NQ D / 16 of them), the shared memory the stages.  D = 128, 8 rows: two tiles a step on 12 warps give each
+// warp more to do between its waits (1.1 GB of contexts of up to 16,000 tokens: 223 -> 212 us); one on 16 warps
+// starts more groups at once (512 rows of 64 to 300 tokens: 75 us against 92).
+template <int D, int NQ, int TP> struct AtCfg;
+template <> struct AtCfg<64, 1, 1> { static constexpr int NW = 16, ST = 6; };
+template <> struct AtCfg<64, 2, 1> { static constexpr int NW = 16, ST = 6; };
+template <> struct AtCfg<64, 4, 1> { static constexpr int NW = 12, ST = 8; };
+template <> struct AtCfg<128, 1, 1> { static constexpr int NW = 16, ST = 3; };
+template <> struct AtCfg<128, 1, 2> { static constexpr int NW = 12, ST = 4; };
+template <> struct AtCfg<128, 2, 1> { static constexpr int NW = 12, ST = 4; };
+template <> struct AtCfg<128, 4, 1> { static constexpr int NW = 8, ST = 6; };
+template <> struct AtCfg<256, 1, 1> { static constexpr int NW = 8, ST = 3; };
+template <> struct AtCfg<256, 2, 1> { static constexpr int NW = 8, ST = 3; };
 // Floats of one piece in the workspace: m, l, W of its rows, then the sums.
 __host__ __device__ constexpr int at_piece(int D, int NQ) { return 8 * NQ * (3 + D); }
 
@@ -200,9 +203,9 @@ __device__ __forceinline__ void at_join(const AttendArgs& a, PieceAt piece_at, i
 // warp and those after it.  Inside a CTA they are added up already, in the place of the first of them; so what
 // counts is the one before, the first warp of each CTA that follows, and the last warp, whose first piece may
 // stand alone.
-template <int D, int DT, int NQ>
+template <int D, int DT, int NQ, int TP>
 __device__ __forceinline__ void at_join_cut(const AttendArgs& a, int64_t worker, const int4& me, int t0, int nth) {
-  constexpr int NW = AtCfg<D, NQ>::NW;
+  constexpr int NW = AtCfg<D, NQ, TP>::NW;
   constexpr int64_t PS = at_piece(D, NQ);
   const int64_t end = worker + me.z - 2, cta = (worker + NW - 1) / NW;
   const int ctas = end >= cta * NW ? (int)(end / NW - cta) + 1 : 0;
@@ -237,13 +240,15 @@ __device__ __forceinline__ void at_join_cut(const AttendArgs& a, int64_t worker,
 //
 // Bound by HBM (2 D bytes per token and head) when a row has few queries, by the tensor pipe and the
 // widening of the codes when it has many (they share it 8 NQ rows at a time).
-template <int D, int DT, int NQ>
-__global__ void __launch_bounds__(AtCfg<D, NQ>::NW * 32, 1) lss_attend_kernel(AttendArgs a) {
-  constexpr int NW = AtCfg<D, NQ>::NW, ST = AtCfg<D, NQ>::ST, NTH = NW * 32, R = 8 * NQ;
+template <int D, int DT, int NQ, int TP>
+__global__ void __launch_bounds__(AtCfg<D, NQ, TP>::NW * 32, 1) lss_attend_kernel(AttendArgs a) {
+  constexpr int NW = AtCfg<D, NQ, TP>::NW, ST = AtCfg<D, NQ, TP>::ST, NTH = NW * 32, R = 8 * NQ;
   constexpr int PC = D < 128 ? D : 128, NP = D / PC;  // columns per panel, panels
   constexpr int SP = PC / 16;                         // 16-column steps per panel
   constexpr int STAGE = 32 * D + 16;                  // K tile, V tile, two scales
   constexpr int PIECE = at_piece(D, NQ);
+  constexpr int PD = ST / TP;                         // steps in the ring
+  static_assert(ST % TP == 0 && PD > 1, "a step is computed while another one is under way");
   static_assert(PIECE * 4 <= ST * STAGE, "a piece lies in its warp's ring");
   extern __shared__ __align__(128) unsigned char at_sm[];
   __shared__ int64_t scr[NW];
@@ -374,7 +379,7 @@ __global__ void __launch_bounds__(AtCfg<D, NQ>::NW * 32, 1) lss_attend_kernel(At
     };
     __syncwarp();
 #pragma unroll
-    for (int s = 0; s < ST - 1; ++s) issue(tile0 + s, s);
+    for (int s = 0; s < (PD - 1) * TP; ++s) issue(tile0 + s, s);
 
     // ---- queries: lane (g, c) holds row g of each eight, its columns; factors of rows 2c, 2c + 1
     uint32_t qf[NQ][NP * SP][2];
@@ -455,86 +460,118 @@ __global__ void __launch_bounds__(AtCfg<D, NQ>::NW * 32, 1) lss_attend_kernel(At
 #pragma unroll
         for (int q = 0; q < 4; ++q) o[i][nq][q] = 0.0f;
 
-    uint32_t stage = 0, fill = (ST - 1);
-    for (int t = tile0; t < tend; ++t) {
-      cp_async_wait_group<ST - 2>();
+    uint32_t stage = 0, fill = (PD - 1) * TP;
+    for (int t0 = tile0; t0 < tend; t0 += TP) {
+      // TP tiles a step: the places of the step before are free once all lanes are here.
       __syncwarp();
-      issue(t + ST - 1, (int)fill);
-      fill = fill + 1 == ST ? 0 : fill + 1;
-      const uint32_t kt = ring + stage * STAGE, vt = kt + 16 * D;
-      const bool wrong = (bad >> stage) & 1u;
-      stage = stage + 1 == ST ? 0 : stage + 1;
-      const float kscale = lds32f(kt + 32 * D), lv = lg2(lds32f(kt + 32 * D + 4));
+#pragma unroll
+      for (int u = 0; u < TP; ++u) {
+        issue(t0 + (PD - 1) * TP + u, (int)fill);
+        fill = fill + 1 == ST ? 0 : fill + 1;
+      }
+      cp_async_wait_group<(PD - 1) * TP>();
+      __syncwarp();
+      uint32_t kt[TP];
+      bool wrong[TP], masked[TP];
+      float lv[TP], f[TP][NQ][2], s[TP][NQ][4];
+      bool any_masked = false;
+#pragma unroll
+      for (int u = 0; u < TP; ++u) {
+        kt[u] = ring + stage * STAGE;
+        wrong[u] = ((bad >> stage) & 1u) || t0 + u >= tend;
+        stage = stage + 1 == ST ? 0 : stage + 1;
+        masked[u] = wrong[u] || ((t0 + u) << 4) + 16 > see_first;
+        any_masked |= masked[u];
+        const float kscale = lds32f(kt[u] + 32 * D);
+        lv[u] = lg2(lds32f(kt[u] + 32 * D + 4));
+        if (wrong[u]) lv[u] = 0.0f;  // what lies there may be anything
+#pragma unroll
+        for (int nq = 0; nq < NQ; ++nq) {
+          f[u][nq][0] = fq[nq][0] * kscale;
+          f[u][nq][1] = fq[nq][1] * kscale;
+        }
+      }
 
       // scores: rows of the product are tokens g and g + 8
-      float s[NQ][4];
 #pragma unroll
-      for (int nq = 0; nq < NQ; ++nq)
+      for (int u = 0; u < TP; ++u)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[nq][e] = 0.0f;
+        for (int nq = 0; nq < NQ; ++nq)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[u][nq][e] = 0.0f;
 #pragma unroll
       for (int p = 0; p < NP; ++p) {
 #pragma unroll
         for (int i = 0; i < SP / 4; ++i) {
-          const uint4 x = lds128(kt + p * (16 * PC) + at_offset<PC>(g, c * (SP / 4) + i));
-          const uint4 y = lds128(kt + p * (16 * PC) + at_offset<PC>(g + 8, c * (SP / 4) + i));
-          const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t ka[4] = {f16_of_e4m3(xw[j]), f16_of_e4m3(yw[j]), f16_of_e4m3(xw[j] >> 16), f16_of_e4m3(yw[j] >> 16)};
+          for (int u = 0; u < TP; ++u) {
+            const uint4 x = lds128(kt[u] + p * (16 * PC) + at_offset<PC>(g, c * (SP / 4) + i));
+            const uint4 y = lds128(kt[u] + p * (16 * PC) + at_offset<PC>(g + 8, c * (SP / 4) + i));
+            const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-            for (int nq = 0; nq < NQ; ++nq) mma_f16(s[nq], ka, qf[nq][p * SP + 4 * i + j][0], qf[nq][p * SP + 4 * i + j][1]);
+            for (int j = 0; j < 4; ++j) {
+              const uint32_t ka[4] = {f16_of_e4m3(xw[j]), f16_of_e4m3(yw[j]), f16_of_e4m3(xw[j] >> 16), f16_of_e4m3(yw[j] >> 16)};
+#pragma unroll
+              for (int nq = 0; nq < NQ; ++nq) mma_f16(s[u][nq], ka, qf[nq][p * SP + 4 * i + j][0], qf[nq][p * SP + 4 * i + j][1]);
+            }
           }
         }
       }
-      const bool masked = wrong || (t << 4) + 16 > see_first;
       // log2 of a token's share of the softmax over 2^m (y), and of its weight of V (z)
-      uint32_t pb[NQ][2];
-      float f[NQ][2];
-      float y[NQ][4], z[NQ][4];
+      uint32_t pb[TP][NQ][2];
+      float y[TP][NQ][4], z[TP][NQ][4];
       bool over = false;
       auto exponents = [&]() {
 #pragma unroll
-        for (int nq = 0; nq < NQ; ++nq)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float mu = m[nq][e & 1], add = lv - w[nq][e & 1] + AT_BIAS;
-            y[nq][e] = fmaf(s[nq][e], f[nq][e & 1], -mu);
-            z[nq][e] = fmaf(s[nq][e], f[nq][e & 1], add);
-          }
-        if (masked) {
+        for (int u = 0; u < TP; ++u)
 #pragma unroll
           for (int nq = 0; nq < NQ; ++nq)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (wrong || (t << 4) + g + 8 * (e >> 1) >= sees(8 * nq + 2 * c + (e & 1))) y[nq][e] = z[nq][e] = -INFINITY;
+            for (int e = 0; e < 4; ++e) {
+              const float mu = m[nq][e & 1], add = lv[u] - w[nq][e & 1] + AT_BIAS;
+              y[u][nq][e] = fmaf(s[u][nq][e], f[u][nq][e & 1], -mu);
+              z[u][nq][e] = fmaf(s[u][nq][e], f[u][nq][e & 1], add);
+            }
+        if (any_masked) {
+#pragma unroll
+          for (int u = 0; u < TP; ++u)
+#pragma unroll
+            for (int nq = 0; nq < NQ; ++nq)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (wrong[u] || ((t0 + u) << 4) + g + 8 * (e >> 1) >= sees(8 * nq + 2 * c + (e & 1))) y[u][nq][e] = z[u][nq][e] = -INFINITY;
         }
       };
-#pragma unroll
-      for (int nq = 0; nq < NQ; ++nq) {
-        f[nq][0] = fq[nq][0] * kscale;
-        f[nq][1] = fq[nq][1] * kscale;
-      }
       exponents();
 #pragma unroll
-      for (int nq = 0; nq < NQ; ++nq)
+      for (int u = 0; u < TP; ++u)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) over |= y[nq][e] > AT_SLACK || z[nq][e] > AT_BIAS + AT_SLACK;
-      if (__any_sync(0xffffffffu, over)) {  // the first tile, and where the maxima move
+        for (int nq = 0; nq < NQ; ++nq)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) over |= y[u][nq][e] > AT_SLACK || z[u][nq][e] > AT_BIAS + AT_SLACK;
+      if (__any_sync(0xffffffffu, over)) {  // the first step, and where the maxima move
 #pragma unroll
         for (int nq = 0; nq < NQ; ++nq)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float top = -INFINITY;
+            float top = -INFINITY, topw = -INFINITY;
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              const bool see = !masked || (!wrong && (t << 4) + g + 8 * q < sees(8 * nq + 2 * c + e));
-              if (see) top = fmaxf(top, s[nq][2 * q + e] * f[nq][e]);
+            for (int u = 0; u < TP; ++u) {
+              float tu = -INFINITY;
+#pragma unroll
+              for (int q = 0; q < 2; ++q) {
+                const bool see = !any_masked || (!wrong[u] && ((t0 + u) << 4) + g + 8 * q < sees(8 * nq + 2 * c + e));
+                if (see) tu = fmaxf(tu, s[u][nq][2 * q + e] * f[u][nq][e]);
+              }
+              top = fmaxf(top, tu);
+              topw = fmaxf(topw, tu + lv[u]);
             }
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-            const float mn = fmaxf(m[nq][e], top), wn = fmaxf(w[nq][e], top + lv);
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) {
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+              topw = fmaxf(topw, __shfl_xor_sync(0xffffffffu, topw, x));
+            }
+            const float mn = fmaxf(m[nq][e], top), wn = fmaxf(w[nq][e], topw);
             l[nq][e] *= ex2(m[nq][e] - (mn == -INFINITY ? 0.0f : mn));
             const float shrink = ex2(w[nq][e] - (wn == -INFINITY ? 0.0f : wn));
             m[nq][e] = mn;
@@ -548,16 +585,19 @@ __global__ void __launch_bounds__(AtCfg<D, NQ>::NW * 32, 1) lss_attend_kernel(At
         exponents();
       }
 #pragma unroll
-      for (int nq = 0; nq < NQ; ++nq) {
-        l[nq][0] += ex2(y[nq][0]) + ex2(y[nq][2]);
-        l[nq][1] += ex2(y[nq][1]) + ex2(y[nq][3]);
-        const __half2 lo = __floats2half2_rn(ex2(z[nq][0]), ex2(z[nq][1])), hi = __floats2half2_rn(ex2(z[nq][2]), ex2(z[nq][3]));
-        pb[nq][0] = transpose8(*reinterpret_cast<const uint32_t*>(&lo));
-        pb[nq][1] = transpose8(*reinterpret_cast<const uint32_t*>(&hi));
-      }
+      for (int u = 0; u < TP; ++u)
+#pragma unroll
+        for (int nq = 0; nq < NQ; ++nq) {
+          l[nq][0] += ex2(y[u][nq][0]) + ex2(y[u][nq][2]);
+          l[nq][1] += ex2(y[u][nq][1]) + ex2(y[u][nq][3]);
+          const __half2 lo = __floats2half2_rn(ex2(z[u][nq][0]), ex2(z[u][nq][1])), hi = __floats2half2_rn(ex2(z[u][nq][2]), ex2(z[u][nq][3]));
+          pb[u][nq][0] = transpose8(*reinterpret_cast<const uint32_t*>(&lo));
+          pb[u][nq][1] = transpose8(*reinterpret_cast<const uint32_t*>(&hi));
+        }
 
       // weights times values: rows of the product are columns of V
-      const bool tail = wrong || (t << 4) + 16 > see_last;  // tokens that no query of the group sees
+#pragma unroll
+      for (int u = 0; u < TP; ++u)
 #pragma unroll
       for (int p = 0; p < NP; ++p) {
         uint32_t vw[4][PC / 32];  // tokens 2c, 2c+1, 2c+8, 2c+9; the lane's columns
@@ -565,22 +605,22 @@ __global__ void __launch_bounds__(AtCfg<D, NQ>::NW * 32, 1) lss_attend_kernel(At
         for (int r = 0; r < 4; ++r) {
           const int token = 2 * c + (r & 1) + 8 * (r >> 1);
           if constexpr (PC == 128) {
-            const uint4 v = lds128(vt + p * (16 * PC) + at_offset<PC>(token, g));
+            const uint4 v = lds128(kt[u] + 16 * D + p * (16 * PC) + at_offset<PC>(token, g));
             vw[r][0] = v.x;
             vw[r][1] = v.y;
             vw[r][2] = v.z;
             vw[r][3] = v.w;
           } else {
-            const uint2 v = lds64(vt + at_offset<PC>(token, g >> 1) + (g & 1) * 8);
+            const uint2 v = lds64(kt[u] + 16 * D + at_offset<PC>(token, g >> 1) + (g & 1) * 8);
             vw[r][0] = v.x;
             vw[r][1] = v.y;
           }
         }
-        if (masked) {
-          if (tail) {  // 0 times what lies there may be NaN
+        if (masked[u]) {
+          if (wrong[u] || ((t0 + u) << 4) + 16 > see_last) {  // tokens that no query of the group sees: 0 times what lies there may be NaN
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-              if (wrong || (t << 4) + 2 * c + (r & 1) + 8 * (r >> 1) >= see_last) {
+              if (wrong[u] || ((t0 + u) << 4) + 2 * c + (r & 1) + 8 * (r >> 1) >= see_last) {
 #pragma unroll
                 for (int i = 0; i < PC / 32; ++i) vw[r][i] = 0u;
               }
@@ -609,7 +649,7 @@ __global__ void __launch_bounds__(AtCfg<D, NQ>::NW * 32, 1) lss_attend_kernel(At
                 const uint32_t na[4] = {f16_of_e4m3(n0), f16_of_e4m3(n0 >> 16), f16_of_e4m3(n1), f16_of_e4m3(n1 >> 16)};
 #pragma unroll
                 for (int nq = 0; nq < NQ; ++nq) {
-                  const int lim = sees(8 * nq + g), tk = (t << 4) + 2 * c;
+                  const int lim = sees(8 * nq + g), tk = ((t0 + u) << 4) + 2 * c;
                   float count[4] = {};
                   mma_f16(count, na, (tk < lim ? 0x3c00u : 0u) | (tk + 1 < lim ? 0x3c000000u : 0u),
                           (tk + 8 < lim ? 0x3c00u : 0u) | (tk + 9 < lim ? 0x3c000000u : 0u));
@@ -629,7 +669,7 @@ __global__ void __launch_bounds__(AtCfg<D, NQ>::NW * 32, 1) lss_attend_kernel(At
             const uint32_t t0 = __byte_perm(vw[0][i], vw[1][i], sel), t1 = __byte_perm(vw[2][i], vw[3][i], sel);
             const uint32_t va[4] = {f16_of_e4m3(t0), f16_of_e4m3(t0 >> 16), f16_of_e4m3(t1), f16_of_e4m3(t1 >> 16)};
 #pragma unroll
-            for (int nq = 0; nq < NQ; ++nq) mma_f16(o[p * SP + 2 * i + q][nq], va, pb[nq][0], pb[nq][1]);
+            for (int nq = 0; nq < NQ; ++nq) mma_f16(o[p * SP + 2 * i + q][nq], va, pb[u][nq][0], pb[u][nq][1]);
           }
       }
     }  // the next tile's __syncwarp lets its place be written again
@@ -745,7 +785,7 @@ __global__ void __launch_bounds__(AtCfg<D, NQ>::NW * 32, 1) lss_attend_kernel(At
     if (lane == 0) w_last[warp] = join;
     __syncthreads();
     for (int i = 0; i < NW; ++i)
-      if (w_last[i].z > 0) at_join_cut<D, DT, NQ>(a, first_w + i, w_last[i], tid, NTH);
+      if (w_last[i].z > 0) at_join_cut<D, DT, NQ, TP>(a, first_w + i, w_last[i], tid, NTH);
   } else if (lane == 0) {
     a.meta[worker] = join;
   }
@@ -753,11 +793,11 @@ __global__ void __launch_bounds__(AtCfg<D, NQ>::NW * 32, 1) lss_attend_kernel(At
 
 // Adds up the pieces of the groups that were cut between CTAs: one CTA per warp of the first kernel,
 // most with nothing to do.
-template <int D, int DT, int NQ>
+template <int D, int DT, int NQ, int TP>
 __global__ void __launch_bounds__(256) lss_attend_join_kernel(AttendArgs a) {
   pdl_wait();
   const int4 me = a.meta[blockIdx.x];
-  if (me.z > 0) at_join_cut<D, DT, NQ>(a, blockIdx.x, me, threadIdx.x, 256);
+  if (me.z > 0) at_join_cut<D, DT, NQ, TP>(a, blockIdx.x, me, threadIdx.x, 256);
 }
 
 }  // namespace lss

@@ -100,19 +100,19 @@ static bool table_ok(const void* table, int64_t stride, int width, int B, int bs
 // ---------------------------------------------------------------- attention
 static constexpr int AT_CAP_CTAS = 160;  // CTAs that the workspace has room for
 
-template <int D, int NQ>
+template <int D, int NQ, int TP>
 static size_t attend_bytes() {
-  const size_t workers = (size_t)AT_CAP_CTAS * AtCfg<D, NQ>::NW;
+  const size_t workers = (size_t)AT_CAP_CTAS * AtCfg<D, NQ, TP>::NW;
   return workers * (sizeof(int4) + 2 * at_piece(D, NQ) * sizeof(float));
 }
 
-template <int D, int DT, int NQ>
+template <int D, int DT, int NQ, int TP = 1>
 static cudaError_t launch_attend(AttendArgs a, void* ws, cudaStream_t st) {
   static SmemSet set;
   const int dev = device_index();
-  constexpr int NW = AtCfg<D, NQ>::NW;
-  constexpr int smem = NW * AtCfg<D, NQ>::ST * (32 * D + 16);
-  cudaError_t e = allow_smem(lss_attend_kernel<D, DT, NQ>, set, dev, smem);
+  constexpr int NW = AtCfg<D, NQ, TP>::NW;
+  constexpr int smem = NW * AtCfg<D, NQ, TP>::ST * (32 * D + 16);
+  cudaError_t e = allow_smem(lss_attend_kernel<D, DT, NQ, TP>, set, dev, smem);
   if (e != cudaSuccess) return e;
   // No more warps than there can be units.
   const int64_t groups = a.B + (int64_t)a.T * a.per / (8 * NQ) + 1;
@@ -125,11 +125,11 @@ static cudaError_t launch_attend(AttendArgs a, void* ws, cudaStream_t st) {
   a.fused = units <= 8 * NW * 2;
   if (a.fused) {
     const int size = ctas <= 1 ? 1 : ctas <= 2 ? 2 : ctas <= 4 ? 4 : 8;
-    return launch(lss_attend_kernel<D, DT, NQ>, (unsigned)size, NW * 32, smem, size, false, st, a);
+    return launch(lss_attend_kernel<D, DT, NQ, TP>, (unsigned)size, NW * 32, smem, size, false, st, a);
   }
-  e = launch(lss_attend_kernel<D, DT, NQ>, (unsigned)ctas, NW * 32, smem, 1, false, st, a);
+  e = launch(lss_attend_kernel<D, DT, NQ, TP>, (unsigned)ctas, NW * 32, smem, 1, false, st, a);
   if (e != cudaSuccess) return e;
-  return launch(lss_attend_join_kernel<D, DT, NQ>, (unsigned)(ctas * NW), 256, 0, 1, true, st, a);
+  return launch(lss_attend_join_kernel<D, DT, NQ, TP>, (unsigned)(ctas * NW), 256, 0, 1, true, st, a);
 }
 
 template <int D>
@@ -157,7 +157,13 @@ static cudaError_t launch_attend_tc(AttendArgs a, void* ws, cudaStream_t st) {
 template <int D, int DT>
 static cudaError_t launch_attend_rows(const AttendArgs& a, void* ws, cudaStream_t st) {
   const int64_t rows = (int64_t)a.per * ((a.T + (int64_t)a.B - 1) / a.B);
-  if (rows <= 8) return launch_attend<D, DT, 1>(a, ws, st);
+  if (rows <= 8) {
+    // Long contexts take two tiles a step (AtCfg); how long they are only the table's width tells here.
+    if constexpr (D == 128) {
+      if (((int64_t)a.width << a.bs_shift) >= 1024) return launch_attend<D, DT, 1, 2>(a, ws, st);
+    }
+    return launch_attend<D, DT, 1>(a, ws, st);
+  }
   if constexpr (D < 256) {
     if (rows >= 128 && (int64_t)a.heads * a.per * a.T >= (int64_t)PA_ROWS * sm_count(device_index()) / 4) return launch_attend_tc<D, DT>(a, ws, st);
     if (rows > 16) return launch_attend<D, DT, 4>(a, ws, st);
@@ -415,9 +421,9 @@ int lss_kv_append(const void* k, int64_t k_token_stride, int64_t k_head_stride, 
 
 size_t lss_attend_workspace_bytes(int dim) {
   switch (dim) {
-    case 64: return std::max({attend_bytes<64, 1>(), attend_bytes<64, 2>(), attend_bytes<64, 4>(), attend_tc_bytes<64>()});
-    case 128: return std::max({attend_bytes<128, 1>(), attend_bytes<128, 2>(), attend_bytes<128, 4>(), attend_tc_bytes<128>()});
-    case 256: return std::max(attend_bytes<256, 1>(), attend_bytes<256, 2>());
+    case 64: return std::max({attend_bytes<64, 1, 1>(), attend_bytes<64, 2, 1>(), attend_bytes<64, 4, 1>(), attend_tc_bytes<64>()});
+    case 128: return std::max({attend_bytes<128, 1, 1>(), attend_bytes<128, 1, 2>(), attend_bytes<128, 2, 1>(), attend_bytes<128, 4, 1>(), attend_tc_bytes<128>()});
+    case 256: return std::max(attend_bytes<256, 1, 1>(), attend_bytes<256, 2, 1>());
     default: return 0;
   }
 }
