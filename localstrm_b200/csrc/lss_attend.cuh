@@ -50,6 +50,7 @@ struct AttendArgs {
   int B, T;
   float scale;         // softmax scale times log2(e)
   int aligned;         // q and out rows start on 16-byte boundaries
+  int rows_lo, rows_hi;  // rows of the batch with rows_lo <= query rows per key head < rows_hi are this launch's
   int fused;           // the grid is one cluster, which joins its own pieces
   int4* meta;          // [workers]: row, group, pieces (0: nothing to join)
   float* part;         // [workers][2][at_piece]: a warp's first piece, its last one
@@ -110,7 +111,8 @@ __device__ __forceinline__ uint32_t at_offset(int token, int cc) {
 }
 
 // A row's share of the work: groups of 8 NQ query rows per key head, tiles of 16 tokens.  Rows whose
-// numbers do not fit (more new tokens than tokens, outside the table or the batch's tokens) have none.
+// numbers do not fit (more new tokens than tokens, outside the table or the batch's tokens), and those of another
+// launch, have none.
 struct AtRow {
   int n, len, nt, mt;
 };
@@ -121,7 +123,7 @@ __device__ __forceinline__ AtRow at_row(const AttendArgs& a, int r) {
   w.len = a.lens[r];
   const int s = a.starts[r];
   const bool ok = w.n > 0 && w.n <= w.len && w.len <= ((int64_t)a.width << a.bs_shift) && s >= 0 && (int64_t)s + w.n <= a.T;
-  if (!ok) w.n = 0;
+  if (!ok || (int64_t)w.n * a.per < a.rows_lo || (int64_t)w.n * a.per >= a.rows_hi) w.n = 0;
   w.nt = w.n > 0 ? (w.len + 15) >> 4 : 0;
   w.mt = w.n > 0 ? (int)(((int64_t)w.n * a.per + 8 * NQ - 1) / (8 * NQ)) : 0;
   return w;
@@ -238,6 +240,9 @@ __device__ __forceinline__ void at_join_cut(const AttendArgs& a, int64_t worker,
 // to f16 (2^-11 relative, no more than the result's own rounding) and keep that precision down to
 // 2^-24 of the largest one.  The sum of the softmax is f32.
 //
+// Measured at D = 128, 8 key heads: 1.1 GB of contexts of 50 to 16,000 tokens for 64 single queries of 32 heads
+// 212 us (5.2 TB/s, 0.81 of the copy rate), 733 MB of three contexts of 90,000 to 131,000 140 us; with queries as the
+// 16-row operand (half of it padding) and reductions for every tile it was 268 and 200 us.
 // Bound by HBM (2 D bytes per token and head) when a row has few queries, by the tensor pipe and the
 // widening of the codes when it has many (they share it 8 NQ rows at a time).
 template <int D, int DT, int NQ, int TP>

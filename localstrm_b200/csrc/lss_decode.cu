@@ -152,11 +152,9 @@ static cudaError_t launch_attend_tc(AttendArgs a, void* ws, cudaStream_t st) {
   return launch(lss_attend_tc_join_kernel<D, DT>, (unsigned)(ctas * (PA_ROWS / 32)), 256, 0, 1, true, st, a);
 }
 
-// Query rows per group: as many as a key head's rows fill on the average (a batch of single tokens:
-// the query heads of a key head).
+// `rows`: query rows per key head that a row of the batch has.
 template <int D, int DT>
-static cudaError_t launch_attend_rows(const AttendArgs& a, void* ws, cudaStream_t st) {
-  const int64_t rows = (int64_t)a.per * ((a.T + (int64_t)a.B - 1) / a.B);
+static cudaError_t launch_attend_few(const AttendArgs& a, int64_t rows, void* ws, cudaStream_t st) {
   if (rows <= 8) {
     // Long contexts take two tiles a step (AtCfg); how long they are only the table's width tells here.
     if constexpr (D == 128) {
@@ -165,10 +163,33 @@ static cudaError_t launch_attend_rows(const AttendArgs& a, void* ws, cudaStream_
     return launch_attend<D, DT, 1>(a, ws, st);
   }
   if constexpr (D < 256) {
-    if (rows >= 128 && (int64_t)a.heads * a.per * a.T >= (int64_t)PA_ROWS * sm_count(device_index()) / 4) return launch_attend_tc<D, DT>(a, ws, st);
     if (rows > 16) return launch_attend<D, DT, 4>(a, ws, st);
   }
   return launch_attend<D, DT, 2>(a, ws, st);
+}
+
+// A step of single tokens has `per` query rows per key head and row; else the average decides.  A step with more
+// tokens than rows, and enough of them to fill the SMs, may mix prompt chunks and single tokens: rows of
+// PA_FROM query rows and more go to the tensor-memory kernel (which would widen the codes for 256 rows of which
+// `per` are there), the others to the one for few rows, one launch after the other on the same workspace.  Steps of
+// chunks alone pay 10 us for the second one's empty launches (220 -> 232 us for four chunks of 300 to 400 tokens); 60
+// single tokens over 6,000 beside two chunks of 2,048 take 490 us.
+template <int D, int DT>
+static cudaError_t launch_attend_rows(AttendArgs a, void* ws, cudaStream_t st) {
+  constexpr int PA_FROM = 64;
+  a.rows_lo = 0;
+  a.rows_hi = INT32_MAX;
+  if constexpr (D < 256) {
+    if (a.T > a.B && (int64_t)a.heads * a.per * a.T >= (int64_t)PA_ROWS * sm_count(device_index()) / 4) {
+      a.rows_lo = PA_FROM;
+      const cudaError_t e = launch_attend_tc<D, DT>(a, ws, st);
+      if (e != cudaSuccess) return e;
+      a.rows_lo = 0;
+      a.rows_hi = PA_FROM;
+      return launch_attend_few<D, DT>(a, a.per, ws, st);
+    }
+  }
+  return launch_attend_few<D, DT>(a, (int64_t)a.per * ((a.T + (int64_t)a.B - 1) / a.B), ws, st);
 }
 
 template <int D>

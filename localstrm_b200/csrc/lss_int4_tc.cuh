@@ -125,6 +125,9 @@ __global__ void __launch_bounds__(256) lss_int4_operand_kernel(Int4Args a, int r
 // scales them in f32 and adds them up in registers.  The codes never go to shared memory as 16-bit
 // values, whose bandwidth (128 B per cycle and SM) could not carry them at the rate of HBM.  The teams drift
 // apart by up to XS - 1 units, so that the widening of one overlaps the products of another.
+// Measured, 128,256 x 4096, groups of 128, bf16: 64 rows 120 us, 16 rows 86 us (lss_int4_kernel eight rows at a
+// time: 591 and 164 us).  Bound by the instructions of the widening, as there, and by the last wave: a
+// CTA's four row blocks at a time divide 1,002 into 1.7 waves of 148.
 // Tensor memory: 64 columns of left operand and 64 of sums per team, all 512.
 // A range of columns per CTA (ks of them) where there are few row blocks; lss_int4_sum_kernel adds up.
 template <int DT, int SPG, int NR>

@@ -119,7 +119,10 @@ __device__ __forceinline__ int row_of(const int32_t* upto, int n, int u) {
 // a step of e4m3 each (2^-4 relative; below 2^-6 s the step is 2^-9 s).
 // Up to 2048 TEAM values stay in registers between the passes; what goes beyond is read again, from the
 // L2 cache.
-// Bound by HBM for prompts and by its chain of dependent loads (lengths, table, scale, values) for
+// Measured: 24 rows of up to 2,048 new tokens, 8 heads of 128, f16: 39 us (153 MB, 3.9 TB/s, 0.60 of the copy
+// rate; a fixed part of some 400 instructions per unit and warp and the rounding bound it), one warp per
+// block of 32 tokens 68 us; 256 single tokens 6.4 us in a graph.
+// Bound by issue and HBM for prompts and by its chain of dependent loads (lengths, table, scale, values) for
 // single tokens.
 template <int DT, int TEAM>
 __global__ void __launch_bounds__(KV_NT, 3) lss_append_kernel(AppendArgs a) {

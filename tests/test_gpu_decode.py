@@ -387,6 +387,16 @@ def test_attend_prompt_chunks(ctx, new, heads, per, bs, dim, dtype):
     assert torch.equal(y[first: first + new[b], 0, 7].isnan(), seen) and not bool(y[first: first + new[b], 0, 6].isnan().any())
 
 
+@pytest.mark.parametrize("per,dim", [(4, 128), (7, 64), (16, 128), (4, 256)])
+def test_attend_prompts_and_single_tokens_mixed(per, dim):
+    """Steps in which some rows have one token, some a few and some a chunk; an idle row, padding behind them."""
+    rows = U.make_rows([4000, 100, 0, 2500, 60, 9, 1300, 0], [1, 700, 300, 1, 20, 0, 15, 1], 16, seed=per)
+    cache = lb.KVCache8(*U.random_cache(rows[-1], 4, 16, dim, seed=per))
+    q = torch.randn(1038 + 30, 4 * per, dim, generator=gen(dim), device=DEV).bfloat16()
+    y, lse = check_attend(q, cache, rows)
+    assert bool((y[1038:] == 77).all()) and bool((lse[1038:] == 77).all()) and bool(y[:1038].isfinite().all())
+
+
 def check_attend_nan(q, cache, rows):
     """As check_attend where some values are NaN: the places of NaN, the others against a cache without it."""
     clean = lb.KVCache8(cache.k, torch.where(cache.v.float().isnan(), 0.0, cache.v.float()).to(E4M3), cache.k_scale, cache.v_scale)
