@@ -223,7 +223,7 @@ int lss_read_row_paths(const void* workspace, int B, int32_t* paths_out, void* s
  * The decode step around the sampler: the 4-bit vocabulary projection that makes the logits, the
  * block tables and slot maps of a paged key/value cache, its 8-bit form, and the attention that
  * reads it.  LocalStrm runs these as eager torch code (src/kernels/quantization.py,
- * src/memory/block_manager.py, src/kernels/paged_attention.py); the formats below are this
+ * src/memory/, src/kernels/paged_attention.py); the formats below are this
  * library's own.  All pointers are device pointers, all calls are asynchronous on `stream`.
  * ------------------------------------------------------------------------------------------ */
 

@@ -4,8 +4,8 @@ A step runs ``plan_blocks`` (a place for every request's new tokens), ``append_k
 values, in 8 bits with one scale per block and head) and ``attend`` per layer; after sampling,
 ``release_blocks`` takes the codes of ``check_stop_batch`` and returns the blocks of the requests
 that stopped.  Everything stays on the device: no call reads a length back, so a step can be
-captured in a CUDA graph.  LocalStrm's counterparts are the host-side ``BlockManager``
-(``src/memory/block_manager.py``) and the gather + SDPA of ``src/kernels/paged_attention.py``.
+captured in a CUDA graph.  LocalStrm's counterparts are the host-side block manager
+(``src/memory/``) and the gather + SDPA of ``src/kernels/paged_attention.py``.
 """
 from __future__ import annotations
 
