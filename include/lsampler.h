@@ -234,12 +234,11 @@ int lss_read_row_paths(const void* workspace, int B, int32_t* paths_out, void* s
  *            16-byte aligned
  *   scales   [N][K / group], dtype LSS_DTYPE_BF16 or LSS_DTYPE_F16; group: 32, 64 or a multiple of 128
  *            that divides K
- *   y        [rows] x [y_stride elements], dtype LSS_DTYPE_*
- *   workspace  lss_int4_workspace_bytes(rows, K, x_dtype, N) bytes (0 for up to eight rows: NULL will do),
- *              16-byte aligned, of this call alone until it is done
- * LSS_ERR_UNSUPPORTED for up to eight rows when one row of x does not fit the shared memory of an SM (K
- * beyond 49,152 for 16-bit x, 16,384 for f32).  A wait inside the kernel for more than eight rows that gives
- * up after about a second leaves NaN in y. */
+ *   y        [rows] x [y_stride elements], dtype LSS_DTYPE_*; shares no memory with x
+ *   workspace  lss_int4_workspace_bytes(rows, K, x_dtype, N) bytes, 16-byte aligned, of this call alone until
+ *              it is done.  0 (NULL will do) for up to eight rows of K up to 49,152 (f32: 16,384) columns;
+ *              longer rows may take the kernel for more than eight
+ * A wait inside the kernel for more than eight rows that gives up after about a second leaves NaN in y. */
 size_t lss_int4_workspace_bytes(int rows, int K, int x_dtype, int N);
 int lss_int4_matvec(const void* x, int x_dtype, int rows, int K, int64_t x_stride, const uint8_t* packed,
                     const void* scales, int scale_dtype, int N, int group, void* y, int y_dtype,
@@ -260,7 +259,7 @@ int lss_int4_matvec(const void* x, int x_dtype, int rows, int K, int64_t x_strid
  *   positions   int32 [capacity]: the token's position in its row; 0 behind the last token
  *   starts      int32 [B + 1], at most capacity
  *   granted     int32 [B]: new_lens[b] or 0
- *   lens_out    int32 [B]: lens + granted; may be `lens` itself
+ *   lens_out    int32 [B]: lens + granted; may be `lens` itself (overlapping it in part: LSS_ERR_INVALID_ARG)
  *   n_free_out  int32 [1]; may be `n_free` itself
  * lss_block_release returns the blocks of the rows with codes[b] != 0 (lss_stop_check's codes) to
  * the free list, in row and block order, and sets their lengths to 0.

@@ -80,6 +80,17 @@ static int status_of(cudaError_t e) {
 static bool aligned_to(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 static bool known_dtype(int d) { return d == LSS_DTYPE_F32 || d == LSS_DTYPE_BF16 || d == LSS_DTYPE_F16; }
 static bool block_size_ok(int bs) { return bs == 16 || bs == 32 || bs == 64 || bs == 128 || bs == 256; }
+// Rows of two matrices (start, bytes between rows, bytes of a row) that share memory.  Rows of one pitch may lie
+// beside each other.
+static bool rows_overlap(const void* x, int64_t x_pitch, int64_t x_row, const void* y, int64_t y_pitch, int64_t y_row, int rows) {
+  const int64_t d = (int64_t)(reinterpret_cast<intptr_t>(y) - reinterpret_cast<intptr_t>(x));
+  if (d >= (rows - 1) * x_pitch + x_row || -d >= (rows - 1) * y_pitch + y_row) return false;
+  if (rows == 1 || x_pitch != y_pitch) return true;
+  const int64_t at = (d % x_pitch + x_pitch) % x_pitch;  // where y's rows start in x's pitch
+  return at < x_row || at + y_row > x_pitch;
+}
+// Arrays of n entries of which one begins inside the other.
+static bool cut(const int32_t* x, const int32_t* y, int64_t n) { return x != y && x < y + n && y < x + n; }
 static int log2_of(int v) {
   int s = 0;
   while ((1 << s) < v) ++s;
@@ -200,48 +211,48 @@ static cudaError_t launch_attend_dt(int dtype, const AttendArgs& a, void* ws, cu
 // ---------------------------------------------------------------- 4-bit products
 static constexpr int I4_SMEM = 227 * 1024;
 
-template <int DT, int SPG>
-static cudaError_t launch_int4(const Int4Args& a, cudaStream_t st, bool& fits) {
-  static SmemSet set;
-  const int dev = device_index(), sms = sm_count(dev);
-  constexpr int planes = DT == LSS_DTYPE_F32 ? 3 : 1;
-  constexpr int fixed = I4_NW * I4_ST * (I4_RB * I4_KB / 2) + I4_NW * 2 * I4_SUMS * 4;
-  const int NB = (a.N + I4_RB - 1) / I4_RB, KB = (a.K + I4_KB - 1) / I4_KB;
-  // CTAs per row block range: the split with the fewest units in the fullest CTA.  A cluster's
-  // exchange costs about as much as 8 units, and its row blocks' sums take 16 KB at most.
-  int ks = 1, nclusters = std::min(NB, sms);
+// Split of lss_int4_kernel: CTAs per row block range (ks), ranges, rows of x that a launch's shared memory takes (0:
+// not even one in any split).  The split with the fewest units in the fullest CTA; a cluster's exchange costs about
+// as much as 8 units, and its row blocks' sums take 16 KB at most.
+struct I4Plan {
+  int ks, nclusters, sums, most;  // sums: bytes of the row blocks' sums
+};
+static constexpr int I4_FIXED = I4_NW * I4_ST * (I4_RB * I4_KB / 2) + I4_NW * 2 * I4_SUMS * 4;
+static I4Plan i4_plan(int N, int K, int planes, int sms) {
+  const int NB = (N + I4_RB - 1) / I4_RB, KB = (K + I4_KB - 1) / I4_KB;
+  I4Plan p{1, 0, 0, 0};
   int64_t best = INT64_MAX;
   for (int k = 1; k <= 8 && k <= KB; k <<= 1) {
-    const int nc = std::min(NB, std::max(1, sms / k));
-    const int nrb = (NB + nc - 1) / nc;
+    const int nc = std::min(NB, std::max(1, sms / k)), nrb = (NB + nc - 1) / nc, units = (KB + k - 1) / k;
     if (k > 1 && nrb > 16) continue;
-    const int64_t cost = (int64_t)nrb * ((KB + k - 1) / k) + (k > 1 ? 8 : 0);
-    if (cost < best) {
+    const int sums = k > 1 ? nrb * I4_SUMS * 4 : 0;
+    const int64_t most = (I4_SMEM - I4_FIXED - sums) / ((int64_t)units * I4_KB * 2 * planes);
+    const int64_t cost = (int64_t)nrb * units + (k > 1 ? 8 : 0);
+    if (most >= 1 && cost < best) {
       best = cost;
-      ks = k;
-      nclusters = nc;
+      p = I4Plan{k, nc, sums, (int)std::min((int64_t)I4_ROWS, most)};
     }
   }
-  auto room = [&](int k) {  // rows of x that fit
-    const int nc = std::min(NB, std::max(1, sms / k));
-    const int left = I4_SMEM - fixed - (k > 1 ? (NB + nc - 1) / nc * I4_SUMS * 4 : 0);
-    return left / (((KB + k - 1) / k) * I4_KB * 2 * planes);
-  };
-  fits = room(ks) >= 1;
-  if (!fits) return cudaSuccess;
-  const int most = std::min(I4_ROWS, room(ks));
-  for (int r0 = 0; r0 < a.rows; r0 += most) {
-    const int rows = std::min(most, a.rows - r0);
-    const int smem = fixed + (ks > 1 ? (NB + nclusters - 1) / nclusters * I4_SUMS * 4 : 0) + rows * ((KB + ks - 1) / ks) * I4_KB * 2 * planes;
-    cudaError_t e = allow_smem(lss_int4_kernel<DT, SPG>, set, dev, smem);
+  return p;
+}
+
+template <int DT, int SPG>
+static cudaError_t launch_int4(const Int4Args& a, const I4Plan& p, cudaStream_t st) {
+  static SmemSet set;
+  constexpr int planes = DT == LSS_DTYPE_F32 ? 3 : 1;
+  const int KB = (a.K + I4_KB - 1) / I4_KB;
+  for (int r0 = 0; r0 < a.rows; r0 += p.most) {
+    const int rows = std::min(p.most, a.rows - r0);
+    const int smem = I4_FIXED + p.sums + rows * ((KB + p.ks - 1) / p.ks) * I4_KB * 2 * planes;
+    cudaError_t e = allow_smem(lss_int4_kernel<DT, SPG>, set, device_index(), smem);
     if (e != cudaSuccess) return e;
-    e = launch(lss_int4_kernel<DT, SPG>, (unsigned)(nclusters * ks), I4_NT, smem, ks, false, st, a, r0, rows, ks);
+    e = launch(lss_int4_kernel<DT, SPG>, (unsigned)(p.nclusters * p.ks), I4_NT, smem, p.ks, false, st, a, r0, rows, p.ks);
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;
 }
 
-// Nine rows and more: the tensor-memory kernel, 64 rows of x at a time.
+// Nine rows and more, and rows of x too long for shared memory: the tensor-memory kernel, 64 rows of x at a time.
 struct TcPlan {
   int blocks, ks;  // row blocks (teams) and column slices: teams on all SMs first, then slices
   size_t xop, part;
@@ -275,18 +286,13 @@ static cudaError_t launch_int4_tc(const Int4Args& a, int row0, int rows, const T
 }
 
 template <int DT, int SPG>
-static cudaError_t launch_int4_rows(const Int4Args& a, void* ws, size_t ws_bytes, cudaStream_t st, int& status) {
+static cudaError_t launch_int4_rows(const Int4Args& a, void* ws, cudaStream_t st) {
+  const int sms = sm_count(device_index());
   if (a.rows <= I4_ROWS) {
-    bool fits = true;
-    const cudaError_t e = launch_int4<DT, SPG>(a, st, fits);
-    if (!fits) status = LSS_ERR_UNSUPPORTED;
-    return e;
+    const I4Plan p = i4_plan(a.N, a.K, DT == LSS_DTYPE_F32 ? 3 : 1, sms);
+    if (p.most > 0) return launch_int4<DT, SPG>(a, p, st);
   }
-  const TcPlan p = tc_plan(a.rows, a.N, a.K, DT, sm_count(device_index()));
-  if (!ws || ws_bytes < p.xop + p.part || !aligned_to(ws, 16)) {
-    status = LSS_ERR_WORKSPACE;
-    return cudaSuccess;
-  }
+  const TcPlan p = tc_plan(a.rows, a.N, a.K, DT, sms);
   unsigned char* w = reinterpret_cast<unsigned char*>(ws);
   for (int r0 = 0; r0 < a.rows; r0 += 64) {
     const int rows = std::min(64, a.rows - r0);
@@ -299,17 +305,19 @@ static cudaError_t launch_int4_rows(const Int4Args& a, void* ws, size_t ws_bytes
 }
 
 template <int DT>
-static cudaError_t launch_int4_group(const Int4Args& a, void* ws, size_t ws_bytes, cudaStream_t st, int& status) {
-  if (a.group == 32) return launch_int4_rows<DT, 1>(a, ws, ws_bytes, st, status);
-  if (a.group == 64) return launch_int4_rows<DT, 2>(a, ws, ws_bytes, st, status);
-  return launch_int4_rows<DT, 4>(a, ws, ws_bytes, st, status);
+static cudaError_t launch_int4_group(const Int4Args& a, void* ws, cudaStream_t st) {
+  if (a.group == 32) return launch_int4_rows<DT, 1>(a, ws, st);
+  if (a.group == 64) return launch_int4_rows<DT, 2>(a, ws, st);
+  return launch_int4_rows<DT, 4>(a, ws, st);
 }
 
 extern "C" {
 
 size_t lss_int4_workspace_bytes(int rows, int K, int x_dtype, int N) {
-  if (rows <= I4_ROWS || K < 1 || N < 1) return 0;
-  const TcPlan p = tc_plan(rows, N, K, x_dtype, sm_count(device_index()));
+  if (rows < 1 || K < 1 || N < 1) return 0;
+  const int sms = sm_count(device_index());
+  if (rows <= I4_ROWS && i4_plan(N, K, x_dtype == LSS_DTYPE_F32 ? 3 : 1, sms).most > 0) return 0;
+  const TcPlan p = tc_plan(rows, N, K, x_dtype, sms);
   return p.xop + p.part;
 }
 
@@ -322,6 +330,10 @@ int lss_int4_matvec(const void* x, int x_dtype, int rows, int K, int64_t x_strid
   if ((group != 32 && group != 64 && (group < 128 || group % 128 != 0)) || K % group != 0) return LSS_ERR_INVALID_ARG;
   if (rows == 0) return LSS_OK;
   if (!x || !packed || !scales || !y || !aligned_to(packed, 16) || !aligned_to(scales, 2)) return LSS_ERR_INVALID_ARG;
+  const size_t need = lss_int4_workspace_bytes(rows, K, x_dtype, N);
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned_to(workspace, 16))) return LSS_ERR_WORKSPACE;
+  const int64_t xe = x_dtype == LSS_DTYPE_F32 ? 4 : 2, ye = y_dtype == LSS_DTYPE_F32 ? 4 : 2;
+  if (rows_overlap(x, x_stride * xe, K * xe, y, y_stride * ye, N * ye, rows)) return LSS_ERR_INVALID_ARG;
   Int4Args a{};
   a.x = x;
   a.x_stride = x_stride;
@@ -337,14 +349,13 @@ int lss_int4_matvec(const void* x, int x_dtype, int rows, int K, int64_t x_strid
   a.y_stride = y_stride;
   a.x_aligned = aligned_to(x, 16) && x_stride % 8 == 0;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  int status = LSS_OK;
   cudaError_t e;
   switch (x_dtype) {
-    case LSS_DTYPE_F32: e = launch_int4_group<LSS_DTYPE_F32>(a, workspace, workspace_bytes, st, status); break;
-    case LSS_DTYPE_BF16: e = launch_int4_group<LSS_DTYPE_BF16>(a, workspace, workspace_bytes, st, status); break;
-    default: e = launch_int4_group<LSS_DTYPE_F16>(a, workspace, workspace_bytes, st, status); break;
+    case LSS_DTYPE_F32: e = launch_int4_group<LSS_DTYPE_F32>(a, workspace, st); break;
+    case LSS_DTYPE_BF16: e = launch_int4_group<LSS_DTYPE_BF16>(a, workspace, st); break;
+    default: e = launch_int4_group<LSS_DTYPE_F16>(a, workspace, st); break;
   }
-  return e != cudaSuccess ? status_of(e) : status;
+  return status_of(e);
 }
 
 int lss_block_plan(int32_t* table, int64_t table_stride, int width, const int32_t* lens,
@@ -356,6 +367,7 @@ int lss_block_plan(int32_t* table, int64_t table_stride, int width, const int32_
   if (!free_blocks || !n_free || !starts || !n_free_out) return LSS_ERR_INVALID_ARG;
   if (B > 0 && (!lens || !new_lens || !granted || !lens_out)) return LSS_ERR_INVALID_ARG;
   if (capacity > 0 && (!slots || !positions)) return LSS_ERR_INVALID_ARG;
+  if (cut(lens_out, lens, B) || cut(lens_out, new_lens, B)) return LSS_ERR_INVALID_ARG;
   PlanArgs a{table, table_stride, width, lens, new_lens, B, block_size, num_blocks, capacity, free_blocks,
              n_free, slots, positions, starts, granted, lens_out, n_free_out};
   static SmemSet set;
@@ -365,7 +377,7 @@ int lss_block_plan(int32_t* table, int64_t table_stride, int width, const int32_
     if (e != cudaSuccess) return status_of(e);
   }
   const int64_t want = ((int64_t)capacity + BL_NT - 1) / BL_NT;
-  const bool in_place = n_free_out == n_free || (lens_out < lens + B && lens < lens_out + B);
+  const bool in_place = n_free_out == n_free || lens_out == lens || lens_out == new_lens;
   const int ctas = in_place ? cluster_for(want, BL_MAXCL) : (int)std::max((int64_t)1, std::min(want, (int64_t)sm_count(dev)));
   return status_of(launch(lss_plan_kernel, (unsigned)ctas, BL_NT, (size_t)smem, in_place ? ctas : 1, false,
                           reinterpret_cast<cudaStream_t>(stream), a));
@@ -378,6 +390,7 @@ int lss_block_release(const int32_t* table, int64_t table_stride, int width, con
   if (B > LSS_BLOCK_MAX_ROWS) return LSS_ERR_UNSUPPORTED;
   if (!free_blocks || !n_free || !n_free_out) return LSS_ERR_INVALID_ARG;
   if (B > 0 && (!lens || !codes || !lens_out)) return LSS_ERR_INVALID_ARG;
+  if (cut(lens_out, lens, B) || cut(lens_out, codes, B)) return LSS_ERR_INVALID_ARG;
   ReleaseArgs a{table, table_stride, width, lens, codes, B, block_size, num_blocks, free_blocks, n_free, lens_out, n_free_out};
   static SmemSet set;
   const int dev = device_index(), smem = 4 * B;

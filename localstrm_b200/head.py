@@ -75,7 +75,7 @@ class Int4Weight:
 def int4_matvec(x: torch.Tensor, weight: Int4Weight, out_dtype: Optional[torch.dtype] = None,
                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``x @ W.T`` for ``x [rows, K]`` or ``[K]`` (f32, bf16 or f16), sums in f32, one rounding to
-    ``out_dtype`` (default: x's).  One pass over the matrix serves 64 rows."""
+    ``out_dtype`` (default: x's).  One pass over the matrix serves 64 rows.  ``out`` shares no memory with x."""
     _require_cuda(x)
     packed, scales = weight.packed, weight.scales
     shape, dev = x.shape, x.get_device()
@@ -121,8 +121,9 @@ def int4_matvec(x: torch.Tensor, weight: Int4Weight, out_dtype: Optional[torch.d
     lib = _lib.load()
     with _on(dev):
         ws, size = None, 0
-        if rows > 8:  # from torch's allocator for every call: other streams and captured calls have their own
+        if rows > 8 or k > 16384:
             size = lib.lss_int4_workspace_bytes(rows, k, _CODES[x.dtype], n)
+            # From torch's allocator for every call: other streams and captured calls have their own.
             ws = torch.empty(size, dtype=torch.uint8, device=x.device)
         _lib.check("lss_int4_matvec", lib.lss_int4_matvec(
             x.data_ptr(), _CODES[x.dtype], rows, k, x_stride, packed.data_ptr(), scales.data_ptr(), scale_code, n, k // groups,

@@ -134,3 +134,20 @@ def test_plain_forms_on_known_values():
     x = torch.tensor([0.0, 1.0625, 1.1875, 448.0, 500.0, 2.0 ** -9, 2.0 ** -10, 3 * 2.0 ** -10, -17.0], dtype=torch.float64)
     assert U.to_e4m3(x).tolist() == [0.0, 1.0, 1.25, 448.0, 448.0, 2.0 ** -9, 0.0, 2.0 ** -8, -16.0]
     assert torch.equal(U.to_e4m3(x), x.clamp(-448, 448).float().to(torch.float8_e4m3fn).double())
+
+
+def test_int4_refuses_overlap_and_asks_for_workspace_for_long_rows():
+    a = dict(x=1 << 20, xs=4000, rows=3, K=64, N=40, ys=4000)  # bf16 x, f32 y
+    for bad in (dict(y=(1 << 20) + 2 * 63), dict(y=(1 << 20) - 4 * 39), dict(y=(1 << 20) + 2 * (2 * 4000 + 63)),
+                dict(y=(1 << 20) + 8000 - 4 * 39, yd=0, ys=2000), dict(y=(1 << 20) + 8000 + 2 * 63, ys=2000)):
+        assert int4(**{**a, **bad}) == INVALID, bad
+    lib = _lib.load()
+    for xd, k in ((1, 49152), (0, 16384)):
+        assert lib.lss_int4_workspace_bytes(8, k, xd, 200000) == 0
+        assert lib.lss_int4_workspace_bytes(1, 2 * k, xd, 200000) > 0
+        assert int4(x=1 << 20, y=1 << 30, K=2 * k, xs=2 * k, xd=xd, N=200000, ys=200000) == WORKSPACE
+
+
+def test_block_state_that_overlaps_in_part():
+    for fn in ("lss_block_plan", "lss_block_release"):
+        assert plan(fn, B=3, lens_out=20) == INVALID and plan(fn, B=3, lens=64, new=20) == INVALID

@@ -83,6 +83,37 @@ def test_int4_layouts_and_values():
     assert bool(y[1].isnan().all()) and not bool(y[3].isfinite().any())
 
 
+@pytest.mark.parametrize("rows,n,k,dtype", [(1, 200, 20480, "f32"), (3, 5000, 20480, "f32"), (2, 130, 150016, "bf16"), (8, 5000, 51200, "f16")])
+def test_int4_long_rows(rows, n, k, dtype):
+    """Rows that do not fit the shared memory of an SM, or only when several SMs share them."""
+    w, x = int4_case(rows, n, k, 128, seed=rows + k)
+    x = x.to(DTYPES[dtype])
+    int4_check(lb.int4_matvec(x, w), x, w)
+
+
+def test_int4_output_beside_and_over_the_input():
+    w, x = int4_case(3, 64, 128, 32, seed=31)
+    both = torch.zeros(3, 200, device=DEV)
+    both[:, :128] = x
+    lb.int4_matvec(both[:, :128], w, out=both[:, 128:192])
+    int4_check(both[:, 128:192].contiguous(), x, w)
+    for out in (both[:, :64], both[:, 100:164]):
+        with pytest.raises((RuntimeError, ValueError)):
+            lb.int4_matvec(both[:, :128], w, out=out)
+    assert torch.equal(both[:, :128], x)
+
+
+def test_plan_writes_lengths_over_the_new_ones():
+    """65,536 tokens of 4,096 rows: many CTAs, if the state were not written in place."""
+    B, bs = 4096, 16
+    table = torch.arange(B, dtype=torch.int32, device=DEV).view(B, 1).contiguous()
+    lens, free, nf = ints([0] * B), ints(list(range(B))), ints([B])
+    for _ in range(20):
+        new = ints([16] * B)
+        p = lb.plan_blocks(table, lens, new, free, nf, bs, 16 * B, lens_out=new)
+        assert p.starts.tolist() == list(range(0, 16 * B + 1, 16)) and bool((new == 16).all()) and bool((p.granted == 16).all())
+
+
 def test_int4_quantize_and_sample_hidden():
     w = torch.randn(777, 256, generator=gen(9), device=DEV)
     q = lb.Int4Weight.quantize(w, group=64)
