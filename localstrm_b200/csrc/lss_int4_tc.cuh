@@ -17,7 +17,7 @@ struct Int4TcArgs {
   Int4Args a;
   const unsigned char* xop;  // x as matrix operand, see lss_int4_operand_kernel
   float* part;               // [ks][rows][N] sums of the column slices (ks > 1)
-  int row0, rows, ks, blocks;  // blocks: row blocks per CTA, one per team
+  int row0, rows, ks, full, rest;  // row blocks per CTA, one per team: T4_TEAMS in the first `full`, `rest` in the others
 };
 
 __device__ __forceinline__ void tc_alloc(uint32_t* out, uint32_t cols) {
@@ -146,8 +146,9 @@ __global__ void __launch_bounds__(T4_NT, 1) lss_int4_tc_kernel(Int4TcArgs t) {
   const Int4Args& a = t.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, team = warp >> 2, quarter = warp & 3;
   const int NB = (a.N + T4_RB - 1) / T4_RB, KB = (a.K + I4_KB - 1) / I4_KB, ng = a.K / a.group;
-  const int slice = blockIdx.x % t.ks, block0 = blockIdx.x / t.ks * t.blocks;
-  const int active = min(t.blocks, NB - block0);             // teams with work
+  const int slice = blockIdx.x % t.ks, cta = blockIdx.x / t.ks;
+  const int block0 = cta < t.full ? cta * T4_TEAMS : t.full * T4_TEAMS + (cta - t.full) * t.rest;
+  const int active = min(cta < t.full ? T4_TEAMS : t.rest, NB - block0);  // teams with work
   const int kb0 = (int)((int64_t)KB * slice / t.ks), nu = (int)((int64_t)KB * (slice + 1) / t.ks) - kb0;
   // 1024-byte alignment of the operand within the dynamic part
   unsigned char* xs = t4_sm + ((1024 - (saddr(t4_sm) & 1023)) & 1023);
