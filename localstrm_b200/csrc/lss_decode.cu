@@ -254,22 +254,26 @@ static cudaError_t launch_int4(const Int4Args& a, const I4Plan& p, cudaStream_t 
 
 // Nine rows and more, and rows of x too long for shared memory: the tensor-memory kernel, 64 rows of x at a time.
 struct TcPlan {
-  int ctas, full, rest, ks;  // CTAs (the first `full` of T4_TEAMS row blocks, the others of `rest`), column slices of each
+  int ctas, full, rest, ks, first;  // CTAs; the first `full` have T4_TEAMS row blocks, the others `rest` and a slice of
+                                    // the columns; first matrix row of the others
   size_t xop, part;
 };
-// Teams on all SMs first, then slices.  The row blocks behind the last full wave of T4_TEAMS per SM are dealt to all SMs:
-// fewer teams in a CTA are done sooner.
+// Teams on all SMs first, then slices.  The row blocks behind the last full wave of T4_TEAMS per SM are dealt to all SMs,
+// as fewer teams in a CTA are done sooner (64 rows, 128,256 x 4096: 120 -> 109 us), and sliced where they are few
+// (151,936 x 4096, three behind two waves: 150 -> 128 us).
 static TcPlan tc_plan(int rows, int N, int K, int x_dtype, int sms) {
   TcPlan p;
   const int NB = (N + T4_RB - 1) / T4_RB, KB = (K + I4_KB - 1) / I4_KB;
   p.full = (NB - 1) / (T4_TEAMS * sms) * sms;
   const int left = NB - p.full * T4_TEAMS;
   p.rest = (left + sms - 1) / sms;
-  p.ctas = p.full + (left + p.rest - 1) / p.rest;
-  p.ks = std::max(1, std::min(KB, sms / p.ctas));
+  const int behind = (left + p.rest - 1) / p.rest;
+  p.ks = std::max(1, std::min(KB, sms / behind));
+  p.ctas = p.full + behind * p.ks;
+  p.first = p.full * T4_TEAMS * T4_RB;
   const int most = std::min(rows, 64);
   p.xop = (size_t)KB * (x_dtype == LSS_DTYPE_F32 ? 3 : 1) * 64 * 256;
-  p.part = p.ks > 1 ? (size_t)p.ks * most * N * sizeof(float) : 0;
+  p.part = p.ks > 1 ? (size_t)p.ks * most * (N - p.first) * sizeof(float) : 0;
   return p;
 }
 
@@ -281,12 +285,12 @@ static cudaError_t launch_int4_tc(const Int4Args& a, int row0, int rows, const T
   cudaError_t e = allow_smem(lss_int4_tc_kernel<DT, SPG, NR>, set, device_index(), smem);
   if (e != cudaSuccess) return e;
   const int KB = (a.K + I4_KB - 1) / I4_KB;
-  Int4TcArgs t{a, ws, reinterpret_cast<float*>(ws + p.xop), row0, rows, p.ks, p.full, p.rest};
+  Int4TcArgs t{a, ws, reinterpret_cast<float*>(ws + p.xop), row0, rows, p.ks, p.full, p.rest, p.first};
   e = launch(lss_int4_operand_kernel<DT, NR>, (unsigned)((KB * NR * 16 + 255) / 256), 256, 0, 1, false, st, a, row0, rows, ws);
   if (e != cudaSuccess) return e;
-  e = launch(lss_int4_tc_kernel<DT, SPG, NR>, (unsigned)(p.ctas * p.ks), T4_NT, smem, 1, true, st, t);
+  e = launch(lss_int4_tc_kernel<DT, SPG, NR>, (unsigned)p.ctas, T4_NT, smem, 1, true, st, t);
   if (e != cudaSuccess || p.ks == 1) return e;
-  return launch(lss_int4_sum_kernel, (unsigned)(((int64_t)rows * a.N + 255) / 256), 256, 0, 1, false, st, t);
+  return launch(lss_int4_sum_kernel, (unsigned)(((int64_t)rows * (a.N - p.first) + 255) / 256), 256, 0, 1, false, st, t);
 }
 
 template <int DT, int SPG>

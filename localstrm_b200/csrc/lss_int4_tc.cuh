@@ -16,8 +16,9 @@ constexpr long long T4_WAIT = 2000000000LL;  // about a second
 struct Int4TcArgs {
   Int4Args a;
   const unsigned char* xop;  // x as matrix operand, see lss_int4_operand_kernel
-  float* part;               // [ks][rows][N] sums of the column slices (ks > 1)
+  float* part;               // [ks][rows][N - first] sums of the column slices (ks > 1)
   int row0, rows, ks, full, rest;  // row blocks per CTA, one per team: T4_TEAMS in the first `full`, `rest` in the others
+  int first;                 // first matrix row of the others, which have ks column slices each
 };
 
 __device__ __forceinline__ void tc_alloc(uint32_t* out, uint32_t cols) {
@@ -125,11 +126,12 @@ __global__ void __launch_bounds__(256) lss_int4_operand_kernel(Int4Args a, int r
 // scales them in f32 and adds them up in registers.  The codes never go to shared memory as 16-bit
 // values, whose bandwidth (128 B per cycle and SM) could not carry them at the rate of HBM.  The teams drift
 // apart by up to XS - 1 units, so that the widening of one overlaps the products of another.
-// Measured, 128,256 x 4096, groups of 128, bf16: 64 rows 120 us, 16 rows 86 us (lss_int4_kernel eight rows at a
-// time: 591 and 164 us).  Bound by the instructions of the widening, as there, and by the last wave: a
-// CTA's four row blocks at a time divide 1,002 into 1.7 waves of 148.
+// Measured, 128,256 x 4096, groups of 128, bf16: 64 rows 109 us, 16 rows 86 us (lss_int4_kernel eight rows at a
+// time: 591 and 164 us).  Bound by the instructions of the widening, as there, and by the chain of a unit (codes,
+// widening, products, sums), which four teams a CTA hide in part.
 // Tensor memory: 64 columns of left operand and 64 of sums per team, all 512.
-// A range of columns per CTA (ks of them) where there are few row blocks; lss_int4_sum_kernel adds up.
+// A range of columns per CTA (ks of them) where there are few row blocks, or few behind the last full wave;
+// lss_int4_sum_kernel adds up.
 template <int DT, int SPG, int NR>
 __global__ void __launch_bounds__(T4_NT, 1) lss_int4_tc_kernel(Int4TcArgs t) {
   constexpr bool BF = DT != LSS_DTYPE_F16;
@@ -146,10 +148,11 @@ __global__ void __launch_bounds__(T4_NT, 1) lss_int4_tc_kernel(Int4TcArgs t) {
   const Int4Args& a = t.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, team = warp >> 2, quarter = warp & 3;
   const int NB = (a.N + T4_RB - 1) / T4_RB, KB = (a.K + I4_KB - 1) / I4_KB, ng = a.K / a.group;
-  const int slice = blockIdx.x % t.ks, cta = blockIdx.x / t.ks;
+  const int ks = (int)blockIdx.x < t.full ? 1 : t.ks, behind = (int)blockIdx.x - t.full;
+  const int slice = ks > 1 ? behind % ks : 0, cta = ks > 1 ? t.full + behind / ks : (int)blockIdx.x;
   const int block0 = cta < t.full ? cta * T4_TEAMS : t.full * T4_TEAMS + (cta - t.full) * t.rest;
   const int active = min(cta < t.full ? T4_TEAMS : t.rest, NB - block0);  // teams with work
-  const int kb0 = (int)((int64_t)KB * slice / t.ks), nu = (int)((int64_t)KB * (slice + 1) / t.ks) - kb0;
+  const int kb0 = (int)((int64_t)KB * slice / ks), nu = (int)((int64_t)KB * (slice + 1) / ks) - kb0;
   // 1024-byte alignment of the operand within the dynamic part
   unsigned char* xs = t4_sm + ((1024 - (saddr(t4_sm) & 1023)) & 1023);
   const uint32_t ring = saddr(xs) + XS * XB + (uint32_t)warp * (T4_ST * STAGE);
@@ -315,7 +318,7 @@ __global__ void __launch_bounds__(T4_NT, 1) lss_int4_tc_kernel(Int4TcArgs t) {
       for (int i = 0; i < NR; ++i)
         if (i < t.rows) {
           const float v = bad ? __int_as_float(0x7fffffff) : acc[i];
-          if (t.ks > 1) t.part[((size_t)slice * t.rows + i) * a.N + n] = v;
+          if (ks > 1) t.part[((size_t)slice * t.rows + i) * (a.N - t.first) + n - t.first] = v;
           else i4_store(a, t.row0 + i, n, v);
         }
     }
@@ -333,12 +336,12 @@ __global__ void __launch_bounds__(T4_NT, 1) lss_int4_tc_kernel(Int4TcArgs t) {
 
 // Adds up the column slices' sums, in order.
 static __global__ void __launch_bounds__(256) lss_int4_sum_kernel(Int4TcArgs t) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, size = (int64_t)t.rows * t.a.N;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, cols = t.a.N - t.first, size = t.rows * cols;
   if (i >= size) return;
   float v = 0.0f;
   for (int s = 0; s < t.ks; ++s) v += t.part[s * size + i];
-  const int r = (int)(i / t.a.N);
-  i4_store(t.a, t.row0 + r, (int)(i - (int64_t)r * t.a.N), v);
+  const int r = (int)(i / cols);
+  i4_store(t.a, t.row0 + r, t.first + (int)(i - r * cols), v);
 }
 
 }  // namespace lss

@@ -91,6 +91,17 @@ def test_int4_long_rows(rows, n, k, dtype):
     int4_check(lb.int4_matvec(x, w), x, w)
 
 
+@pytest.mark.parametrize("rows,n,k,dtype", [(9, 76000, 512, "bf16"), (64, 76100, 384, "f16"), (20, 76001, 256, "f32"), (16, 100000, 128, "bf16"),
+                                            (70, 82000, 640, "bf16"), (33, 151936, 160, "f16")])
+def test_int4_waves(rows, n, k, dtype):
+    """More row blocks than fit the SMs at a time, with few and many of them left for the last turn."""
+    w, x = int4_case(rows, n, k, 32, seed=n)
+    x = x.to(DTYPES[dtype])
+    y = lb.int4_matvec(x, w, out_dtype=torch.float32)
+    int4_check(y, x, w)
+    assert torch.equal(y, lb.int4_matvec(x, w, out_dtype=torch.float32))
+
+
 def test_int4_output_beside_and_over_the_input():
     w, x = int4_case(3, 64, 128, 32, seed=31)
     both = torch.zeros(3, 200, device=DEV)
