@@ -258,18 +258,30 @@ struct TcPlan {
                                     // the columns; first matrix row of the others
   size_t xop, part;
 };
-// Teams on all SMs first, then slices.  The row blocks behind the last full wave of T4_TEAMS per SM are dealt to all SMs,
-// as fewer teams in a CTA are done sooner (64 rows, 128,256 x 4096: 120 -> 109 us), and sliced where they are few
-// (151,936 x 4096, three behind two waves: 150 -> 128 us).
+// The row blocks behind the last full wave of T4_TEAMS per SM: a unit of 128 columns takes about 1 us and an eighth of
+// one per team (its chain of codes, widening, products and sums is only in part hidden by the other teams), a CTA's
+// start and end eight units, slices a second launch and 1 ns per 300 of their sums.  So few teams per CTA on all SMs (64 rows, 128,256
+// x 4096: 120 -> 109 us), or more of them with a slice of the columns each (151,936 x 4096, three blocks behind two
+// waves: 150 -> 128 us; 100,000 x 4096, 190 behind one: 104 -> 102 us, 14,336 x 4096: 45 -> 36), whichever is less.
 static TcPlan tc_plan(int rows, int N, int K, int x_dtype, int sms) {
   TcPlan p;
   const int NB = (N + T4_RB - 1) / T4_RB, KB = (K + I4_KB - 1) / I4_KB;
   p.full = (NB - 1) / (T4_TEAMS * sms) * sms;
   const int left = NB - p.full * T4_TEAMS;
-  p.rest = (left + sms - 1) / sms;
-  const int behind = (left + p.rest - 1) / p.rest;
-  p.ks = std::max(1, std::min(KB, sms / behind));
-  p.ctas = p.full + behind * p.ks;
+  int64_t best = INT64_MAX;
+  for (int t = 1; t <= T4_TEAMS; ++t) {
+    const int behind = (left + t - 1) / t;
+    if (behind > sms) continue;
+    const int units = (KB + std::min(KB, sms / behind) - 1) / std::min(KB, sms / behind), ks = (KB + units - 1) / units;
+    // ns
+    const int64_t cost = (int64_t)(units + 8) * (1000 + 125 * t) + (ks > 1 ? 2500 + (int64_t)ks * std::min(rows, 64) * left * T4_RB / 300 : 0);
+    if (cost < best) {
+      best = cost;
+      p.rest = t;
+      p.ks = ks;
+      p.ctas = p.full + behind * ks;
+    }
+  }
   p.first = p.full * T4_TEAMS * T4_RB;
   const int most = std::min(rows, 64);
   p.xop = (size_t)KB * (x_dtype == LSS_DTYPE_F32 ? 3 : 1) * 64 * 256;
