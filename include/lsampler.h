@@ -262,7 +262,9 @@ int lss_int4_matvec(const void* x, int x_dtype, int rows, int K, int64_t x_strid
  *   lens_out    int32 [B]: lens + granted; may be `lens` itself (overlapping it in part: LSS_ERR_INVALID_ARG)
  *   n_free_out  int32 [1]; may be `n_free` itself
  * lss_block_release returns the blocks of the rows with codes[b] != 0 (lss_stop_check's codes) to
- * the free list, in row and block order, and sets their lengths to 0.
+ * the free list, in row and block order, and sets their lengths to 0.  codes[b] has to be 0 for rows without
+ * a sampled token of their own in the step (granted[b] == 0, or a prompt that goes on): starts[b + 1] - 1 is
+ * another row's token there, whose code would free a live request.
  * Both: B at most LSS_BLOCK_MAX_ROWS; n_free is taken as within [0, num_blocks]. */
 #define LSS_BLOCK_MAX_ROWS 16384
 int lss_block_plan(int32_t* table, int64_t table_stride, int width, const int32_t* lens,

@@ -2,8 +2,8 @@
 
 A step runs ``plan_blocks`` (a place for every request's new tokens), ``append_kv`` (their keys and
 values, in 8 bits with one scale per block and head) and ``attend`` per layer; after sampling,
-``release_blocks`` takes the codes of ``check_stop_batch`` and returns the blocks of the requests
-that stopped.  Everything stays on the device: no call reads a length back, so a step can be
+``release_blocks`` takes the codes of ``check_stop_batch`` (those of the rows that had a token of their own:
+``StepPlan.stops``) and returns the blocks of the requests that stopped.  Everything stays on the device: no call reads a length back, so a step can be
 captured in a CUDA graph.  LocalStrm's counterparts are the host-side block manager
 (``src/memory/``) and the gather + SDPA of ``src/kernels/paged_attention.py``.
 """
@@ -35,6 +35,22 @@ class StepPlan:
     slots: Optional[torch.Tensor] = None
     positions: Optional[torch.Tensor] = None
     n_free: Optional[torch.Tensor] = None
+
+    def stops(self, codes: torch.Tensor, prompt_lens: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """The codes (``check_stop_batch``'s) of the rows that sampled a token of their own in this step,
+        0 for the others: what ``release_blocks`` may be given.
+
+        A row without tokens in the step (idle or refused) has no last token: ``starts[b + 1] - 1`` is
+        another row's, or one that ``attend`` passed over, and a code for it would free a live request.
+        With ``prompt_lens [B]`` rows that do not hold their whole prompt yet are left out too.  The
+        tokens of all rows left out mean nothing.  To be called before ``lens`` changes again."""
+        own = self.granted > 0
+        for name, t in (("codes", codes), ("prompt_lens", prompt_lens)):
+            if t is not None and (t.dtype is not _I32 or t.shape != own.shape or t.device != own.device):
+                raise ValueError(f"{name}: expected int32 {list(own.shape)} on {own.device}")
+        if prompt_lens is not None:
+            own = own & (self.lens >= prompt_lens)
+        return torch.where(own, codes, 0)
 
 
 @dataclass
@@ -128,8 +144,8 @@ def plan_blocks(block_table: torch.Tensor, lens: torch.Tensor, new_lens: torch.T
 def release_blocks(block_table: torch.Tensor, lens: torch.Tensor, codes: torch.Tensor, free_blocks: torch.Tensor,
                    n_free: torch.Tensor, block_size: int, lens_out: Optional[torch.Tensor] = None,
                    n_free_out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
-    """Returns the blocks of the rows with a non-zero code (``check_stop_batch``'s) to ``free_blocks``, in
-    row and block order; their lengths become 0.  Gives ``(lens, n_free)`` afterwards; ``lens_out`` and
+    """Returns the blocks of the rows with a non-zero code (``check_stop_batch``'s, through
+    ``StepPlan.stops``) to ``free_blocks``, in row and block order; their lengths become 0.  Gives ``(lens, n_free)`` afterwards; ``lens_out`` and
     ``n_free_out`` as for ``plan_blocks``.  Blocks that rows share must be released once."""
     dev, B, width, stride = _table(block_table)
     lens_at, codes_at = _ints("lens", lens, B, dev), _ints("codes", codes, B, dev)

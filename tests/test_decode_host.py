@@ -151,3 +151,16 @@ def test_int4_refuses_overlap_and_asks_for_workspace_for_long_rows():
 def test_block_state_that_overlaps_in_part():
     for fn in ("lss_block_plan", "lss_block_release"):
         assert plan(fn, B=3, lens_out=20) == INVALID and plan(fn, B=3, lens=64, new=20) == INVALID
+
+
+def test_stops_leaves_out_rows_without_a_token_of_their_own():
+    i = lambda *v: torch.tensor(v, dtype=torch.int32)
+    # rows: a token, idle, refused, the middle of a prompt, the end of a prompt, a token and no stop
+    p = lb.StepPlan(i(0, 1, 1, 4, 6, 9, 10), i(1, 0, 0, 2, 3, 1), i(8, 5, 0, 6, 7, 9))
+    codes = i(1, 1, 2, 1, 2, 0)
+    assert p.stops(codes).tolist() == [1, 0, 0, 1, 2, 0]
+    got = p.stops(codes, i(3, 3, 9, 7, 7, 9))
+    assert got.tolist() == [1, 0, 0, 0, 2, 0] and got.dtype is torch.int32 and got.is_contiguous()
+    for bad in ((codes.long(),), (codes[:5],), (codes, i(1, 2)), (codes, codes.float())):
+        with pytest.raises(ValueError):
+            p.stops(*bad)

@@ -616,6 +616,30 @@ def test_decode_loop_against_64_bits():
     assert len(left) == int(m.n_free) and left | live == set(range(40)) and not left & live and held >= live
 
 
+def test_loop_keeps_rows_that_had_no_token_of_their_own():
+    """An idle row, a refused one and one inside its prompt behind rows that sample their EOS: the codes of the
+    tokens that stand in their places would free them."""
+    m = Loop()
+    m.step(27)
+    before = m.lens.clone()
+    m.new = ints([1, 0, 4, 1, 200, 0])  # row 4 does not fit the step
+    plan, _, _, _, last, tok = m.step(27)
+    assert plan.granted.tolist() == [1, 0, 4, 1, 0, 0] and int(last[1]) == int(last[0]) and int(tok[1]) == int(tok[0])
+    codes = S.check_stop_batch(tok, tok.tolist())  # whatever stands there is the row's EOS
+    assert bool((codes == S.STOP_EOS).all())
+    prompts = before.clone()
+    prompts[2] = int(plan.lens[2]) + 1
+    codes = plan.stops(codes, prompts)
+    assert codes.tolist() == [S.STOP_EOS, 0, 0, S.STOP_EOS, 0, 0]
+    held = [m.table[b, : -(-int(plan.lens[b]) // m.bs)].tolist() for b in range(m.rows)]
+    lb.release_blocks(m.table, m.lens, codes, m.free, m.n_free, m.bs, lens_out=m.lens, n_free_out=m.n_free)
+    left = set(m.free[: int(m.n_free)].tolist())
+    assert m.lens.tolist() == [0, int(before[1]), int(before[2]) + 4, 0, int(before[4]), int(before[5])]
+    for b in (1, 2, 4, 5):
+        assert not left & set(held[b])
+    assert set(held[0]) | set(held[3]) <= left
+
+
 def test_decode_loop_captured_and_replayed():
     """The captured step against eager ones, several steps on: state in place, no host reads."""
     eager, graph = Loop(), Loop()
