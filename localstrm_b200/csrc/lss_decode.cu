@@ -1,7 +1,9 @@
 // lss_decode.cu — C ABI of the decode-step operators around the sampler: 4-bit products, block
 // tables, the 8-bit key/value cache and its attention.
 #include <algorithm>
+#include <cstdlib>
 #include <mutex>
+#include <utility>
 
 #include "lss_attend_tc.cuh"
 #include "lss_blocks.cuh"
@@ -88,6 +90,27 @@ static bool rows_overlap(const void* x, int64_t x_pitch, int64_t x_row, const vo
   if (rows == 1 || x_pitch != y_pitch) return true;
   const int64_t at = (d % x_pitch + x_pitch) % x_pitch;  // where y's rows start in x's pitch
   return at < x_row || at + y_row > x_pitch;
+}
+// Two arrays of T x H rows of n bytes (start, bytes between tokens and between heads) that share memory without
+// being the same rows: a result would be written where another CTA still reads its query.  With equal strides
+// exactly, else wherever the extents meet.
+static bool rows_shifted(const void* x, int64_t x_st, int64_t x_sh, const void* y, int64_t y_st, int64_t y_sh, int64_t T, int64_t H, int64_t n) {
+  if (T == 1) x_st = y_st = 0;  // one token, one head: the stride says nothing
+  if (H == 1) x_sh = y_sh = 0;
+  const int64_t d = (int64_t)(reinterpret_cast<intptr_t>(y) - reinterpret_cast<intptr_t>(x));
+  if (d >= (T - 1) * x_st + (H - 1) * x_sh + n || -d >= (T - 1) * y_st + (H - 1) * y_sh + n) return false;
+  if (x_st != y_st || x_sh != y_sh) return true;
+  if (d == 0) return false;
+  if (T < H) {  // the walk below is over the shorter side
+    std::swap(T, H);
+    std::swap(x_st, x_sh);
+  }
+  for (int64_t j = 1 - H; j < H; ++j) {  // rows i tokens and j heads apart begin d - i st - j sh bytes apart
+    const int64_t r = d - j * x_sh, i0 = x_st > 0 ? (r >= 0 ? r / x_st : -((-r + x_st - 1) / x_st)) : 0;
+    for (int64_t i = i0; i <= i0 + 1; ++i)
+      if (i > -T && i < T && std::abs(r - i * x_st) < n) return true;
+  }
+  return false;
 }
 // Arrays of n entries of which one begins inside the other.
 static bool cut(const int32_t* x, const int32_t* y, int64_t n) { return x != y && x < y + n && y < x + n; }
@@ -499,6 +522,8 @@ int lss_attend(const void* q, int64_t q_token_stride, int64_t q_head_stride, int
   if (!q || !out || !k_cache || !v_cache || !k_scale || !v_scale || !starts || !granted || !lens)
     return LSS_ERR_INVALID_ARG;
   if (!aligned_to(k_cache, 16) || !aligned_to(v_cache, 16)) return LSS_ERR_INVALID_ARG;
+  if (rows_shifted(q, 2 * q_token_stride, 2 * q_head_stride, out, 2 * out_token_stride, 2 * out_head_stride, T, q_heads, 2 * (int64_t)dim))
+    return LSS_ERR_INVALID_ARG;
   if (!workspace || workspace_bytes < lss_attend_workspace_bytes(dim) || !aligned_to(workspace, 16)) return LSS_ERR_WORKSPACE;
   AttendArgs a{};
   a.q = q;

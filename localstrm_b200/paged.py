@@ -203,7 +203,8 @@ def attend(q: torch.Tensor, cache: KVCache8, block_table: torch.Tensor, plan: St
 
     The queries of row b see its positions up to their own, the step's own tokens among them (append
     first).  ``scale`` defaults to ``dim ** -0.5``; ``lse_out`` (float32 ``[T, q_heads]``) receives the natural
-    log of the softmax sums.  Tokens of refused rows, and those behind the last row, are left as they
+    log of the softmax sums.  ``out`` may be ``q`` itself; where it overlaps q in any other way the call is
+    refused.  Tokens of refused rows, and those behind the last row, are left as they
     are in ``out`` and ``lse_out`` (in a fresh ``out``: undefined)."""
     dev, B, width, stride = _table(block_table)
     blocks, heads, bs, dim = cache.check(dev)

@@ -164,3 +164,23 @@ def test_stops_leaves_out_rows_without_a_token_of_their_own():
     for bad in ((codes.long(),), (codes[:5],), (codes, i(1, 2)), (codes, codes.float())):
         with pytest.raises(ValueError):
             p.stops(*bad)
+
+
+def test_attend_refuses_results_shifted_over_the_queries():
+    """Every row of a small layout against brute force: q at 4096 (bytes), 16-bit values."""
+    rows = lambda at, st, sh, T, H: [at + 2 * (t * st + h * sh) for t in range(T) for h in range(H)]
+    kinds = [(2, 4, 256, 64), (2, 4, 64, 128), (3, 2, 384, 64), (1, 4, 7, 64), (2, 2, 256, 64), (3, 4, 512, 128)]
+    for T, hq, st, sh in kinds:
+        for ot, oh in {(st, sh), (256, 64), (300, 72), (512, 128)}:
+            if oh < 64 or (T > 1 and ot < (hq - 1) * oh + 64 and oh < (T - 1) * ot + 64):
+                continue
+            q = rows(4096, st, sh, T, hq)
+            for at in [4096 + 16 * i for i in range(-200, 201, 3)] + [4096, 4096 + 2 * sh, 4096 + 2 * st, 4096 - 2 * st, 4096 + 128, 4096 + 126]:
+                o = rows(at, ot, oh, T, hq)
+                meet = any(abs(a - b) < 128 for a in q for b in o)
+                apart = max(q) + 128 <= min(o) or max(o) + 128 <= min(q)
+                got = attend(q=4096, qt=st, qh=sh, T=T, hq=hq, out=at, ot=ot, oh=oh, ws=None)
+                if o == q or not meet and (apart or (ot, oh) == (st, sh)):
+                    assert got == WORKSPACE, (T, hq, st, sh, ot, oh, at)
+                elif meet:
+                    assert got == INVALID, (T, hq, st, sh, ot, oh, at)
