@@ -302,7 +302,8 @@ int lss_kv_append(const void* k, int64_t k_token_stride, int64_t k_head_stride, 
  * dim 64, 128 or 256.  `scale` multiplies the products.  lse (f32 [T][q_heads], natural log of the
  * sum) may be NULL.  Queries that see nothing (all of their blocks outside [0, num_blocks)) give 0
  * and -inf; tokens of no granted row are left as they were in out and lse.  out may be q itself (same address
- * and strides), and shares no other memory with it (LSS_ERR_INVALID_ARG).
+ * and strides), and shares no other memory with it (LSS_ERR_INVALID_ARG); its rows lie token by
+ * token or head by head, none over another.
  * workspace: lss_attend_workspace_bytes(dim) bytes, 16-byte aligned, of this call alone until it is
  * done. */
 size_t lss_attend_workspace_bytes(int dim);

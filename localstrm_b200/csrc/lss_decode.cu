@@ -522,6 +522,9 @@ int lss_attend(const void* q, int64_t q_token_stride, int64_t q_head_stride, int
   if (!q || !out || !k_cache || !v_cache || !k_scale || !v_scale || !starts || !granted || !lens)
     return LSS_ERR_INVALID_ARG;
   if (!aligned_to(k_cache, 16) || !aligned_to(v_cache, 16)) return LSS_ERR_INVALID_ARG;
+  if (T > 1 && out_token_stride < (q_heads - 1) * out_head_stride + dim &&
+      (out_token_stride < dim || out_head_stride < (T - 1) * out_token_stride + dim))
+    return LSS_ERR_INVALID_ARG;  // rows of the result lie over each other, whether tokens or heads are outside
   if (rows_shifted(q, 2 * q_token_stride, 2 * q_head_stride, out, 2 * out_token_stride, 2 * out_head_stride, T, q_heads, 2 * (int64_t)dim))
     return LSS_ERR_INVALID_ARG;
   if (!workspace || workspace_bytes < lss_attend_workspace_bytes(dim) || !aligned_to(workspace, 16)) return LSS_ERR_WORKSPACE;

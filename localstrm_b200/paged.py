@@ -222,8 +222,9 @@ def attend(q: torch.Tensor, cache: KVCache8, block_table: torch.Tensor, plan: St
         os = out.stride()
     else:
         os = out.stride()
-        if out.shape != shape or out.dtype is not dtype or out.get_device() != dev or os[2] != 1 or os[1] < dim \
-                or (shape[0] > 1 and os[0] < (shape[1] - 1) * os[1] + dim):
+        if out.shape != shape or out.dtype is not dtype or out.get_device() != dev or os[2] != 1 \
+                or (shape[1] > 1 and os[1] < dim) or (shape[0] > 1 and os[0] < dim) \
+                or (shape[0] > 1 and os[0] < (shape[1] - 1) * os[1] + dim and os[1] < (shape[0] - 1) * os[0] + dim):
             raise ValueError(f"out: expected {dtype} {list(shape)} on cuda:{dev}, rows of stride 1 that do not overlap")
     if lse_out is not None and (lse_out.dtype is not _F32 or lse_out.shape != shape[:2] or lse_out.get_device() != dev
                                 or not lse_out.is_contiguous()):
@@ -239,7 +240,7 @@ def attend(q: torch.Tensor, cache: KVCache8, block_table: torch.Tensor, plan: St
             q.data_ptr(), qs[0], qs[1], _CODES[dtype], shape[0], shape[1], heads, dim, cache.k.data_ptr(), cache.v.data_ptr(),
             cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), blocks, bs, block_table.data_ptr(), stride, width,
             _ints("plan.starts", plan.starts, B + 1, dev), _ints("plan.granted", plan.granted, B, dev),
-            _ints("plan.lens", plan.lens, B, dev), B, dim ** -0.5 if scale is None else scale, out.data_ptr(), os[0], os[1],
+            _ints("plan.lens", plan.lens, B, dev), B, dim ** -0.5 if scale is None else scale, out.data_ptr(), os[0], max(os[1], dim),
             None if lse_out is None else lse_out.data_ptr(), ws.data_ptr(), size, _stream(dev)))
     return out
 

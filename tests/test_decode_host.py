@@ -184,3 +184,10 @@ def test_attend_refuses_results_shifted_over_the_queries():
                     assert got == WORKSPACE, (T, hq, st, sh, ot, oh, at)
                 elif meet:
                     assert got == INVALID, (T, hq, st, sh, ot, oh, at)
+
+
+def test_attend_takes_results_head_by_head():
+    for bad in (dict(ot=255), dict(ot=0), dict(ot=64, oh=127), dict(ot=65, oh=128), dict(T=3, ot=64, oh=191)):
+        assert attend(out=1 << 20, ws=None, **bad) == INVALID, bad
+    for good in (dict(ot=256), dict(ot=64, oh=128), dict(T=3, ot=70, oh=204), dict(T=1, ot=0), dict(hq=2, ot=128)):
+        assert attend(out=1 << 20, ws=None, **good) == WORKSPACE, good

@@ -487,6 +487,25 @@ def test_attend_layouts_and_scales():
     check_attend(q, cache, rows)
 
 
+def test_attend_results_head_by_head():
+    """Tokens inside heads in the result, and a result between the queries' rows."""
+    rows = U.make_rows([100, 33], [1, 20], 16)
+    cache = lb.KVCache8(*U.random_cache(rows[-1], 2, 16, 128))
+    both = torch.randn(21, 6, 256, generator=gen(2), device=DEV).half()
+    q, plan = both[:, :, :128], lb.StepPlan(*rows[2:5])
+    want = lb.attend(q, cache, rows[1], plan)
+    out = torch.zeros(6, 21, 128, dtype=torch.float16, device=DEV).transpose(0, 1)
+    assert torch.equal(lb.attend(q, cache, rows[1], plan, out=out), want)
+    keep = q.clone()
+    assert torch.equal(lb.attend(q, cache, rows[1], plan, out=both[:, :, 128:]), want) and torch.equal(q, keep)
+    flat = torch.zeros(40 * 6 * 128, dtype=torch.float16, device=DEV)
+    for sizes in ((128 * 5, 128, 1), (128, 128 * 20, 1), (0, 128, 1)):
+        with pytest.raises(ValueError):
+            lb.attend(q, cache, rows[1], plan, out=flat.as_strided((21, 6, 128), sizes))
+    with pytest.raises(lb.SamplerError):
+        lb.attend(q, cache, rows[1], plan, out=both[:, :, 64:192])
+
+
 def test_attend_small_weights_are_not_lost():
     """One token far above 60,000 others: together they hold a good part of the sum."""
     n, dim = 60000, 64
