@@ -185,7 +185,8 @@ __device__ __forceinline__ void at_join(const AttendArgs& a, PieceAt piece_at, i
       continue;
     }
     const float f = ex2(w - AT_BIAS - m) / l;
-    const uint32_t y0 = l == 0.0f ? 0u : at_pack<DT>(o.x * f, o.y * f), y1 = l == 0.0f ? 0u : at_pack<DT>(o.z * f, o.w * f);
+    const bool none = m == -INFINITY;  // it sees nothing
+    const uint32_t y0 = none ? 0u : at_pack<DT>(o.x * f, o.y * f), y1 = none ? 0u : at_pack<DT>(o.z * f, o.w * f);
     const int r2 = mt * R + rr, qi = r2 / a.per, qh = head * a.per + r2 - qi * a.per;
     const int64_t tok = a.starts[row] + qi;
     uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + tok * a.o_st + (int64_t)qh * a.o_sh + d;
@@ -197,7 +198,7 @@ __device__ __forceinline__ void at_join(const AttendArgs& a, PieceAt piece_at, i
       out[2] = (uint16_t)y1;
       out[3] = (uint16_t)(y1 >> 16);
     }
-    if (a.lse && d == 0) a.lse[tok * (a.heads * a.per) + qh] = l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
+    if (a.lse && d == 0) a.lse[tok * (a.heads * a.per) + qh] = none ? -INFINITY : (m + log2f(l)) * LN2;
   }
 }
 
@@ -553,7 +554,7 @@ __global__ void __launch_bounds__(AtCfg<D, NQ, TP>::NW * 32, 1) lss_attend_kerne
 #pragma unroll
         for (int nq = 0; nq < NQ; ++nq)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) over |= y[u][nq][e] > AT_SLACK || z[u][nq][e] > AT_BIAS + AT_SLACK;
+          for (int e = 0; e < 4; ++e) over |= !(y[u][nq][e] <= AT_SLACK && z[u][nq][e] <= AT_BIAS + AT_SLACK);  // NaN too: -inf less a maximum of -inf
       if (__any_sync(0xffffffffu, over)) {  // the first step, and where the maxima move
 #pragma unroll
         for (int nq = 0; nq < NQ; ++nq)
@@ -566,7 +567,9 @@ __global__ void __launch_bounds__(AtCfg<D, NQ, TP>::NW * 32, 1) lss_attend_kerne
 #pragma unroll
               for (int q = 0; q < 2; ++q) {
                 const bool see = !any_masked || (!wrong[u] && ((t0 + u) << 4) + g + 8 * q < sees(8 * nq + 2 * c + e));
-                if (see) tu = fmaxf(tu, s[u][nq][2 * q + e] * f[u][nq][e]);
+                // A score of -inf is above "none seen": maxima of what is seen are finite at least, so that such a
+                // score has no weight beside others, and no sum at all alone (0 / 0 at the end).
+                if (see) tu = fmaxf(tu, fmaxf(s[u][nq][2 * q + e] * f[u][nq][e], -FLT_MAX));
               }
               top = fmaxf(top, tu);
               topw = fmaxf(topw, tu + lv[u]);
@@ -700,7 +703,7 @@ __global__ void __launch_bounds__(AtCfg<D, NQ, TP>::NW * 32, 1) lss_attend_kerne
         if (rr < rows_here) {
           if (whole) {
             const int r2 = mt * R + rr, qi = r2 / a.per, qh = head * a.per + r2 - qi * a.per;
-            const bool none = l[nq][e] == 0.0f;
+            const bool none = m[nq][e] == -INFINITY;
             const float f = ex2(w[nq][e] - AT_BIAS - m[nq][e]) / l[nq][e];
             uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + (int64_t)(start + qi) * a.o_st + (int64_t)qh * a.o_sh;
 #pragma unroll

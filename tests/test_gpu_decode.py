@@ -506,6 +506,49 @@ def test_attend_results_head_by_head():
         lb.attend(q, cache, rows[1], plan, out=both[:, :, 64:192])
 
 
+# few query rows (each group size of that kernel, one and two tiles a step), prompt chunks
+SCORES = [([700, 900], [1, 1], 2, 4, 128), ([1500], [1], 2, 4, 128), ([700], [4], 2, 4, 64), ([700], [7], 2, 4, 128), ([700], [3], 1, 4, 256),
+          ([700, 1000], [900, 300], 8, 4, 128), ([650], [1300], 8, 2, 64)]
+
+
+@pytest.mark.parametrize("ctx,new,heads,per,dim", SCORES[:5])
+def test_attend_scores_that_are_all_minus_infinity(ctx, new, heads, per, dim):
+    """A query whose products are all -inf has no softmax: NaN, not the 0 of one that sees nothing."""
+    rows = U.make_rows(ctx, new, 16, seed=dim)
+    table, t, starts, granted, lens, blocks = rows
+    k, v, ks, vs = U.random_cache(blocks, heads, 16, dim, seed=per)
+    k.view(torch.uint8)[..., 0] = 0x38  # 1
+    cache = lb.KVCache8(k, v, ks, vs)
+    q = torch.randn(sum(new), heads * per, dim, generator=gen(dim), device=DEV).bfloat16()
+    hit = torch.zeros(q.shape[:2], dtype=torch.bool, device=DEV)
+    hit[0, 0] = hit[-1, -1] = hit[sum(new) // 2, heads] = True
+    q[..., 0][hit] = -math.inf
+    lse = torch.full(q.shape[:2], 77.0, device=DEV)
+    y = lb.attend(q, cache, t, lb.StepPlan(starts, granted, lens), lse_out=lse)
+    assert bool(y[hit].isnan().all()) and bool((lse[hit] == -math.inf).all())
+    want, mag, wl = U.attend_reference(q, k, v, ks, vs, table, starts.tolist(), granted.tolist(), lens.tolist(), dim ** -0.5)
+    tol = 1.25 * 2.0 ** -11 * mag + 2.0 ** -8 * want.abs()
+    assert bool(((y.double() - want).abs() <= tol)[~hit].all()) and bool(((lse.double() - wl).abs() <= 2.0 ** -16 * (1 + wl.abs()))[~hit].all())
+
+
+@pytest.mark.parametrize("ctx,new,heads,per,dim", SCORES)
+def test_attend_scores_that_overflow_to_minus_infinity(ctx, new, heads, per, dim):
+    """Tokens whose scores fall below the range of f32 have no weight, wherever they lie."""
+    rows = U.make_rows(ctx, new, 16, seed=dim)
+    table, t, starts, granted, lens, blocks = rows
+    k, v, ks, vs = U.random_cache(blocks, heads, 16, dim, seed=per)
+    k.view(torch.uint8)[:] = 0
+    for a, b in ((0, 600), (40, 100), (620, 640)):  # from the first token on, in the middle, near the end
+        k.view(torch.uint8)[:] = 0
+        for row in table:
+            for p in range(a, b):
+                k.view(torch.uint8)[row[p // 16], :, p % 16, 0] = 0x7E  # 448
+        q = torch.zeros(sum(new), heads * per, dim, dtype=torch.bfloat16, device=DEV)
+        q[..., 0] = -2.0 ** 127
+        y, lse = check_attend(q, lb.KVCache8(k, v, torch.ones_like(ks), vs), rows, scale=1.0)
+        assert bool(y.isfinite().all()) and bool(lse.isfinite().all())
+
+
 def test_attend_small_weights_are_not_lost():
     """One token far above 60,000 others: together they hold a good part of the sum."""
     n, dim = 60000, 64
