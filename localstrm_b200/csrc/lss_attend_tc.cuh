@@ -299,8 +299,8 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
 #pragma unroll
               for (int e = 0; e < 16; ++e)
                 if (!with_mask || at + 16 * g + e < limit) t = fmaxf(t, __uint_as_float(x[g][e]));
-              if (with_mask && (k.x < 0.0f || t == -INFINITY)) continue;
-              t *= fq * k.x;
+              if (with_mask && (k.x < 0.0f || at + 16 * g >= limit)) continue;
+              t = fmaxf(t * (fq * k.x), -FLT_MAX);  // -inf and NaN: seen, unlike what leaves m at -inf
               top = fmaxf(top, t);
               topw = fmaxf(topw, t + k.y);
               least = fminf(least, k.y);
@@ -377,7 +377,7 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
           piece[PA_ROWS + rr] = l;
           piece[2 * PA_ROWS + rr] = w;
         }
-        const bool none = l == 0.0f, bad = *(volatile int*)&failed, spoiled = bad || any_nan;
+        const bool none = m == -INFINITY, bad = *(volatile int*)&failed, spoiled = bad || any_nan;
         const float fin = ex2(w - AT_BIAS - m) / l;
 #pragma unroll 1
         for (int i = 0; i < D; i += 16) {
@@ -657,13 +657,14 @@ __global__ void __launch_bounds__(256) lss_attend_tc_join_kernel(AttendArgs a) {
       o[2] += v.z * f;
       o[3] += v.w * f;
     }
+    const bool none = m == -INFINITY;  // it sees nothing
     const float f = ex2(w - AT_BIAS - m) / l;
     const int r2 = mt * PA_ROWS + rr, qi = r2 / a.per, qh = head * a.per + r2 - qi * a.per;
     const int limit = rw.len - rw.n + qi + 1;
     const int64_t tok = a.starts[me.x] + qi;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      o[e] = l == 0.0f ? 0.0f : o[e] * f;
+      o[e] = none ? 0.0f : o[e] * f;
       if (nan[e] < limit) o[e] = __int_as_float(0x7fffffff);
     }
     const uint32_t y0 = at_pack<DT>(o[0], o[1]), y1 = at_pack<DT>(o[2], o[3]);
@@ -672,7 +673,7 @@ __global__ void __launch_bounds__(256) lss_attend_tc_join_kernel(AttendArgs a) {
     out[1] = (uint16_t)(y0 >> 16);
     out[2] = (uint16_t)y1;
     out[3] = (uint16_t)(y1 >> 16);
-    if (a.lse && d == 0) a.lse[tok * (a.heads * a.per) + qh] = l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
+    if (a.lse && d == 0) a.lse[tok * (a.heads * a.per) + qh] = none ? -INFINITY : (m + log2f(l)) * LN2;
   }
 }
 

@@ -511,7 +511,7 @@ SCORES = [([700, 900], [1, 1], 2, 4, 128), ([1500], [1], 2, 4, 128), ([700], [4]
           ([700, 1000], [900, 300], 8, 4, 128), ([650], [1300], 8, 2, 64)]
 
 
-@pytest.mark.parametrize("ctx,new,heads,per,dim", SCORES[:5])
+@pytest.mark.parametrize("ctx,new,heads,per,dim", SCORES)
 def test_attend_scores_that_are_all_minus_infinity(ctx, new, heads, per, dim):
     """A query whose products are all -inf has no softmax: NaN, not the 0 of one that sees nothing."""
     rows = U.make_rows(ctx, new, 16, seed=dim)
