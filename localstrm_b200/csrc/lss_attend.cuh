@@ -140,6 +140,19 @@ __device__ __forceinline__ uint32_t at_pack(float x0, float x1) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+// What turns a row's sums into its result, 2^(W - AT_BIAS - m) / l, as f times g: with the smallest scales of V
+// the power alone would be flushed to zero.
+struct AtFactor {
+  float f, g;
+  __device__ __forceinline__ AtFactor(float m, float l, float w) {
+    const float e = w - AT_BIAS - m;
+    const bool low = e < -64.0f;
+    f = ex2(low ? e + 64.0f : e) / l;
+    g = low ? 5.42101086242752217e-20f : 1.0f;  // 2^-64
+  }
+  __device__ __forceinline__ float operator()(float x) const { return x * f * g; }
+};
+
 // Adds up `n` pieces (at p(i), laid out as in the workspace) of one group and writes the result: the
 // output where `last`, else a piece at `dst`.  Threads t0, t0 + nth, ... share the elements.
 template <int D, int DT, int NQ, class PieceAt>
@@ -184,9 +197,9 @@ __device__ __forceinline__ void at_join(const AttendArgs& a, PieceAt piece_at, i
       *reinterpret_cast<float4*>(dst + 3 * R + rr * D + d) = o;
       continue;
     }
-    const float f = ex2(w - AT_BIAS - m) / l;
+    const AtFactor f(m, l, w);
     const bool none = m == -INFINITY;  // it sees nothing
-    const uint32_t y0 = none ? 0u : at_pack<DT>(o.x * f, o.y * f), y1 = none ? 0u : at_pack<DT>(o.z * f, o.w * f);
+    const uint32_t y0 = none ? 0u : at_pack<DT>(f(o.x), f(o.y)), y1 = none ? 0u : at_pack<DT>(f(o.z), f(o.w));
     const int r2 = mt * R + rr, qi = r2 / a.per, qh = head * a.per + r2 - qi * a.per;
     const int64_t tok = a.starts[row] + qi;
     uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + tok * a.o_st + (int64_t)qh * a.o_sh + d;
@@ -704,7 +717,7 @@ __global__ void __launch_bounds__(AtCfg<D, NQ, TP>::NW * 32, 1) lss_attend_kerne
           if (whole) {
             const int r2 = mt * R + rr, qi = r2 / a.per, qh = head * a.per + r2 - qi * a.per;
             const bool none = m[nq][e] == -INFINITY;
-            const float f = ex2(w[nq][e] - AT_BIAS - m[nq][e]) / l[nq][e];
+            const AtFactor f(m[nq][e], l[nq][e], w[nq][e]);
             uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + (int64_t)(start + qi) * a.o_st + (int64_t)qh * a.o_sh;
 #pragma unroll
             for (int p = 0; p < NP; ++p)
@@ -713,7 +726,7 @@ __global__ void __launch_bounds__(AtCfg<D, NQ, TP>::NW * 32, 1) lss_attend_kerne
                 uint32_t pk[4];
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
-                  pk[q] = none ? 0u : at_pack<DT>(o[p * SP + i + q][nq][e] * f, o[p * SP + i + q][nq][2 + e] * f);
+                  pk[q] = none ? 0u : at_pack<DT>(f(o[p * SP + i + q][nq][e]), f(o[p * SP + i + q][nq][2 + e]));
                 uint16_t* d = out + p * PC + g * (PC / 8) + 2 * i;
                 if (a.aligned) {
                   *reinterpret_cast<uint4*>(d) = make_uint4(pk[0], pk[1], pk[2], pk[3]);

@@ -378,7 +378,7 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
           piece[2 * PA_ROWS + rr] = w;
         }
         const bool none = m == -INFINITY, bad = *(volatile int*)&failed, spoiled = bad || any_nan;
-        const float fin = ex2(w - AT_BIAS - m) / l;
+        const AtFactor fin(m, l, w);
 #pragma unroll 1
         for (int i = 0; i < D; i += 16) {
           uint32_t x[16];
@@ -397,7 +397,7 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
               float y[2];
 #pragma unroll
               for (int z = 0; z < 2; ++z) {
-                y[z] = none ? 0.0f : __uint_as_float(x[2 * e + z]) * fin;
+                y[z] = none ? 0.0f : fin(__uint_as_float(x[2 * e + z]));
                 if (spoiled && (bad || nan_from[i + 2 * e + z] < limit)) y[z] = __int_as_float(0x7fffffff);
               }
               pk[e] = at_pack<DT>(y[0], y[1]);
@@ -658,13 +658,13 @@ __global__ void __launch_bounds__(256) lss_attend_tc_join_kernel(AttendArgs a) {
       o[3] += v.w * f;
     }
     const bool none = m == -INFINITY;  // it sees nothing
-    const float f = ex2(w - AT_BIAS - m) / l;
+    const AtFactor f(m, l, w);
     const int r2 = mt * PA_ROWS + rr, qi = r2 / a.per, qh = head * a.per + r2 - qi * a.per;
     const int limit = rw.len - rw.n + qi + 1;
     const int64_t tok = a.starts[me.x] + qi;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      o[e] = none ? 0.0f : o[e] * f;
+      o[e] = none ? 0.0f : f(o[e]);
       if (nan[e] < limit) o[e] = __int_as_float(0x7fffffff);
     }
     const uint32_t y0 = at_pack<DT>(o[0], o[1]), y1 = at_pack<DT>(o[2], o[3]);

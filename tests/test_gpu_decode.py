@@ -549,6 +549,18 @@ def test_attend_scores_that_overflow_to_minus_infinity(ctx, new, heads, per, dim
         assert bool(y.isfinite().all()) and bool(lse.isfinite().all())
 
 
+@pytest.mark.parametrize("ctx,new,heads,per,dim", SCORES)
+def test_attend_smallest_value_scales(ctx, new, heads, per, dim):
+    """Values near the smallest scale of a block (2^-126): bf16 results hold them."""
+    rows = U.make_rows(ctx, new, 16, seed=dim)
+    k, v, ks, vs = U.random_cache(rows[-1], heads, 16, dim, seed=per)
+    q = torch.randn(sum(new), heads * per, dim, generator=gen(dim), device=DEV).bfloat16()
+    for lo, hi in ((-126, -126), (-126, -100), (-126, 100), (110, 118)):
+        scales = torch.exp2(torch.randint(lo, hi + 1, vs.shape, generator=gen(lo + hi), device=DEV).float())
+        y, _ = check_attend(q, lb.KVCache8(k, v, ks, scales), rows)
+        assert bool((y != 0).any())
+
+
 def test_attend_small_weights_are_not_lost():
     """One token far above 60,000 others: together they hold a good part of the sum."""
     n, dim = 60000, 64
