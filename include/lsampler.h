@@ -251,7 +251,9 @@ int lss_int4_matvec(const void* x, int x_dtype, int rows, int K, int64_t x_strid
  * lss_block_plan gives every row a place for its new_lens[b] tokens (0 and less: none), rows in
  * order.  A row is granted all of its tokens or none: none if they end behind `capacity` in the
  * step's token order, behind the table's width, or if the blocks that it and the rows before it
- * need (refused ones of this last kind among them, so that no later row overtakes) exceed the free list.
+ * need exceed the free list.  Rows refused for this last reason count among "the rows before": once one is, no
+ * later row gets a new block.  A later row whose tokens fit the blocks that it holds is still granted, and a row
+ * refused for the capacity or the width needs no blocks, so that the free list passes on to the rows behind it.
  * The step's tokens lie row after row, starts[b] the first one of row b (granted or not).
  *   table       int32 [B] x [table_stride], width entries used; entries of new blocks are written
  *   slots       int64 [capacity]: block * block_size + offset of each token; -1 for tokens of refused

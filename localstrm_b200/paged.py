@@ -117,8 +117,9 @@ def plan_blocks(block_table: torch.Tensor, lens: torch.Tensor, new_lens: torch.T
     ``lens [B]``: tokens that the rows hold; ``free_blocks [num_blocks]`` with ``n_free [1]``: a stack of
     free block ids, its top taken first; ``capacity``: tokens that the step has room for.  Rows are
     served in order, each with all of its tokens or none: none if they end behind the capacity or the
-    table's width, or if the free list does not hold the blocks for it and the rows before it.  New
-    blocks are written into the table.  ``lens_out`` / ``n_free_out`` may be ``lens`` / ``n_free``
+    table's width, or if the free list does not hold the blocks for it and the rows before it (those
+    refused for this reason among them: once one is, no later row gets a new block; one that needs none is
+    granted all the same).  New blocks are written into the table.  ``lens_out`` / ``n_free_out`` may be ``lens`` / ``n_free``
     (state updated in place, as a captured step needs it); otherwise both inputs are left as they are.
     """
     dev, B, width, stride = _table(block_table)

@@ -244,6 +244,20 @@ def test_plan_odd_inputs():
         assert p.n_free.tolist() == want["n_free"] and p.starts.tolist() == want["starts"]
 
 
+def test_plan_order_of_service():
+    """Who goes on behind a refused row: rows that need no block always, the others only if blocks were not the reason."""
+    table = [[0, 1, -1, -1], [2, -1, -1, -1], [3, -1, -1, -1], [4, -1, -1, -1]]
+    plan = lambda new, capacity: lb.plan_blocks(ints(table), ints([20, 3, 16, 4]), ints(new), ints([5, 6, 0, 0, 0, 0, 0]), ints([1]), 16, capacity)
+    # row 0 lacks a block: row 1 needs none and goes on, row 2 needs the one that is left and does not get it
+    p = plan([40, 2, 1, 3], 60)
+    assert p.granted.tolist() == [0, 2, 0, 3] and p.n_free.tolist() == [1]
+    # row 0 is too long for the table: the block is row 2's
+    p = plan([45, 2, 1, 3], 60)
+    assert p.granted.tolist() == [0, 2, 1, 3] and p.n_free.tolist() == [0] and p.slots.tolist()[47] == 5 * 16
+    # row 0 ends behind the capacity, and so do all rows behind it in the step's order
+    assert plan([16, 2, 1, 3], 15).granted.tolist() == [0, 0, 0, 0]
+
+
 @pytest.mark.parametrize("rows,bs,hi", [(1, 16, 0), (5, 16, 100), (1000, 32, 700), (3000, 4, 60)])
 def test_release_then_plan_again(rows, bs, hi):
     table, lens, _, free, n_free = plan_case(rows, bs, hi, 1, 10, seed=rows)
