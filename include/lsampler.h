@@ -228,18 +228,22 @@ int lss_read_row_paths(const void* workspace, int B, int32_t* paths_out, void* s
  * ------------------------------------------------------------------------------------------ */
 
 /* y[r, n] = sum_k x[r, k] * (code[n, k] - 8) * scale[n, k / group], sums in f32, one rounding to
- * y's type.  Meant for the rows of a decode step: the matrix is read once for up to 64 of them.
+ * y's type.  Meant for the rows of a decode step: the matrix is read once for up to 64 of them, given
+ * lss_int4_workspace_one_pass_bytes of workspace.
  *   x        [rows] x [x_stride elements], dtype LSS_DTYPE_*; K a multiple of 32
  *   packed   uint8 [N][K / 2], column 2i in the low four bits of byte i, 2i + 1 in the high ones;
  *            16-byte aligned
  *   scales   [N][K / group], dtype LSS_DTYPE_BF16 or LSS_DTYPE_F16; group: 32, 64 or a multiple of 128
  *            that divides K
  *   y        [rows] x [y_stride elements], dtype LSS_DTYPE_*; shares no memory with x
- *   workspace  lss_int4_workspace_bytes(rows, K, x_dtype, N) bytes, 16-byte aligned, of this call alone until
+ *   workspace  lss_int4_workspace_bytes(rows, K, x_dtype, N) bytes at least, 16-byte aligned, of this call alone until
  *              it is done.  0 (NULL will do) for up to eight rows of K up to 49,152 (f32: 16,384) columns;
- *              longer rows may take the kernel for more than eight
+ *              longer rows may take the kernel for more than eight.  Two to eight rows that do not fit the shared
+ *              memory of the SMs together are taken a few at a time, the matrix read again for each turn, unless
+ *              the workspace has lss_int4_workspace_one_pass_bytes (never less than the other; 0 where one pass needs none)
  * A wait inside the kernel for more than eight rows that gives up after about a second leaves NaN in y. */
 size_t lss_int4_workspace_bytes(int rows, int K, int x_dtype, int N);
+size_t lss_int4_workspace_one_pass_bytes(int rows, int K, int x_dtype, int N);
 int lss_int4_matvec(const void* x, int x_dtype, int rows, int K, int64_t x_stride, const uint8_t* packed,
                     const void* scales, int scale_dtype, int N, int group, void* y, int y_dtype,
                     int64_t y_stride, void* workspace, size_t workspace_bytes, void* stream);

@@ -68,6 +68,8 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.lss_int4_matvec.argtypes = [P, c_int, c_int, c_int, c_int64, P, P, c_int, c_int, c_int, P, c_int, c_int64, P, c_size_t, P]
     lib.lss_int4_workspace_bytes.restype = c_size_t
     lib.lss_int4_workspace_bytes.argtypes = [c_int, c_int, c_int, c_int]
+    lib.lss_int4_workspace_one_pass_bytes.restype = c_size_t
+    lib.lss_int4_workspace_one_pass_bytes.argtypes = [c_int, c_int, c_int, c_int]
     lib.lss_block_plan.restype = c_int
     lib.lss_block_plan.argtypes = [P, c_int64, c_int, P, P, c_int, c_int, P, c_int, P, c_int, P, P, P, P, P, P, P]
     lib.lss_block_release.restype = c_int

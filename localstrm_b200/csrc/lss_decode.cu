@@ -235,28 +235,33 @@ static cudaError_t launch_attend_dt(int dtype, const AttendArgs& a, void* ws, cu
 static constexpr int I4_SMEM = 227 * 1024;
 
 // Split of lss_int4_kernel: CTAs per row block range (ks), ranges, rows of x that a launch's shared memory takes (0:
-// not even one in any split).  The split with the fewest units in the fullest CTA; a cluster's exchange costs about
-// as much as 8 units, and its row blocks' sums take 16 KB at most.
+// not even one in any split).  The matrix is read once per `most` rows: of the splits with the fewest passes the one
+// with the fewest units in the fullest CTA; a cluster's exchange costs about as much as 8 units, and its row blocks'
+// sums take 16 KB at most.  (Fewest units alone: 8 rows of 4096 x 14,336 in three passes, 60 us in bf16, and eight,
+// 169 us in f32.)
 struct I4Plan {
   int ks, nclusters, sums, most;  // sums: bytes of the row blocks' sums
+  int passes(int rows) const { return (rows + most - 1) / most; }
 };
 static constexpr int I4_FIXED = I4_NW * I4_ST * (I4_RB * I4_KB / 2) + I4_NW * 2 * I4_SUMS * 4;
-static I4Plan i4_plan(int N, int K, int planes, int sms) {
+static I4Plan i4_plan(int rows, int N, int K, int planes, int sms) {
   const int NB = (N + I4_RB - 1) / I4_RB, KB = (K + I4_KB - 1) / I4_KB;
-  I4Plan p{1, 0, 0, 0};
-  int64_t best = INT64_MAX;
+  I4Plan best{1, 0, 0, 0};
+  int64_t best_cost = 0;
   for (int k = 1; k <= 8 && k <= KB; k <<= 1) {
     const int nc = std::min(NB, std::max(1, sms / k)), nrb = (NB + nc - 1) / nc, units = (KB + k - 1) / k;
     if (k > 1 && nrb > 16) continue;
     const int sums = k > 1 ? nrb * I4_SUMS * 4 : 0;
     const int64_t most = (I4_SMEM - I4_FIXED - sums) / ((int64_t)units * I4_KB * 2 * planes);
     const int64_t cost = (int64_t)nrb * units + (k > 1 ? 8 : 0);
-    if (most >= 1 && cost < best) {
-      best = cost;
-      p = I4Plan{k, nc, sums, (int)std::min((int64_t)I4_ROWS, most)};
+    if (most < 1) continue;
+    const I4Plan p{k, nc, sums, (int)std::min((int64_t)I4_ROWS, most)};
+    if (best.most == 0 || p.passes(rows) < best.passes(rows) || (p.passes(rows) == best.passes(rows) && cost < best_cost)) {
+      best_cost = cost;
+      best = p;
     }
   }
-  return p;
+  return best;
 }
 
 template <int DT, int SPG>
@@ -328,12 +333,16 @@ static cudaError_t launch_int4_tc(const Int4Args& a, int row0, int rows, const T
   return launch(lss_int4_sum_kernel, (unsigned)(((int64_t)rows * (a.N - p.first) + 255) / 256), 256, 0, 1, false, st, t);
 }
 
+// Up to eight rows: lss_int4_kernel, unless it would need more than one pass and the workspace has room for the other
+// one (or x does not fit at all, when the workspace has to).
 template <int DT, int SPG>
-static cudaError_t launch_int4_rows(const Int4Args& a, void* ws, cudaStream_t st) {
+static cudaError_t launch_int4_rows(const Int4Args& a, void* ws, size_t ws_bytes, cudaStream_t st) {
   const int sms = sm_count(device_index());
   if (a.rows <= I4_ROWS) {
-    const I4Plan p = i4_plan(a.N, a.K, DT == LSS_DTYPE_F32 ? 3 : 1, sms);
-    if (p.most > 0) return launch_int4<DT, SPG>(a, p, st);
+    const I4Plan p = i4_plan(a.rows, a.N, a.K, DT == LSS_DTYPE_F32 ? 3 : 1, sms);
+    const TcPlan t = tc_plan(a.rows, a.N, a.K, DT, sms);
+    const bool room = ws && aligned_to(ws, 16) && ws_bytes >= t.xop + t.part;
+    if (p.most > 0 && (p.passes(a.rows) == 1 || !room)) return launch_int4<DT, SPG>(a, p, st);
   }
   const TcPlan p = tc_plan(a.rows, a.N, a.K, DT, sms);
   unsigned char* w = reinterpret_cast<unsigned char*>(ws);
@@ -348,10 +357,10 @@ static cudaError_t launch_int4_rows(const Int4Args& a, void* ws, cudaStream_t st
 }
 
 template <int DT>
-static cudaError_t launch_int4_group(const Int4Args& a, void* ws, cudaStream_t st) {
-  if (a.group == 32) return launch_int4_rows<DT, 1>(a, ws, st);
-  if (a.group == 64) return launch_int4_rows<DT, 2>(a, ws, st);
-  return launch_int4_rows<DT, 4>(a, ws, st);
+static cudaError_t launch_int4_group(const Int4Args& a, void* ws, size_t ws_bytes, cudaStream_t st) {
+  if (a.group == 32) return launch_int4_rows<DT, 1>(a, ws, ws_bytes, st);
+  if (a.group == 64) return launch_int4_rows<DT, 2>(a, ws, ws_bytes, st);
+  return launch_int4_rows<DT, 4>(a, ws, ws_bytes, st);
 }
 
 extern "C" {
@@ -359,7 +368,18 @@ extern "C" {
 size_t lss_int4_workspace_bytes(int rows, int K, int x_dtype, int N) {
   if (rows < 1 || K < 1 || N < 1) return 0;
   const int sms = sm_count(device_index());
-  if (rows <= I4_ROWS && i4_plan(N, K, x_dtype == LSS_DTYPE_F32 ? 3 : 1, sms).most > 0) return 0;
+  if (rows <= I4_ROWS && i4_plan(rows, N, K, x_dtype == LSS_DTYPE_F32 ? 3 : 1, sms).most > 0) return 0;
+  const TcPlan p = tc_plan(rows, N, K, x_dtype, sms);
+  return p.xop + p.part;
+}
+
+size_t lss_int4_workspace_one_pass_bytes(int rows, int K, int x_dtype, int N) {
+  if (rows < 1 || K < 1 || N < 1) return 0;
+  const int sms = sm_count(device_index());
+  if (rows <= I4_ROWS) {
+    const I4Plan p = i4_plan(rows, N, K, x_dtype == LSS_DTYPE_F32 ? 3 : 1, sms);
+    if (p.most > 0 && p.passes(rows) == 1) return 0;
+  }
   const TcPlan p = tc_plan(rows, N, K, x_dtype, sms);
   return p.xop + p.part;
 }
@@ -394,9 +414,9 @@ int lss_int4_matvec(const void* x, int x_dtype, int rows, int K, int64_t x_strid
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   cudaError_t e;
   switch (x_dtype) {
-    case LSS_DTYPE_F32: e = launch_int4_group<LSS_DTYPE_F32>(a, workspace, st); break;
-    case LSS_DTYPE_BF16: e = launch_int4_group<LSS_DTYPE_BF16>(a, workspace, st); break;
-    default: e = launch_int4_group<LSS_DTYPE_F16>(a, workspace, st); break;
+    case LSS_DTYPE_F32: e = launch_int4_group<LSS_DTYPE_F32>(a, workspace, workspace_bytes, st); break;
+    case LSS_DTYPE_BF16: e = launch_int4_group<LSS_DTYPE_BF16>(a, workspace, workspace_bytes, st); break;
+    default: e = launch_int4_group<LSS_DTYPE_F16>(a, workspace, workspace_bytes, st); break;
   }
   return status_of(e);
 }

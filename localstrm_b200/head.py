@@ -121,8 +121,9 @@ def int4_matvec(x: torch.Tensor, weight: Int4Weight, out_dtype: Optional[torch.d
     lib = _lib.load()
     with _on(dev):
         ws, size = None, 0
-        if rows > 8 or k > 16384:
-            size = lib.lss_int4_workspace_bytes(rows, k, _CODES[x.dtype], n)
+        # Few and short rows fit the shared memory of any SM.
+        if rows > 8 or k > 16384 or rows * k * (6 if x.dtype is torch.float32 else 2) > 96000:
+            size = lib.lss_int4_workspace_one_pass_bytes(rows, k, _CODES[x.dtype], n)
             # From torch's allocator for every call: other streams and captured calls have their own.
             ws = torch.empty(size, dtype=torch.uint8, device=x.device)
         _lib.check("lss_int4_matvec", lib.lss_int4_matvec(

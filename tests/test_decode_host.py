@@ -191,3 +191,17 @@ def test_attend_takes_results_head_by_head():
         assert attend(out=1 << 20, ws=None, **bad) == INVALID, bad
     for good in (dict(ot=256), dict(ot=64, oh=128), dict(T=3, ot=70, oh=204), dict(T=1, ot=0), dict(hq=2, ot=128)):
         assert attend(out=1 << 20, ws=None, **good) == WORKSPACE, good
+
+
+def test_int4_workspace_of_one_pass():
+    """148 SMs: two to eight rows that fit some split of an SM's shared memory need none; others the other kernel's."""
+    f = _lib.load().lss_int4_workspace_one_pass_bytes
+    bf16, f32 = 1, 0
+    for rows, k, dt, n in ((1, 49152, bf16, 200000), (1, 16384, f32, 200000), (8, 4096, bf16, 151936), (4, 4096, f32, 151936), (8, 14336, bf16, 4096),
+                           (8, 14336, f32, 4096), (8, 11008, bf16, 4096), (8, 28672, bf16, 4096), (6, 8192, bf16, 151936)):
+        assert f(rows, k, dt, n) == 0, (rows, k, dt, n)
+    for rows, k, dt, n in ((8, 8192, bf16, 151936), (8, 8192, f32, 151936), (8, 4096, f32, 151936), (2, 49152, bf16, 200000), (8, 16384, f32, 128256)):
+        assert f(rows, k, dt, n) > 0 and _lib.load().lss_int4_workspace_bytes(rows, k, dt, n) == 0, (rows, k, dt, n)
+    for rows, k, dt, n in ((9, 4096, bf16, 128256), (64, 896, f32, 2000), (1, 98304, bf16, 200000)):
+        assert f(rows, k, dt, n) == _lib.load().lss_int4_workspace_bytes(rows, k, dt, n) > 0
+    assert f(0, 64, bf16, 4) == f(1, 0, bf16, 4) == f(1, 64, bf16, 0) == 0

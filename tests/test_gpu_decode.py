@@ -91,6 +91,35 @@ def test_int4_long_rows(rows, n, k, dtype):
     int4_check(lb.int4_matvec(x, w), x, w)
 
 
+def launches(f):
+    """Kernel launches of a call, counted in a graph that captures it."""
+    rt = pytest.importorskip("cuda.bindings.runtime")
+    g = torch.cuda.CUDAGraph(keep_graph=True)
+    f()
+    with torch.cuda.graph(g):
+        f()
+    err, _, n = rt.cudaGraphGetNodes(g.raw_cuda_graph(), 0)
+    err, nodes, n = rt.cudaGraphGetNodes(g.raw_cuda_graph(), n)
+    return sum(rt.cudaGraphNodeGetType(x)[1] == rt.cudaGraphNodeType.cudaGraphNodeTypeKernel for x in nodes[:n])
+
+
+@pytest.mark.parametrize("rows,n,k,dtype,most", [
+    (8, 1000, 14336, "f32", 1), (8, 4096, 14336, "bf16", 1), (3, 4096, 14336, "f32", 1), (4, 1000, 28672, "f16", 1), (2, 2057, 11008, "f32", 1),
+    (8, 40000, 8192, "bf16", 3), (8, 40000, 4096, "f32", 3), (5, 40003, 4096, "f32", 3), (2, 40000, 16384, "f32", 3), (7, 40000, 8224, "f16", 3)])
+def test_int4_few_rows_read_the_matrix_once(rows, n, k, dtype, most):
+    """Two to eight long rows: one launch for all of them, or the operand, the product and the sum of the other kernel."""
+    w, x = int4_case(rows, n, k, 32, seed=rows + k)
+    x = x.to(DTYPES[dtype])
+    int4_check(lb.int4_matvec(x, w), x, w)
+    assert launches(lambda: lb.int4_matvec(x, w)) <= most
+    # without a workspace of that size, as a C caller may: the same result in more passes
+    lib, y = lb._lib.load(), torch.empty(rows, n, device=DEV)
+    code = {"f32": 0, "bf16": 1, "f16": 2}
+    assert lib.lss_int4_matvec(x.data_ptr(), code[dtype], rows, k, k, w.packed.data_ptr(), w.scales.data_ptr(), 2, n, 32, y.data_ptr(), 0, n, None, 0,
+                               torch.cuda.current_stream().cuda_stream) == 0
+    int4_check(y, x, w)
+
+
 @pytest.mark.parametrize("rows,n,k,dtype", [(9, 76000, 512, "bf16"), (64, 76100, 384, "f16"), (20, 76001, 256, "f32"), (16, 100000, 128, "bf16"),
                                             (70, 82000, 640, "bf16"), (33, 151936, 160, "f16")])
 def test_int4_waves(rows, n, k, dtype):
