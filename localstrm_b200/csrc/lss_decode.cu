@@ -234,22 +234,53 @@ static cudaError_t launch_attend_dt(int dtype, const AttendArgs& a, void* ws, cu
 // ---------------------------------------------------------------- 4-bit products
 static constexpr int I4_SMEM = 227 * 1024;
 
+// Clusters of k CTAs with an SM's whole shared memory that run at a time: fewer than SMs / k, as a cluster lies in one
+// group of SMs whose number need not be a multiple of k.  Asked once per device; without one, SMs / k.
+static int cluster_count(int dev, int k, int sms) {
+  static int n[MAX_DEV][4] = {};
+  int& got = n[dev][log2_of(k)];
+  std::lock_guard<std::mutex> lock(g_mu);
+  if (got == 0) {
+    auto* kern = lss_int4_kernel<LSS_DTYPE_BF16, 4>;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(k * sms), 1, 1);
+    cfg.blockDim = dim3(I4_NT, 1, 1);
+    cfg.dynamicSmemBytes = I4_SMEM;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)k;
+    at[0].val.clusterDim.y = 1;
+    at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    int c = 0;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, I4_SMEM) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&c, kern, &cfg) != cudaSuccess || c < 1) {
+      cudaGetLastError();
+      return std::max(1, sms / k);
+    }
+    got = c;
+  }
+  return got;
+}
+
 // Split of lss_int4_kernel: CTAs per row block range (ks), ranges, rows of x that a launch's shared memory takes (0:
 // not even one in any split).  The matrix is read once per `most` rows: of the splits with the fewest passes the one
 // with the fewest units in the fullest CTA; a cluster's exchange costs about as much as 8 units, and its row blocks'
 // sums take 16 KB at most.  (Fewest units alone: 8 rows of 4096 x 14,336 in three passes, 60 us in bf16, and eight,
-// 169 us in f32.)
+// 169 us in f32.)  There are no more ranges than clusters run at a time (one row of 14,336 x 4096 in SMs / 4 ranges:
+// two waves, 37 us).
 struct I4Plan {
   int ks, nclusters, sums, most;  // sums: bytes of the row blocks' sums
   int passes(int rows) const { return (rows + most - 1) / most; }
 };
 static constexpr int I4_FIXED = I4_NW * I4_ST * (I4_RB * I4_KB / 2) + I4_NW * 2 * I4_SUMS * 4;
-static I4Plan i4_plan(int rows, int N, int K, int planes, int sms) {
-  const int NB = (N + I4_RB - 1) / I4_RB, KB = (K + I4_KB - 1) / I4_KB;
+static I4Plan i4_plan(int rows, int N, int K, int planes, int dev) {
+  const int NB = (N + I4_RB - 1) / I4_RB, KB = (K + I4_KB - 1) / I4_KB, sms = sm_count(dev);
   I4Plan best{1, 0, 0, 0};
   int64_t best_cost = 0;
   for (int k = 1; k <= 8 && k <= KB; k <<= 1) {
-    const int nc = std::min(NB, std::max(1, sms / k)), nrb = (NB + nc - 1) / nc, units = (KB + k - 1) / k;
+    const int nc = std::min(NB, k == 1 ? sms : cluster_count(dev, k, sms)), nrb = (NB + nc - 1) / nc, units = (KB + k - 1) / k;
     if (k > 1 && nrb > 16) continue;
     const int sums = k > 1 ? nrb * I4_SUMS * 4 : 0;
     const int64_t most = (I4_SMEM - I4_FIXED - sums) / ((int64_t)units * I4_KB * 2 * planes);
@@ -337,9 +368,9 @@ static cudaError_t launch_int4_tc(const Int4Args& a, int row0, int rows, const T
 // one (or x does not fit at all, when the workspace has to).
 template <int DT, int SPG>
 static cudaError_t launch_int4_rows(const Int4Args& a, void* ws, size_t ws_bytes, cudaStream_t st) {
-  const int sms = sm_count(device_index());
+  const int dev = device_index(), sms = sm_count(dev);
   if (a.rows <= I4_ROWS) {
-    const I4Plan p = i4_plan(a.rows, a.N, a.K, DT == LSS_DTYPE_F32 ? 3 : 1, sms);
+    const I4Plan p = i4_plan(a.rows, a.N, a.K, DT == LSS_DTYPE_F32 ? 3 : 1, dev);
     const TcPlan t = tc_plan(a.rows, a.N, a.K, DT, sms);
     const bool room = ws && aligned_to(ws, 16) && ws_bytes >= t.xop + t.part;
     if (p.most > 0 && (p.passes(a.rows) == 1 || !room)) return launch_int4<DT, SPG>(a, p, st);
@@ -367,17 +398,17 @@ extern "C" {
 
 size_t lss_int4_workspace_bytes(int rows, int K, int x_dtype, int N) {
   if (rows < 1 || K < 1 || N < 1) return 0;
-  const int sms = sm_count(device_index());
-  if (rows <= I4_ROWS && i4_plan(rows, N, K, x_dtype == LSS_DTYPE_F32 ? 3 : 1, sms).most > 0) return 0;
+  const int dev = device_index(), sms = sm_count(dev);
+  if (rows <= I4_ROWS && i4_plan(rows, N, K, x_dtype == LSS_DTYPE_F32 ? 3 : 1, dev).most > 0) return 0;
   const TcPlan p = tc_plan(rows, N, K, x_dtype, sms);
   return p.xop + p.part;
 }
 
 size_t lss_int4_workspace_one_pass_bytes(int rows, int K, int x_dtype, int N) {
   if (rows < 1 || K < 1 || N < 1) return 0;
-  const int sms = sm_count(device_index());
+  const int dev = device_index(), sms = sm_count(dev);
   if (rows <= I4_ROWS) {
-    const I4Plan p = i4_plan(rows, N, K, x_dtype == LSS_DTYPE_F32 ? 3 : 1, sms);
+    const I4Plan p = i4_plan(rows, N, K, x_dtype == LSS_DTYPE_F32 ? 3 : 1, dev);
     if (p.most > 0 && p.passes(rows) == 1) return 0;
   }
   const TcPlan p = tc_plan(rows, N, K, x_dtype, sms);

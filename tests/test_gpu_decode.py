@@ -120,6 +120,32 @@ def test_int4_few_rows_read_the_matrix_once(rows, n, k, dtype, most):
     int4_check(y, x, w)
 
 
+@pytest.mark.parametrize("rows,n,k,dtype", [(1, 14336, 4096, "bf16"), (8, 4096, 14336, "bf16"), (8, 4096, 14336, "f32"), (1, 9000, 2048, "f16")])
+def test_int4_clusters_run_at_one_time(rows, n, k, dtype):
+    """No second wave for a split of the columns: its clusters are all on the device at once."""
+    drv = pytest.importorskip("cuda.bindings.driver")
+    w, x = int4_case(rows, n, k, 128, seed=n)
+    x = x.to(DTYPES[dtype])
+    int4_check(lb.int4_matvec(x, w), x, w)
+    g = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(g):
+        lb.int4_matvec(x, w)
+    graph = drv.CUgraph(g.raw_cuda_graph())
+    _, _, count = drv.cuGraphGetNodes(graph, 0)
+    _, (node,), count = drv.cuGraphGetNodes(graph, count)
+    assert count == 1
+    _, p = drv.cuGraphKernelNodeGetParams(node)
+    kind = drv.CUlaunchAttributeID.CU_LAUNCH_ATTRIBUTE_CLUSTER_DIMENSION
+    size = max(1, drv.cuGraphKernelNodeGetAttribute(node, kind)[1].clusterDim.x)
+    cfg, at = drv.CUlaunchConfig(), drv.CUlaunchAttribute()
+    cfg.gridDimX, cfg.blockDimX, cfg.sharedMemBytes = p.gridDimX, p.blockDimX, p.sharedMemBytes
+    cfg.gridDimY = cfg.gridDimZ = cfg.blockDimY = cfg.blockDimZ = 1
+    at.id, at.value.clusterDim.x, at.value.clusterDim.y, at.value.clusterDim.z = kind, size, 1, 1
+    cfg.attrs, cfg.numAttrs = [at], 1
+    err, active = drv.cuOccupancyMaxActiveClusters(p.func, cfg)
+    assert int(err) == 0 and p.gridDimX // size <= active
+
+
 @pytest.mark.parametrize("rows,n,k,dtype", [(9, 76000, 512, "bf16"), (64, 76100, 384, "f16"), (20, 76001, 256, "f32"), (16, 100000, 128, "bf16"),
                                             (70, 82000, 640, "bf16"), (33, 151936, 160, "f16")])
 def test_int4_waves(rows, n, k, dtype):
