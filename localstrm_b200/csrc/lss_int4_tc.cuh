@@ -99,7 +99,7 @@ __device__ __forceinline__ bool tc_wait(uint64_t* bar, uint32_t parity, volatile
 }
 
 // Writes x as the operand that the product kernel copies: [unit of 128 columns][plane][half][NR rows][128
-// bytes], 16-byte pieces in the order of int4_unpack's pairs and permuted by row (tc_desc128); zero
+// bytes], 16-byte pieces in the order of int4_unpack's pairs and permuted by row (tc_desc_lo); zero
 // behind the last row and column.  f32 values become three bf16 planes that add up to them.
 template <int DT, int NR>
 __global__ void __launch_bounds__(256) lss_int4_operand_kernel(Int4Args a, int row0, int rows, unsigned char* xop) {

@@ -247,6 +247,26 @@ def test_attend_in_place_and_at_once():
         assert all(torch.equal(o, want) for o in outs)
 
 
+@pytest.mark.parametrize("group", [32, 64, 128, 256])
+@pytest.mark.parametrize("rows", [5, 16, 30, 64])
+def test_int4_f32_rows_are_exact(rows, group):
+    """One value of 24 bits per row, weights that are powers of two: the product is that value at another place, so
+    all three parts of it have to arrive, in the right order and column."""
+    g, n, k = gen(group + rows), 150, 768
+    codes = torch.tensor([0, 4, 6, 7, 9, 10, 12], dtype=torch.uint8, device=DEV)[torch.randint(0, 7, (n, k), generator=g, device=DEV)]
+    scales = torch.exp2(torch.randint(-6, 7, (n, k // group), generator=g, device=DEV).float()).half()
+    w = lb.Int4Weight(codes[:, ::2] | (codes[:, 1::2] << 4), scales)
+    dense = (codes.double() - 8) * scales.double().repeat_interleave(group, 1)
+    at = torch.arange(rows, device=DEV)
+    for shift in range(0, k, rows):
+        v = (torch.randint(0, 1 << 23, (rows,), generator=g, device=DEV) | (1 << 23) | 1).float() * torch.exp2(torch.randint(-40, 20, (rows,), generator=g, device=DEV).float())
+        v = torch.where(at % 2 == 0, v, -v)
+        cols = (shift + at) % k
+        x = torch.zeros(rows, k, device=DEV)
+        x[at, cols] = v
+        assert torch.equal(lb.int4_matvec(x, w).double(), v.double()[:, None] * dense[:, cols].t()), shift
+
+
 # --------------------------------------------------------------------------------- block tables
 def plan_case(rows, bs, hi_ctx, hi_new, spare, seed, width_cut=0):
     g = torch.Generator().manual_seed(seed)
