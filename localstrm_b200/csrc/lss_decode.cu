@@ -203,27 +203,36 @@ static cudaError_t launch_attend_few(const AttendArgs& a, int64_t rows, void* ws
 }
 
 // A step of single tokens has `per` query rows per key head and row; else the average decides.  A step with more
-// tokens than rows, and enough of them to fill the SMs, may mix prompt chunks and single tokens: rows of
-// PA_FROM query rows and more go to the tensor-memory kernel (which would widen the codes for 256 rows of which
-// `per` are there), the others to the one for few rows, one launch after the other on the same workspace.  Steps of
-// chunks alone pay 10 us for the second one's empty launches (220 -> 232 us for four chunks of 300 to 400 tokens); 60
-// single tokens over 6,000 beside two chunks of 2,048 take 490 us.
+// tokens than rows, and enough of them to fill the SMs, may mix prompt chunks, rows of a few tokens and single
+// tokens, and only the device knows which is which: rows of pa_from query rows and more go to the tensor-memory
+// kernel (which would widen the codes for 256 rows of which `per` are there), the others to the one for few rows, one
+// launch after the other on the same workspace.  Its group is that of a single token, or of 16 rows where the average
+// row is a short one.  Measured at 64 rows over 50 to 16,000 tokens, 8 key heads of 4 queries of 128 (in groups of 8 for comparison):
+// 5 tokens each 512 us (606), 8 tokens 532 (813), 9 tokens 750 (977); tensor memory from 41 rows on, 12 tokens 944 (1,190); single tokens
+// beside one chunk of 449 pay for it, 244 (219).  At D = 64 and with more heads per key head the tensor-memory kernel
+// is slower than groups of 16 up to 63 rows (9 tokens of D = 64: 668 us, 435).  Steps of chunks alone pay 10 us for the
+// second one's empty launches (220 -> 232 us for four chunks of 300 to 400 tokens); 60 single tokens over 6,000 beside two
+// chunks of 2,048 take 420 us.
+// A step of no more tokens than rows counts as one of single tokens: a chunk among idle rows is right, but goes in
+// groups of `per` rows (200 tokens over 8,000 beside 255 idle rows 213 us), as a launch more would cost every step of
+// single tokens 8 us.
 template <int D, int DT>
 static cudaError_t launch_attend_rows(AttendArgs a, void* ws, cudaStream_t st) {
-  constexpr int PA_FROM = 64;
+  const int64_t average = (int64_t)a.per * ((a.T + (int64_t)a.B - 1) / a.B);
   a.rows_lo = 0;
   a.rows_hi = INT32_MAX;
   if constexpr (D < 256) {
     if (a.T > a.B && (int64_t)a.heads * a.per * a.T >= (int64_t)PA_ROWS * sm_count(device_index()) / 4) {
-      a.rows_lo = PA_FROM;
+      const int pa_from = D == 128 && a.per <= 8 ? 41 : 64;
+      a.rows_lo = pa_from;
       const cudaError_t e = launch_attend_tc<D, DT>(a, ws, st);
       if (e != cudaSuccess) return e;
       a.rows_lo = 0;
-      a.rows_hi = PA_FROM;
-      return launch_attend_few<D, DT>(a, a.per, ws, st);
+      a.rows_hi = pa_from;
+      return launch_attend_few<D, DT>(a, average < pa_from ? std::max((int64_t)a.per, std::min(average, (int64_t)16)) : a.per, ws, st);
     }
   }
-  return launch_attend_few<D, DT>(a, (int64_t)a.per * ((a.T + (int64_t)a.B - 1) / a.B), ws, st);
+  return launch_attend_few<D, DT>(a, average, ws, st);
 }
 
 template <int D>

@@ -203,7 +203,8 @@ def attend(q: torch.Tensor, cache: KVCache8, block_table: torch.Tensor, plan: St
     256) over the cache, one token per row or many; query head h reads key head ``h // (q_heads / heads)``.
 
     The queries of row b see its positions up to their own, the step's own tokens among them (append
-    first).  ``scale`` defaults to ``dim ** -0.5``; ``lse_out`` (float32 ``[T, q_heads]``) receives the natural
+    first).  A step of no more tokens than rows is taken for one of single tokens; a chunk among many idle rows
+    runs faster where only the rows with tokens are passed.  ``scale`` defaults to ``dim ** -0.5``; ``lse_out`` (float32 ``[T, q_heads]``) receives the natural
     log of the softmax sums.  ``out`` may be ``q`` itself; where it overlaps q in any other way the call is
     refused.  Tokens of refused rows, and those behind the last row, are left as they
     are in ``out`` and ``lse_out`` (in a fresh ``out``: undefined)."""

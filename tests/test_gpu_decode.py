@@ -528,6 +528,40 @@ def test_attend_prompts_and_single_tokens_mixed(per, dim):
     assert bool((y[1038:] == 77).all()) and bool((lse[1038:] == 77).all()) and bool(y[:1038].isfinite().all())
 
 
+def kernels(f):
+    """Names of the kernels that a call launches, from a graph that captures it."""
+    drv = pytest.importorskip("cuda.bindings.driver")
+    f()
+    g = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(g):
+        f()
+    graph = drv.CUgraph(g.raw_cuda_graph())
+    _, _, n = drv.cuGraphGetNodes(graph, 0)
+    _, nodes, n = drv.cuGraphGetNodes(graph, n)
+    return [drv.cuFuncGetName(drv.cuGraphKernelNodeGetParams(x)[1].func)[1].decode() for x in nodes[:n]]
+
+
+@pytest.mark.parametrize("n,per,dim", [(5, 4, 128), (10, 4, 128), (11, 4, 128), (5, 4, 64), (15, 4, 64), (3, 16, 128), (0, 4, 128), (0, 7, 64)])
+def test_attend_a_few_tokens_per_row(n, per, dim):
+    """Batches on both sides of the borders between the kernels: n tokens in every row (0: 1 to 16 of them)."""
+    new = [n or 1 + (i * 5) % 16 for i in range(64)]
+    rows = U.make_rows([(53 * i) % 300 for i in range(64)], new, 16, seed=n)
+    cache = lb.KVCache8(*U.random_cache(rows[-1], 8, 16, dim, seed=per))
+    q = torch.randn(sum(new), 8 * per, dim, generator=gen(dim + n), device=DEV).bfloat16()
+    y, _ = check_attend(q, cache, rows)
+    assert bool(y.isfinite().all())
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attend_short_rows_share_their_tiles(dim):
+    """Eight tokens of four query heads each, 32 query rows: not in groups of eight, which read the cache four times."""
+    rows = U.make_rows([100] * 64, [8] * 64, 16)
+    cache = lb.KVCache8(*U.random_cache(rows[-1], 8, 16, dim))
+    q = torch.zeros(512, 32, dim, dtype=torch.float16, device=DEV)
+    names = kernels(lambda: lb.attend(q, cache, rows[1], lb.StepPlan(*rows[2:5])))
+    assert names and not [x for x in names if f"lss_attend_kernelILi{dim}ELi2ELi1E" in x], names
+
+
 def check_attend_nan(q, cache, rows):
     """As check_attend where some values are NaN: the places of NaN, the others against a cache without it."""
     clean = lb.KVCache8(cache.k, torch.where(cache.v.float().isnan(), 0.0, cache.v.float()).to(E4M3), cache.k_scale, cache.v_scale)
