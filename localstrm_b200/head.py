@@ -62,6 +62,8 @@ class Int4Weight:
         n, k = weight.shape
         w = weight.float().view(n, k // group, group)
         scales = (w.abs().amax(-1) / 7.0).to(scale_dtype)
+        if not bool(scales.isfinite().all()):  # an infinite scale times the code 0 of a small weight is NaN
+            raise ValueError(f"weight: not finite, or a group's largest magnitude / 7 is beyond {scale_dtype}")
         step = scales.float().clamp(min=torch.finfo(torch.float32).tiny)[..., None]
         codes = (torch.round(w / step).clamp(-7, 7) + 8).to(torch.uint8).view(n, k)
         return cls((codes[:, 0::2] | (codes[:, 1::2] << 4)).contiguous(), scales.contiguous())
@@ -75,7 +77,8 @@ class Int4Weight:
 def int4_matvec(x: torch.Tensor, weight: Int4Weight, out_dtype: Optional[torch.dtype] = None,
                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``x @ W.T`` for ``x [rows, K]`` or ``[K]`` (f32, bf16 or f16), sums in f32, one rounding to
-    ``out_dtype`` (default: x's).  One pass over the matrix serves 64 rows.  ``out`` shares no memory with x."""
+    ``out_dtype`` (default: x's).  One pass over the matrix serves 64 rows.  ``out`` shares no memory with x.
+    A group is summed before its scale is applied: these sums, up to 8 times those of ``|x|``, have to lie within f32."""
     _require_cuda(x)
     packed, scales = weight.packed, weight.scales
     shape, dev = x.shape, x.get_device()

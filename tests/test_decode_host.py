@@ -205,3 +205,15 @@ def test_int4_workspace_of_one_pass():
     for rows, k, dt, n in ((9, 4096, bf16, 128256), (64, 896, f32, 2000), (1, 98304, bf16, 200000)):
         assert f(rows, k, dt, n) == _lib.load().lss_int4_workspace_bytes(rows, k, dt, n) > 0
     assert f(0, 64, bf16, 4) == f(1, 0, bf16, 4) == f(1, 64, bf16, 0) == 0
+
+
+def test_quantize_refuses_what_its_scales_cannot_hold():
+    w = torch.ones(3, 64)
+    w[1, 40] = 7 * 65504.0
+    assert bool(lb.Int4Weight.quantize(w, 32).dequantize().isfinite().all())
+    for bad in (7 * 65600.0, float("inf"), float("nan")):
+        w[1, 40] = bad
+        with pytest.raises(ValueError):
+            lb.Int4Weight.quantize(w, 32)
+    w[1, 40] = 7 * 65600.0
+    assert bool(lb.Int4Weight.quantize(w, 32, torch.bfloat16).dequantize().isfinite().all())
