@@ -228,7 +228,8 @@ int lss_read_row_paths(const void* workspace, int B, int32_t* paths_out, void* s
  * ------------------------------------------------------------------------------------------ */
 
 /* y[r, n] = sum_k x[r, k] * (code[n, k] - 8) * scale[n, k / group], sums in f32, one rounding to
- * y's type.  Meant for the rows of a decode step: the matrix is read once for up to 64 of them, given
+ * y's type.  A group is summed before its scale is applied: these sums (up to 8 times those of |x|) have to lie
+ * within f32.  Meant for the rows of a decode step: the matrix is read once for up to 64 of them, given
  * lss_int4_workspace_one_pass_bytes of workspace.
  *   x        [rows] x [x_stride elements], dtype LSS_DTYPE_*; K a multiple of 32
  *   packed   uint8 [N][K / 2], column 2i in the low four bits of byte i, 2i + 1 in the high ones;

@@ -255,8 +255,9 @@ __device__ __forceinline__ void at_join_cut(const AttendArgs& a, int64_t worker,
 // 2^-24 of the largest one.  The sum of the softmax is f32.
 //
 // Measured at D = 128, 8 key heads: 1.1 GB of contexts of 50 to 16,000 tokens for 64 single queries of 32 heads
-// 212 us (5.2 TB/s, 0.81 of the copy rate), 733 MB of three contexts of 90,000 to 131,000 140 us; with queries as the
-// 16-row operand (half of it padding) and reductions for every tile it was 268 and 200 us.
+// 212 us (5.2 TB/s, 0.81 of the copy rate), 733 MB of three contexts of 90,000 to 131,000 140 us (226 and 146 with other
+// work between the calls); with queries as the 16-row operand (half of it padding) and reductions for every tile it was
+// 268 and 200 us.  The first at D = 64 138 us (0.62 of the copy rate), at D = 256 400 us (0.86).
 // Bound by HBM (2 D bytes per token and head) when a row has few queries, by the tensor pipe and the
 // widening of the codes when it has many (they share it 8 NQ rows at a time).
 template <int D, int DT, int NQ, int TP>

@@ -84,8 +84,8 @@ __device__ __forceinline__ uint32_t pa_place(int r, int q) {
 // held as the first position per column from which it is seen.
 // The units (group, tile of 128 tokens that it sees) are cut into equal ranges, one per CTA; pieces of a
 // group are added up by lss_attend_tc_join_kernel.
-// Measured: 296 to 416 new tokens over 3,000 to 5,300 (four rows, 32 query, 8 key heads of 128) 220 us, 450 TFLOP/s, against
-// 640 us with lss_attend_kernel; D = 64 165 us.  About 5,000 cycles per 256 x 128 scores at 48 % issue: waits for
+// Measured: 296 to 416 new tokens over 3,000 to 5,300 (four rows, 32 query, 8 key heads of 128) 222 to 240 us, 410 to 450
+// TFLOP/s, against 640 us with lss_attend_kernel; D = 64 165 to 185 us.  About 5,000 cycles per 256 x 128 scores at 48 % issue: waits for
 // tensor memory and barriers between steps are what is left above the bounds.
 // Bound by the exponentials (16 per cycle and SM: 2048 cycles per 256 x 128 scores) and the tensor pipe (the same
 // number of cycles at D = 128).

@@ -214,8 +214,8 @@ static cudaError_t launch_attend_few(const AttendArgs& a, int64_t rows, void* ws
 // second one's empty launches (220 -> 232 us for four chunks of 300 to 400 tokens); 60 single tokens over 6,000 beside two
 // chunks of 2,048 take 420 us.
 // A step of no more tokens than rows counts as one of single tokens: a chunk among idle rows is right, but goes in
-// groups of `per` rows (200 tokens over 8,000 beside 255 idle rows 213 us), as a launch more would cost every step of
-// single tokens 8 us.
+// their groups (200 tokens over 8,000 beside 255 idle rows 213 us, alone 201; 500 beside 511 507 us, alone 171), as the
+// launches for chunks would cost every step of single tokens 8 to 10 us.
 template <int D, int DT>
 static cudaError_t launch_attend_rows(AttendArgs a, void* ws, cudaStream_t st) {
   const int64_t average = (int64_t)a.per * ((a.T + (int64_t)a.B - 1) / a.B);

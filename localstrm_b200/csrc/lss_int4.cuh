@@ -191,8 +191,8 @@ __device__ __forceinline__ void i4_stage_x(const Int4Args& a, int row0, int rows
 // instructions, about 360 per unit and warp, half of them the widening (11 per 8 weights in bf16, 9 in f16;
 // the integer pipe takes 7 and 5 of those at two warps a cycle).  Units of 32 rows instead of 16 share a load
 // of x and the loop's bookkeeping: 102 -> 82 us.
-// Measured, 151,936 x 4096, groups of 128: one row 82 us in bf16 (3.9 TB/s, 0.61 of the copy rate), 76 us in
-// f16, 114 us in f32; eight rows of bf16 86 us.
+// Measured, 151,936 x 4096, groups of 128: one row 82 us in bf16 (3.9 TB/s, 0.61 of the copy rate; 86 to 96 us with the
+// L2 cache swept between calls), 76 us in f16, 114 us in f32 (four rows 125); eight rows of bf16 86 us.
 template <int DT, int SPG>  // SPG: 32-column steps per group (1, 2, or 4 for groups of 128 and more)
 __global__ void __launch_bounds__(I4_NT, 1) lss_int4_kernel(Int4Args a, int row0, int rows, int ks) {
   constexpr bool BF = DT != LSS_DTYPE_F16;

@@ -126,8 +126,9 @@ __global__ void __launch_bounds__(256) lss_int4_operand_kernel(Int4Args a, int r
 // scales them in f32 and adds them up in registers.  The codes never go to shared memory as 16-bit
 // values, whose bandwidth (128 B per cycle and SM) could not carry them at the rate of HBM.  The teams drift
 // apart by up to XS - 1 units, so that the widening of one overlaps the products of another.
-// Measured, 128,256 x 4096, groups of 128, bf16: 64 rows 109 us, 16 rows 86 us (lss_int4_kernel eight rows at a
-// time: 591 and 164 us).  Bound by the instructions of the widening, as there, and by the chain of a unit (codes,
+// Measured, 128,256 x 4096, groups of 128, bf16: 64 rows 109 us (122 with the L2 cache swept between calls), 16 rows
+// 86 us (lss_int4_kernel eight rows at a time: 591 and 164 us).  f32 x, three products per unit, cache swept: 16 rows 104 us,
+// 32 rows 128, 64 rows 190.  More than 64 rows repeat all of it (151,936 x 4096, bf16: 128 rows 264 us, 256 rows 520).  Bound by the instructions of the widening, as there, and by the chain of a unit (codes,
 // widening, products, sums), which four teams a CTA hide in part.
 // Tensor memory: 64 columns of left operand and 64 of sums per team, all 512.
 // A range of columns per CTA (ks of them) where there are few row blocks, or few behind the last full wave;

@@ -121,7 +121,7 @@ __device__ __forceinline__ int row_of(const int32_t* upto, int n, int u) {
 // L2 cache.
 // Measured: 24 rows of up to 2,048 new tokens, 8 heads of 128, f16: 39 us (153 MB, 3.9 TB/s, 0.60 of the copy
 // rate; a fixed part of some 400 instructions per unit and warp and the rounding bound it), one warp per
-// block of 32 tokens 68 us; 256 single tokens 6.4 us in a graph.
+// block of 32 tokens 68 us; in f32 (254 MB, half the values held in registers) 60 us; 256 single tokens 6.4 us in a graph.
 // Bound by issue and HBM for prompts and by its chain of dependent loads (lengths, table, scale, values) for
 // single tokens.
 template <int DT, int TEAM>
