@@ -16,7 +16,8 @@ constexpr float LN2 = 0.6931471805599453f;
 // CTA (one CTA per SM), stages of the copy ring per warp.  Registers set the warps (queries and sums take
 // 6 NQ D / 16 of them), the shared memory the stages.  D = 128, 8 rows: two tiles a step on 12 warps give each
 // warp more to do between its waits (1.1 GB of contexts of up to 16,000 tokens: 223 -> 212 us); one on 16 warps
-// starts more groups at once (512 rows of 64 to 300 tokens: 75 us against 92).
+// starts more groups at once (512 rows of 64 to 300 tokens: 75 us against 92).  At D = 256 the registers are full with one
+// tile; D = 64 has not been built with two.
 template <int D, int NQ, int TP> struct AtCfg;
 template <> struct AtCfg<64, 1, 1> { static constexpr int NW = 16, ST = 6; };
 template <> struct AtCfg<64, 2, 1> { static constexpr int NW = 16, ST = 6; };
