@@ -322,6 +322,111 @@ int lss_attend(const void* q, int64_t q_token_stride, int64_t q_head_stride, int
                int64_t out_token_stride, int64_t out_head_stride, float* lse, void* workspace,
                size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Decode steps with several tokens per request, drafted as trees, and blocks that several requests
+ * hold.  LocalStrm has neither (it decodes token by token, and its block manager shares blocks on
+ * the host); conventions and formats are those of the operators above.
+ * ------------------------------------------------------------------------------------------ */
+
+/* Norms of queries and keys for each head, with the position rotation in the same pass:
+ *   y = x / sqrt(mean(x^2) + eps) * weight      per token and head, where there is a weight (NULL: y = x),
+ *   (a, b) -> (a cos - b sin, b cos + a sin)    angle = positions[t] * freqs[i], i in [0, rot / 2),
+ * of the pairs (y[i], y[i + rot / 2]), or (y[2 i], y[2 i + 1]) where `interleaved`; y[rot ..] stays.  Sums and products
+ * in f32, the angle is reduced in f64, one rounding to the type of x.
+ *   q, k       [T][heads][dim], innermost stride 1, the other strides in elements; dim even, at most 512
+ *   q_out, k_out  may be q and k themselves (same address and strides), and share no other memory with them or each
+ *              other; their rows lie token by token or head by head, none over another (else LSS_ERR_INVALID_ARG)
+ *   freqs      f32 [rot / 2]; rot even, 0 to dim
+ *   weights    [dim], both of weight_dtype, either may be NULL
+ * dim a multiple of 16 and rot one of 16, with 16-byte aligned rows, take the wide loads. */
+int lss_norm_rotate(const void* q, int64_t q_token_stride, int64_t q_head_stride, void* q_out, int64_t q_out_token_stride,
+                    int64_t q_out_head_stride, int q_heads, const void* k, int64_t k_token_stride, int64_t k_head_stride,
+                    void* k_out, int64_t k_out_token_stride, int64_t k_out_head_stride, int k_heads, int dtype, int T, int dim,
+                    const int32_t* positions, const float* freqs, int rot, int interleaved, const void* q_weight,
+                    const void* k_weight, int weight_dtype, float eps, void* stream);
+
+/* Trees of drafted tokens.  The new tokens of a row (starts[b] .. starts[b] + granted[b] of the step's T tokens, as
+ * lss_block_plan lays them out) are the nodes of a forest: parents[t] is the node, counted from the row's first new
+ * token, that token t goes on from; parents come first, and -1 (or anything that is no earlier node) goes on from the
+ * context.  A row of more than LSS_TREE_MAX_TOKENS new tokens is a prompt chunk: each token goes on from the one
+ * before, whatever its parents say.
+ *
+ * lss_tree_plan, once per step:
+ *   span       int32 [T][2], 8-byte aligned: the token's place in the pre-order of its row's forest (children in
+ *              order) and the number of tokens of its branch; token j is i or an ancestor of it where
+ *              0 <= place(i) - place(j) < size(j)
+ *   positions  int32 [T]: context + depth, for the rotation
+ * Both are 0 for tokens of no granted row.
+ *
+ * lss_tree_accept: the tokens that the sampled ones confirm.  `drafts` are the step's tokens, `targets` the ones sampled
+ * after each of them.  The first given[b] tokens (NULL: 1; at least 1: the token sampled last; the whole chunk of a
+ * prompt) are accepted as they are; from the last of them the walk goes on, from a token to the first of its children
+ * that is the token's target, until there is none, or the target has a code other than 0 (codes: lss_stop_check's, of
+ * the T targets; NULL: none).
+ *   path       int32 [T]: path[starts[b] + i] is the i-th accepted node of the row, -1 behind the last
+ *   tokens     int32 [T]: tokens[starts[b] + i] is the i-th new token of the request (the targets of the given
+ *              tokens' last and of those behind it), -1 behind the last
+ *   counts     int32 [B]: accepted tokens (0 for rows that are not granted); counts - given + 1 are new
+ *   lens_out   int32 [B]: lens - granted + counts; may be `lens` itself
+ *   last       int32 [B]: the last new token, the next step's first; -1 for rows that are not granted
+ *   codes_out  int32 [B]: its code
+ * Rows whose numbers do not fit (granted > lens, tokens outside [0, T)) count as not granted.  B at most LSS_BLOCK_MAX_ROWS. */
+#define LSS_TREE_MAX_TOKENS 1024
+int lss_tree_plan(const int32_t* starts, const int32_t* granted, const int32_t* lens, int B, const int32_t* parents, int T,
+                  int32_t* span, int32_t* positions, void* stream);
+int lss_tree_accept(const int32_t* starts, const int32_t* granted, const int32_t* lens, int B, const int32_t* parents,
+                    const int32_t* drafts, const int32_t* targets, const int32_t* codes, const int32_t* given, int T, int32_t* path,
+                    int32_t* tokens, int32_t* counts, int32_t* lens_out, int32_t* last, int32_t* codes_out, void* stream);
+
+/* lss_attend for such a step: a query sees the tokens before its row's new ones and, of these, itself and its ancestors
+ * (by `span`).  All else is as for lss_attend, the workspace too. */
+int lss_attend_tree(const void* q, int64_t q_token_stride, int64_t q_head_stride, int dtype, int T, int q_heads, int heads,
+                    int dim, const uint8_t* k_cache, const uint8_t* v_cache, const float* k_scale, const float* v_scale,
+                    int num_blocks, int block_size, const int32_t* table, int64_t table_stride, int width,
+                    const int32_t* starts, const int32_t* granted, const int32_t* lens, int B, float scale, void* out,
+                    int64_t out_token_stride, int64_t out_head_stride, float* lse, void* workspace, size_t workspace_bytes,
+                    const int32_t* span, void* stream);
+
+/* What an accepted branch leaves in the cache: the keys and values of new token path[starts[b] + i] of row b become those
+ * of its new token i, for i < counts[b] (lss_tree_accept's; path[i] >= i, other entries stay where they are).  `lens` are
+ * those with all new tokens.  A block that takes in tokens gets the largest of the scales of the blocks that its tokens
+ * come from (its own among them where tokens stay in it), and codes of other scales are rounded again, to nearest even.
+ * What lies behind the accepted tokens is left as it was.  Blocks of one row only, as for lss_kv_append. */
+int lss_kv_compact(uint8_t* k_cache, uint8_t* v_cache, float* k_scale, float* v_scale, int num_blocks, int heads, int block_size,
+                   int dim, const int32_t* table, int64_t table_stride, int width, const int32_t* starts, const int32_t* granted,
+                   const int32_t* lens, int B, const int32_t* path, const int32_t* counts, int T, void* stream);
+
+/* Blocks that several rows hold: shares[block], int32 [num_blocks], counts the holders beyond the first (0 for free
+ * blocks and those of one row, as all are at first).  Only full blocks are shared; a block that is written has one holder.
+ *
+ * lss_block_fork: row dst_rows[i], idle (length 0), goes on from the tokens of row src_rows[i], at most upto[i] of them
+ * (NULL: all).  It gets the ids of their full blocks, each with a holder more, and for the tokens behind these a block
+ * of its own from the free list.  Forks are served in order, by the free list as the rows of lss_block_plan are; one
+ * is refused (granted 0) where the rows are outside [0, B), the destination is not idle or an earlier fork's, or there
+ * is nothing to take.  All lengths are those before the call.
+ *   granted     int32 [n]: tokens taken
+ *   copies      int32 [n][2]: block to copy and the block it is copied to, for lss_kv_copy on every layer's
+ *               cache; -1, -1 where there is none
+ *   lens_out    int32 [B], may be `lens` itself; n_free_out may be `n_free` itself
+ * n at most LSS_BLOCK_MAX_ROWS.
+ *
+ * lss_kv_copy copies whole blocks with their scales, copies[i][0] to copies[i][1]; pairs outside [0, num_blocks) are
+ * passed over.  No block is copied to twice, or copied from and to, in one call.  dim a multiple of 8.
+ *
+ * lss_block_give is lss_block_release for such blocks, and for rows that keep a part of theirs: a row with a code (NULL:
+ * none has) gives all of its blocks back, any other those behind its first keep[b] tokens (NULL: it keeps all), which
+ * become its length.  A block returns to the free list with the last of its holders, in row and block order of these;
+ * shares NULL: no block is shared.  Entries outside [0, num_blocks) are passed over.  B * width at most 2^30. */
+int lss_block_fork(int32_t* table, int64_t table_stride, int width, const int32_t* lens, int B, int block_size,
+                   const int32_t* src_rows, const int32_t* dst_rows, const int32_t* upto, int n, int32_t* shares,
+                   const int32_t* free_blocks, int num_blocks, const int32_t* n_free, int32_t* granted, int32_t* copies,
+                   int32_t* lens_out, int32_t* n_free_out, void* stream);
+int lss_kv_copy(uint8_t* k_cache, uint8_t* v_cache, float* k_scale, float* v_scale, int num_blocks, int heads, int block_size,
+                int dim, const int32_t* copies, int n, void* stream);
+int lss_block_give(const int32_t* table, int64_t table_stride, int width, const int32_t* lens, const int32_t* codes,
+                   const int32_t* keep, int B, int block_size, int32_t* shares, int32_t* free_blocks, int num_blocks,
+                   const int32_t* n_free, int32_t* lens_out, int32_t* n_free_out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -82,6 +82,23 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.lss_attend.restype = c_int
     lib.lss_attend.argtypes = [P, c_int64, c_int64, c_int, c_int, c_int, c_int, c_int, P, P, P, P, c_int, c_int,
                                P, c_int64, c_int, P, P, P, c_int, c_float, P, c_int64, c_int64, P, P, c_size_t, P]
+    lib.lss_norm_rotate.restype = c_int
+    lib.lss_norm_rotate.argtypes = [P, c_int64, c_int64, P, c_int64, c_int64, c_int, P, c_int64, c_int64, P, c_int64, c_int64, c_int,
+                                    c_int, c_int, c_int, P, P, c_int, c_int, P, P, c_int, c_float, P]
+    lib.lss_tree_plan.restype = c_int
+    lib.lss_tree_plan.argtypes = [P, P, P, c_int, P, c_int, P, P, P]
+    lib.lss_tree_accept.restype = c_int
+    lib.lss_tree_accept.argtypes = [P, P, P, c_int, P, P, P, P, P, c_int, P, P, P, P, P, P, P]
+    lib.lss_attend_tree.restype = c_int
+    lib.lss_attend_tree.argtypes = lib.lss_attend.argtypes[:-1] + [P, P]
+    lib.lss_kv_compact.restype = c_int
+    lib.lss_kv_compact.argtypes = [P, P, P, P, c_int, c_int, c_int, c_int, P, c_int64, c_int, P, P, P, c_int, P, P, c_int, P]
+    lib.lss_block_fork.restype = c_int
+    lib.lss_block_fork.argtypes = [P, c_int64, c_int, P, c_int, c_int, P, P, P, c_int, P, P, c_int, P, P, P, P, P, P]
+    lib.lss_kv_copy.restype = c_int
+    lib.lss_kv_copy.argtypes = [P, P, P, P, c_int, c_int, c_int, c_int, P, c_int, P]
+    lib.lss_block_give.restype = c_int
+    lib.lss_block_give.argtypes = [P, c_int64, c_int, P, P, P, c_int, c_int, P, P, c_int, P, P, P, P]
     lib.lss_read_status.restype = c_int
     lib.lss_read_status.argtypes = [P, ctypes.POINTER(c_uint32), P]
     lib.lss_read_row_paths.restype = c_int

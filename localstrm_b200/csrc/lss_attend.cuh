@@ -48,6 +48,7 @@ struct AttendArgs {
   const int32_t* starts;
   const int32_t* granted;
   const int32_t* lens;
+  const int2* span;    // [T]: place in its tree's pre-order and size of its branch (kernels with TREE)
   int B, T;
   float scale;         // softmax scale times log2(e)
   int aligned;         // q and out rows start on 16-byte boundaries
@@ -261,7 +262,13 @@ __device__ __forceinline__ void at_join_cut(const AttendArgs& a, int64_t worker,
 // 268 and 200 us.  The first at D = 64 138 us (0.62 of the copy rate), at D = 256 400 us (0.86).
 // Bound by HBM (2 D bytes per token and head) when a row has few queries, by the tensor pipe and the
 // widening of the codes when it has many (they share it 8 NQ rows at a time).
-template <int D, int DT, int NQ, int TP>
+//
+// With TREE the row's new tokens are the nodes of a tree (parents before children): a query sees the tokens before
+// them and, of them, those in whose branch it lies.  With a node's place in the pre-order and the size of its branch
+// that is one unsigned comparison per new token, 0 <= place(query) - place(token) < size(token), in the tiles that hold
+// new tokens; all others take the same path as without.  As parents come first, the last token that a group of
+// queries can see, and with it the split of the work, is that of the causal form.
+template <int D, int DT, int NQ, int TP, bool TREE>
 __global__ void __launch_bounds__(AtCfg<D, NQ, TP>::NW * 32, 1) lss_attend_kernel(AttendArgs a) {
   constexpr int NW = AtCfg<D, NQ, TP>::NW, ST = AtCfg<D, NQ, TP>::ST, NTH = NW * 32, R = 8 * NQ;
   constexpr int PC = D < 128 ? D : 128, NP = D / PC;  // columns per panel, panels
@@ -355,10 +362,24 @@ __global__ void __launch_bounds__(AtCfg<D, NQ, TP>::NW * 32, 1) lss_attend_kerne
     const int start = a.starts[row], ctx = rw.len - rw.n;
     const int rows_here = min(R, rw.n * a.per - mt * R);
     // Tokens that the first and the last query of the group see.
-    const int see_first = ctx + mt * R / a.per + 1;
+    const int see_first = TREE ? ctx : ctx + mt * R / a.per + 1;
     const int see_last = ctx + (mt * R + rows_here - 1) / a.per + 1;
     const int tend = min(tile1, (see_last + 15) >> 4);
     auto sees = [&](int rr) { return rr < rows_here ? ctx + (mt * R + rr) / a.per + 1 : 0; };
+    // TREE: place of a row's query in its tree; what a token shows, and to whom (below see_last only).
+    auto place = [&](int rr) { return rr < rows_here ? __ldg(&a.span[start + (mt * R + rr) / a.per].x) : -1; };
+    auto branch = [&](int token) {
+      if (token < ctx) return make_int2(INT32_MIN, -1);  // any place is in it
+      return token < see_last ? __ldg(&a.span[start + token - ctx]) : make_int2(0, 0);
+    };
+    auto within = [](int at, const int2& b) { return (uint32_t)at - (uint32_t)b.x < (uint32_t)b.y; };
+    int at_place[NQ][2];
+    if constexpr (TREE) {
+#pragma unroll
+      for (int nq = 0; nq < NQ; ++nq)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) at_place[nq][e] = place(8 * nq + 2 * c + e);
+    }
 
     // ---- copies: block ids of 32 tiles at a time, one per lane
     const int32_t* trow = a.table + row * a.table_stride;
@@ -542,6 +563,20 @@ __global__ void __launch_bounds__(AtCfg<D, NQ, TP>::NW * 32, 1) lss_attend_kerne
       uint32_t pb[TP][NQ][2];
       float y[TP][NQ][4], z[TP][NQ][4];
       bool over = false;
+      uint32_t hidden = 0;  // TREE: bit 4 (u NQ + nq) + e
+      if (TREE && any_masked) {
+#pragma unroll
+        for (int u = 0; u < TP; ++u)
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            const int2 b = branch(((t0 + u) << 4) + g + 8 * q);
+#pragma unroll
+            for (int nq = 0; nq < NQ; ++nq)
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                if (wrong[u] || !within(at_place[nq][e], b)) hidden |= 1u << (4 * (u * NQ + nq) + 2 * q + e);
+          }
+      }
       auto exponents = [&]() {
 #pragma unroll
         for (int u = 0; u < TP; ++u)
@@ -560,7 +595,8 @@ __global__ void __launch_bounds__(AtCfg<D, NQ, TP>::NW * 32, 1) lss_attend_kerne
             for (int nq = 0; nq < NQ; ++nq)
 #pragma unroll
               for (int e = 0; e < 4; ++e)
-                if (wrong[u] || ((t0 + u) << 4) + g + 8 * (e >> 1) >= sees(8 * nq + 2 * c + (e & 1))) y[u][nq][e] = z[u][nq][e] = -INFINITY;
+                if (TREE ? (hidden >> (4 * (u * NQ + nq) + e)) & 1u : wrong[u] || ((t0 + u) << 4) + g + 8 * (e >> 1) >= sees(8 * nq + 2 * c + (e & 1)))
+                  y[u][nq][e] = z[u][nq][e] = -INFINITY;
         }
       };
       exponents();
@@ -581,7 +617,8 @@ __global__ void __launch_bounds__(AtCfg<D, NQ, TP>::NW * 32, 1) lss_attend_kerne
               float tu = -INFINITY;
 #pragma unroll
               for (int q = 0; q < 2; ++q) {
-                const bool see = !any_masked || (!wrong[u] && ((t0 + u) << 4) + g + 8 * q < sees(8 * nq + 2 * c + e));
+                const bool see = !any_masked || (TREE ? !((hidden >> (4 * (u * NQ + nq) + 2 * q + e)) & 1u)
+                                                      : !wrong[u] && ((t0 + u) << 4) + g + 8 * q < sees(8 * nq + 2 * c + e));
                 // A score of -inf is above "none seen": maxima of what is seen are finite at least, so that such a
                 // score has no weight beside others, and no sum at all alone (0 / 0 at the end).
                 if (see) tu = fmaxf(tu, fmaxf(s[u][nq][2 * q + e] * f[u][nq][e], -FLT_MAX));
@@ -673,9 +710,11 @@ __global__ void __launch_bounds__(AtCfg<D, NQ, TP>::NW * 32, 1) lss_attend_kerne
 #pragma unroll
                 for (int nq = 0; nq < NQ; ++nq) {
                   const int lim = sees(8 * nq + g), tk = ((t0 + u) << 4) + 2 * c;
+                  const int at = TREE ? place(8 * nq + g) : 0;
+                  auto seen = [&](int t) { return TREE ? within(at, branch(t)) : t < lim; };
                   float count[4] = {};
-                  mma_f16(count, na, (tk < lim ? 0x3c00u : 0u) | (tk + 1 < lim ? 0x3c000000u : 0u),
-                          (tk + 8 < lim ? 0x3c00u : 0u) | (tk + 9 < lim ? 0x3c000000u : 0u));
+                  mma_f16(count, na, (seen(tk) ? 0x3c00u : 0u) | (seen(tk + 1) ? 0x3c000000u : 0u),
+                          (seen(tk + 8) ? 0x3c00u : 0u) | (seen(tk + 9) ? 0x3c000000u : 0u));
 #pragma unroll
                   for (int e = 0; e < 4; ++e)
                     if (count[e] > 0.0f) o[p * SP + 2 * i + q][nq][e] = __int_as_float(0x7fffffff);
@@ -816,7 +855,7 @@ __global__ void __launch_bounds__(AtCfg<D, NQ, TP>::NW * 32, 1) lss_attend_kerne
 
 // Adds up the pieces of the groups that were cut between CTAs: one CTA per warp of the first kernel,
 // most with nothing to do.
-template <int D, int DT, int NQ, int TP>
+template <int D, int DT, int NQ, int TP, bool TREE>
 __global__ void __launch_bounds__(256) lss_attend_join_kernel(AttendArgs a) {
   pdl_wait();
   const int4 me = a.meta[blockIdx.x];

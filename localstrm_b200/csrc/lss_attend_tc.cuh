@@ -34,7 +34,7 @@ __device__ __forceinline__ int pa_tiles(const AttendArgs& a, const AtRow& w, int
   const int last = min((mt + 1) * PA_ROWS, w.n * a.per) - 1;
   return (w.len - w.n + last / a.per + 1 + PA_KT - 1) / PA_KT;
 }
-__device__ __noinline__ int64_t pa_units(const AttendArgs& a, int r) {
+static __device__ __noinline__ int64_t pa_units(const AttendArgs& a, int r) {
   const AtRow w = at_row<PA_ROWS / 8>(a, r);
   int64_t n = 0;
   for (int mt = 0; mt < w.mt; ++mt) n += pa_tiles(a, w, mt);
@@ -89,7 +89,11 @@ __device__ __forceinline__ uint32_t pa_place(int r, int q) {
 // tensor memory and barriers between steps are what is left above the bounds.
 // Bound by the exponentials (16 per cycle and SM: 2048 cycles per 256 x 128 scores) and the tensor pipe (the same
 // number of cycles at D = 128).
-template <int D, int DT>
+//
+// With TREE (see lss_attend_kernel) a step that holds new tokens begins with a thread's 64 comparisons, kept as
+// bits.  NaN among the new tokens' values, which only their own branches see, is looked for again by the rows that see
+// them, once a group, where there was any.
+template <int D, int DT, bool TREE>
 __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
   constexpr int CH = D / 8;                // 16-byte pieces of a row in f16
   constexpr int OPB = 128 * D * 2;         // bytes of a 128-row operand
@@ -103,7 +107,7 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
   __shared__ float2 sscale[4][8];          // scales of the tile's 16-token parts: of K (< 0: not seen), log2 of that of V
   __shared__ int nan_from[D];              // first position with a NaN among the values of a column
   __shared__ int64_t scr[PA_NT / 32], found_lo;
-  __shared__ int found, any_nan;
+  __shared__ int found, any_nan, branch_nan;  // branch_nan: NaN among the values of new tokens (TREE)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   unsigned char* base = pa_dyn + ((1024 - (saddr(pa_dyn) & 1023)) & 1023);
   unsigned char* qs = base;                // two query operands
@@ -194,7 +198,7 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
     const int i0 = tile0 * 2, i1 = min(tile1 * 2, (see_last + PA_HT - 1) / PA_HT);  // steps of 64 tokens
     float* piece = a.part + ((size_t)blockIdx.x * 2 + (tile0 == 0 ? 1 : 0)) * pa_piece(D);
     for (int i = tid; i < D; i += PA_NT) nan_from[i] = NOWHERE;
-    if (tid == 0) any_nan = 0;
+    if (tid == 0) any_nan = branch_nan = 0;
     __syncthreads();  // and nobody reads the last group's any more
 
     if (warp < 8) {
@@ -203,7 +207,12 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
       const bool in = rr < rows_here;
       const int qi = in ? (mt * PA_ROWS + rr) / a.per : 0;
       const int qh = head * a.per + (in ? mt * PA_ROWS + rr - qi * a.per : 0);
-      const int limit = in ? ctx + qi + 1 : 0;
+      const int limit = !in ? 0 : TREE ? ctx : ctx + qi + 1;  // TREE: and what `shows` says
+      const int at_place = TREE && in ? __ldg(&a.span[start + qi].x) : 0;
+      auto shows = [&](int t) {  // new token t, below see_last
+        const int2 b = __ldg(&a.span[start + t - ctx]);
+        return in && (uint32_t)at_place - (uint32_t)b.x < (uint32_t)b.y;
+      };
       const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
       float fq = fabsf(a.scale);
       // Loops of this part, and of the one behind the tiles, stay rolled: code that runs once per group comes from
@@ -273,7 +282,7 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
       float m = -INFINITY, l = 0.0f, w = -INFINITY;
       if (q < nq) {
         // The first row of the warp sees least.
-        const int see_warp = ctx + (mt * PA_ROWS + q * 128 + (warp & 3) * 32) / a.per + 1;
+        const int see_warp = TREE ? ctx : ctx + (mt * PA_ROWS + q * 128 + (warp & 3) * 32) / a.per + 1;
         for (int i = i0; i < i1; ++i, ++steps) {
           const int half = i & 1, at = i * PA_HT;
           tc_wait(&sfull[q][half], (phases >> half) & 1, &failed);
@@ -288,6 +297,15 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
 #pragma unroll
           for (int g = 0; g < 4; ++g) tc_ld16(s_here + 16 * g, x[g]);
           tc_wait_ld();
+          uint64_t seen = 0;  // TREE, masked: the step's tokens that this row sees
+          if (TREE && masked) {
+            const int old = min(max(limit - at, 0), PA_HT), upto = min(see_last - at, PA_HT);
+            if (old > 0) seen = ~0ull >> (PA_HT - old);
+#pragma unroll 8
+            for (int e = max(ctx - at, 0); e < upto; ++e)
+              if (shows(at + e)) seen |= 1ull << e;
+          }
+          auto sees = [&](int e) { return TREE ? ((seen >> e) & 1) != 0 : at + e < limit; };
           // Largest score, and largest weight of V.
           float top = -INFINITY, topw = -INFINITY, least = INFINITY;
           auto maxima = [&](auto mask_c) {
@@ -298,8 +316,8 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
               float t = -INFINITY;
 #pragma unroll
               for (int e = 0; e < 16; ++e)
-                if (!with_mask || at + 16 * g + e < limit) t = fmaxf(t, __uint_as_float(x[g][e]));
-              if (with_mask && (k.x < 0.0f || at + 16 * g >= limit)) continue;
+                if (!with_mask || sees(16 * g + e)) t = fmaxf(t, __uint_as_float(x[g][e]));
+              if (with_mask && (k.x < 0.0f || (TREE ? ((seen >> (16 * g)) & 0xffff) == 0 : at + 16 * g >= limit))) continue;
               t = fmaxf(t * (fq * k.x), -FLT_MAX);  // -inf and NaN: seen, unlike what leaves m at -inf
               top = fmaxf(top, t);
               topw = fmaxf(topw, t + k.y);
@@ -345,8 +363,8 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
               for (int e = 0; e < 16; e += 2) {
                 float y0 = fmaf(__uint_as_float(x[g][e]), fg, add), y1 = fmaf(__uint_as_float(x[g][e + 1]), fg, add);
                 if (with_mask) {
-                  if (k.x < 0.0f || at + 16 * g + e >= limit) y0 = -INFINITY;
-                  if (k.x < 0.0f || at + 16 * g + e + 1 >= limit) y1 = -INFINITY;
+                  if (k.x < 0.0f || !sees(16 * g + e)) y0 = -INFINITY;
+                  if (k.x < 0.0f || !sees(16 * g + e + 1)) y1 = -INFINITY;
                 }
                 float p0 = ex2(y0), p1 = ex2(y1);
                 part += p0 + p1;
@@ -384,6 +402,19 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
           uint32_t x[16];
           tc_ld16(o_at[q] + lanes + i, x);
           tc_wait_ld();
+          if (TREE && branch_nan) {
+#pragma unroll 1
+            for (int t = max(ctx, tile0 * PA_KT); t < min(see_last, tile1 * PA_KT); ++t) {
+              const int page = __ldg(a.table + row * a.table_stride + (t >> a.bs_shift));
+              if (!shows(t) || (unsigned)page >= (unsigned)a.num_blocks) continue;
+              const uint4 v = __ldg(reinterpret_cast<const uint4*>(
+                  a.vc + (((((int64_t)page * a.heads + head) << a.bs_shift) + (t & ((1 << a.bs_shift) - 1))) * D + i)));
+              const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+              for (int e = 0; e < 16; ++e)
+                if (((u[e >> 2] >> (8 * (e & 3))) & 0x7fu) == 0x7fu) x[e] = 0x7fffffffu;
+            }
+          }
           if (!whole) {
             float* to = piece + 3 * PA_ROWS + rr * D + i;
             if (in)
@@ -523,7 +554,10 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
             for (int e = 0; e < 4; ++e) {
               const uint32_t nan = __vcmpeq4(u[e] & 0x7f7f7f7fu, 0x7f7f7f7fu);
               for (int z = 0; z < 4; ++z)
-                if ((nan >> (8 * z)) & 1u) atomicMin(&nan_from[cc * 16 + 4 * e + z], j * PA_KT + t);
+                if ((nan >> (8 * z)) & 1u) {
+                  if (TREE && j * PA_KT + t >= ctx) branch_nan = 1;
+                  else atomicMin(&nan_from[cc * 16 + 4 * e + z], j * PA_KT + t);
+                }
               u[e] &= ~nan;
             }
           }
@@ -620,7 +654,7 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
 
 // Adds up the pieces of a group that was cut, the last one of the CTA before and the first ones of this
 // CTA and those after it; 32 rows per CTA.
-template <int D, int DT>
+template <int D, int DT, bool TREE>
 __global__ void __launch_bounds__(256) lss_attend_tc_join_kernel(AttendArgs a) {
   pdl_wait();
   const int cta = blockIdx.x / (PA_ROWS / 32), r0 = blockIdx.x % (PA_ROWS / 32) * 32;

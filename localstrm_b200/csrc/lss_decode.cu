@@ -1,244 +1,9 @@
 // lss_decode.cu — C ABI of the decode-step operators around the sampler: 4-bit products, block
 // tables, the 8-bit key/value cache and its attention.
-#include <algorithm>
-#include <cstdlib>
-#include <mutex>
-#include <utility>
-
-#include "lss_attend_tc.cuh"
+#include "lss_attend_host.cuh"
 #include "lss_blocks.cuh"
 #include "lss_int4_tc.cuh"
 #include "lss_kvcache.cuh"
-
-using namespace lss;
-
-static constexpr int MAX_DEV = 64;
-
-static int device_index() {
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= MAX_DEV) dev = 0;
-  return dev;
-}
-
-static std::mutex g_mu;
-
-static int sm_count(int dev) {
-  static int n[MAX_DEV] = {};
-  std::lock_guard<std::mutex> lock(g_mu);
-  if (n[dev] == 0 && (cudaDeviceGetAttribute(&n[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n[dev] < 1)) {
-    cudaGetLastError();
-    n[dev] = 0;
-    return 148;
-  }
-  return n[dev];
-}
-
-// Raises a kernel's dynamic shared memory limit, once per device and size.
-struct SmemSet {
-  int bytes[MAX_DEV] = {};
-};
-template <class K>
-static cudaError_t allow_smem(K kern, SmemSet& set, int dev, int bytes) {
-  std::lock_guard<std::mutex> lock(g_mu);
-  if (bytes <= set.bytes[dev]) return cudaSuccess;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e == cudaSuccess) set.bytes[dev] = bytes;
-  return e;
-}
-
-template <class... KA, class... A>
-static cudaError_t launch(void (*kern)(KA...), unsigned grid, unsigned block, size_t smem, int cluster, bool pdl,
-                          cudaStream_t st, A... args) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(grid, 1, 1);
-  cfg.blockDim = dim3(block, 1, 1);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute at[2];
-  int na = 0;
-  if (cluster > 1) {
-    at[na].id = cudaLaunchAttributeClusterDimension;
-    at[na].val.clusterDim.x = (unsigned)cluster;
-    at[na].val.clusterDim.y = 1;
-    at[na].val.clusterDim.z = 1;
-    ++na;
-  }
-  if (pdl) {
-    at[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[na].val.programmaticStreamSerializationAllowed = 1;
-    ++na;
-  }
-  cfg.attrs = at;
-  cfg.numAttrs = (unsigned)na;
-  return cudaLaunchKernelEx(&cfg, kern, args...);
-}
-
-static int status_of(cudaError_t e) {
-  if (e == cudaSuccess) return LSS_OK;
-  cudaGetLastError();
-  return LSS_ERR_CUDA;
-}
-
-static bool aligned_to(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
-static bool known_dtype(int d) { return d == LSS_DTYPE_F32 || d == LSS_DTYPE_BF16 || d == LSS_DTYPE_F16; }
-static bool block_size_ok(int bs) { return bs == 16 || bs == 32 || bs == 64 || bs == 128 || bs == 256; }
-// Rows of two matrices (start, bytes between rows, bytes of a row) that share memory.  Rows of one pitch may lie
-// beside each other.
-static bool rows_overlap(const void* x, int64_t x_pitch, int64_t x_row, const void* y, int64_t y_pitch, int64_t y_row, int rows) {
-  const int64_t d = (int64_t)(reinterpret_cast<intptr_t>(y) - reinterpret_cast<intptr_t>(x));
-  if (d >= (rows - 1) * x_pitch + x_row || -d >= (rows - 1) * y_pitch + y_row) return false;
-  if (rows == 1 || x_pitch != y_pitch) return true;
-  const int64_t at = (d % x_pitch + x_pitch) % x_pitch;  // where y's rows start in x's pitch
-  return at < x_row || at + y_row > x_pitch;
-}
-// Two arrays of T x H rows of n bytes (start, bytes between tokens and between heads) that share memory without
-// being the same rows: a result would be written where another CTA still reads its query.  With equal strides
-// exactly, else wherever the extents meet.
-static bool rows_shifted(const void* x, int64_t x_st, int64_t x_sh, const void* y, int64_t y_st, int64_t y_sh, int64_t T, int64_t H, int64_t n) {
-  if (T == 1) x_st = y_st = 0;  // one token, one head: the stride says nothing
-  if (H == 1) x_sh = y_sh = 0;
-  const int64_t d = (int64_t)(reinterpret_cast<intptr_t>(y) - reinterpret_cast<intptr_t>(x));
-  if (d >= (T - 1) * x_st + (H - 1) * x_sh + n || -d >= (T - 1) * y_st + (H - 1) * y_sh + n) return false;
-  if (x_st != y_st || x_sh != y_sh) return true;
-  if (d == 0) return false;
-  if (T < H) {  // the walk below is over the shorter side
-    std::swap(T, H);
-    std::swap(x_st, x_sh);
-  }
-  for (int64_t j = 1 - H; j < H; ++j) {  // rows i tokens and j heads apart begin d - i st - j sh bytes apart
-    const int64_t r = d - j * x_sh, i0 = x_st > 0 ? (r >= 0 ? r / x_st : -((-r + x_st - 1) / x_st)) : 0;
-    for (int64_t i = i0; i <= i0 + 1; ++i)
-      if (i > -T && i < T && std::abs(r - i * x_st) < n) return true;
-  }
-  return false;
-}
-// Arrays of n entries of which one begins inside the other.
-static bool cut(const int32_t* x, const int32_t* y, int64_t n) { return x != y && x < y + n && y < x + n; }
-static int log2_of(int v) {
-  int s = 0;
-  while ((1 << s) < v) ++s;
-  return s;
-}
-static int cluster_for(int64_t ctas, int most) {
-  int c = 1;
-  while (c < most && c < ctas) c <<= 1;
-  return c;
-}
-
-// ---------------------------------------------------------------- block tables
-static bool table_ok(const void* table, int64_t stride, int width, int B, int bs, int num_blocks) {
-  return (table || B == 0) && width >= 1 && stride >= width && B >= 0 && bs >= 1 && num_blocks >= 1 &&
-         (int64_t)width * bs <= (1 << 30);
-}
-
-// ---------------------------------------------------------------- attention
-static constexpr int AT_CAP_CTAS = 160;  // CTAs that the workspace has room for
-
-template <int D, int NQ, int TP>
-static size_t attend_bytes() {
-  const size_t workers = (size_t)AT_CAP_CTAS * AtCfg<D, NQ, TP>::NW;
-  return workers * (sizeof(int4) + 2 * at_piece(D, NQ) * sizeof(float));
-}
-
-template <int D, int DT, int NQ, int TP = 1>
-static cudaError_t launch_attend(AttendArgs a, void* ws, cudaStream_t st) {
-  static SmemSet set;
-  const int dev = device_index();
-  constexpr int NW = AtCfg<D, NQ, TP>::NW;
-  constexpr int smem = NW * AtCfg<D, NQ, TP>::ST * (32 * D + 16);
-  cudaError_t e = allow_smem(lss_attend_kernel<D, DT, NQ, TP>, set, dev, smem);
-  if (e != cudaSuccess) return e;
-  // No more warps than there can be units.
-  const int64_t groups = a.B + (int64_t)a.T * a.per / (8 * NQ) + 1;
-  const int64_t units = groups * a.heads * ((((int64_t)a.width << a.bs_shift) + 15) >> 4);
-  const int ctas = (int)std::min((int64_t)std::min(sm_count(dev), AT_CAP_CTAS), (units + NW - 1) / NW);
-  a.meta = reinterpret_cast<int4*>(ws);
-  a.part = reinterpret_cast<float*>(a.meta + (size_t)ctas * NW);
-  // Two tiles a warp and less on eight SMs: one launch (a call for one short request 20.6 -> 17.5 us on the host); with
-  // more tiles eight SMs' share of the bandwidth would cost more than the second launch.
-  a.fused = units <= 8 * NW * 2;
-  if (a.fused) {
-    const int size = ctas <= 1 ? 1 : ctas <= 2 ? 2 : ctas <= 4 ? 4 : 8;
-    return launch(lss_attend_kernel<D, DT, NQ, TP>, (unsigned)size, NW * 32, smem, size, false, st, a);
-  }
-  e = launch(lss_attend_kernel<D, DT, NQ, TP>, (unsigned)ctas, NW * 32, smem, 1, false, st, a);
-  if (e != cudaSuccess) return e;
-  return launch(lss_attend_join_kernel<D, DT, NQ, TP>, (unsigned)(ctas * NW), 256, 0, 1, true, st, a);
-}
-
-template <int D>
-static size_t attend_tc_bytes() {
-  return (size_t)AT_CAP_CTAS * (sizeof(int4) + 2 * pa_piece(D) * sizeof(float));
-}
-
-template <int D, int DT>
-static cudaError_t launch_attend_tc(AttendArgs a, void* ws, cudaStream_t st) {
-  static SmemSet set;
-  const int dev = device_index();
-  constexpr int smem = 1024 + 6 * 128 * D * 2;
-  cudaError_t e = allow_smem(lss_attend_tc_kernel<D, DT>, set, dev, smem);
-  if (e != cudaSuccess) return e;
-  const int ctas = std::min(sm_count(dev), AT_CAP_CTAS);
-  a.meta = reinterpret_cast<int4*>(ws);
-  a.part = reinterpret_cast<float*>(a.meta + AT_CAP_CTAS);
-  e = launch(lss_attend_tc_kernel<D, DT>, (unsigned)ctas, PA_NT, smem, 1, false, st, a);
-  if (e != cudaSuccess) return e;
-  return launch(lss_attend_tc_join_kernel<D, DT>, (unsigned)(ctas * (PA_ROWS / 32)), 256, 0, 1, true, st, a);
-}
-
-// `rows`: query rows per key head that a row of the batch has.
-template <int D, int DT>
-static cudaError_t launch_attend_few(const AttendArgs& a, int64_t rows, void* ws, cudaStream_t st) {
-  if (rows <= 8) {
-    // Long contexts take two tiles a step (AtCfg); how long they are only the table's width tells here.
-    if constexpr (D == 128) {
-      if (((int64_t)a.width << a.bs_shift) >= 1024) return launch_attend<D, DT, 1, 2>(a, ws, st);
-    }
-    return launch_attend<D, DT, 1>(a, ws, st);
-  }
-  if constexpr (D < 256) {
-    if (rows > 16) return launch_attend<D, DT, 4>(a, ws, st);
-  }
-  return launch_attend<D, DT, 2>(a, ws, st);
-}
-
-// A step of single tokens has `per` query rows per key head and row; else the average decides.  A step with more
-// tokens than rows, and enough of them to fill the SMs, may mix prompt chunks, rows of a few tokens and single
-// tokens, and only the device knows which is which: rows of pa_from query rows and more go to the tensor-memory
-// kernel (which would widen the codes for 256 rows of which `per` are there), the others to the one for few rows, one
-// launch after the other on the same workspace.  Its group is that of a single token, or of 16 rows where the average
-// row is a short one.  Measured at 64 rows over 50 to 16,000 tokens, 8 key heads of 4 queries of 128 (in groups of 8 for comparison):
-// 5 tokens each 512 us (606), 8 tokens 532 (813), 9 tokens 750 (977); tensor memory from 41 rows on, 12 tokens 944 (1,190); single tokens
-// beside one chunk of 449 pay for it, 244 (219).  At D = 64 and with more heads per key head the tensor-memory kernel
-// is slower than groups of 16 up to 63 rows (9 tokens of D = 64: 668 us, 435).  Steps of chunks alone pay 10 us for the
-// second one's empty launches (220 -> 232 us for four chunks of 300 to 400 tokens); 60 single tokens over 6,000 beside two
-// chunks of 2,048 take 420 us.
-// A step of no more tokens than rows counts as one of single tokens: a chunk among idle rows is right, but goes in
-// their groups (200 tokens over 8,000 beside 255 idle rows 213 us, alone 201; 500 beside 511 507 us, alone 171), as the
-// launches for chunks would cost every step of single tokens 8 to 10 us.
-template <int D, int DT>
-static cudaError_t launch_attend_rows(AttendArgs a, void* ws, cudaStream_t st) {
-  const int64_t average = (int64_t)a.per * ((a.T + (int64_t)a.B - 1) / a.B);
-  a.rows_lo = 0;
-  a.rows_hi = INT32_MAX;
-  if constexpr (D < 256) {
-    if (a.T > a.B && (int64_t)a.heads * a.per * a.T >= (int64_t)PA_ROWS * sm_count(device_index()) / 4) {
-      const int pa_from = D == 128 && a.per <= 8 ? 41 : 64;
-      a.rows_lo = pa_from;
-      const cudaError_t e = launch_attend_tc<D, DT>(a, ws, st);
-      if (e != cudaSuccess) return e;
-      a.rows_lo = 0;
-      a.rows_hi = pa_from;
-      return launch_attend_few<D, DT>(a, average < pa_from ? std::max((int64_t)a.per, std::min(average, (int64_t)16)) : a.per, ws, st);
-    }
-  }
-  return launch_attend_few<D, DT>(a, average, ws, st);
-}
-
-template <int D>
-static cudaError_t launch_attend_dt(int dtype, const AttendArgs& a, void* ws, cudaStream_t st) {
-  return dtype == LSS_DTYPE_BF16 ? launch_attend_rows<D, LSS_DTYPE_BF16>(a, ws, st) : launch_attend_rows<D, LSS_DTYPE_F16>(a, ws, st);
-}
 
 // ---------------------------------------------------------------- 4-bit products
 static constexpr int I4_SMEM = 227 * 1024;
@@ -571,56 +336,7 @@ int lss_attend(const void* q, int64_t q_token_stride, int64_t q_head_stride, int
                int width, const int32_t* starts, const int32_t* granted, const int32_t* lens, int B, float scale,
                void* out, int64_t out_token_stride, int64_t out_head_stride, float* lse, void* workspace,
                size_t workspace_bytes, void* stream) {
-  if ((dtype != LSS_DTYPE_BF16 && dtype != LSS_DTYPE_F16) || T < 0 || heads < 1 || q_heads < heads ||
-      q_heads % heads != 0 || !block_size_ok(block_size))
-    return LSS_ERR_INVALID_ARG;
-  if (q_token_stride < 0 || q_head_stride < 0 || out_token_stride < 0 || out_head_stride < dim) return LSS_ERR_INVALID_ARG;
-  if (!table_ok(table, table_stride, width, B, block_size, num_blocks)) return LSS_ERR_INVALID_ARG;
-  if (dim != 64 && dim != 128 && dim != 256) return LSS_ERR_UNSUPPORTED;
-  if (heads > 65536 || (int64_t)T * q_heads > (1 << 30)) return LSS_ERR_UNSUPPORTED;
-  if (B == 0 || T == 0) return LSS_OK;
-  if (!q || !out || !k_cache || !v_cache || !k_scale || !v_scale || !starts || !granted || !lens)
-    return LSS_ERR_INVALID_ARG;
-  if (!aligned_to(k_cache, 16) || !aligned_to(v_cache, 16)) return LSS_ERR_INVALID_ARG;
-  if (T > 1 && out_token_stride < (q_heads - 1) * out_head_stride + dim &&
-      (out_token_stride < dim || out_head_stride < (T - 1) * out_token_stride + dim))
-    return LSS_ERR_INVALID_ARG;  // rows of the result lie over each other, whether tokens or heads are outside
-  if (rows_shifted(q, 2 * q_token_stride, 2 * q_head_stride, out, 2 * out_token_stride, 2 * out_head_stride, T, q_heads, 2 * (int64_t)dim))
-    return LSS_ERR_INVALID_ARG;
-  if (!workspace || workspace_bytes < lss_attend_workspace_bytes(dim) || !aligned_to(workspace, 16)) return LSS_ERR_WORKSPACE;
-  AttendArgs a{};
-  a.q = q;
-  a.q_st = q_token_stride;
-  a.q_sh = q_head_stride;
-  a.out = out;
-  a.o_st = out_token_stride;
-  a.o_sh = out_head_stride;
-  a.lse = lse;
-  a.kc = k_cache;
-  a.vc = v_cache;
-  a.ks = k_scale;
-  a.vs = v_scale;
-  a.num_blocks = num_blocks;
-  a.heads = heads;
-  a.per = q_heads / heads;
-  a.bs_shift = log2_of(block_size);
-  a.table = table;
-  a.table_stride = table_stride;
-  a.width = width;
-  a.starts = starts;
-  a.granted = granted;
-  a.lens = lens;
-  a.B = B;
-  a.T = T;
-  a.scale = scale * LOG2E;
-  a.aligned = aligned_to(q, 16) && aligned_to(out, 16) && q_token_stride % 8 == 0 && q_head_stride % 8 == 0 &&
-              out_token_stride % 8 == 0 && out_head_stride % 8 == 0;
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  switch (dim) {
-    case 64: return status_of(launch_attend_dt<64>(dtype, a, workspace, st));
-    case 128: return status_of(launch_attend_dt<128>(dtype, a, workspace, st));
-    default: return status_of(launch_attend_dt<256>(dtype, a, workspace, st));
-  }
+  return attend_entry<false>(q, q_token_stride, q_head_stride, dtype, T, q_heads, heads, dim, k_cache, v_cache, k_scale, v_scale, num_blocks, block_size, table, table_stride, width, starts, granted, lens, B, scale, out, out_token_stride, out_head_stride, lse, workspace, workspace_bytes, nullptr, stream);
 }
 
 }  // extern "C"

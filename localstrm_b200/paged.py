@@ -17,7 +17,7 @@ import torch
 from . import _lib
 from .head import _CODES, _on, _stream
 
-__all__ = ["StepPlan", "KVCache8", "plan_blocks", "release_blocks", "append_kv", "attend"]
+__all__ = ["StepPlan", "TreePlan", "Forks", "KVCache8", "plan_blocks", "release_blocks", "fork_blocks", "copy_blocks", "append_kv", "attend"]
 
 
 @dataclass
@@ -51,6 +51,30 @@ class StepPlan:
         if prompt_lens is not None:
             own = own & (self.lens >= prompt_lens)
         return torch.where(own, codes, 0)
+
+
+@dataclass
+class TreePlan:
+    """The trees of a step's new tokens, as ``plan_tree`` makes them (int32 on the device).
+
+    ``span [T, 2]``: a token's place in the pre-order of its row's tree and the number of tokens of its branch (token j is
+    i or an ancestor of it where ``0 <= span[i, 0] - span[j, 0] < span[j, 1]``); ``positions [T]``: context and depth,
+    for the rotation; ``parents [T]``: what ``plan_tree`` was given.
+    """
+    span: torch.Tensor
+    positions: torch.Tensor
+    parents: torch.Tensor
+
+
+@dataclass
+class Forks:
+    """What ``fork_blocks`` did (int32 on the device): ``lens [B]`` and ``n_free [1]`` afterwards; ``granted [n]``: tokens
+    that a fork took (0: refused); ``copies [n, 2]``: the block to copy for it and the one it is copied to (-1, -1: none),
+    for ``copy_blocks`` on every layer's cache."""
+    lens: torch.Tensor
+    n_free: torch.Tensor
+    granted: torch.Tensor
+    copies: torch.Tensor
 
 
 @dataclass
@@ -144,10 +168,15 @@ def plan_blocks(block_table: torch.Tensor, lens: torch.Tensor, new_lens: torch.T
 
 def release_blocks(block_table: torch.Tensor, lens: torch.Tensor, codes: torch.Tensor, free_blocks: torch.Tensor,
                    n_free: torch.Tensor, block_size: int, lens_out: Optional[torch.Tensor] = None,
-                   n_free_out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+                   n_free_out: Optional[torch.Tensor] = None, keep: Optional[torch.Tensor] = None,
+                   shares: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """Returns the blocks of the rows with a non-zero code (``check_stop_batch``'s, through
     ``StepPlan.stops``) to ``free_blocks``, in row and block order; their lengths become 0.  Gives ``(lens, n_free)`` afterwards; ``lens_out`` and
-    ``n_free_out`` as for ``plan_blocks``.  Blocks that rows share must be released once."""
+    ``n_free_out`` as for ``plan_blocks``.
+
+    With ``keep [B]`` the other rows give back what lies behind their first ``keep[b]`` tokens, which become their length
+    (``Accepted.lens``).  With ``shares [num_blocks]`` (as ``fork_blocks`` keeps them) a block goes back with the last of its
+    holders, in the order of these; without, blocks that rows share must be released once."""
     dev, B, width, stride = _table(block_table)
     lens_at, codes_at = _ints("lens", lens, B, dev), _ints("codes", codes, B, dev)
     blocks = free_blocks.numel()
@@ -158,12 +187,68 @@ def release_blocks(block_table: torch.Tensor, lens: torch.Tensor, codes: torch.T
         lens_out = torch.empty(B, dtype=_I32, device=block_table.device)
     if n_free_out is None:
         n_free_out = torch.empty(1, dtype=_I32, device=block_table.device)
+    lens_out_at, n_free_out_at = _ints("lens_out", lens_out, B, dev), _ints("n_free_out", n_free_out, 1, dev)
     lib = _lib.load()
     with _on(dev):
-        _lib.check("lss_block_release", lib.lss_block_release(
-            block_table.data_ptr(), stride, width, lens_at, codes_at, B, block_size, free_at, blocks, n_free_at,
-            _ints("lens_out", lens_out, B, dev), _ints("n_free_out", n_free_out, 1, dev), _stream(dev)))
+        if keep is None and shares is None:
+            _lib.check("lss_block_release", lib.lss_block_release(
+                block_table.data_ptr(), stride, width, lens_at, codes_at, B, block_size, free_at, blocks, n_free_at,
+                lens_out_at, n_free_out_at, _stream(dev)))
+        else:
+            _lib.check("lss_block_give", lib.lss_block_give(
+                block_table.data_ptr(), stride, width, lens_at, codes_at, None if keep is None else _ints("keep", keep, B, dev), B,
+                block_size, None if shares is None else _ints("shares", shares, blocks, dev), free_at, blocks, n_free_at,
+                lens_out_at, n_free_out_at, _stream(dev)))
     return lens_out, n_free_out
+
+
+def fork_blocks(block_table: torch.Tensor, lens: torch.Tensor, src_rows: torch.Tensor, dst_rows: torch.Tensor,
+                shares: torch.Tensor, free_blocks: torch.Tensor, n_free: torch.Tensor, block_size: int,
+                upto: Optional[torch.Tensor] = None, lens_out: Optional[torch.Tensor] = None,
+                n_free_out: Optional[torch.Tensor] = None) -> Forks:
+    """Lets the idle rows ``dst_rows [n]`` go on from the tokens of the rows ``src_rows [n]``, from the first ``upto [n]`` of
+    them where given: more samples of a prompt, or a prompt whose beginning another row holds.
+
+    Their full blocks are shared: ``shares [num_blocks]`` (int32, zeros at first) counts the holders beyond the first, in
+    place; the tokens behind these get a block of their own from the free list, to be filled by ``copy_blocks`` on every layer's
+    cache.  Forks are served in order, as the rows of ``plan_blocks`` are; one is refused where its rows are outside the
+    table, the destination is not idle or an earlier fork's, or there is nothing to take.  Lengths are those before the call.
+    ``lens_out`` / ``n_free_out`` as for ``plan_blocks``.  Blocks so shared are given back with ``release_blocks(shares=)``."""
+    dev, B, width, stride = _table(block_table)
+    n, blocks = src_rows.numel(), free_blocks.numel()
+    if blocks < 1:
+        raise ValueError("free_blocks must not be empty")
+    lens_at = _ints("lens", lens, B, dev)
+    free_at, n_free_at = _ints("free_blocks", free_blocks, blocks, dev), _ints("n_free", n_free, 1, dev)
+    # One allocation for the results.
+    copies, granted, new_state, new_free = torch.empty(3 * n + B + 1, dtype=_I32, device=block_table.device).split_with_sizes((2 * n, n, B, 1))
+    lens_out, n_free_out = new_state if lens_out is None else lens_out, new_free if n_free_out is None else n_free_out
+    lib = _lib.load()
+    with _on(dev):
+        _lib.check("lss_block_fork", lib.lss_block_fork(
+            block_table.data_ptr(), stride, width, lens_at, B, block_size, _ints("src_rows", src_rows, n, dev),
+            _ints("dst_rows", dst_rows, n, dev), None if upto is None else _ints("upto", upto, n, dev), n,
+            _ints("shares", shares, blocks, dev), free_at, blocks, n_free_at, granted.data_ptr(), copies.data_ptr(),
+            _ints("lens_out", lens_out, B, dev), _ints("n_free_out", n_free_out, 1, dev), _stream(dev)))
+    return Forks(lens_out, n_free_out, granted, copies.view(n, 2))
+
+
+def copy_blocks(cache: "KVCache8", copies: torch.Tensor) -> None:
+    """Copies whole blocks of one layer's cache, with their scales: ``copies`` int32 ``[n, 2]``, from and to (``Forks.copies``).
+    Pairs that are not two blocks of the cache are passed over.  No block may be copied to twice, or both copied from and
+    to, in one call."""
+    if not isinstance(copies, torch.Tensor) or not copies.is_cuda:
+        raise RuntimeError("copies: a CUDA tensor is needed (no CPU fallback)")
+    dev = copies.get_device()
+    blocks, heads, bs, dim = cache.check(dev)
+    if copies.dim() != 2 or copies.shape[1] != 2:
+        raise ValueError("copies: expected int32 [n, 2]")
+    n = copies.shape[0]
+    lib = _lib.load()
+    with _on(dev):
+        _lib.check("lss_kv_copy", lib.lss_kv_copy(
+            cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), blocks, heads, bs, dim,
+            _ints("copies", copies, 2 * n, dev), n, _stream(dev)))
 
 
 def append_kv(cache: KVCache8, k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor, plan: StepPlan) -> None:
@@ -198,12 +283,14 @@ def append_kv(cache: KVCache8, k: torch.Tensor, v: torch.Tensor, block_table: to
 
 
 def attend(q: torch.Tensor, cache: KVCache8, block_table: torch.Tensor, plan: StepPlan, scale: Optional[float] = None,
-           out: Optional[torch.Tensor] = None, lse_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+           out: Optional[torch.Tensor] = None, lse_out: Optional[torch.Tensor] = None,
+           tree: Optional[TreePlan] = None) -> torch.Tensor:
     """Causal softmax attention of the step's queries ``[T, q_heads, dim]`` (bf16 or f16; dim 64, 128 or
     256) over the cache, one token per row or many; query head h reads key head ``h // (q_heads / heads)``.
 
     The queries of row b see its positions up to their own, the step's own tokens among them (append
-    first).  A step of no more tokens than rows is taken for one of single tokens; a chunk among many idle rows
+    first).  With a ``tree`` (``plan_tree``'s) the step's tokens lie in the cache in their order, and a query sees the tokens before
+    them, itself and its ancestors.  A step of no more tokens than rows is taken for one of single tokens; a chunk among many idle rows
     runs faster where only the rows with tokens are passed.  ``scale`` defaults to ``dim ** -0.5``; ``lse_out`` (float32 ``[T, q_heads]``) receives the natural
     log of the softmax sums.  ``out`` may be ``q`` itself; where it overlaps q in any other way the call is
     refused.  Tokens of refused rows, and those behind the last row, are left as they
@@ -231,6 +318,12 @@ def attend(q: torch.Tensor, cache: KVCache8, block_table: torch.Tensor, plan: St
     if lse_out is not None and (lse_out.dtype is not _F32 or lse_out.shape != shape[:2] or lse_out.get_device() != dev
                                 or not lse_out.is_contiguous()):
         raise ValueError(f"lse_out: expected a contiguous float32 {list(shape[:2])} on cuda:{dev}")
+    extra = ()
+    if tree is not None:
+        span = tree.span
+        if span.dim() != 2 or span.shape[0] != shape[0]:
+            raise ValueError(f"tree.span: expected int32 [{shape[0]}, 2]")
+        extra = (_ints("tree.span", span, 2 * shape[0], dev),)
     lib = _lib.load()
     with _on(dev):
         # From torch's allocator for every call: calls on other streams, and captured ones, have their own.
@@ -238,12 +331,13 @@ def attend(q: torch.Tensor, cache: KVCache8, block_table: torch.Tensor, plan: St
         if size is None:
             size = _WORKSPACE[dim] = int(lib.lss_attend_workspace_bytes(dim))
         ws = torch.empty(size, dtype=torch.uint8, device=block_table.device)
-        _lib.check("lss_attend", lib.lss_attend(
+        name = "lss_attend" if tree is None else "lss_attend_tree"
+        _lib.check(name, getattr(lib, name)(
             q.data_ptr(), qs[0], qs[1], _CODES[dtype], shape[0], shape[1], heads, dim, cache.k.data_ptr(), cache.v.data_ptr(),
             cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), blocks, bs, block_table.data_ptr(), stride, width,
             _ints("plan.starts", plan.starts, B + 1, dev), _ints("plan.granted", plan.granted, B, dev),
             _ints("plan.lens", plan.lens, B, dev), B, dim ** -0.5 if scale is None else scale, out.data_ptr(), os[0], max(os[1], dim),
-            None if lse_out is None else lse_out.data_ptr(), ws.data_ptr(), size, _stream(dev)))
+            None if lse_out is None else lse_out.data_ptr(), ws.data_ptr(), size, *extra, _stream(dev)))
     return out
 
 
