@@ -13,22 +13,40 @@ static bool tokens_overlap(const void* x, int64_t x_st, int64_t x_sh, int x_head
   return rows_overlap(x, x_st, (x_heads - 1) * x_sh + n, y, y_st, (y_heads - 1) * y_sh + n, T);
 }
 
-template <int DT, int N, int L>
+template <int DT, int N, int L, bool PAIRS>
 static cudaError_t launch_rotate(const RotateArgs& a, cudaStream_t st) {
-  const int hs = a.side[0].heads + a.side[1].heads, teams = RO_NT / L, sms = sm_count(device_index());
-  // Tokens per CTA: four heads a team, as long as there are six CTAs per SM, and 32 KB of cosines and sines.
-  int tk = std::max(1, std::min((4 * teams + hs - 1) / hs, a.T / (6 * sms)));
-  if (a.half > 0) tk = std::min(tk, std::max(1, 4096 / a.half));
-  const size_t smem = (size_t)tk * a.half * 8 + (size_t)a.dim * 8;
-  return launch(lss_rotate_kernel<DT, N, L>, (unsigned)((a.T + tk - 1) / tk), RO_NT, smem, 1, false, st, a, tk);
+  const int teams = RO_NT / L, sms = sm_count(device_index());
+  // Tokens per CTA, a power of two.  A wave of three CTAs per SM takes about as long as its teams' heads and four more
+  // (start, weights, sines): 1,000 tokens of 32 + 8 heads of 128 one by one 22 us, four by four 14; 8,192 by 8 or 32 39 us, by 16 45.
+  int tk = 1;
+  int64_t best = INT64_MAX;
+  for (int t = 1; t <= teams; t *= 2) {
+    const int per = teams / t, ctas = (a.T + t - 1) / t;
+    const int64_t cost = (int64_t)((ctas + 3 * sms - 1) / (3 * sms)) * (4 + (a.side[0].heads + per - 1) / per + (a.side[1].heads + per - 1) / per);
+    if (cost < best) {
+      best = cost;
+      tk = t;
+    }
+  }
+  const int ring = N > 1 ? RO_ST * 2 * 16 * RO_NT : 0;
+  const int smem = ring + a.dim * 8 + tk * a.half * 8;
+  static SmemSet set;
+  const cudaError_t e = allow_smem(lss_rotate_kernel<DT, N, L, PAIRS>, set, device_index(), smem);
+  if (e != cudaSuccess) return e;
+  return launch(lss_rotate_kernel<DT, N, L, PAIRS>, (unsigned)((a.T + tk - 1) / tk), RO_NT, smem, 1, false, st, a, tk);
+}
+template <int DT, bool PAIRS>
+static cudaError_t launch_rotate_dim(const RotateArgs& a, bool wide, cudaStream_t st) {
+  constexpr int N = DT == LSS_DTYPE_F32 ? 4 : 8;  // values in 16 bytes
+  if (!wide) return launch_rotate<DT, 1, 32, PAIRS>(a, st);
+  if (a.dim <= 8 * N) return launch_rotate<DT, N, 4, PAIRS>(a, st);
+  if (a.dim <= 16 * N) return launch_rotate<DT, N, 8, PAIRS>(a, st);
+  if (a.dim <= 32 * N) return launch_rotate<DT, N, 16, PAIRS>(a, st);
+  return launch_rotate<DT, N, 32, PAIRS>(a, st);
 }
 template <int DT>
 static cudaError_t launch_rotate_dt(const RotateArgs& a, bool wide, cudaStream_t st) {
-  if (!wide) return launch_rotate<DT, 1, 32>(a, st);
-  if (a.dim <= 64) return launch_rotate<DT, 8, 4>(a, st);
-  if (a.dim <= 128) return launch_rotate<DT, 8, 8>(a, st);
-  if (a.dim <= 256) return launch_rotate<DT, 8, 16>(a, st);
-  return launch_rotate<DT, 8, 32>(a, st);
+  return a.interleaved ? launch_rotate_dim<DT, true>(a, wide, st) : launch_rotate_dim<DT, false>(a, wide, st);
 }
 
 static bool rows_ok(const void* x, int64_t st, int64_t sh, int heads, int T, int dim) {
@@ -73,8 +91,9 @@ int lss_norm_rotate(const void* q, int64_t q_token_stride, int64_t q_head_stride
   a.w_dtype = weight_dtype;
   a.interleaved = interleaved != 0;
   a.eps = eps;
-  // Eight values at a time where all groups of eight lie on 16-byte boundaries and turn with one other group.
-  bool wide = dim % 16 == 0 && a.half % 8 == 0;
+  // 16 bytes at a time where all groups of values lie on 16-byte boundaries and turn with one other group; f32 up to
+  // a dim of 256 (a lane's 8 values times 32).
+  bool wide = dim % 16 == 0 && a.half % 8 == 0 && dim * e <= 1024;
   for (const RotateSide& s : a.side) {
     const int64_t per16 = 16 / e;
     wide = wide && aligned_to(s.x, 16) && aligned_to(s.y, 16) && s.x_st % per16 == 0 && s.x_sh % per16 == 0 && s.y_st % per16 == 0 &&
