@@ -47,7 +47,7 @@ template <int D, int DT, bool TREE>
 static inline cudaError_t launch_attend_tc(AttendArgs a, void* ws, cudaStream_t st) {
   static SmemSet set;
   const int dev = device_index();
-  constexpr int smem = 1024 + 6 * 128 * D * 2;
+  constexpr int smem = pa_smem(D);
   cudaError_t e = allow_smem(lss_attend_tc_kernel<D, DT, TREE>, set, dev, smem);
   if (e != cudaSuccess) return e;
   const int ctas = std::min(sm_count(dev), AT_CAP_CTAS);

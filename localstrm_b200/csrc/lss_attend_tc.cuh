@@ -10,10 +10,15 @@
 namespace lss {
 
 constexpr int PA_ROWS = 256;   // query rows of a group: two tiles of 128
-constexpr int PA_KT = 128;     // tokens of a tile of keys and values
-constexpr int PA_HT = 64;      // tokens that a softmax step takes: half a tile
-constexpr int PA_CONV = 7;     // warps that widen keys and values (16 in all: 128 registers a thread)
-constexpr int PA_NT = (8 + PA_CONV + 1) * 32;
+constexpr int PA_KT = 128;     // tokens of a unit of work
+constexpr int PA_HT = 64;      // tokens of a step: of the copies, the widening, the products and the softmax
+constexpr int PA_CONV = 4;     // warps that widen keys and values
+constexpr int PA_NT = (8 + PA_CONV + 3) * 32;  // and two that issue products, one that issues copies
+constexpr int PA_OP = 3;       // stages of widened keys, and of values
+constexpr int PA_SC = 8;       // stages of scales: steps between the copies and the softmax, and some
+// Stages of keys and values as they come: 48 KB.
+__host__ __device__ constexpr int pa_raw(int D) { return D == 64 ? 6 : 3; }
+__host__ __device__ constexpr int pa_smem(int D) { return 1024 + 2 * 128 * D * 2 + 2 * PA_OP * PA_HT * D * 2 + pa_raw(D) * 2 * PA_HT * D; }
 
 // D (+)= A B, both operands in shared memory.
 __device__ __forceinline__ void tc_mma_ss(uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, bool add) {
@@ -64,31 +69,31 @@ __device__ __forceinline__ int64_t pa_sum(int64_t v, int64_t* scr) {
 // Floats of one piece in the workspace: m, l, W of its rows, the sums, the first positions with NaN.
 __host__ __device__ constexpr int pa_piece(int D) { return PA_ROWS * (3 + D) + D; }
 
-// Where 16 bytes (8 values) `q` of row `r` lie in an operand of 128 rows: panels of 64 columns, a
+// Where 16 bytes (8 values) `q` of row `r` lie in an operand of ROWS rows: panels of 64 columns, a
 // 128-byte line per row, pieces permuted by the row (the 128-byte swizzle).
+template <int ROWS = 128>
 __device__ __forceinline__ uint32_t pa_place(int r, int q) {
-  return (uint32_t)((q >> 3) * (128 * 128) + r * 128 + (((q & 7) ^ (r & 7)) << 4));
+  return (uint32_t)((q >> 3) * (ROWS * 128) + r * 128 + (((q & 7) ^ (r & 7)) << 4));
 }
 
 // o = softmax(c q K^T) V for groups of 256 query rows (`per` heads times new tokens of one row and key head).
 //
-// Two tiles of 128 rows have a warpgroup each, a thread per row, and take 64 tokens a step: while it takes the
-// softmax of a step's scores, the next step's are under way.  Scores S = Q K^T (two places of 128 x 64, f32) lie in
-// tensor memory, the weights take their place as f16, the sums O stay there for the whole group.  Keys and
-// values come as e4m3 and are widened to f16 by seven warps into two stages of shared memory, once for
-// 256 rows (exact; 16 rows at a time, the widening is what bounds lss_attend_kernel here).
+// Two streams of work, each a warpgroup with a thread per query row, a warp that issues its products and its own part
+// of tensor memory: scores S = Q K^T of 64 tokens (two places of 128 x 64, f32), which the weights replace as f16, and the
+// sums O, which stay there for the whole group.  A group of more than 128 rows has a tile of 128 in each stream; in
+// one of fewer rows the streams take the same rows and every other step of 64 tokens each, and are added up at the end
+// (128 rows over 192,000 tokens and 8 heads: the second warpgroup idle 424 us).
+// Keys and values come as e4m3 through bulk copies that one warp issues, 48 KB on their way, and are widened to f16 by four
+// warps into three stages each, once for all rows (exact; 16 rows at a time, the widening is what bounds
+// lss_attend_kernel here).
 // Scales and the power of two of a query row act as in lss_attend_kernel; the weight of V is
 // p 2^(m + log2(v scale) - W + 10) from the softmax's own p, one exponential per score.  Both running
 // maxima may lag by 2^5, so that O is rarely rescaled.
-// NaN among the values is kept out of the products (0 NaN of a masked place would spoil the row) and
-// held as the first position per column from which it is seen.
+// NaN among values that all rows of the group see takes its way through the products.  In steps that some rows do not
+// see whole it is kept out of them (0 NaN of a masked place would spoil the row) and held as the first position
+// per column from which it is seen.
 // The units (group, tile of 128 tokens that it sees) are cut into equal ranges, one per CTA; pieces of a
 // group are added up by lss_attend_tc_join_kernel.
-// Measured: 296 to 416 new tokens over 3,000 to 5,300 (four rows, 32 query, 8 key heads of 128) 222 to 240 us, 410 to 450
-// TFLOP/s, against 640 us with lss_attend_kernel; D = 64 165 to 185 us.  About 5,000 cycles per 256 x 128 scores at 48 % issue: waits for
-// tensor memory and barriers between steps are what is left above the bounds.
-// Bound by the exponentials (16 per cycle and SM: 2048 cycles per 256 x 128 scores) and the tensor pipe (the same
-// number of cycles at D = 128).
 //
 // With TREE (see lss_attend_kernel) a step that holds new tokens begins with a thread's 64 comparisons, kept as
 // bits.  NaN among the new tokens' values, which only their own branches see, is looked for again by the rows that see
@@ -97,31 +102,41 @@ template <int D, int DT, bool TREE>
 __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
   constexpr int CH = D / 8;                // 16-byte pieces of a row in f16
   constexpr int OPB = 128 * D * 2;         // bytes of a 128-row operand
-  constexpr int PIECES = PA_KT * D / 16;   // 16-byte pieces of a tile in e4m3
-  constexpr int PER_T = (PIECES + PA_CONV * 32 - 1) / (PA_CONV * 32);
+  constexpr int STB = PA_HT * D * 2;       // bytes of a step's keys or values, widened
+  constexpr int RAWB = PA_HT * D;          // and as they come
+  constexpr int RS = pa_raw(D), OP = PA_OP;
+  constexpr int PIECES = RAWB / 16 / (PA_CONV * 32);  // 16-byte pieces of a step's keys (or values) per widening thread
   constexpr uint32_t NOWHERE = 0x7fffffff;
   extern __shared__ __align__(1024) unsigned char pa_dyn[];
-  __shared__ __align__(8) uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sfull[2][2], pready[2][2], pvdone[2], ofull[2], qready;
+  __shared__ __align__(8) uint64_t rfull[RS], rempty[RS], kfull[OP], kempty[OP], vfull[OP], vempty[OP], sfull[2][2], pready[2][2], pvdone[2], ofull[2], qready;
   __shared__ uint32_t tmem_base;
   __shared__ int failed;
-  __shared__ float2 sscale[4][8];          // scales of the tile's 16-token parts: of K (< 0: not seen), log2 of that of V
+  __shared__ __align__(16) float2 sscale[PA_SC][4];      // scales of the step's 16-token parts: of K (< 0: not seen), log2 of that of V
   __shared__ int nan_from[D];              // first position with a NaN among the values of a column
+  __shared__ float row_factor[128];
   __shared__ int64_t scr[PA_NT / 32], found_lo;
   __shared__ int found, any_nan, branch_nan;  // branch_nan: NaN among the values of new tokens (TREE)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   unsigned char* base = pa_dyn + ((1024 - (saddr(pa_dyn) & 1023)) & 1023);
   unsigned char* qs = base;                // two query operands
-  unsigned char* ksm = base + 2 * OPB;     // two stages of keys
-  unsigned char* vsm = base + 4 * OPB;     // two stages of values
+  unsigned char* ksm = base + 2 * OPB;     // stages of keys
+  unsigned char* vsm = ksm + OP * STB;     // stages of values
+  unsigned char* raw = vsm + OP * STB;     // stages of both as they come
 
   if (warp == 0) tc_alloc(&tmem_base, 512);
   if (tid == 0) {
     failed = 0;
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < RS; ++i) {
+      mbar_init(&rfull[i], 1);
+      mbar_init(&rempty[i], PA_CONV);
+    }
+    for (int i = 0; i < OP; ++i) {
       mbar_init(&kfull[i], PA_CONV);
       mbar_init(&vfull[i], PA_CONV);
-      mbar_init(&kempty[i], 1);
-      mbar_init(&vempty[i], 1);
+      mbar_init(&kempty[i], 2);
+      mbar_init(&vempty[i], 2);
+    }
+    for (int i = 0; i < 2; ++i) {
       for (int h = 0; h < 2; ++h) {
         mbar_init(&sfull[i][h], 1);
         mbar_init(&pready[i][h], 4);
@@ -136,7 +151,6 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
   __syncthreads();
   tc_after_sync();
   const uint32_t tmem = tmem_base;
-  const uint32_t s_at[2] = {tmem, tmem + 128}, o_at[2] = {tmem + 256, tmem + 256 + 128};
 
   // ---- the CTA's range of units (group of query rows, tile of tokens)
   int64_t total = 0;
@@ -147,9 +161,9 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
   const int64_t end = min(pos + each, total);
   int4 join = make_int4(0, 0, 0, 0);
 
-  uint32_t tiles = 0;       // K/V tiles of earlier groups
-  uint32_t phases = 0;      // of the score barriers (softmax) or the weight barriers (products): bit 2 q + half
-  uint32_t steps = 0, groups = 0;  // steps: of this warpgroup's query tile
+  uint32_t steps = 0;       // of earlier groups: their numbers choose the stages
+  uint32_t turns = 0;       // this stream's steps: their numbers choose the place of the scores
+  uint32_t groups = 0;
   int row = -1, head = 0, mt = 0, tile0 = 0;
   if (pos < end) {  // where it begins: rows' units counted up by all threads
     int64_t before = 0;
@@ -191,8 +205,9 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
     const AtRow rw = at_row<PA_ROWS / 8>(a, row);
     const int start = a.starts[row], ctx = rw.len - rw.n;
     const int rows_here = min(PA_ROWS, rw.n * a.per - mt * PA_ROWS);
-    const int nq = rows_here > 128 ? 2 : 1;
+    const bool narrow = rows_here <= 128;
     const int see_last = ctx + (mt * PA_ROWS + rows_here - 1) / a.per + 1;
+    const int see_all = TREE ? ctx : ctx + mt * PA_ROWS / a.per + 1;  // tokens that every row of the group sees
     const int nt = pa_tiles(a, rw, mt), tile1 = (int)min((int64_t)nt, tile0 + (end - pos));
     const bool whole = tile0 == 0 && tile1 == nt;
     const int i0 = tile0 * 2, i1 = min(tile1 * 2, (see_last + PA_HT - 1) / PA_HT);  // steps of 64 tokens
@@ -203,7 +218,7 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
 
     if (warp < 8) {
       // ---- a thread per query row
-      const int q = warp >> 2, r = (warp & 3) * 32 + lane, rr = q * 128 + r;
+      const int q = warp >> 2, tile = narrow ? 0 : q, r = (warp & 3) * 32 + lane, rr = tile * 128 + r;
       const bool in = rr < rows_here;
       const int qi = in ? (mt * PA_ROWS + rr) / a.per : 0;
       const int qh = head * a.per + (in ? mt * PA_ROWS + rr - qi * a.per : 0);
@@ -214,17 +229,18 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
         return in && (uint32_t)at_place - (uint32_t)b.x < (uint32_t)b.y;
       };
       const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+      const uint32_t s_at = tmem + 128 * q + lanes, o_at = tmem + 256 + 128 * q + lanes;
       float fq = fabsf(a.scale);
-      // Loops of this part, and of the one behind the tiles, stay rolled: code that runs once per group comes from
+      // Loops of this part, and of the one behind the steps, stay rolled: code that runs once per group comes from
       // the L2 cache instruction line by instruction line (unrolled, they took 15 us per group).
-      if (q < nq) {
-        unsigned char* mine = qs + q * OPB;
+      if (!narrow || q == 0) {
+        unsigned char* mine = qs + tile * OPB;
         // The warp's 32 rows, CH lanes each, as they are.
-        PaRows walk(a, mt * PA_ROWS + q * 128 + (warp & 3) * 32 + lane / CH);
+        PaRows walk(a, mt * PA_ROWS + tile * 128 + (warp & 3) * 32 + lane / CH);
 #pragma unroll 1
         for (int i = 0; i < CH; ++i) {
           const int r2 = (warp & 3) * 32 + (i * 32 + lane) / CH;
-          const bool in2 = q * 128 + r2 < rows_here;
+          const bool in2 = tile * 128 + r2 < rows_here;
           const uint16_t* src = reinterpret_cast<const uint16_t*>(a.q) +
                                 (in2 ? (int64_t)(start + walk.qi) * a.q_st + (int64_t)(head * a.per + walk.h) * a.q_sh + (lane % CH) * 8 : 0);
           unsigned char* to = mine + pa_place(r2, lane % CH);
@@ -274,54 +290,96 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
             *at = make_uint4(u[0], u[1], u[2], u[3]);
           }
         }
+        if (narrow) row_factor[r] = fq;
       }
       fence_proxy_async();
       __syncwarp();
       if (lane == 0) mbar_arrive_local(&qready);
+      if (narrow && q == 1) {  // the same rows
+        tc_wait(&qready, groups & 1, &failed);
+        fq = row_factor[r];
+      }
 
       float m = -INFINITY, l = 0.0f, w = -INFINITY;
-      if (q < nq) {
-        // The first row of the warp sees least.
-        const int see_warp = TREE ? ctx : ctx + (mt * PA_ROWS + q * 128 + (warp & 3) * 32) / a.per + 1;
-        for (int i = i0; i < i1; ++i, ++steps) {
-          const int half = i & 1, at = i * PA_HT;
-          tc_wait(&sfull[q][half], (phases >> half) & 1, &failed);
-          phases ^= 1u << half;
-          tc_after_sync();
-          const uint32_t s_here = s_at[q] + lanes + 64 * half;
-          const float2* sc = &sscale[(tiles + (i >> 1) - tile0) & 3][4 * half];
-          bool masked = at + PA_HT > see_warp;
+      // The first row of the warp sees least.
+      const int see_warp = TREE ? ctx : ctx + (mt * PA_ROWS + tile * 128 + (warp & 3) * 32) / a.per + 1;
+      const int first = narrow ? i0 + q : i0, by = narrow ? 2 : 1;
+      for (int i = first; i < i1; i += by, ++turns) {
+        const int half = turns & 1, at = i * PA_HT;
+        tc_wait(&sfull[q][half], (turns >> 1) & 1, &failed);
+        tc_after_sync();
+        const uint32_t s_here = s_at + 64 * half;
+        const float2* sc = sscale[(steps + i - i0) & (PA_SC - 1)];
+        // Without a mask the weights are first taken with the maxima as they are: if one, or a share of the softmax, is
+        // too large for them (or NaN) they move and the weights are taken again.  A token's weight of V is 2^z,
+        // z = s + log2(v scale) - W + 10; its share p = 2^(s - m) of the softmax differs by a factor of its part, so that
+        // one exponential does for both: p = 2^z 2^(-shift).  Where the factor is far from 1 (a block of zeros has the
+        // scale 2^-126) p would be lost: then p itself is taken.
+        auto shift_of = [&](float ky) { return fminf((m == -INFINITY ? 0.0f : m) + ky - (w == -INFINITY ? 0.0f : w) + AT_BIAS, 126.0f); };
+        const float4 k01 = *reinterpret_cast<const float4*>(sc), k23 = *reinterpret_cast<const float4*>(sc + 2);
+        const float kx[4] = {k01.x, k01.z, k23.x, k23.z}, ky[4] = {k01.y, k01.w, k23.y, k23.w};
+        const float least = fminf(fminf(ky[0], ky[1]), fminf(ky[2], ky[3]));
+        bool over = at + PA_HT > see_warp || fminf(fminf(kx[0], kx[1]), fminf(kx[2], kx[3])) < 0.0f;
+        const bool masked = over;
+        over |= m == -INFINITY || shift_of(least) < -60.0f;
+        float more = 0.0f;
+        if (!__any_sync(0xffffffffu, over)) {
+          uint32_t x[4][16], p[4][8];
 #pragma unroll
-          for (int g = 0; g < 4; ++g) masked |= sc[g].x < 0.0f;
+          for (int g = 0; g < 4; ++g) tc_ld16(s_here + 16 * g, x[g]);
+          tc_wait_ld();
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const float fg = fq * kx[g], add = ky[g] - w + AT_BIAS;
+            float2 part = make_float2(0.0f, 0.0f);
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) {
+              const float2 y = fma2(make_float2(__uint_as_float(x[g][e]), __uint_as_float(x[g][e + 1])), make_float2(fg, fg), make_float2(add, add));
+              const float2 v = make_float2(ex2(y.x), ex2(y.y));
+              part = add2(part, v);
+              const __half2 h = __floats2half2_rn(v.x, v.y);
+              p[g][e / 2] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+            const float sum = part.x + part.y, share = sum * ex2(-shift_of(ky[g]));
+            over |= !(sum <= 32768.0f && share <= 1024.0f);  // 2^(AT_BIAS + AT_SLACK): each weight is an f16 below the largest
+            more += share;
+          }
+          if (!__any_sync(0xffffffffu, over)) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) tc_st8(s_here + 8 * g, p[g]);  // over scores that have been read
+          }
+        }
+        if (__any_sync(0xffffffffu, over)) {
           uint32_t x[4][16];
 #pragma unroll
           for (int g = 0; g < 4; ++g) tc_ld16(s_here + 16 * g, x[g]);
           tc_wait_ld();
-          uint64_t seen = 0;  // TREE, masked: the step's tokens that this row sees
+          uint32_t seen[2] = {0u, 0u};  // TREE, masked: the step's tokens that this row sees
           if (TREE && masked) {
-            const int old = min(max(limit - at, 0), PA_HT), upto = min(see_last - at, PA_HT);
-            if (old > 0) seen = ~0ull >> (PA_HT - old);
-#pragma unroll 8
-            for (int e = max(ctx - at, 0); e < upto; ++e)
-              if (shows(at + e)) seen |= 1ull << e;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int t0 = at + 32 * h, old = min(max(limit - t0, 0), 32), upto = min(see_last - t0, 32);
+              if (old > 0) seen[h] = 0xffffffffu >> (32 - old);
+#pragma unroll 4
+              for (int e = max(ctx - t0, 0); e < upto; ++e)
+                if (shows(t0 + e)) seen[h] |= 1u << e;
+            }
           }
-          auto sees = [&](int e) { return TREE ? ((seen >> e) & 1) != 0 : at + e < limit; };
+          auto sees = [&](int e) { return TREE ? ((seen[e >> 5] >> (e & 31)) & 1u) != 0u : at + e < limit; };
           // Largest score, and largest weight of V.
-          float top = -INFINITY, topw = -INFINITY, least = INFINITY;
+          float top = -INFINITY, topw = -INFINITY;
           auto maxima = [&](auto mask_c) {
             constexpr bool with_mask = decltype(mask_c)::value;
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-              const float2 k = sc[g];
               float t = -INFINITY;
 #pragma unroll
               for (int e = 0; e < 16; ++e)
                 if (!with_mask || sees(16 * g + e)) t = fmaxf(t, __uint_as_float(x[g][e]));
-              if (with_mask && (k.x < 0.0f || (TREE ? ((seen >> (16 * g)) & 0xffff) == 0 : at + 16 * g >= limit))) continue;
-              t = fmaxf(t * (fq * k.x), -FLT_MAX);  // -inf and NaN: seen, unlike what leaves m at -inf
+              if (with_mask && (kx[g] < 0.0f || (TREE ? ((seen[g >> 1] >> (16 * (g & 1))) & 0xffffu) == 0u : at + 16 * g >= limit))) continue;
+              t = fmaxf(t * (fq * kx[g]), -FLT_MAX);  // -inf and NaN: seen, unlike what leaves m at -inf
               top = fmaxf(top, t);
-              topw = fmaxf(topw, t + k.y);
-              least = fminf(least, k.y);
+              topw = fmaxf(topw, t + ky[g]);
             }
           };
           if (masked) maxima(std::true_type{}); else maxima(std::false_type{});
@@ -331,65 +389,89 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
             const float shrink = ex2(w - (wn == -INFINITY ? 0.0f : wn));
             m = mn;
             w = wn;
-            if (i > i0) {  // the sums so far, once the products of the step before are in them
-              tc_wait(&pvdone[q], (steps - 1) & 1, &failed);
+            if (i > first) {  // the sums so far, once the products of the step before are in them
+              tc_wait(&pvdone[q], (turns - 1) & 1, &failed);
               tc_after_sync();
 #pragma unroll 1
               for (int d = 0; d < D; d += 16) {
-                uint32_t x[16];
-                tc_ld16(o_at[q] + lanes + d, x);
+                uint32_t o[16];
+                tc_ld16(o_at + d, o);
                 tc_wait_ld();
 #pragma unroll
-                for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * shrink);
-                tc_st16(o_at[q] + lanes + d, x);
+                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * shrink);
+                tc_st16(o_at + d, o);
               }
             }
           }
-          const float mu = m == -INFINITY ? 0.0f : m, wu = w == -INFINITY ? 0.0f : w;
-          // A token's weight of V is 2^z, z = s + log2(v scale) - W + 10; its share p = 2^(s - m) of the softmax
-          // differs by a factor of its part, so that one exponential does for both: p = 2^z 2^(-shift).  Where the factor
-          // is far from 1 (a block of zeros has the scale 2^-126) p would be lost: then p itself is taken.
-          const bool apart = __any_sync(0xffffffffu, mu + least - wu + AT_BIAS < -60.0f);
-          auto weights = [&](auto mask_c, auto share_c) {
-            constexpr bool with_mask = decltype(mask_c)::value, by_share = decltype(share_c)::value;
+          const float mu = m == -INFINITY ? 0.0f : m;
+          more = 0.0f;
+          auto weights = [&](auto mask_c) {
+            constexpr bool with_mask = decltype(mask_c)::value;
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-              const float2 k = sc[g];
-              const float fg = fq * k.x, shift = fminf(mu + k.y - wu + AT_BIAS, 126.0f);
-              const float add = by_share ? -mu : k.y - wu + AT_BIAS, gain = by_share ? ex2(shift) : 0.0f;
+              const float fg = fq * kx[g], gain = ex2(shift_of(ky[g]));
               uint32_t p[8];
-              float part = 0.0f;
 #pragma unroll
               for (int e = 0; e < 16; e += 2) {
-                float y0 = fmaf(__uint_as_float(x[g][e]), fg, add), y1 = fmaf(__uint_as_float(x[g][e + 1]), fg, add);
+                float y0 = fmaf(__uint_as_float(x[g][e]), fg, -mu), y1 = fmaf(__uint_as_float(x[g][e + 1]), fg, -mu);
                 if (with_mask) {
-                  if (k.x < 0.0f || !sees(16 * g + e)) y0 = -INFINITY;
-                  if (k.x < 0.0f || !sees(16 * g + e + 1)) y1 = -INFINITY;
+                  if (kx[g] < 0.0f || !sees(16 * g + e)) y0 = -INFINITY;
+                  if (kx[g] < 0.0f || !sees(16 * g + e + 1)) y1 = -INFINITY;
                 }
-                float p0 = ex2(y0), p1 = ex2(y1);
-                part += p0 + p1;
-                if (by_share) {
-                  p0 *= gain;
-                  p1 *= gain;
-                }
-                const __half2 v = __floats2half2_rn(p0, p1);
+                const float p0 = ex2(y0), p1 = ex2(y1);
+                more += p0 + p1;
+                const __half2 v = __floats2half2_rn(p0 * gain, p1 * gain);
                 p[e / 2] = *reinterpret_cast<const uint32_t*>(&v);
               }
-              if (by_share) l += part;
-              else if (!with_mask || part != 0.0f) l = fmaf(part, ex2(-shift), l);
-              tc_st8(s_here + 8 * g, p);  // over scores that have been read
+              tc_st8(s_here + 8 * g, p);
             }
           };
-          if (masked) weights(std::true_type{}, std::true_type{});
-          else if (apart) weights(std::false_type{}, std::true_type{});
-          else weights(std::false_type{}, std::false_type{});
-          tc_wait_st();
-          tc_before_sync();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_local(&pready[q][half]);
+          if (masked) weights(std::true_type{}); else weights(std::false_type{});
         }
-        tc_wait(&ofull[q], groups & 1, &failed);
-        tc_after_sync();
+        l += more;
+        tc_wait_st();
+        tc_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_local(&pready[q][half]);
+      }
+      tc_wait(&ofull[q], groups & 1, &failed);
+      tc_after_sync();
+      // Two streams of the same rows: the second one leaves its state and sums in the stages of keys and values, which
+      // no product reads any more, four columns of all rows after the other.
+      float4* other = reinterpret_cast<float4*>(ksm);
+      if (narrow) {
+        if (q == 1) {
+          tc_wait(&ofull[0], groups & 1, &failed);
+          float* state = reinterpret_cast<float*>(other + 128 * (D / 4));
+          state[r] = m;
+          state[128 + r] = l;
+          state[256 + r] = w;
+          if (first < i1) {
+#pragma unroll 1
+            for (int i = 0; i < D; i += 16) {
+              uint32_t x[16];
+              tc_ld16(o_at + i, x);
+              tc_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                other[(i / 4 + e) * 128 + r] = make_float4(__uint_as_float(x[4 * e]), __uint_as_float(x[4 * e + 1]), __uint_as_float(x[4 * e + 2]), __uint_as_float(x[4 * e + 3]));
+            }
+          }
+        }
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+      }
+      if (!narrow || q == 0) {
+        float f0 = 1.0f, f1 = 0.0f;  // of this stream's sums and of the other's
+        if (narrow && i0 + 1 < i1) {
+          const float* state = reinterpret_cast<const float*>(other + 128 * (D / 4));
+          const float m1 = state[r], l1 = state[128 + r], w1 = state[256 + r];
+          const float mn = fmaxf(m, m1), wn = fmaxf(w, w1), mu = mn == -INFINITY ? 0.0f : mn, wu = wn == -INFINITY ? 0.0f : wn;
+          l = l * ex2(m - mu) + l1 * ex2(m1 - mu);
+          f0 = ex2(w - wu);
+          f1 = ex2(w1 - wu);
+          m = mn;
+          w = wn;
+        }
         if (!whole && rr < rows_here) {  // a piece: its state as it is
           piece[rr] = m;
           piece[PA_ROWS + rr] = l;
@@ -400,8 +482,18 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
 #pragma unroll 1
         for (int i = 0; i < D; i += 16) {
           uint32_t x[16];
-          tc_ld16(o_at[q] + lanes + i, x);
+          tc_ld16(o_at + i, x);
           tc_wait_ld();
+          if (narrow && i0 + 1 < i1) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float4 v = other[(i / 4 + e) * 128 + r];
+              x[4 * e] = __float_as_uint(fmaf(v.x, f1, __uint_as_float(x[4 * e]) * f0));
+              x[4 * e + 1] = __float_as_uint(fmaf(v.y, f1, __uint_as_float(x[4 * e + 1]) * f0));
+              x[4 * e + 2] = __float_as_uint(fmaf(v.z, f1, __uint_as_float(x[4 * e + 2]) * f0));
+              x[4 * e + 3] = __float_as_uint(fmaf(v.w, f1, __uint_as_float(x[4 * e + 3]) * f0));
+            }
+          }
           if (TREE && branch_nan) {
 #pragma unroll 1
             for (int t = max(ctx, tile0 * PA_KT); t < min(see_last, tile1 * PA_KT); ++t) {
@@ -434,19 +526,19 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
               pk[e] = at_pack<DT>(y[0], y[1]);
             }
             // Into the place of the queries, which no product reads any more.
-            *reinterpret_cast<uint4*>(qs + q * OPB + pa_place(r, i / 8)) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
-            *reinterpret_cast<uint4*>(qs + q * OPB + pa_place(r, i / 8 + 1)) = make_uint4(pk[4], pk[5], pk[6], pk[7]);
+            *reinterpret_cast<uint4*>(qs + tile * OPB + pa_place(r, i / 8)) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+            *reinterpret_cast<uint4*>(qs + tile * OPB + pa_place(r, i / 8 + 1)) = make_uint4(pk[4], pk[5], pk[6], pk[7]);
           }
         }
         if (whole) {
           __syncwarp();
-          PaRows walk(a, mt * PA_ROWS + q * 128 + (warp & 3) * 32 + lane / CH);
+          PaRows walk(a, mt * PA_ROWS + tile * 128 + (warp & 3) * 32 + lane / CH);
 #pragma unroll 1
           for (int i = 0; i < CH; ++i) {
             const int r2 = (warp & 3) * 32 + (i * 32 + lane) / CH;
-            if (q * 128 + r2 < rows_here) {
+            if (tile * 128 + r2 < rows_here) {
               uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + (int64_t)(start + walk.qi) * a.o_st + (int64_t)(head * a.per + walk.h) * a.o_sh + (lane % CH) * 8;
-              const uint4 v = *reinterpret_cast<const uint4*>(qs + q * OPB + pa_place(r2, lane % CH));
+              const uint4 v = *reinterpret_cast<const uint4*>(qs + tile * OPB + pa_place(r2, lane % CH));
               if (a.aligned) {
                 *reinterpret_cast<uint4*>(out) = v;
               } else {
@@ -462,162 +554,184 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
           }
         }
         if (in && whole && a.lse) a.lse[(int64_t)(start + qi) * (a.heads * a.per) + qh] = none ? -INFINITY : (m + log2f(l)) * LN2;
-        tc_before_sync();
       }
+      tc_before_sync();
     } else if (warp < 8 + PA_CONV) {
-      // ---- widens keys and values, a tile ahead of the products
+      // ---- widens keys and values
       const int ct = tid - 256;
-      const int32_t* trow = a.table + row * a.table_stride;
-      const int bsm = (1 << a.bs_shift) - 1;
-      uint4 kr[PER_T], vr[PER_T];
-      int ids[PER_T], ids_next[PER_T], part_id = -1, part_next = -1;
-      float ksn = 0.0f, lvn = 0.0f;
-      // Block ids of the thread's pieces of tile j (-1: not seen), a tile ahead of their use; then keys with the
-      // scales, and values, each as soon as the registers of the tile before are free.
-      auto locate = [&](int j) {
-        auto id = [&](int t) {
-          const int page = t < see_last && j < tile1 ? __ldg(trow + (t >> a.bs_shift)) : -1;
-          return (unsigned)page < (unsigned)a.num_blocks ? page : -1;
-        };
-#pragma unroll
-        for (int i = 0; i < PER_T; ++i) {
-          const int p = ct + i * PA_CONV * 32;
-          ids_next[i] = p < PIECES ? id(j * PA_KT + p / (D / 16)) : -1;
-        }
-        if (ct < 8) part_next = id(j * PA_KT + ct * 16);
-      };
-      auto advance = [&]() {
-#pragma unroll
-        for (int i = 0; i < PER_T; ++i) ids[i] = ids_next[i];
-        part_id = part_next;
-      };
-      auto fetch = [&](const uint8_t* from, uint4 (&to)[PER_T], int j) {
-#pragma unroll
-        for (int i = 0; i < PER_T; ++i) {
-          const int p = ct + i * PA_CONV * 32, t = j * PA_KT + p / (D / 16), cc = p % (D / 16);
-          to[i] = ids[i] >= 0 ? __ldg(reinterpret_cast<const uint4*>(from + (((int64_t)ids[i] * a.heads + head) << a.bs_shift) * D + (t & bsm) * D + cc * 16))
-                              : make_uint4(0, 0, 0, 0);
-        }
-      };
-      auto fetch_scales = [&]() {
-        if (ct < 8) {
-          ksn = part_id >= 0 ? __ldg(a.ks + (int64_t)part_id * a.heads + head) : -1.0f;
-          lvn = part_id >= 0 ? lg2(__ldg(a.vs + (int64_t)part_id * a.heads + head)) : -INFINITY;
-        }
-      };
-      auto widen = [&](const uint4& v, unsigned char* to, int t, int cc) {
+      // Piece k of the thread: token (ct + k * threads) / (D / 16), and the same 16 columns each time.
+      constexpr int PT = PA_CONV * 32 / (D / 16);  // tokens between the thread's pieces
+      const int cc = ct % (D / 16);
+      const int token = ct / (D / 16) ^ (D > 64 && cc >= 4);  // lanes of the second panel take the neighbour: 8 lanes, 8 bank groups
+      const int piece0 = token * (D / 16) + cc;
+      // Tokens PT apart lie PT lines apart, permuted alike.
+      static_assert(PT % 8 == 0, "a thread's tokens are permuted alike");
+      const uint32_t to0 = pa_place<PA_HT>(token, 2 * cc), to1 = pa_place<PA_HT>(token, 2 * cc + 1);
+      auto widen = [&](const uint4& v, unsigned char* to) {
         const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-        const uint4 lo = make_uint4(f16_of_e4m3(u[0]), f16_of_e4m3(u[0] >> 16), f16_of_e4m3(u[1]), f16_of_e4m3(u[1] >> 16));
-        const uint4 hi = make_uint4(f16_of_e4m3(u[2]), f16_of_e4m3(u[2] >> 16), f16_of_e4m3(u[3]), f16_of_e4m3(u[3] >> 16));
-        // Lanes of the second panel store their second piece first: 8 lanes, 8 bank groups.
-        const bool swap = D > 64 && cc >= 4;
-        *reinterpret_cast<uint4*>(to + pa_place(t, 2 * cc + swap)) = swap ? hi : lo;
-        *reinterpret_cast<uint4*>(to + pa_place(t, 2 * cc + !swap)) = swap ? lo : hi;
+        *reinterpret_cast<uint4*>(to + to0) = make_uint4(f16_of_e4m3(u[0]), f16_of_e4m3(u[0] >> 16), f16_of_e4m3(u[1]), f16_of_e4m3(u[1] >> 16));
+        *reinterpret_cast<uint4*>(to + to1) = make_uint4(f16_of_e4m3(u[2]), f16_of_e4m3(u[2] >> 16), f16_of_e4m3(u[3]), f16_of_e4m3(u[3] >> 16));
       };
-      locate(tile0);
-      advance();
-      locate(tile0 + 1);
-      fetch(a.kc, kr, tile0);
-      fetch_scales();
-      fetch(a.vc, vr, tile0);
-      for (int j = tile0; j < tile1; ++j) {
-        const uint32_t n = tiles + j - tile0, st = n & 1;
-        if (n >= 2) tc_wait(&kempty[st], ((n >> 1) - 1) & 1, &failed);
+      for (int i = i0; i < i1; ++i) {
+        const uint32_t n = steps + i - i0, rst = n % RS, st = n % OP;
+        tc_wait(&rfull[rst], (n / RS) & 1, &failed);
+        const uint4* from = reinterpret_cast<const uint4*>(raw + rst * 2 * RAWB) + piece0;
+        uint4 v[PIECES];
 #pragma unroll
-        for (int i = 0; i < PER_T; ++i) {
-          const int p = ct + i * PA_CONV * 32;
-          if (p < PIECES) widen(kr[i], ksm + st * OPB, p / (D / 16), p % (D / 16));
-        }
-        if (ct < 8) {
-          sscale[n & 3][ct] = make_float2(ksn, lvn);
-        }
+        for (int k = 0; k < PIECES; ++k) v[k] = from[k * PA_CONV * 32];
+        if (n >= OP) tc_wait(&kempty[st], (n / OP - 1) & 1, &failed);
+#pragma unroll
+        for (int k = 0; k < PIECES; ++k) widen(v[k], ksm + st * STB + k * PT * 128);
         fence_proxy_async();
         __syncwarp();
         if (lane == 0) mbar_arrive_local(&kfull[st]);
-        advance();
-        if (j + 1 < tile1) {
-          fetch(a.kc, kr, j + 1);
-          fetch_scales();
-          locate(j + 2);
-        }
-        if (n >= 2) tc_wait(&vempty[st], ((n >> 1) - 1) & 1, &failed);
 #pragma unroll
-        for (int i = 0; i < PER_T; ++i) {
-          const int p = ct + i * PA_CONV * 32, t = p / (D / 16), cc = p % (D / 16);
-          uint32_t u[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
-          uint32_t any = 0;
+        for (int k = 0; k < PIECES; ++k) v[k] = from[RAWB / 16 + k * PA_CONV * 32];
+        const float2* sc = sscale[n & (PA_SC - 1)];
+        bool cut = i * PA_HT + PA_HT > see_all;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) any |= (u[e] & 0x7f7f7f7fu) + 0x01010101u;  // a byte of 0x7f carries into its sign
-          if (any & 0x80808080u) {
-            any_nan = 1;
+        for (int g = 0; g < 4; ++g) cut |= sc[g].x < 0.0f;
+        if (cut) {  // nothing of parts and tokens that are not there, and no NaN
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint32_t nan = __vcmpeq4(u[e] & 0x7f7f7f7fu, 0x7f7f7f7fu);
-              for (int z = 0; z < 4; ++z)
-                if ((nan >> (8 * z)) & 1u) {
-                  if (TREE && j * PA_KT + t >= ctx) branch_nan = 1;
-                  else atomicMin(&nan_from[cc * 16 + 4 * e + z], j * PA_KT + t);
-                }
-              u[e] &= ~nan;
+          for (int k = 0; k < PIECES; ++k) {
+            const int t = token + k * PT;
+            if (sc[t >> 4].x < 0.0f || i * PA_HT + t >= see_last) v[k] = make_uint4(0, 0, 0, 0);
+            uint32_t u[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+            uint32_t any = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) any |= (u[e] & 0x7f7f7f7fu) + 0x01010101u;  // a byte of 0x7f carries into its sign
+            if (any & 0x80808080u) {
+              any_nan = 1;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const uint32_t nan = __vcmpeq4(u[e] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+                for (int z = 0; z < 4; ++z)
+                  if ((nan >> (8 * z)) & 1u) {
+                    if (TREE && i * PA_HT + t >= ctx) branch_nan = 1;
+                    else atomicMin(&nan_from[cc * 16 + 4 * e + z], i * PA_HT + t);
+                  }
+                u[e] &= ~nan;
+              }
+              v[k] = make_uint4(u[0], u[1], u[2], u[3]);
             }
           }
-          if (p < PIECES) widen(make_uint4(u[0], u[1], u[2], u[3]), vsm + st * OPB, t, cc);
         }
-        if (j + 1 < tile1) fetch(a.vc, vr, j + 1);
+        __syncwarp();  // all of the stage is in registers
+        if (lane == 0) mbar_arrive_local(&rempty[rst]);
+        if (n >= OP) tc_wait(&vempty[st], (n / OP - 1) & 1, &failed);
+#pragma unroll
+        for (int k = 0; k < PIECES; ++k) widen(v[k], vsm + st * STB + k * PT * 128);
         fence_proxy_async();
         __syncwarp();
         if (lane == 0) mbar_arrive_local(&vfull[st]);
       }
-    } else {
-      // ---- issues the products: scores of tile j follow the weighted values of tile j - 1, query tiles in turn
+    } else if (warp < 8 + PA_CONV + 2) {
+      // ---- issues a stream's products: scores are two of its steps ahead of the weighted values
       constexpr uint32_t is = tc_idesc(false, PA_HT), io = tc_idesc(false, D) | (1u << 16);  // values: columns lie together
+      const int q = warp - 8 - PA_CONV;
+      const int first = narrow ? i0 + q : i0, by = narrow ? 2 : 1;
+      const uint32_t s_at = tmem + 128 * q, o_at = tmem + 256 + 128 * q;
+      const uint32_t q0 = tc_desc_lo(saddr(qs + (narrow ? 0 : q) * OPB));
       tc_wait(&qready, groups & 1, &failed);
-      auto score = [&](int q, int i) {
-        const uint32_t n = tiles + (i >> 1) - tile0, st = n & 1, half = i & 1;
-        if (q == 0 && half == 0) tc_wait(&kfull[st], (n >> 1) & 1, &failed);
+      auto score = [&](int i, uint32_t turn) {
+        const uint32_t n = steps + i - i0, st = n % OP, half = turn & 1;
+        const bool ok = tc_wait(&kfull[st], (n / OP) & 1, &failed);
         tc_after_sync();
         __syncwarp();
-        if (!tc_elect() || *(volatile int*)&failed) return;
-        const uint32_t q0 = tc_desc_lo(saddr(qs + q * OPB)), k0 = tc_desc_lo(saddr(ksm + st * OPB) + half * (PA_HT * 128));
+        if (tc_elect()) {
+          const uint32_t k0 = tc_desc_lo(saddr(ksm + st * STB));
+          if (ok) {
 #pragma unroll
-        for (int s = 0; s < D / 16; ++s) {
-          const uint32_t off = (uint32_t)((s >> 2) * (128 * 128) + (s & 3) * 32) / 16;
-          tc_mma_ss(s_at[q] + 64 * half, q0 + off, TC_DESC_HI, k0 + off, TC_DESC_HI, is, s > 0);
+            for (int s = 0; s < D / 16; ++s)
+              tc_mma_ss(s_at + 64 * half, q0 + ((s >> 2) * (128 * 128) + (s & 3) * 32) / 16, TC_DESC_HI, k0 + ((s >> 2) * (PA_HT * 128) + (s & 3) * 32) / 16,
+                        TC_DESC_HI, is, s > 0);
+          }
+          tc_commit(&sfull[q][half]);
+          tc_commit(&kempty[st]);
+          if (narrow) mbar_arrive_local(&kempty[st]);  // for the other stream
         }
-        tc_commit(&sfull[q][half]);
-        if (q == nq - 1 && (half == 1 || i == i1 - 1)) tc_commit(&kempty[st]);
+        __syncwarp();
       };
-      auto weigh = [&](int q, int i) {
-        const uint32_t n = tiles + (i >> 1) - tile0, st = n & 1, half = i & 1;
-        tc_wait(&pready[q][half], (phases >> (2 * q + half)) & 1, &failed);
-        phases ^= 1u << (2 * q + half);
-        if (q == 0 && half == 0) tc_wait(&vfull[st], (n >> 1) & 1, &failed);
+      auto weigh = [&](int i, uint32_t turn) {
+        const uint32_t n = steps + i - i0, st = n % OP, half = turn & 1;
+        bool ok = tc_wait(&vfull[st], (n / OP) & 1, &failed);
+        ok = tc_wait(&pready[q][half], (turn >> 1) & 1, &failed) && ok;
         tc_after_sync();
         __syncwarp();
-        if (!tc_elect() || *(volatile int*)&failed) return;
-        // panels of 64 columns are 16 KB apart, groups of 8 tokens 1 KB
-        const uint32_t v0 = (((saddr(vsm + st * OPB) + half * (PA_HT * 128)) >> 4) & 0x3fffu) | ((128u * 128u >> 4) << 16);
+        if (tc_elect()) {
+          // panels of 64 columns are 8 KB apart, groups of 8 tokens 1 KB
+          const uint32_t v0 = ((saddr(vsm + st * STB) >> 4) & 0x3fffu) | ((PA_HT * 128u >> 4) << 16);
+          if (ok) {
 #pragma unroll
-        for (int s = 0; s < PA_HT / 16; ++s)
-          tc_mma_ts(o_at[q], s_at[q] + 64 * half + 8 * s, v0 + s * (2048 / 16), TC_DESC_HI, io, i > i0 || s > 0);
-        tc_commit(&pvdone[q]);
-        if (q == nq - 1 && (half == 1 || i == i1 - 1)) tc_commit(&vempty[st]);
+            for (int s = 0; s < PA_HT / 16; ++s)
+              tc_mma_ts(o_at, s_at + 64 * half + 8 * s, v0 + s * (2048 / 16), TC_DESC_HI, io, i > first || s > 0);
+          }
+          tc_commit(&pvdone[q]);
+          tc_commit(&vempty[st]);
+          if (narrow) mbar_arrive_local(&vempty[st]);
+        }
+        __syncwarp();
       };
-      // Scores are two steps ahead of the weighted values: the next ones wait when a warpgroup has its weights.
-      for (int i = i0; i < min(i0 + 2, i1); ++i)
-        for (int q = 0; q < nq; ++q) score(q, i);
+      for (int j = 0; j < 2; ++j)
+        if (first + j * by < i1) score(first + j * by, turns + j);
 #pragma unroll 1
+      for (int i = first; i < i1; i += by, ++turns) {
+        weigh(i, turns);
+        if (i + 2 * by < i1) score(i + 2 * by, turns + 2);
+      }
+      if (tc_elect()) tc_commit(&ofull[q]);
+      __syncwarp();
+    } else {
+      // ---- issues the copies: lanes 0 to 3 the keys of the step's parts of 16 tokens, 4 to 7 the values, each with
+      // the part's scale; block ids of 32 parts at a time, one per lane
+      const int32_t* trow = a.table + row * a.table_stride;
+      const int bsm = (1 << a.bs_shift) - 1, part = lane & 3;
+      const bool is_v = (lane & 4) != 0;
+      const uint8_t* codes = is_v ? a.vc : a.kc;
+      const float* scales = is_v ? a.vs : a.ks;
+      auto load_ids = [&](int from) {  // of parts [from, from + 32)
+        const int t = (from + lane) * 16;
+        const int page = t < see_last ? __ldg(trow + (t >> a.bs_shift)) : -1;
+        return (unsigned)page < (unsigned)a.num_blocks ? page : -1;
+      };
+      int at = i0 * 4, ids = load_ids(at), ids_next = load_ids(at + 32);
+      auto page_of = [&](int i) {  // of this lane's part of step i: called for steps in order
+        if (i * 4 - at >= 32) {
+          at += 32;
+          ids = ids_next;
+          ids_next = load_ids(at + 32);
+        }
+        return __shfl_sync(0xffffffffu, ids, i * 4 + part - at);
+      };
+      auto scale_of = [&](int page) { return page >= 0 ? __ldg(scales + (int64_t)page * a.heads + head) : -1.0f; };
+      int page = page_of(i0);
+      float scale = scale_of(page);
       for (int i = i0; i < i1; ++i) {
-#pragma unroll 1
-        for (int q = 0; q < nq; ++q) {
-          weigh(q, i);
-          __syncwarp();
-          if (i == i1 - 1 && tc_elect()) tc_commit(&ofull[q]);
-          if (i + 2 < i1) score(q, i + 2);
+        const uint32_t n = steps + i - i0, rst = n % RS;
+        const int page_now = page;
+        const float scale_now = scale;
+        if (i + 1 < i1) {
+          page = page_of(i + 1);
+          scale = scale_of(page);
+        }
+        bool ok = n < RS || tc_wait(&rempty[rst], (n / RS - 1) & 1, &failed);
+        ok = ok && !*(volatile int*)&failed;
+        if (lane < 8) {
+          float2* sc = &sscale[n & (PA_SC - 1)][part];
+          if (is_v) sc->y = page_now >= 0 ? lg2(scale_now) : -INFINITY;
+          else sc->x = scale_now;
+        }
+        const bool mine = ok && lane < 8 && page_now >= 0;
+        const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, mine)) * 16 * D;
+        __syncwarp();
+        if (lane == 0) mbar_expect_tx(&rfull[rst], bytes);
+        __syncwarp();
+        if (mine) {
+          const int t = i * PA_HT + part * 16;
+          bulk_g2s(raw + rst * 2 * RAWB + (is_v ? RAWB : 0) + part * 16 * D, codes + ((((int64_t)page_now * a.heads + head) << a.bs_shift) + (t & bsm)) * D, 16 * D,
+                   &rfull[rst]);
         }
       }
-      __syncwarp();
-      if (nq == 1 && tc_elect()) tc_commit(&ofull[1]);  // its phase goes with the groups
     }
     __syncwarp();
     __syncthreads();
@@ -627,7 +741,7 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
       const int64_t from = pos - tile0;
       if (from >= ((int64_t)blockIdx.x - 1) * each) join = make_int4(row, mt * a.heads + head, (int)((from + nt - 1) / each) - (int)blockIdx.x + 2, 0);
     }
-    tiles += tile1 - tile0;
+    steps += i1 - i0;
     ++groups;
     pos += tile1 - tile0;
     tile0 = 0;
@@ -644,7 +758,7 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
   tc_before_sync();
   __syncthreads();
   tc_after_sync();
-  if (*(volatile int*)&failed) {  // products may still run: they get a quarter of a second
+  if (*(volatile int*)&failed) {  // products and copies may still run: they get a quarter of a second
     const long long t0 = clock64();
     while (clock64() - t0 < T4_WAIT / 4) __nanosleep(1000);
     __syncthreads();

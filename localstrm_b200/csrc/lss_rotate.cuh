@@ -84,20 +84,6 @@ __device__ __forceinline__ float ro_weight(const void* w, int dtype, int i) {
                                    : __half2float(reinterpret_cast<const __half*>(w)[i]);
 }
 
-// Two f32 values at a time.
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  float2 r;
-  asm("{\n .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mul.rn.f32x2 x, x, y;\n mov.b64 {%0, %1}, x;\n}\n"
-      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return r;
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 r;
-  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n fma.rn.f32x2 x, x, y, z;\n mov.b64 {%0, %1}, x;\n}\n"
-      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return r;
-}
-
 // y = x / sqrt(mean(x^2) + eps) * w for each head (where there is a weight), then each pair (a, b) of the first
 // 2 half values turned by the angle positions[t] * freqs[i]:  (a cos - b sin, b cos + a sin); pairs are (i, i + half),
 // or (2 i, 2 i + 1) where interleaved.  Squares, sums and products are f32, one rounding at the end.
