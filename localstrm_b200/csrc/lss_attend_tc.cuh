@@ -12,12 +12,13 @@ namespace lss {
 constexpr int PA_ROWS = 256;   // query rows of a group: two tiles of 128
 constexpr int PA_KT = 128;     // tokens of a unit of work
 constexpr int PA_HT = 64;      // tokens of a step: of the copies, the widening, the products and the softmax
-constexpr int PA_CONV = 4;     // warps that widen keys and values
-constexpr int PA_NT = (8 + PA_CONV + 3) * 32;  // and two that issue products, one that issues copies
-constexpr int PA_OP = 3;       // stages of widened keys, and of values
-constexpr int PA_SC = 8;       // stages of scales: steps between the copies and the softmax, and some
-// Stages of keys and values as they come: 48 KB.
-__host__ __device__ constexpr int pa_raw(int D) { return D == 64 ? 6 : 3; }
+// Warpgroups: two of a thread per query row, one that widens keys, one that widens values, one with two warps that issue
+// products and two that issue copies.  Registers go from the last three to the first two: 8 x 144 + 12 x 64 of 20 x 96.
+constexpr int PA_NT = 5 * 128;
+constexpr int PA_OP = 2;       // stages of widened keys, and of values: a multiple of the streams
+constexpr int PA_SC = 16;      // stages of scales: more than the steps between the copies and the softmax
+// Stages of keys and values as they come: 64 KB.
+__host__ __device__ constexpr int pa_raw(int D) { return D == 64 ? 8 : 4; }
 __host__ __device__ constexpr int pa_smem(int D) { return 1024 + 2 * 128 * D * 2 + 2 * PA_OP * PA_HT * D * 2 + pa_raw(D) * 2 * PA_HT * D; }
 
 // D (+)= A B, both operands in shared memory.
@@ -39,7 +40,7 @@ __device__ __forceinline__ int pa_tiles(const AttendArgs& a, const AtRow& w, int
   const int last = min((mt + 1) * PA_ROWS, w.n * a.per) - 1;
   return (w.len - w.n + last / a.per + 1 + PA_KT - 1) / PA_KT;
 }
-static __device__ __noinline__ int64_t pa_units(const AttendArgs& a, int r) {
+static __device__ __forceinline__ int64_t pa_units(const AttendArgs& a, int r) {
   const AtRow w = at_row<PA_ROWS / 8>(a, r);
   int64_t n = 0;
   for (int mt = 0; mt < w.mt; ++mt) n += pa_tiles(a, w, mt);
@@ -83,8 +84,8 @@ __device__ __forceinline__ uint32_t pa_place(int r, int q) {
 // sums O, which stay there for the whole group.  A group of more than 128 rows has a tile of 128 in each stream; in
 // one of fewer rows the streams take the same rows and every other step of 64 tokens each, and are added up at the end
 // (128 rows over 192,000 tokens and 8 heads: the second warpgroup idle 424 us).
-// Keys and values come as e4m3 through bulk copies that one warp issues, 48 KB on their way, and are widened to f16 by four
-// warps into three stages each, once for all rows (exact; 16 rows at a time, the widening is what bounds
+// Keys and values come as e4m3 through bulk copies that one warp issues, 64 KB on their way, and are widened to f16 by four
+// warps each into two stages, once for all rows (exact; 16 rows at a time, the widening is what bounds
 // lss_attend_kernel here).
 // Scales and the power of two of a query row act as in lss_attend_kernel; the weight of V is
 // p 2^(m + log2(v scale) - W + 10) from the softmax's own p, one exponential per score.  Both running
@@ -98,6 +99,57 @@ __device__ __forceinline__ uint32_t pa_place(int r, int q) {
 // With TREE (see lss_attend_kernel) a step that holds new tokens begins with a thread's 64 comparisons, kept as
 // bits.  NaN among the new tokens' values, which only their own branches see, is looked for again by the rows that see
 // them, once a group, where there was any.
+//
+// The warps go through the groups on their own, held together by the barriers of what they pass on alone: copies and
+// widening run ahead into the next group while the softmax finishes one and fetches its queries.  A stage of widened
+// keys or values belongs to steps of one parity, so that a stream that takes every other step sees all of its phases.
+struct PaGroup {  // a group of query rows, and the tiles of it that a CTA takes
+  int row, head, mt, tile0, tile1, nt;
+  int start, ctx, n, rows, see_last, see_all, i0, i1;  // steps [i0, i1)
+  bool narrow, whole;
+};
+template <bool TREE>
+struct PaWalk {
+  int64_t pos, end;
+  int row, head, mt, tile0;
+  uint32_t steps, groups, wides;  // of earlier groups: their numbers choose stages and phases
+  __device__ __forceinline__ bool get(const AttendArgs& a, PaGroup& g) const {
+    if (pos >= end) return false;
+    const AtRow w = at_row<PA_ROWS / 8>(a, row);
+    g.row = row;
+    g.head = head;
+    g.mt = mt;
+    g.n = w.n;
+    g.start = a.starts[row];
+    g.ctx = w.len - w.n;
+    g.rows = min(PA_ROWS, w.n * a.per - mt * PA_ROWS);
+    g.narrow = g.rows <= 128;
+    g.see_last = g.ctx + (mt * PA_ROWS + g.rows - 1) / a.per + 1;
+    g.see_all = TREE ? g.ctx : g.ctx + mt * PA_ROWS / a.per + 1;  // tokens that every row of the group sees
+    g.nt = pa_tiles(a, w, mt);
+    g.tile0 = tile0;
+    g.tile1 = (int)min((int64_t)g.nt, tile0 + (end - pos));
+    g.whole = tile0 == 0 && g.tile1 == g.nt;
+    g.i0 = tile0 * 2;
+    g.i1 = min(g.tile1 * 2, (g.see_last + PA_HT - 1) / PA_HT);
+    return true;
+  }
+  __device__ __forceinline__ void next(const AttendArgs& a, const PaGroup& g) {
+    steps += g.i1 - g.i0;
+    ++groups;
+    wides += !g.narrow;
+    pos += g.tile1 - g.tile0;
+    tile0 = 0;
+    if (pos < end && --mt < 0) {  // next group of the head, next head, next row with work
+      if (++head == a.heads) {
+        head = 0;
+        do ++row; while (row < a.B - 1 && at_row<PA_ROWS / 8>(a, row).n == 0);
+      }
+      mt = at_row<PA_ROWS / 8>(a, row).mt - 1;
+    }
+  }
+};
+
 template <int D, int DT, bool TREE>
 __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
   constexpr int CH = D / 8;                // 16-byte pieces of a row in f16
@@ -105,17 +157,21 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
   constexpr int STB = PA_HT * D * 2;       // bytes of a step's keys or values, widened
   constexpr int RAWB = PA_HT * D;          // and as they come
   constexpr int RS = pa_raw(D), OP = PA_OP;
-  constexpr int PIECES = RAWB / 16 / (PA_CONV * 32);  // 16-byte pieces of a step's keys (or values) per widening thread
+  constexpr int PIECES = RAWB / 16 / 128;  // 16-byte pieces of a step's keys (or values) per widening thread
   constexpr uint32_t NOWHERE = 0x7fffffff;
+  constexpr int NN = 4;                    // the widening is two steps, so two groups at most, ahead of the softmax
+  static_assert(OP % 2 == 0, "a stage belongs to one stream");
   extern __shared__ __align__(1024) unsigned char pa_dyn[];
-  __shared__ __align__(8) uint64_t rfull[RS], rempty[RS], kfull[OP], kempty[OP], vfull[OP], vempty[OP], sfull[2][2], pready[2][2], pvdone[2], ofull[2], qready;
+  __shared__ __align__(8) uint64_t rfull[2][RS], rempty[2][RS], kfull[OP], kempty[OP], vfull[OP], vempty[OP], sfull[2][2], pready[2][2], pvdone[2], ofull[2], qready[2];
   __shared__ uint32_t tmem_base;
   __shared__ int failed;
-  __shared__ __align__(16) float2 sscale[PA_SC][4];      // scales of the step's 16-token parts: of K (< 0: not seen), log2 of that of V
-  __shared__ int nan_from[D];              // first position with a NaN among the values of a column
-  __shared__ float row_factor[128];
+  __shared__ __align__(16) float2 sscale[PA_SC][4];  // scales of the step's 16-token parts: of K (< 0: not seen), log2 of that of V
+  __shared__ uint32_t parts[PA_SC];        // bit p: part p of the step's values is there
+  __shared__ int nan_from[NN][D];          // first position with a NaN among the values of a column
+  __shared__ int any_nan[NN], branch_nan[NN];  // branch_nan: NaN among the values of new tokens (TREE)
+  __shared__ float row_factor[128], state[3][128];
   __shared__ int64_t scr[PA_NT / 32], found_lo;
-  __shared__ int found, any_nan, branch_nan;  // branch_nan: NaN among the values of new tokens (TREE)
+  __shared__ int found;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   unsigned char* base = pa_dyn + ((1024 - (saddr(pa_dyn) & 1023)) & 1023);
   unsigned char* qs = base;                // two query operands
@@ -127,12 +183,14 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
   if (tid == 0) {
     failed = 0;
     for (int i = 0; i < RS; ++i) {
-      mbar_init(&rfull[i], 1);
-      mbar_init(&rempty[i], PA_CONV);
+      for (int h = 0; h < 2; ++h) {
+        mbar_init(&rfull[h][i], 1);
+        mbar_init(&rempty[h][i], 4);
+      }
     }
     for (int i = 0; i < OP; ++i) {
-      mbar_init(&kfull[i], PA_CONV);
-      mbar_init(&vfull[i], PA_CONV);
+      mbar_init(&kfull[i], 4);
+      mbar_init(&vfull[i], 4);
       mbar_init(&kempty[i], 2);
       mbar_init(&vempty[i], 2);
     }
@@ -143,31 +201,29 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
       }
       mbar_init(&pvdone[i], 1);
       mbar_init(&ofull[i], 1);
+      mbar_init(&qready[i], 4);
     }
-    mbar_init(&qready, 8);
     fence_barrier_init();
   }
-  tc_before_sync();
-  __syncthreads();
-  tc_after_sync();
-  const uint32_t tmem = tmem_base;
 
   // ---- the CTA's range of units (group of query rows, tile of tokens)
   int64_t total = 0;
   for (int r = tid; r < a.B; r += PA_NT) total += pa_units(a, r);
+  tc_before_sync();
   total = pa_sum(total, scr);
+  tc_after_sync();
+  const uint32_t tmem = tmem_base;
   const int64_t each = max((total + gridDim.x - 1) / (int64_t)gridDim.x, (int64_t)1);
-  int64_t pos = blockIdx.x * each;
-  const int64_t end = min(pos + each, total);
+  PaWalk<TREE> walk;
+  walk.pos = blockIdx.x * each;
+  walk.end = min(walk.pos + each, total);
+  walk.row = -1;
+  walk.head = walk.mt = walk.tile0 = 0;
+  walk.steps = walk.groups = walk.wides = 0;
   int4 join = make_int4(0, 0, 0, 0);
-
-  uint32_t steps = 0;       // of earlier groups: their numbers choose the stages
-  uint32_t turns = 0;       // this stream's steps: their numbers choose the place of the scores
-  uint32_t groups = 0;
-  int row = -1, head = 0, mt = 0, tile0 = 0;
-  if (pos < end) {  // where it begins: rows' units counted up by all threads
+  if (walk.pos < walk.end) {  // where it begins: rows' units counted up by all threads
     int64_t before = 0;
-    for (int r0 = 0; r0 < a.B && row < 0; r0 += PA_NT) {
+    for (int r0 = 0; r0 < a.B && walk.row < 0; r0 += PA_NT) {
       const int r = r0 + tid;
       const int64_t n = r < a.B ? pa_units(a, r) : 0;
       int64_t x = n;
@@ -186,85 +242,72 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
         if (i < warp) lo += scr[i];
         before += scr[i];
       }
-      if (pos >= lo && pos < lo + n) {
+      if (walk.pos >= lo && walk.pos < lo + n) {
         found = r;
         found_lo = lo;
       }
       __syncthreads();
-      row = found;
+      walk.row = found;
     }
-    const AtRow rw = at_row<PA_ROWS / 8>(a, row);
-    const int64_t per_head = pa_units(a, row) / a.heads, rel = pos - found_lo;
-    head = (int)(rel / per_head);
-    int64_t u = rel - head * per_head;
-    mt = rw.mt - 1;  // later groups see more: they come first
-    while (u >= pa_tiles(a, rw, mt)) u -= pa_tiles(a, rw, mt--);
-    tile0 = (int)u;
+    const AtRow rw = at_row<PA_ROWS / 8>(a, walk.row);
+    const int64_t per_head = pa_units(a, walk.row) / a.heads, rel = walk.pos - found_lo;
+    walk.head = (int)(rel / per_head);
+    int64_t u = rel - walk.head * per_head;
+    walk.mt = rw.mt - 1;  // later groups see more: they come first
+    while (u >= pa_tiles(a, rw, walk.mt)) u -= pa_tiles(a, rw, walk.mt--);
+    walk.tile0 = (int)u;
+    // The first cut inside its group joins the pieces.
+    const int64_t from = walk.pos - walk.tile0;
+    if (walk.tile0 > 0 && from >= ((int64_t)blockIdx.x - 1) * each)
+      join = make_int4(walk.row, walk.mt * a.heads + walk.head, (int)((from + pa_tiles(a, rw, walk.mt) - 1) / each) - (int)blockIdx.x + 2, 0);
   }
-  while (pos < end) {
-    const AtRow rw = at_row<PA_ROWS / 8>(a, row);
-    const int start = a.starts[row], ctx = rw.len - rw.n;
-    const int rows_here = min(PA_ROWS, rw.n * a.per - mt * PA_ROWS);
-    const bool narrow = rows_here <= 128;
-    const int see_last = ctx + (mt * PA_ROWS + rows_here - 1) / a.per + 1;
-    const int see_all = TREE ? ctx : ctx + mt * PA_ROWS / a.per + 1;  // tokens that every row of the group sees
-    const int nt = pa_tiles(a, rw, mt), tile1 = (int)min((int64_t)nt, tile0 + (end - pos));
-    const bool whole = tile0 == 0 && tile1 == nt;
-    const int i0 = tile0 * 2, i1 = min(tile1 * 2, (see_last + PA_HT - 1) / PA_HT);  // steps of 64 tokens
-    float* piece = a.part + ((size_t)blockIdx.x * 2 + (tile0 == 0 ? 1 : 0)) * pa_piece(D);
-    for (int i = tid; i < D; i += PA_NT) nan_from[i] = NOWHERE;
-    if (tid == 0) any_nan = branch_nan = 0;
-    __syncthreads();  // and nobody reads the last group's any more
+  if (tid == 0) a.meta[blockIdx.x] = join;
 
-    if (warp < 8) {
-      // ---- a thread per query row
-      const int q = warp >> 2, tile = narrow ? 0 : q, r = (warp & 3) * 32 + lane, rr = tile * 128 + r;
-      const bool in = rr < rows_here;
-      const int qi = in ? (mt * PA_ROWS + rr) / a.per : 0;
-      const int qh = head * a.per + (in ? mt * PA_ROWS + rr - qi * a.per : 0);
+  PaGroup g;
+  if (warp < 8) {
+    // ---- a thread per query row
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
+    const int q = warp >> 2, r = (warp & 3) * 32 + lane;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_at = tmem + 128 * q + lanes, o_at = tmem + 256 + 128 * q + lanes;
+    uint32_t turns = 0;  // this stream's steps: their numbers choose the place of the scores
+    for (; walk.get(a, g); walk.next(a, g)) {
+      const bool narrow = g.narrow;
+      const int tile = narrow ? 0 : q, rr = tile * 128 + r, ctx = g.ctx, start = g.start, see_last = g.see_last;
+      const bool in = rr < g.rows;
+      const int qi = in ? (g.mt * PA_ROWS + rr) / a.per : 0;
+      const int qh = g.head * a.per + (in ? g.mt * PA_ROWS + rr - qi * a.per : 0);
       const int limit = !in ? 0 : TREE ? ctx : ctx + qi + 1;  // TREE: and what `shows` says
       const int at_place = TREE && in ? __ldg(&a.span[start + qi].x) : 0;
       auto shows = [&](int t) {  // new token t, below see_last
         const int2 b = __ldg(&a.span[start + t - ctx]);
         return in && (uint32_t)at_place - (uint32_t)b.x < (uint32_t)b.y;
       };
-      const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-      const uint32_t s_at = tmem + 128 * q + lanes, o_at = tmem + 256 + 128 * q + lanes;
       float fq = fabsf(a.scale);
-      // Loops of this part, and of the one behind the steps, stay rolled: code that runs once per group comes from
-      // the L2 cache instruction line by instruction line (unrolled, they took 15 us per group).
       if (!narrow || q == 0) {
-        unsigned char* mine = qs + tile * OPB;
-        // The warp's 32 rows, CH lanes each, as they are.
-        PaRows walk(a, mt * PA_ROWS + tile * 128 + (warp & 3) * 32 + lane / CH);
-#pragma unroll 1
-        for (int i = 0; i < CH; ++i) {
-          const int r2 = (warp & 3) * 32 + (i * 32 + lane) / CH;
-          const bool in2 = tile * 128 + r2 < rows_here;
-          const uint16_t* src = reinterpret_cast<const uint16_t*>(a.q) +
-                                (in2 ? (int64_t)(start + walk.qi) * a.q_st + (int64_t)(head * a.per + walk.h) * a.q_sh + (lane % CH) * 8 : 0);
-          unsigned char* to = mine + pa_place(r2, lane % CH);
-          if (a.aligned) {
-            cp_async16z(saddr(to), src, in2 ? 16 : 0);
-          } else {
-            uint32_t u[4] = {0, 0, 0, 0};
-            if (in2) {
+        // The row's 16-byte pieces, twice: for its largest exponent, which goes to 0 (bf16 to f16; the power of two goes
+        // into the row's factor), and as operand.
+        const uint16_t* src = reinterpret_cast<const uint16_t*>(a.q) + (int64_t)(start + qi) * a.q_st + (int64_t)qh * a.q_sh;
+        auto piece_of = [&](int i) {
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (in) {
+            if (a.aligned) {
+              v = __ldg(reinterpret_cast<const uint4*>(src) + i);
+            } else {
+              uint32_t u[4];
 #pragma unroll
-              for (int e = 0; e < 4; ++e) u[e] = (uint32_t)src[2 * e] | ((uint32_t)src[2 * e + 1] << 16);
+              for (int e = 0; e < 4; ++e) u[e] = (uint32_t)src[8 * i + 2 * e] | ((uint32_t)src[8 * i + 2 * e + 1] << 16);
+              v = make_uint4(u[0], u[1], u[2], u[3]);
             }
-            *reinterpret_cast<uint4*>(to) = make_uint4(u[0], u[1], u[2], u[3]);
           }
-          walk.next(a, 32 / CH);
-        }
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        __syncwarp();
-        // bf16 to f16, a thread per row: largest exponent to 0, the power of two goes into the row's factor.
+          return v;
+        };
         float down = 1.0f;
         if (DT == LSS_DTYPE_BF16) {
           uint32_t top = 0;  // magnitudes of bf16 order as whole numbers do
-#pragma unroll 4
+#pragma unroll 8
           for (int i = 0; i < CH; ++i) {
-            const uint4 v = *reinterpret_cast<const uint4*>(mine + pa_place(r, i));
+            const uint4 v = piece_of(i);
             top = __vmaxu2(__vmaxu2(top, v.x & 0x7fff7fffu), __vmaxu2(v.y & 0x7fff7fffu, __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
           }
           top = max(top & 0xffffu, top >> 16);
@@ -273,43 +316,39 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
           fq *= __uint_as_float((uint32_t)(127 + e) << 23);
         }
         const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;  // scores are compared before they are scaled
-        if (DT == LSS_DTYPE_BF16 || sign != 0u) {
-#pragma unroll 2
-          for (int i = 0; i < CH; ++i) {
-            uint4* at = reinterpret_cast<uint4*>(mine + pa_place(r, i));
-            const uint4 v = *at;
-            uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll 8
+        for (int i = 0; i < CH; ++i) {
+          const uint4 v = piece_of(i);
+          uint32_t u[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              if (DT == LSS_DTYPE_BF16) {
-                const __half2 h = __floats2half2_rn(__uint_as_float(u[e] << 16) * down, __uint_as_float(u[e] & 0xffff0000u) * down);
-                u[e] = *reinterpret_cast<const uint32_t*>(&h);
-              }
-              u[e] ^= sign;
+          for (int e = 0; e < 4; ++e) {
+            if (DT == LSS_DTYPE_BF16) {
+              const __half2 h = __floats2half2_rn(__uint_as_float(u[e] << 16) * down, __uint_as_float(u[e] & 0xffff0000u) * down);
+              u[e] = *reinterpret_cast<const uint32_t*>(&h);
             }
-            *at = make_uint4(u[0], u[1], u[2], u[3]);
+            u[e] ^= sign;
           }
+          *reinterpret_cast<uint4*>(qs + tile * OPB + pa_place(r, i)) = make_uint4(u[0], u[1], u[2], u[3]);
         }
         if (narrow) row_factor[r] = fq;
-      }
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_local(&qready);
-      if (narrow && q == 1) {  // the same rows
-        tc_wait(&qready, groups & 1, &failed);
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_local(&qready[q]);
+      } else {  // the same rows
+        tc_wait(&qready[0], walk.groups & 1, &failed);
         fq = row_factor[r];
       }
 
       float m = -INFINITY, l = 0.0f, w = -INFINITY;
       // The first row of the warp sees least.
-      const int see_warp = TREE ? ctx : ctx + (mt * PA_ROWS + tile * 128 + (warp & 3) * 32) / a.per + 1;
-      const int first = narrow ? i0 + q : i0, by = narrow ? 2 : 1;
+      const int see_warp = TREE ? ctx : ctx + (g.mt * PA_ROWS + tile * 128 + (warp & 3) * 32) / a.per + 1;
+      const int first = narrow ? g.i0 + ((walk.steps ^ q) & 1) : g.i0, by = narrow ? 2 : 1, i1 = g.i1;
       for (int i = first; i < i1; i += by, ++turns) {
         const int half = turns & 1, at = i * PA_HT;
         tc_wait(&sfull[q][half], (turns >> 1) & 1, &failed);
         tc_after_sync();
         const uint32_t s_here = s_at + 64 * half;
-        const float2* sc = sscale[(steps + i - i0) & (PA_SC - 1)];
+        const float2* sc = sscale[(walk.steps + i - g.i0) & (PA_SC - 1)];
         // Without a mask the weights are first taken with the maxima as they are: if one, or a share of the softmax, is
         // too large for them (or NaN) they move and the weights are taken again.  A token's weight of V is 2^z,
         // z = s + log2(v scale) - W + 10; its share p = 2^(s - m) of the softmax differs by a factor of its part, so that
@@ -434,20 +473,20 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
         __syncwarp();
         if (lane == 0) mbar_arrive_local(&pready[q][half]);
       }
-      tc_wait(&ofull[q], groups & 1, &failed);
+      tc_wait(&ofull[q], walk.groups & 1, &failed);
       tc_after_sync();
-      // Two streams of the same rows: the second one leaves its state and sums in the stages of keys and values, which
-      // no product reads any more, four columns of all rows after the other.
-      float4* other = reinterpret_cast<float4*>(ksm);
+      // Two streams of the same rows: the second one leaves its state, and its sums in the place of the queries, which no
+      // product reads any more, four columns of all rows after the other.
+      float4* other = reinterpret_cast<float4*>(qs);
+      const bool both = narrow && g.i1 - g.i0 > 1;  // each has a step
       if (narrow) {
         if (q == 1) {
-          tc_wait(&ofull[0], groups & 1, &failed);
-          float* state = reinterpret_cast<float*>(other + 128 * (D / 4));
-          state[r] = m;
-          state[128 + r] = l;
-          state[256 + r] = w;
+          tc_wait(&ofull[0], walk.groups & 1, &failed);
+          state[0][r] = m;
+          state[1][r] = l;
+          state[2][r] = w;
           if (first < i1) {
-#pragma unroll 1
+#pragma unroll 2
             for (int i = 0; i < D; i += 16) {
               uint32_t x[16];
               tc_ld16(o_at + i, x);
@@ -462,9 +501,9 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
       }
       if (!narrow || q == 0) {
         float f0 = 1.0f, f1 = 0.0f;  // of this stream's sums and of the other's
-        if (narrow && i0 + 1 < i1) {
-          const float* state = reinterpret_cast<const float*>(other + 128 * (D / 4));
-          const float m1 = state[r], l1 = state[128 + r], w1 = state[256 + r];
+        const bool mine = first < i1;  // a single step may be the other stream's
+        if (narrow) {
+          const float m1 = state[0][r], l1 = state[1][r], w1 = state[2][r];
           const float mn = fmaxf(m, m1), wn = fmaxf(w, w1), mu = mn == -INFINITY ? 0.0f : mn, wu = wn == -INFINITY ? 0.0f : wn;
           l = l * ex2(m - mu) + l1 * ex2(m1 - mu);
           f0 = ex2(w - wu);
@@ -472,48 +511,52 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
           m = mn;
           w = wn;
         }
-        if (!whole && rr < rows_here) {  // a piece: its state as it is
+        float* piece = a.part + ((size_t)blockIdx.x * 2 + (g.tile0 == 0 ? 1 : 0)) * pa_piece(D);
+        const int* nans = nan_from[walk.groups & (NN - 1)];
+        if (!g.whole && in) {  // a piece: its state as it is
           piece[rr] = m;
           piece[PA_ROWS + rr] = l;
           piece[2 * PA_ROWS + rr] = w;
         }
-        const bool none = m == -INFINITY, bad = *(volatile int*)&failed, spoiled = bad || any_nan;
+        if (!g.whole && tile == 0 && r < D) reinterpret_cast<int*>(piece + 3 * PA_ROWS + PA_ROWS * D)[r] = nans[r];
+        const bool none = m == -INFINITY, bad = *(volatile int*)&failed, spoiled = bad || any_nan[walk.groups & (NN - 1)];
+        const bool branches = TREE && branch_nan[walk.groups & (NN - 1)];
         const AtFactor fin(m, l, w);
+        uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + (int64_t)(start + qi) * a.o_st + (int64_t)qh * a.o_sh;
 #pragma unroll 1
         for (int i = 0; i < D; i += 16) {
           uint32_t x[16];
           tc_ld16(o_at + i, x);
           tc_wait_ld();
-          if (narrow && i0 + 1 < i1) {
+          if (narrow && (both || !mine)) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const float4 v = other[(i / 4 + e) * 128 + r];
-              x[4 * e] = __float_as_uint(fmaf(v.x, f1, __uint_as_float(x[4 * e]) * f0));
-              x[4 * e + 1] = __float_as_uint(fmaf(v.y, f1, __uint_as_float(x[4 * e + 1]) * f0));
-              x[4 * e + 2] = __float_as_uint(fmaf(v.z, f1, __uint_as_float(x[4 * e + 2]) * f0));
-              x[4 * e + 3] = __float_as_uint(fmaf(v.w, f1, __uint_as_float(x[4 * e + 3]) * f0));
+              const float z[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+              for (int c = 0; c < 4; ++c) x[4 * e + c] = __float_as_uint(mine ? fmaf(z[c], f1, __uint_as_float(x[4 * e + c]) * f0) : z[c]);
             }
           }
-          if (TREE && branch_nan) {
+          if (branches) {
 #pragma unroll 1
-            for (int t = max(ctx, tile0 * PA_KT); t < min(see_last, tile1 * PA_KT); ++t) {
-              const int page = __ldg(a.table + row * a.table_stride + (t >> a.bs_shift));
+            for (int t = max(ctx, g.tile0 * PA_KT); t < min(see_last, g.tile1 * PA_KT); ++t) {
+              const int page = __ldg(a.table + g.row * a.table_stride + (t >> a.bs_shift));
               if (!shows(t) || (unsigned)page >= (unsigned)a.num_blocks) continue;
               const uint4 v = __ldg(reinterpret_cast<const uint4*>(
-                  a.vc + (((((int64_t)page * a.heads + head) << a.bs_shift) + (t & ((1 << a.bs_shift) - 1))) * D + i)));
+                  a.vc + (((((int64_t)page * a.heads + g.head) << a.bs_shift) + (t & ((1 << a.bs_shift) - 1))) * D + i)));
               const uint32_t u[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
               for (int e = 0; e < 16; ++e)
                 if (((u[e >> 2] >> (8 * (e & 3))) & 0x7fu) == 0x7fu) x[e] = 0x7fffffffu;
             }
           }
-          if (!whole) {
+          if (!g.whole) {
             float* to = piece + 3 * PA_ROWS + rr * D + i;
             if (in)
 #pragma unroll
               for (int e = 0; e < 16; e += 4)
                 *reinterpret_cast<uint4*>(to + e) = bad ? make_uint4(NOWHERE, NOWHERE, NOWHERE, NOWHERE) : make_uint4(x[e], x[e + 1], x[e + 2], x[e + 3]);
-          } else {
+          } else if (in) {
             uint32_t pk[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -521,240 +564,222 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
 #pragma unroll
               for (int z = 0; z < 2; ++z) {
                 y[z] = none ? 0.0f : fin(__uint_as_float(x[2 * e + z]));
-                if (spoiled && (bad || nan_from[i + 2 * e + z] < limit)) y[z] = __int_as_float(0x7fffffff);
+                if (spoiled && (bad || nans[i + 2 * e + z] < limit)) y[z] = __int_as_float(0x7fffffff);
               }
               pk[e] = at_pack<DT>(y[0], y[1]);
             }
-            // Into the place of the queries, which no product reads any more.
-            *reinterpret_cast<uint4*>(qs + tile * OPB + pa_place(r, i / 8)) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
-            *reinterpret_cast<uint4*>(qs + tile * OPB + pa_place(r, i / 8 + 1)) = make_uint4(pk[4], pk[5], pk[6], pk[7]);
-          }
-        }
-        if (whole) {
-          __syncwarp();
-          PaRows walk(a, mt * PA_ROWS + tile * 128 + (warp & 3) * 32 + lane / CH);
-#pragma unroll 1
-          for (int i = 0; i < CH; ++i) {
-            const int r2 = (warp & 3) * 32 + (i * 32 + lane) / CH;
-            if (tile * 128 + r2 < rows_here) {
-              uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + (int64_t)(start + walk.qi) * a.o_st + (int64_t)(head * a.per + walk.h) * a.o_sh + (lane % CH) * 8;
-              const uint4 v = *reinterpret_cast<const uint4*>(qs + tile * OPB + pa_place(r2, lane % CH));
-              if (a.aligned) {
-                *reinterpret_cast<uint4*>(out) = v;
-              } else {
-                const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+            if (a.aligned) {
+              reinterpret_cast<uint4*>(out + i)[0] = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+              reinterpret_cast<uint4*>(out + i)[1] = make_uint4(pk[4], pk[5], pk[6], pk[7]);
+            } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  out[2 * e] = (uint16_t)u[e];
-                  out[2 * e + 1] = (uint16_t)(u[e] >> 16);
-                }
+              for (int e = 0; e < 8; ++e) {
+                out[i + 2 * e] = (uint16_t)pk[e];
+                out[i + 2 * e + 1] = (uint16_t)(pk[e] >> 16);
               }
             }
-            walk.next(a, 32 / CH);
           }
         }
-        if (in && whole && a.lse) a.lse[(int64_t)(start + qi) * (a.heads * a.per) + qh] = none ? -INFINITY : (m + log2f(l)) * LN2;
+        if (in && g.whole && a.lse) a.lse[(int64_t)(start + qi) * (a.heads * a.per) + qh] = none ? -INFINITY : (m + log2f(l)) * LN2;
       }
+      if (narrow) asm volatile("bar.sync 1, 256;" ::: "memory");  // the other stream's sums have been read
       tc_before_sync();
-    } else if (warp < 8 + PA_CONV) {
-      // ---- widens keys and values
-      const int ct = tid - 256;
-      // Piece k of the thread: token (ct + k * threads) / (D / 16), and the same 16 columns each time.
-      constexpr int PT = PA_CONV * 32 / (D / 16);  // tokens between the thread's pieces
-      const int cc = ct % (D / 16);
-      const int token = ct / (D / 16) ^ (D > 64 && cc >= 4);  // lanes of the second panel take the neighbour: 8 lanes, 8 bank groups
-      const int piece0 = token * (D / 16) + cc;
-      // Tokens PT apart lie PT lines apart, permuted alike.
-      static_assert(PT % 8 == 0, "a thread's tokens are permuted alike");
-      const uint32_t to0 = pa_place<PA_HT>(token, 2 * cc), to1 = pa_place<PA_HT>(token, 2 * cc + 1);
-      auto widen = [&](const uint4& v, unsigned char* to) {
-        const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-        *reinterpret_cast<uint4*>(to + to0) = make_uint4(f16_of_e4m3(u[0]), f16_of_e4m3(u[0] >> 16), f16_of_e4m3(u[1]), f16_of_e4m3(u[1] >> 16));
-        *reinterpret_cast<uint4*>(to + to1) = make_uint4(f16_of_e4m3(u[2]), f16_of_e4m3(u[2] >> 16), f16_of_e4m3(u[3]), f16_of_e4m3(u[3] >> 16));
-      };
-      for (int i = i0; i < i1; ++i) {
-        const uint32_t n = steps + i - i0, rst = n % RS, st = n % OP;
-        tc_wait(&rfull[rst], (n / RS) & 1, &failed);
-        const uint4* from = reinterpret_cast<const uint4*>(raw + rst * 2 * RAWB) + piece0;
+    }
+  } else if (warp < 16) {
+    // ---- widen keys (warps 8 to 11) and values
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    const bool is_v = warp >= 12;
+    const int ct = tid & 127;
+    // Piece k of the thread: token + k PT, and the same 16 columns each time.
+    constexpr int PT = 128 / (D / 16);
+    const int cc = ct % (D / 16);
+    const int token = ct / (D / 16) ^ (D > 64 && cc >= 4);  // lanes of the second panel take the neighbour: 8 lanes, 8 bank groups
+    // Tokens PT apart lie PT lines apart, permuted alike.
+    static_assert(PT % 8 == 0, "a thread's tokens are permuted alike");
+    const uint32_t to0 = pa_place<PA_HT>(token, 2 * cc), to1 = pa_place<PA_HT>(token, 2 * cc + 1);
+    const uint4* from0 = reinterpret_cast<const uint4*>(raw + (is_v ? RAWB : 0)) + token * (D / 16) + cc;
+    unsigned char* into = is_v ? vsm : ksm;
+    uint64_t *full = is_v ? vfull : kfull, *empty = is_v ? vempty : kempty;
+    for (; walk.get(a, g); walk.next(a, g)) {
+      int* nans = nan_from[walk.groups & (NN - 1)];
+      if (is_v) {
+        if (ct < D) nans[ct] = NOWHERE;
+        if (ct == 0) any_nan[walk.groups & (NN - 1)] = branch_nan[walk.groups & (NN - 1)] = 0;
+        asm volatile("bar.sync 3, 128;" ::: "memory");
+      }
+      for (int i = g.i0; i < g.i1; ++i) {
+        const uint32_t n = walk.steps + i - g.i0, rst = n % RS, st = n % OP;
+        tc_wait(&rfull[is_v][rst], (n / RS) & 1, &failed);
+        const uint4* from = from0 + rst * (2 * RAWB / 16);
         uint4 v[PIECES];
 #pragma unroll
-        for (int k = 0; k < PIECES; ++k) v[k] = from[k * PA_CONV * 32];
-        if (n >= OP) tc_wait(&kempty[st], (n / OP - 1) & 1, &failed);
+        for (int k = 0; k < PIECES; ++k) v[k] = from[k * 128];
+        if (is_v) {
+          const uint32_t there = parts[n & (PA_SC - 1)];
+          const bool cut = i * PA_HT + PA_HT > g.see_all || there != 15u;
+          if (cut) {  // nothing of parts and tokens that are not there, and no NaN
 #pragma unroll
-        for (int k = 0; k < PIECES; ++k) widen(v[k], ksm + st * STB + k * PT * 128);
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_local(&kfull[st]);
+            for (int k = 0; k < PIECES; ++k) {
+              const int t = token + k * PT;
+              if (!((there >> (t >> 4)) & 1u) || i * PA_HT + t >= g.see_last) v[k] = make_uint4(0, 0, 0, 0);
+              uint32_t u[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+              uint32_t any = 0;
 #pragma unroll
-        for (int k = 0; k < PIECES; ++k) v[k] = from[RAWB / 16 + k * PA_CONV * 32];
-        const float2* sc = sscale[n & (PA_SC - 1)];
-        bool cut = i * PA_HT + PA_HT > see_all;
+              for (int e = 0; e < 4; ++e) any |= (u[e] & 0x7f7f7f7fu) + 0x01010101u;  // a byte of 0x7f carries into its sign
+              if (any & 0x80808080u) {
+                any_nan[walk.groups & (NN - 1)] = 1;
 #pragma unroll
-        for (int g = 0; g < 4; ++g) cut |= sc[g].x < 0.0f;
-        if (cut) {  // nothing of parts and tokens that are not there, and no NaN
-#pragma unroll
-          for (int k = 0; k < PIECES; ++k) {
-            const int t = token + k * PT;
-            if (sc[t >> 4].x < 0.0f || i * PA_HT + t >= see_last) v[k] = make_uint4(0, 0, 0, 0);
-            uint32_t u[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
-            uint32_t any = 0;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) any |= (u[e] & 0x7f7f7f7fu) + 0x01010101u;  // a byte of 0x7f carries into its sign
-            if (any & 0x80808080u) {
-              any_nan = 1;
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const uint32_t nan = __vcmpeq4(u[e] & 0x7f7f7f7fu, 0x7f7f7f7fu);
-                for (int z = 0; z < 4; ++z)
-                  if ((nan >> (8 * z)) & 1u) {
-                    if (TREE && i * PA_HT + t >= ctx) branch_nan = 1;
-                    else atomicMin(&nan_from[cc * 16 + 4 * e + z], i * PA_HT + t);
-                  }
-                u[e] &= ~nan;
+                for (int e = 0; e < 4; ++e) {
+                  const uint32_t nan = __vcmpeq4(u[e] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+                  for (int z = 0; z < 4; ++z)
+                    if ((nan >> (8 * z)) & 1u) {
+                      if (TREE && i * PA_HT + t >= g.ctx) branch_nan[walk.groups & (NN - 1)] = 1;
+                      else atomicMin(&nans[cc * 16 + 4 * e + z], i * PA_HT + t);
+                    }
+                  u[e] &= ~nan;
+                }
+                v[k] = make_uint4(u[0], u[1], u[2], u[3]);
               }
-              v[k] = make_uint4(u[0], u[1], u[2], u[3]);
             }
           }
         }
-        __syncwarp();  // all of the stage is in registers
-        if (lane == 0) mbar_arrive_local(&rempty[rst]);
-        if (n >= OP) tc_wait(&vempty[st], (n / OP - 1) & 1, &failed);
+        if (n >= OP) tc_wait(&empty[st], (n / OP - 1) & 1, &failed);
+        unsigned char* to = into + st * STB;
 #pragma unroll
-        for (int k = 0; k < PIECES; ++k) widen(v[k], vsm + st * STB + k * PT * 128);
+        for (int k = 0; k < PIECES; ++k) {
+          const uint32_t u[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+          *reinterpret_cast<uint4*>(to + k * PT * 128 + to0) = make_uint4(f16_of_e4m3(u[0]), f16_of_e4m3(u[0] >> 16), f16_of_e4m3(u[1]), f16_of_e4m3(u[1] >> 16));
+          *reinterpret_cast<uint4*>(to + k * PT * 128 + to1) = make_uint4(f16_of_e4m3(u[2]), f16_of_e4m3(u[2] >> 16), f16_of_e4m3(u[3]), f16_of_e4m3(u[3] >> 16));
+        }
         fence_proxy_async();
         __syncwarp();
-        if (lane == 0) mbar_arrive_local(&vfull[st]);
+        if (lane == 0) {
+          mbar_arrive_local(&full[st]);
+          mbar_arrive_local(&rempty[is_v][rst]);
+        }
       }
-    } else if (warp < 8 + PA_CONV + 2) {
-      // ---- issues a stream's products: scores are two of its steps ahead of the weighted values
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if (warp < 18) {
+      // ---- issue a stream's products: scores are two of its steps ahead of the weighted values
       constexpr uint32_t is = tc_idesc(false, PA_HT), io = tc_idesc(false, D) | (1u << 16);  // values: columns lie together
-      const int q = warp - 8 - PA_CONV;
-      const int first = narrow ? i0 + q : i0, by = narrow ? 2 : 1;
+      const int q = warp - 16;
       const uint32_t s_at = tmem + 128 * q, o_at = tmem + 256 + 128 * q;
-      const uint32_t q0 = tc_desc_lo(saddr(qs + (narrow ? 0 : q) * OPB));
-      tc_wait(&qready, groups & 1, &failed);
-      auto score = [&](int i, uint32_t turn) {
-        const uint32_t n = steps + i - i0, st = n % OP, half = turn & 1;
-        const bool ok = tc_wait(&kfull[st], (n / OP) & 1, &failed);
-        tc_after_sync();
-        __syncwarp();
-        if (tc_elect()) {
-          const uint32_t k0 = tc_desc_lo(saddr(ksm + st * STB));
-          if (ok) {
+      uint32_t turns = 0;
+      for (; walk.get(a, g); walk.next(a, g)) {
+        const bool narrow = g.narrow;
+        const int first = narrow ? g.i0 + ((walk.steps ^ q) & 1) : g.i0, by = narrow ? 2 : 1;
+        const uint32_t q0 = tc_desc_lo(saddr(qs + (narrow ? 0 : q) * OPB));
+        if (narrow || q == 0) tc_wait(&qready[0], walk.groups & 1, &failed);
+        else tc_wait(&qready[1], walk.wides & 1, &failed);
+        auto score = [&](int i, uint32_t turn) {
+          const uint32_t n = walk.steps + i - g.i0, st = n % OP, half = turn & 1;
+          const bool ok = tc_wait(&kfull[st], (n / OP) & 1, &failed);
+          tc_after_sync();
+          __syncwarp();
+          if (tc_elect()) {
+            const uint32_t k0 = tc_desc_lo(saddr(ksm + st * STB));
+            if (ok) {
 #pragma unroll
-            for (int s = 0; s < D / 16; ++s)
-              tc_mma_ss(s_at + 64 * half, q0 + ((s >> 2) * (128 * 128) + (s & 3) * 32) / 16, TC_DESC_HI, k0 + ((s >> 2) * (PA_HT * 128) + (s & 3) * 32) / 16,
-                        TC_DESC_HI, is, s > 0);
+              for (int s = 0; s < D / 16; ++s)
+                tc_mma_ss(s_at + 64 * half, q0 + ((s >> 2) * (128 * 128) + (s & 3) * 32) / 16, TC_DESC_HI, k0 + ((s >> 2) * (PA_HT * 128) + (s & 3) * 32) / 16,
+                          TC_DESC_HI, is, s > 0);
+            }
+            tc_commit(&sfull[q][half]);
+            tc_commit(&kempty[st]);
+            if (narrow) mbar_arrive_local(&kempty[st]);  // for the other stream
           }
-          tc_commit(&sfull[q][half]);
-          tc_commit(&kempty[st]);
-          if (narrow) mbar_arrive_local(&kempty[st]);  // for the other stream
-        }
-        __syncwarp();
-      };
-      auto weigh = [&](int i, uint32_t turn) {
-        const uint32_t n = steps + i - i0, st = n % OP, half = turn & 1;
-        bool ok = tc_wait(&vfull[st], (n / OP) & 1, &failed);
-        ok = tc_wait(&pready[q][half], (turn >> 1) & 1, &failed) && ok;
-        tc_after_sync();
-        __syncwarp();
-        if (tc_elect()) {
-          // panels of 64 columns are 8 KB apart, groups of 8 tokens 1 KB
-          const uint32_t v0 = ((saddr(vsm + st * STB) >> 4) & 0x3fffu) | ((PA_HT * 128u >> 4) << 16);
-          if (ok) {
+          __syncwarp();
+        };
+        auto weigh = [&](int i, uint32_t turn) {
+          const uint32_t n = walk.steps + i - g.i0, st = n % OP, half = turn & 1;
+          bool ok = tc_wait(&vfull[st], (n / OP) & 1, &failed);
+          ok = tc_wait(&pready[q][half], (turn >> 1) & 1, &failed) && ok;
+          tc_after_sync();
+          __syncwarp();
+          if (tc_elect()) {
+            // panels of 64 columns are 8 KB apart, groups of 8 tokens 1 KB
+            const uint32_t v0 = ((saddr(vsm + st * STB) >> 4) & 0x3fffu) | ((PA_HT * 128u >> 4) << 16);
+            if (ok) {
 #pragma unroll
-            for (int s = 0; s < PA_HT / 16; ++s)
-              tc_mma_ts(o_at, s_at + 64 * half + 8 * s, v0 + s * (2048 / 16), TC_DESC_HI, io, i > first || s > 0);
+              for (int s = 0; s < PA_HT / 16; ++s)
+                tc_mma_ts(o_at, s_at + 64 * half + 8 * s, v0 + s * (2048 / 16), TC_DESC_HI, io, i > first || s > 0);
+            }
+            tc_commit(&pvdone[q]);
+            tc_commit(&vempty[st]);
+            if (narrow) mbar_arrive_local(&vempty[st]);
           }
-          tc_commit(&pvdone[q]);
-          tc_commit(&vempty[st]);
-          if (narrow) mbar_arrive_local(&vempty[st]);
-        }
-        __syncwarp();
-      };
-      for (int j = 0; j < 2; ++j)
-        if (first + j * by < i1) score(first + j * by, turns + j);
+          __syncwarp();
+        };
+        for (int j = 0; j < 2; ++j)
+          if (first + j * by < g.i1) score(first + j * by, turns + j);
 #pragma unroll 1
-      for (int i = first; i < i1; i += by, ++turns) {
-        weigh(i, turns);
-        if (i + 2 * by < i1) score(i + 2 * by, turns + 2);
+        for (int i = first; i < g.i1; i += by, ++turns) {
+          weigh(i, turns);
+          if (i + 2 * by < g.i1) score(i + 2 * by, turns + 2);
+        }
+        if (tc_elect()) tc_commit(&ofull[q]);
+        __syncwarp();
       }
-      if (tc_elect()) tc_commit(&ofull[q]);
-      __syncwarp();
     } else {
-      // ---- issues the copies: lanes 0 to 3 the keys of the step's parts of 16 tokens, 4 to 7 the values, each with
-      // the part's scale; block ids of 32 parts at a time, one per lane
-      const int32_t* trow = a.table + row * a.table_stride;
+      // ---- issue the copies, of the keys (warp 18) and of the values: lanes 0 to 3 a part of 16 tokens each; block ids of
+      // 32 parts at a time, one per lane.  The scales of both go with the keys: the softmax needs them first.
       const int bsm = (1 << a.bs_shift) - 1, part = lane & 3;
-      const bool is_v = (lane & 4) != 0;
+      const bool is_v = warp == 19;
       const uint8_t* codes = is_v ? a.vc : a.kc;
-      const float* scales = is_v ? a.vs : a.ks;
-      auto load_ids = [&](int from) {  // of parts [from, from + 32)
-        const int t = (from + lane) * 16;
-        const int page = t < see_last ? __ldg(trow + (t >> a.bs_shift)) : -1;
-        return (unsigned)page < (unsigned)a.num_blocks ? page : -1;
-      };
-      int at = i0 * 4, ids = load_ids(at), ids_next = load_ids(at + 32);
-      auto page_of = [&](int i) {  // of this lane's part of step i: called for steps in order
-        if (i * 4 - at >= 32) {
-          at += 32;
-          ids = ids_next;
-          ids_next = load_ids(at + 32);
-        }
-        return __shfl_sync(0xffffffffu, ids, i * 4 + part - at);
-      };
-      auto scale_of = [&](int page) { return page >= 0 ? __ldg(scales + (int64_t)page * a.heads + head) : -1.0f; };
-      int page = page_of(i0);
-      float scale = scale_of(page);
-      for (int i = i0; i < i1; ++i) {
-        const uint32_t n = steps + i - i0, rst = n % RS;
-        const int page_now = page;
-        const float scale_now = scale;
-        if (i + 1 < i1) {
-          page = page_of(i + 1);
-          scale = scale_of(page);
-        }
-        bool ok = n < RS || tc_wait(&rempty[rst], (n / RS - 1) & 1, &failed);
-        ok = ok && !*(volatile int*)&failed;
-        if (lane < 8) {
-          float2* sc = &sscale[n & (PA_SC - 1)][part];
-          if (is_v) sc->y = page_now >= 0 ? lg2(scale_now) : -INFINITY;
-          else sc->x = scale_now;
-        }
-        const bool mine = ok && lane < 8 && page_now >= 0;
-        const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, mine)) * 16 * D;
-        __syncwarp();
-        if (lane == 0) mbar_expect_tx(&rfull[rst], bytes);
-        __syncwarp();
-        if (mine) {
-          const int t = i * PA_HT + part * 16;
-          bulk_g2s(raw + rst * 2 * RAWB + (is_v ? RAWB : 0) + part * 16 * D, codes + ((((int64_t)page_now * a.heads + head) << a.bs_shift) + (t & bsm)) * D, 16 * D,
-                   &rfull[rst]);
+      const float* scales = lane & 4 ? a.vs : a.ks;
+      for (; walk.get(a, g); walk.next(a, g)) {
+        const int32_t* trow = a.table + g.row * a.table_stride;
+        auto load_ids = [&](int from) {  // of parts [from, from + 32)
+          const int t = (from + lane) * 16;
+          const int page = t < g.see_last ? __ldg(trow + (t >> a.bs_shift)) : -1;
+          return (unsigned)page < (unsigned)a.num_blocks ? page : -1;
+        };
+        int at = g.i0 * 4, ids = load_ids(at), ids_next = load_ids(at + 32);
+        auto page_of = [&](int i) {  // of this lane's part of step i: called for steps in order
+          if (i * 4 - at >= 32) {
+            at += 32;
+            ids = ids_next;
+            ids_next = load_ids(at + 32);
+          }
+          return __shfl_sync(0xffffffffu, ids, i * 4 + part - at);
+        };
+        auto scale_of = [&](int page) { return page >= 0 && !is_v && lane < 8 ? __ldg(scales + (int64_t)page * a.heads + g.head) : -1.0f; };
+        int page = page_of(g.i0);
+        float scale = scale_of(page);
+        for (int i = g.i0; i < g.i1; ++i) {
+          const uint32_t n = walk.steps + i - g.i0, rst = n % RS;
+          const int page_now = page;
+          const float scale_now = scale;
+          if (i + 1 < g.i1) {
+            page = page_of(i + 1);
+            scale = scale_of(page);
+          }
+          bool ok = n < RS || tc_wait(&rempty[is_v][rst], (n / RS - 1) & 1, &failed);
+          ok = ok && !*(volatile int*)&failed;
+          const bool mine = lane < 4 && page_now >= 0;
+          const uint32_t there = __ballot_sync(0xffffffffu, mine);
+          if (is_v) {
+            if (lane == 0) parts[n & (PA_SC - 1)] = there;
+          } else if (lane < 8) {
+            float2* sc = &sscale[n & (PA_SC - 1)][part];
+            if (lane < 4) sc->x = scale_now;
+            else sc->y = page_now >= 0 ? lg2(scale_now) : -INFINITY;
+          }
+          __syncwarp();
+          if (lane == 0) mbar_expect_tx(&rfull[is_v][rst], ok ? __popc(there) * 16 * D : 0);
+          __syncwarp();
+          if (mine && ok) {
+            const int t = i * PA_HT + part * 16;
+            bulk_g2s(raw + rst * 2 * RAWB + (is_v ? RAWB : 0) + part * 16 * D, codes + ((((int64_t)page_now * a.heads + g.head) << a.bs_shift) + (t & bsm)) * D, 16 * D,
+                     &rfull[is_v][rst]);
+          }
         }
       }
     }
-    __syncwarp();
-    __syncthreads();
-    if (!whole)
-      for (int i = tid; i < D; i += PA_NT) reinterpret_cast<int*>(piece + 3 * PA_ROWS + PA_ROWS * D)[i] = nan_from[i];
-    if (tile0 > 0) {  // the first cut inside its group joins the pieces
-      const int64_t from = pos - tile0;
-      if (from >= ((int64_t)blockIdx.x - 1) * each) join = make_int4(row, mt * a.heads + head, (int)((from + nt - 1) / each) - (int)blockIdx.x + 2, 0);
-    }
-    steps += i1 - i0;
-    ++groups;
-    pos += tile1 - tile0;
-    tile0 = 0;
-    if (pos < end && --mt < 0) {  // next group of the head, next head, next row with work
-      if (++head == a.heads) {
-        head = 0;
-        do ++row; while (row < a.B - 1 && at_row<PA_ROWS / 8>(a, row).n == 0);
-      }
-      mt = at_row<PA_ROWS / 8>(a, row).mt - 1;
-    }
-    __syncthreads();  // the positions of NaN are out
   }
-  if (tid == 0) a.meta[blockIdx.x] = join;
+  __syncwarp();
   tc_before_sync();
   __syncthreads();
   tc_after_sync();
