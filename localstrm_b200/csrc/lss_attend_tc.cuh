@@ -16,6 +16,7 @@ constexpr int PA_HT = 64;      // tokens of a step: of the copies, the widening,
 // products and two that issue copies.  Registers go from the last three to the first two: 8 x 144 + 12 x 64 of 20 x 96.
 constexpr int PA_NT = 5 * 128;
 constexpr int PA_OP = 2;       // stages of widened keys, and of values: a multiple of the streams
+constexpr int PA_EXTRA = 6;    // see pa_extra
 constexpr int PA_SC = 16;      // stages of scales: more than the steps between the copies and the softmax
 // Stages of keys and values as they come: 64 KB.
 __host__ __device__ constexpr int pa_raw(int D) { return D == 64 ? 8 : 4; }
@@ -35,29 +36,21 @@ __device__ __forceinline__ void tc_st8(uint32_t at, const uint32_t (&r)[8]) {
                : "memory");
 }
 
-// Tiles of tokens that the last query of a group sees; units of a row.
+// Tiles of tokens that the last query of a group sees.
 __device__ __forceinline__ int pa_tiles(const AttendArgs& a, const AtRow& w, int mt) {
   const int last = min((mt + 1) * PA_ROWS, w.n * a.per) - 1;
   return (w.len - w.n + last / a.per + 1 + PA_KT - 1) / PA_KT;
 }
+// Units of work that a group's start and end count for: its queries and results take the time of some tiles (a tile of
+// a group of up to 128 rows takes about half as long).  Without them the CTA that got the shortest rows was the last
+// one by far (48 rows of 8 to 32 tokens over 50 to 8,000: 353 us, over 4,000 each 239).
+__device__ __forceinline__ int pa_extra(const AttendArgs& a, const AtRow& w, int mt) { return w.n * a.per - mt * PA_ROWS <= 128 ? PA_EXTRA : PA_EXTRA / 2; }
 static __device__ __forceinline__ int64_t pa_units(const AttendArgs& a, int r) {
   const AtRow w = at_row<PA_ROWS / 8>(a, r);
   int64_t n = 0;
-  for (int mt = 0; mt < w.mt; ++mt) n += pa_tiles(a, w, mt);
+  for (int mt = 0; mt < w.mt; ++mt) n += pa_tiles(a, w, mt) + pa_extra(a, w, mt);
   return n * a.heads;
 }
-// (token, head) of a query row and of the ones that follow it.
-struct PaRows {
-  int qi, h;
-  __device__ __forceinline__ PaRows(const AttendArgs& a, int row) : qi(row / a.per), h(row - row / a.per * a.per) {}
-  __device__ __forceinline__ void next(const AttendArgs& a, int rows) {
-    h += rows;
-    while (h >= a.per) {
-      h -= a.per;
-      ++qi;
-    }
-  }
-};
 __device__ __forceinline__ int64_t pa_sum(int64_t v, int64_t* scr) {
   v = warp_allreduce(v, [](int64_t p, int64_t q) { return p + q; });
   if ((threadIdx.x & 31) == 0) scr[threadIdx.x >> 5] = v;
@@ -110,12 +103,17 @@ struct PaGroup {  // a group of query rows, and the tiles of it that a CTA takes
 };
 template <bool TREE>
 struct PaWalk {
-  int64_t pos, end;
+  int64_t base, end;              // first unit of the group (its extra ones come before its tiles), end of the CTA's range
   int row, head, mt, tile0;
   uint32_t steps, groups, wides;  // of earlier groups: their numbers choose stages and phases
   __device__ __forceinline__ bool get(const AttendArgs& a, PaGroup& g) const {
-    if (pos >= end) return false;
+    if (base >= end) return false;
     const AtRow w = at_row<PA_ROWS / 8>(a, row);
+    const int64_t upto = end - base - pa_extra(a, w, mt);  // tiles of the group before the end of the range
+    g.nt = pa_tiles(a, w, mt);
+    g.tile0 = tile0;
+    g.tile1 = (int)min((int64_t)g.nt, upto);
+    if (upto <= tile0) return false;
     g.row = row;
     g.head = head;
     g.mt = mt;
@@ -126,9 +124,6 @@ struct PaWalk {
     g.narrow = g.rows <= 128;
     g.see_last = g.ctx + (mt * PA_ROWS + g.rows - 1) / a.per + 1;
     g.see_all = TREE ? g.ctx : g.ctx + mt * PA_ROWS / a.per + 1;  // tokens that every row of the group sees
-    g.nt = pa_tiles(a, w, mt);
-    g.tile0 = tile0;
-    g.tile1 = (int)min((int64_t)g.nt, tile0 + (end - pos));
     g.whole = tile0 == 0 && g.tile1 == g.nt;
     g.i0 = tile0 * 2;
     g.i1 = min(g.tile1 * 2, (g.see_last + PA_HT - 1) / PA_HT);
@@ -138,9 +133,9 @@ struct PaWalk {
     steps += g.i1 - g.i0;
     ++groups;
     wides += !g.narrow;
-    pos += g.tile1 - g.tile0;
+    base += g.nt + (g.narrow ? PA_EXTRA : PA_EXTRA / 2);
     tile0 = 0;
-    if (pos < end && --mt < 0) {  // next group of the head, next head, next row with work
+    if (base < end && --mt < 0) {  // next group of the head, next head, next row with work
       if (++head == a.heads) {
         head = 0;
         do ++row; while (row < a.B - 1 && at_row<PA_ROWS / 8>(a, row).n == 0);
@@ -215,13 +210,14 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
   const uint32_t tmem = tmem_base;
   const int64_t each = max((total + gridDim.x - 1) / (int64_t)gridDim.x, (int64_t)1);
   PaWalk<TREE> walk;
-  walk.pos = blockIdx.x * each;
-  walk.end = min(walk.pos + each, total);
+  const int64_t pos = blockIdx.x * each;
+  walk.base = pos;
+  walk.end = min(pos + each, total);
   walk.row = -1;
   walk.head = walk.mt = walk.tile0 = 0;
   walk.steps = walk.groups = walk.wides = 0;
   int4 join = make_int4(0, 0, 0, 0);
-  if (walk.pos < walk.end) {  // where it begins: rows' units counted up by all threads
+  if (pos < walk.end) {  // where it begins: rows' units counted up by all threads
     int64_t before = 0;
     for (int r0 = 0; r0 < a.B && walk.row < 0; r0 += PA_NT) {
       const int r = r0 + tid;
@@ -242,7 +238,7 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
         if (i < warp) lo += scr[i];
         before += scr[i];
       }
-      if (walk.pos >= lo && walk.pos < lo + n) {
+      if (pos >= lo && pos < lo + n) {
         found = r;
         found_lo = lo;
       }
@@ -250,14 +246,16 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
       walk.row = found;
     }
     const AtRow rw = at_row<PA_ROWS / 8>(a, walk.row);
-    const int64_t per_head = pa_units(a, walk.row) / a.heads, rel = walk.pos - found_lo;
+    const int64_t per_head = pa_units(a, walk.row) / a.heads, rel = pos - found_lo;
     walk.head = (int)(rel / per_head);
     int64_t u = rel - walk.head * per_head;
     walk.mt = rw.mt - 1;  // later groups see more: they come first
-    while (u >= pa_tiles(a, rw, walk.mt)) u -= pa_tiles(a, rw, walk.mt--);
-    walk.tile0 = (int)u;
+    for (int here; u >= (here = pa_tiles(a, rw, walk.mt) + pa_extra(a, rw, walk.mt)); --walk.mt) u -= here;
+    const int extra = pa_extra(a, rw, walk.mt);
+    walk.base = pos - u;
+    walk.tile0 = (int)max(u - extra, (int64_t)0);
     // The first cut inside its group joins the pieces.
-    const int64_t from = walk.pos - walk.tile0;
+    const int64_t from = walk.base + extra;
     if (walk.tile0 > 0 && from >= ((int64_t)blockIdx.x - 1) * each)
       join = make_int4(walk.row, walk.mt * a.heads + walk.head, (int)((from + pa_tiles(a, rw, walk.mt) - 1) / each) - (int)blockIdx.x + 2, 0);
   }
@@ -285,40 +283,20 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
       };
       float fq = fabsf(a.scale);
       if (!narrow || q == 0) {
-        // The row's 16-byte pieces, twice: for its largest exponent, which goes to 0 (bf16 to f16; the power of two goes
-        // into the row's factor), and as operand.
+        // Largest exponent of the row to 0 (bf16 to f16); the power of two goes into the row's factor.
         const uint16_t* src = reinterpret_cast<const uint16_t*>(a.q) + (int64_t)(start + qi) * a.q_st + (int64_t)qh * a.q_sh;
-        auto piece_of = [&](int i) {
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (in) {
-            if (a.aligned) {
-              v = __ldg(reinterpret_cast<const uint4*>(src) + i);
-            } else {
-              uint32_t u[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e) u[e] = (uint32_t)src[8 * i + 2 * e] | ((uint32_t)src[8 * i + 2 * e + 1] << 16);
-              v = make_uint4(u[0], u[1], u[2], u[3]);
-            }
-          }
-          return v;
-        };
         float down = 1.0f;
-        if (DT == LSS_DTYPE_BF16) {
-          uint32_t top = 0;  // magnitudes of bf16 order as whole numbers do
-#pragma unroll 8
-          for (int i = 0; i < CH; ++i) {
-            const uint4 v = piece_of(i);
-            top = __vmaxu2(__vmaxu2(top, v.x & 0x7fff7fffu), __vmaxu2(v.y & 0x7fff7fffu, __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
-          }
+        auto top_of = [&](uint32_t top, const uint4& v) {  // magnitudes of bf16 order as whole numbers do
+          return __vmaxu2(__vmaxu2(top, v.x & 0x7fff7fffu), __vmaxu2(v.y & 0x7fff7fffu, __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
+        };
+        auto factor = [&](uint32_t top) {
           top = max(top & 0xffffu, top >> 16);
           const int e = min(max((int)(top >> 7) - 127, -126), 126);
           down = __uint_as_float((uint32_t)(127 - e) << 23);
           fq *= __uint_as_float((uint32_t)(127 + e) << 23);
-        }
+        };
         const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;  // scores are compared before they are scaled
-#pragma unroll 8
-        for (int i = 0; i < CH; ++i) {
-          const uint4 v = piece_of(i);
+        auto put = [&](int i, const uint4& v) {
           uint32_t u[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
@@ -329,6 +307,35 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
             u[e] ^= sign;
           }
           *reinterpret_cast<uint4*>(qs + tile * OPB + pa_place(r, i)) = make_uint4(u[0], u[1], u[2], u[3]);
+        };
+        uint32_t top = 0;
+        if (a.aligned) {
+          uint4 v[CH];
+#pragma unroll
+          for (int i = 0; i < CH; ++i) v[i] = in ? __ldg(reinterpret_cast<const uint4*>(src) + i) : make_uint4(0, 0, 0, 0);
+          if (DT == LSS_DTYPE_BF16) {
+#pragma unroll
+            for (int i = 0; i < CH; ++i) top = top_of(top, v[i]);
+            factor(top);
+          }
+#pragma unroll
+          for (int i = 0; i < CH; ++i) put(i, v[i]);
+        } else {  // value by value, twice
+          auto piece_of = [&](int i) {
+            uint32_t u[4] = {0, 0, 0, 0};
+            if (in) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) u[e] = (uint32_t)src[8 * i + 2 * e] | ((uint32_t)src[8 * i + 2 * e + 1] << 16);
+            }
+            return make_uint4(u[0], u[1], u[2], u[3]);
+          };
+          if (DT == LSS_DTYPE_BF16) {
+#pragma unroll 1
+            for (int i = 0; i < CH; ++i) top = top_of(top, piece_of(i));
+            factor(top);
+          }
+#pragma unroll 1
+          for (int i = 0; i < CH; ++i) put(i, piece_of(i));
         }
         if (narrow) row_factor[r] = fq;
         fence_proxy_async();
