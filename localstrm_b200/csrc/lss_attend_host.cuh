@@ -68,6 +68,12 @@ static inline cudaError_t launch_attend_few(const AttendArgs& a, int64_t rows, v
     }
     return launch_attend<D, DT, 1, 1, TREE>(a, ws, st);
   }
+  if constexpr (TREE) {
+    // Small trees: groups of eight rows where all of their tiles find a warp at once (6 tokens of 7 heads per key head of 64
+    // over 700: 15 us, in groups of 16 20 us, of 32 26 us).
+    const int64_t units = (a.B + (int64_t)a.T * a.per / 8 + 1) * a.heads * ((((int64_t)a.width << a.bs_shift) + 15) >> 4);
+    if (units <= (int64_t)sm_count(device_index()) * AtCfg<D, 1, 1>::NW) return launch_attend<D, DT, 1, 1, TREE>(a, ws, st);
+  }
   if constexpr (D < 256) {
     if (rows > 16) return launch_attend<D, DT, 4, 1, TREE>(a, ws, st);
   }
@@ -88,14 +94,19 @@ static inline cudaError_t launch_attend_few(const AttendArgs& a, int64_t rows, v
 // A step of no more tokens than rows counts as one of single tokens: a chunk among idle rows is right, but goes in
 // their groups (200 tokens over 8,000 beside 255 idle rows 213 us, alone 201; 500 beside 511 507 us, alone 171), as the
 // launches for chunks would cost every step of single tokens 8 to 10 us.
+// Trees: the rows of a batch are mostly alike, a few tokens to some dozens each, and the tensor-memory kernel is the faster one from 17
+// query rows on (D = 64: from 33), also where a single row has tokens enough for the SMs (48 rows over 4,000 tokens, 8
+// key heads of 4 queries of 128, in groups of 16 for comparison: 4 tokens each 161 us, 6 tokens 202 (243), 8 tokens 202 (314), 30 tokens
+// 212 (980); D = 64: 6 tokens 161, 10 tokens 177 (196); 64 tokens of 8 heads per key head over 20,000 alone 120 (300)).
 template <int D, int DT, bool TREE>
 static inline cudaError_t launch_attend_rows(AttendArgs a, void* ws, cudaStream_t st) {
   const int64_t average = (int64_t)a.per * ((a.T + (int64_t)a.B - 1) / a.B);
   a.rows_lo = 0;
   a.rows_hi = INT32_MAX;
   if constexpr (D < 256) {
-    if (a.T > a.B && (int64_t)a.heads * a.per * a.T >= (int64_t)PA_ROWS * sm_count(device_index()) / 4) {
-      const int pa_from = D == 128 && a.per <= 8 ? 41 : 64;
+    const int sms = sm_count(device_index()), pa_from = TREE ? (D == 128 ? 17 : 33) : D == 128 && a.per <= 8 ? 41 : 64;
+    const int64_t tiles = ((((int64_t)a.width << a.bs_shift) + PA_KT - 1) / PA_KT) * a.heads * a.B;
+    if (a.T > a.B && ((int64_t)a.heads * a.per * a.T >= (int64_t)PA_ROWS * sms / 4 || (TREE && average >= pa_from && tiles >= sms))) {
       a.rows_lo = pa_from;
       const cudaError_t e = launch_attend_tc<D, DT, TREE>(a, ws, st);
       if (e != cudaSuccess) return e;

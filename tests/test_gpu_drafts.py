@@ -225,7 +225,7 @@ def test_attend_tree_of_chains_is_causal(ctx, new, heads, per, bs, dim):
     y, lse = check_attend_tree(q, cache, rows, chains)
     lse2 = torch.empty_like(lse)
     causal = lb.attend(q, cache, rows[1], lb.StepPlan(*rows[2:5]), lse_out=lse2)
-    if 8 * per * sum(new) < 9000:  # the kernel for few rows: the same sums of the same terms
+    if dim == 256:  # the kernel for few rows in both forms: the same sums of the same terms
         assert torch.equal(y, causal) and torch.equal(lse, lse2)
     # In tensor memory a step with new tokens rounds the share of the softmax times a factor, others the weight itself:
     # both forms are within the bound of the same exact result (the causal one by its own tests).
