@@ -54,8 +54,7 @@ def plan_tree(plan: StepPlan, parents: torch.Tensor) -> TreePlan:
     dev = _device(plan)
     B, T = plan.granted.numel(), parents.numel()
     at = _ints("parents", parents, T, dev)
-    span = torch.empty(T, 2, dtype=_I32, device=parents.device)
-    positions = torch.empty(T, dtype=_I32, device=parents.device)
+    span, positions = parents.new_empty((T, 2)), parents.new_empty((T,))
     lib = _lib.load()
     with _on(dev):
         _lib.check("lss_tree_plan", lib.lss_tree_plan(
@@ -78,13 +77,14 @@ def accept_drafts(plan: StepPlan, tree: TreePlan, tokens: torch.Tensor, targets:
     ``lens_out`` may be ``plan.lens`` (which ``compact_kv`` and ``plan.stops`` still need as it is)."""
     dev = _device(plan)
     B, T = plan.granted.numel(), tree.parents.numel()
-    new = torch.empty(2 * T + 4 * B, dtype=_I32, device=plan.starts.device)  # one allocation for the results
+    starts_at = _ints("plan.starts", plan.starts, B + 1, dev)
+    new = plan.starts.new_empty((2 * T + 4 * B,))  # one allocation for the results
     path, said, counts, lens, last, stop = new.split_with_sizes((T, T, B, B, B, B))
     lens = lens if lens_out is None else lens_out
     lib = _lib.load()
     with _on(dev):
         _lib.check("lss_tree_accept", lib.lss_tree_accept(
-            _ints("plan.starts", plan.starts, B + 1, dev), _ints("plan.granted", plan.granted, B, dev),
+            starts_at, _ints("plan.granted", plan.granted, B, dev),
             _ints("plan.lens", plan.lens, B, dev), B, _ints("tree.parents", tree.parents, T, dev), _ints("tokens", tokens, T, dev),
             _ints("targets", targets, T, dev), None if codes is None else _ints("codes", codes, T, dev),
             None if given is None else _ints("given", given, B, dev), T, path.data_ptr(), said.data_ptr(), counts.data_ptr(),

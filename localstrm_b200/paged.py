@@ -100,13 +100,12 @@ class KVCache8:
         shape = k.shape
         if len(shape) != 4:
             raise ValueError("cache: k must be [num_blocks, heads, block_size, dim]")
-        for name, t in (("k", k), ("v", v)):
-            if t.dtype is not _E4M3 or t.get_device() != device or not t.is_contiguous() or t.shape != shape:
-                raise ValueError(f"cache: {name} must be a contiguous float8_e4m3fn {list(shape)} on cuda:{device}")
-        for name, t in (("k_scale", ks), ("v_scale", vs)):
-            if t.dtype is not _F32 or t.get_device() != device or not t.is_contiguous() or t.dim() != 2 \
-                    or t.shape[0] != shape[0] or t.shape[1] != shape[1]:
-                raise ValueError(f"cache: {name} must be a contiguous float32 {list(shape[:2])} on cuda:{device}")
+        if not (k.dtype is _E4M3 and v.dtype is _E4M3 and k.get_device() == device and v.get_device() == device and k.is_contiguous()
+                and v.is_contiguous() and v.shape == shape):
+            raise ValueError(f"cache: k and v must be contiguous float8_e4m3fn {list(shape)} on cuda:{device}")
+        if not (ks.dtype is _F32 and vs.dtype is _F32 and ks.get_device() == device and vs.get_device() == device and ks.is_contiguous()
+                and vs.is_contiguous() and ks.shape == shape[:2] and vs.shape == shape[:2]):
+            raise ValueError(f"cache: k_scale and v_scale must be contiguous float32 {list(shape[:2])} on cuda:{device}")
         return shape
 
 
@@ -184,9 +183,9 @@ def release_blocks(block_table: torch.Tensor, lens: torch.Tensor, codes: torch.T
     if blocks < 1:
         raise ValueError("free_blocks must not be empty")
     if lens_out is None:
-        lens_out = torch.empty(B, dtype=_I32, device=block_table.device)
+        lens_out = lens.new_empty((B,))
     if n_free_out is None:
-        n_free_out = torch.empty(1, dtype=_I32, device=block_table.device)
+        n_free_out = lens.new_empty((1,))
     lens_out_at, n_free_out_at = _ints("lens_out", lens_out, B, dev), _ints("n_free_out", n_free_out, 1, dev)
     lib = _lib.load()
     with _on(dev):
@@ -221,7 +220,7 @@ def fork_blocks(block_table: torch.Tensor, lens: torch.Tensor, src_rows: torch.T
     lens_at = _ints("lens", lens, B, dev)
     free_at, n_free_at = _ints("free_blocks", free_blocks, blocks, dev), _ints("n_free", n_free, 1, dev)
     # One allocation for the results.
-    copies, granted, new_state, new_free = torch.empty(3 * n + B + 1, dtype=_I32, device=block_table.device).split_with_sizes((2 * n, n, B, 1))
+    copies, granted, new_state, new_free = lens.new_empty((3 * n + B + 1,)).split_with_sizes((2 * n, n, B, 1))
     lens_out, n_free_out = new_state if lens_out is None else lens_out, new_free if n_free_out is None else n_free_out
     lib = _lib.load()
     with _on(dev):
@@ -307,7 +306,7 @@ def attend(q: torch.Tensor, cache: KVCache8, block_table: torch.Tensor, plan: St
         q = q.contiguous()
         qs = q.stride()
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=block_table.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         os = out.stride()
     else:
         os = out.stride()
@@ -330,7 +329,7 @@ def attend(q: torch.Tensor, cache: KVCache8, block_table: torch.Tensor, plan: St
         size = _WORKSPACE.get(dim)
         if size is None:
             size = _WORKSPACE[dim] = int(lib.lss_attend_workspace_bytes(dim))
-        ws = torch.empty(size, dtype=torch.uint8, device=block_table.device)
+        ws = block_table.new_empty((size // 4,))
         name = "lss_attend" if tree is None else "lss_attend_tree"
         _lib.check(name, getattr(lib, name)(
             q.data_ptr(), qs[0], qs[1], _CODES[dtype], shape[0], shape[1], heads, dim, cache.k.data_ptr(), cache.v.data_ptr(),

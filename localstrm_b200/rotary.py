@@ -16,9 +16,10 @@ from .sampling import _require_cuda
 __all__ = ["norm_rotate"]
 
 
-def _out(name: str, out: Optional[torch.Tensor], x: torch.Tensor) -> torch.Tensor:
-    if out is None:
-        return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+_I32, _F32, _DENSE = torch.int32, torch.float32, torch.contiguous_format
+
+
+def _out(name: str, out: torch.Tensor, x: torch.Tensor) -> torch.Tensor:
     if out.shape != x.shape or out.dtype is not x.dtype or out.get_device() != x.get_device() or out.stride(2) != 1:
         raise ValueError(f"{name}: expected {x.dtype} {list(x.shape)} on {x.device} with rows of stride 1")
     return out
@@ -38,36 +39,43 @@ def norm_rotate(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, freqs
     their fraction), rounded once.  ``q_out`` / ``k_out`` may be ``q`` and ``k`` themselves; results that overlap the inputs
     in another way, or each other, are refused."""
     _require_cuda(q)
-    dev, dtype, shape = q.get_device(), q.dtype, q.shape
-    if len(shape) != 3 or k.dim() != 3 or k.shape[0] != shape[0] or k.shape[2] != shape[2] or k.get_device() != dev:
+    dev, dtype, shape, k_shape = q.get_device(), q.dtype, q.shape, k.shape
+    if len(shape) != 3 or len(k_shape) != 3 or k_shape[0] != shape[0] or k_shape[2] != shape[2] or k.get_device() != dev:
         raise ValueError(f"q, k: expected [T, heads, dim] of the same T and dim on cuda:{dev}")
     if dtype not in _CODES or k.dtype is not dtype:
         raise TypeError(f"unsupported dtypes {dtype}, {k.dtype}")
     T, heads, dim = shape
-    if positions.dtype is not torch.int32 or positions.shape != (T,) or positions.get_device() != dev or not positions.is_contiguous():
+    if positions.dtype is not _I32 or positions.dim() != 1 or positions.numel() != T or positions.get_device() != dev \
+            or not positions.is_contiguous():
         raise ValueError(f"positions: expected a contiguous int32 tensor of {T} entries on cuda:{dev}")
-    if freqs.dtype is not torch.float32 or freqs.dim() != 1 or freqs.get_device() != dev or not freqs.is_contiguous() \
-            or 2 * freqs.shape[0] > dim:
+    half = freqs.numel()
+    if freqs.dtype is not _F32 or freqs.dim() != 1 or freqs.get_device() != dev or not freqs.is_contiguous() or 2 * half > dim:
         raise ValueError(f"freqs: expected a contiguous float32 tensor of at most {dim // 2} entries on cuda:{dev}")
     code = 0
     for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
         if w is None:
             continue
-        if w.shape != (dim,) or w.get_device() != dev or not w.is_contiguous() or w.dtype not in _CODES:
+        if w.dim() != 1 or w.numel() != dim or w.get_device() != dev or not w.is_contiguous() or w.dtype not in _CODES:
             raise ValueError(f"{name}: expected a contiguous float32, bfloat16 or float16 tensor of {dim} entries on cuda:{dev}")
         code = _CODES[w.dtype]
     if q_weight is not None and k_weight is not None and q_weight.dtype is not k_weight.dtype:
         raise TypeError(f"weights of two types: {q_weight.dtype}, {k_weight.dtype}")
-    if q.stride(2) != 1:
+    qs, ks = q.stride(), k.stride()
+    if qs[2] != 1:
         q = q.contiguous()
-    if k.stride(2) != 1:
+        qs = q.stride()
+    if ks[2] != 1:
         k = k.contiguous()
-    q_out, k_out = _out("q_out", q_out, q), _out("k_out", k_out, k)
-    qs, ks, qo, ko = q.stride(), k.stride(), q_out.stride(), k_out.stride()
+        ks = k.stride()
+    q_out = torch.empty_like(q, memory_format=_DENSE) if q_out is None else _out("q_out", q_out, q)
+    k_out = torch.empty_like(k, memory_format=_DENSE) if k_out is None else _out("k_out", k_out, k)
+    qo, ko = q_out.stride(), k_out.stride()
     lib = _lib.load()
     with _on(dev):
-        _lib.check("lss_norm_rotate", lib.lss_norm_rotate(
+        status = lib.lss_norm_rotate(
             q.data_ptr(), qs[0], qs[1], q_out.data_ptr(), qo[0], qo[1], heads, k.data_ptr(), ks[0], ks[1], k_out.data_ptr(), ko[0],
-            ko[1], k.shape[1], _CODES[dtype], T, dim, positions.data_ptr(), freqs.data_ptr(), 2 * freqs.shape[0], interleaved,
-            None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(), code, eps, _stream(dev)))
+            ko[1], k_shape[1], _CODES[dtype], T, dim, positions.data_ptr(), freqs.data_ptr(), 2 * half, interleaved,
+            None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(), code, eps, _stream(dev))
+    if status:
+        _lib.check("lss_norm_rotate", status)
     return q_out, k_out

@@ -225,13 +225,27 @@ def test_attend_tree_of_chains_is_causal(ctx, new, heads, per, bs, dim):
     y, lse = check_attend_tree(q, cache, rows, chains)
     lse2 = torch.empty_like(lse)
     causal = lb.attend(q, cache, rows[1], lb.StepPlan(*rows[2:5]), lse_out=lse2)
-    if dim == 256:  # the kernel for few rows in both forms: the same sums of the same terms
-        assert torch.equal(y, causal) and torch.equal(lse, lse2)
-    # In tensor memory a step with new tokens rounds the share of the softmax times a factor, others the weight itself:
-    # both forms are within the bound of the same exact result (the causal one by its own tests).
+    # The two forms may take other kernels and cut the work elsewhere, so that sums round differently: both are within the
+    # bound of the same exact result (the causal one by its own tests).
     want, mag, _ = U.attend_reference(q, cache.k, cache.v, cache.k_scale, cache.v_scale, rows[0], *(x.tolist() for x in rows[2:5]), dim ** -0.5)
     tol = 1.25 * 2.0 ** -11 * mag + torch.finfo(q.dtype).eps / 2 * want.abs() + 2.0 ** -24
     assert bool(((y.double() - want).abs() <= tol).all()) and bool(((y.double() - causal.double()).abs() <= 2 * tol).all())
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("per", [4, 3])
+def test_attend_chunks_of_whole_and_half_groups(dim, per):
+    """Groups of up to 128 query rows behind ones of 256, causal and as chains: in the first ones the two streams take
+    every other step each, and must not take a stage of keys for one that comes later."""
+    ctx, new = [1000, 2003, 61, 3340], [256, 353, 700, 431]
+    rows = U.make_rows(ctx, new, 16, seed=dim + per)
+    cache = lb.KVCache8(*U.random_cache(rows[-1], 8, 16, dim, seed=per))
+    q = torch.randn(sum(new), 8 * per, dim, generator=gen(dim), device=DEV).bfloat16()
+    y, _ = check_attend_tree(q, cache, rows, [i - 1 for n in new for i in range(n)])
+    want, mag, _ = U.attend_reference(q, cache.k, cache.v, cache.k_scale, cache.v_scale, rows[0], *(x.tolist() for x in rows[2:5]), dim ** -0.5)
+    for _ in range(3):
+        causal = lb.attend(q, cache, rows[1], lb.StepPlan(*rows[2:5]))
+        assert bool(((causal.double() - want).abs() <= 1.25 * 2.0 ** -11 * mag + 2.0 ** -8 * want.abs()).all())
 
 
 @pytest.mark.parametrize("ctx,new,heads,per,dim", [([20, 3], [9, 5], 2, 4, 128), ([20, 100], [64, 70], 8, 4, 128), ([20, 1], [33, 90], 8, 7, 64), ([5, 0], [7, 20], 2, 1, 256)])
