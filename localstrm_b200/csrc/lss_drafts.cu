@@ -55,6 +55,34 @@ static bool rows_ok(const void* x, int64_t st, int64_t sh, int heads, int T, int
          (T == 1 || heads == 1 || st >= (heads - 1) * sh + dim || sh >= (T - 1) * st + dim);
 }
 
+// CTAs that share a release: every entry is a scattered access or two per pass, which eight SMs take longer for than
+// sixteen (37 us against 23 for 46,000 entries); sixteen where the device runs such a cluster with all of its shared memory.
+static int give_ctas(int dev) {
+  static int n[MAX_DEV] = {};
+  std::lock_guard<std::mutex> lock(g_mu);
+  if (n[dev] == 0) {
+    constexpr int smem = 224 * 1024;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(16, 1, 1);
+    cfg.blockDim = dim3(BL_NT, 1, 1);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = 16;
+    at[0].val.clusterDim.y = 1;
+    at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    int c = 0;
+    const bool ok = cudaFuncSetAttribute(lss_give_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
+                    cudaFuncSetAttribute(lss_give_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) == cudaSuccess &&
+                    cudaOccupancyMaxActiveClusters(&c, lss_give_kernel, &cfg) == cudaSuccess && c >= 1;
+    if (!ok) cudaGetLastError();
+    n[dev] = ok ? 16 : BL_MAXCL;
+  }
+  return n[dev];
+}
+
 extern "C" {
 
 int lss_norm_rotate(const void* q, int64_t q_token_stride, int64_t q_head_stride, void* q_out, int64_t q_out_token_stride,
@@ -189,14 +217,17 @@ int lss_block_give(const int32_t* table, int64_t table_stride, int width, const 
   if (B > LSS_BLOCK_MAX_ROWS || (int64_t)B * width > (1 << 30)) return LSS_ERR_UNSUPPORTED;
   if (!free_blocks || !n_free || !n_free_out || (B > 0 && (!lens || !lens_out))) return LSS_ERR_INVALID_ARG;
   if (cut(lens_out, lens, B) || (codes && cut(lens_out, codes, B)) || (keep && cut(lens_out, keep, B))) return LSS_ERR_INVALID_ARG;
-  GiveArgs a{table, table_stride, width, lens, codes, keep, B, block_size, num_blocks, shares, free_blocks, n_free, lens_out, n_free_out};
+  GiveArgs a{table, table_stride, width, lens, codes, keep, B, block_size, num_blocks, shares, free_blocks, n_free, lens_out, n_free_out, 0};
   static SmemSet set;
-  const int smem = 4 * B;
+  const int dev = device_index(), ctas = cluster_for((B + 31) / 32, give_ctas(dev));
+  // Room for the entries of each warp's rows, up to 192 KB per CTA.
+  const int64_t pieces = (int64_t)((B + ctas * 32 - 1) / (ctas * 32)) * (((int64_t)width + 255) / 256);
+  a.held = (int)std::min(pieces, (int64_t)(224 * 1024 - 4 * B) / (32 * 1024));
+  const int smem = 4 * B + a.held * 32 * 1024;
   if (smem > 40 * 1024) {
-    const cudaError_t e = allow_smem(lss_give_kernel, set, device_index(), smem);
+    const cudaError_t e = allow_smem(lss_give_kernel, set, dev, smem);
     if (e != cudaSuccess) return status_of(e);
   }
-  const int ctas = cluster_for((B + 31) / 32, BL_MAXCL);
   return status_of(launch(lss_give_kernel, (unsigned)ctas, BL_NT, (size_t)smem, ctas, false, reinterpret_cast<cudaStream_t>(stream), a));
 }
 
