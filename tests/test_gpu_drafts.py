@@ -507,3 +507,177 @@ def test_state_refusals():
     for bad in (dict(tokens=one), dict(targets=two.long()), dict(codes=one), dict(given=one), dict(lens_out=one)):
         with pytest.raises(ValueError):
             lb.accept_drafts(plan, tree, **{**dict(tokens=two, targets=two), **bad})
+
+
+# ------------------------------------------------------------------------- steps with drafted tokens
+class Toy:
+    """One layer of attention with tied random embeddings: the next token is the largest of W o.  Its state lies in a
+    paged cache; a step takes drafted tokens with their trees."""
+    HEADS, PER, DIM, BS, VOCAB = 2, 2, 64, 16, 40
+
+    def __init__(self, rows, blocks, width, seed):
+        g = gen(seed)
+        q, k = self.HEADS * self.PER * self.DIM, self.HEADS * self.DIM
+        self.embed = torch.randn(self.VOCAB, q + 2 * k, generator=g, device=DEV).half()
+        self.head = torch.randn(q, self.VOCAB, generator=g, device=DEV)
+        self.weights = [(1 + 0.2 * torch.randn(self.DIM, generator=g, device=DEV)).half() for _ in range(2)]
+        self.freqs = (100.0 ** (-torch.arange(0, self.DIM, 2, device=DEV, dtype=torch.float64) / self.DIM)).float()
+        self.cache = lb.KVCache8.empty(blocks, self.HEADS, self.BS, self.DIM, device=DEV)
+        self.table = torch.full((rows, width), -1, dtype=torch.int32, device=DEV)
+        self.lens = torch.zeros(rows, dtype=torch.int32, device=DEV)
+        self.free, self.n_free = torch.arange(blocks, dtype=torch.int32, device=DEV), ints([blocks])
+
+    def step(self, new, tokens, parents, given, eos=-1):
+        T, q, k = tokens.numel(), self.HEADS * self.PER * self.DIM, self.HEADS * self.DIM
+        plan = lb.plan_blocks(self.table, self.lens, new, self.free, self.n_free, self.BS, T, lens_out=self.lens, n_free_out=self.n_free)
+        tree = lb.plan_tree(plan, parents)
+        x = self.embed[tokens.long()]
+        queries, keys, values = (y.unflatten(1, (-1, self.DIM)) for y in x.split((q, k, k), 1))
+        queries, keys = lb.norm_rotate(queries, keys, tree.positions, self.freqs, q_weight=self.weights[0], k_weight=self.weights[1])
+        lb.append_kv(self.cache, keys, values, self.table, plan)
+        o = lb.attend(queries, self.cache, self.table, plan, tree=tree)
+        logits = o.flatten(1).float() @ self.head
+        targets = logits.argmax(-1).int()
+        a = lb.accept_drafts(plan, tree, tokens, targets, codes=(targets == eos).int(), given=given)
+        lb.compact_kv(self.cache, self.table, plan, a.path, a.counts)
+        lb.release_blocks(self.table, self.lens, a.codes, self.free, self.n_free, self.BS, lens_out=self.lens, n_free_out=self.n_free, keep=a.lens)
+        top = logits.topk(2).values
+        return a, top[:, 0] - top[:, 1]
+
+
+def prompt_step(toy, prompts):
+    tokens = ints([t for p in prompts for t in p])
+    return toy.step(ints([len(p) for p in prompts]), tokens, ints([i - 1 for p in prompts for i in range(len(p))]), ints([len(p) for p in prompts]))
+
+
+def test_drafted_steps_give_the_tokens_of_single_ones():
+    """Whatever is drafted, the tokens are those of sampling one by one.  The two ways round differently: f16 results of about
+    0.35 with errors of up to 2^-11 of that, so some 2e-4 between the two, in 256 terms 0.0032 of a logit; where the two
+    largest logits are less than six times that (0.02) apart, the token, and the row behind it, is not decided."""
+    rng = random.Random(11)
+    prompts = [[rng.randrange(40) for _ in range(n)] for n in (5, 16, 31)]
+    want_n = 40
+    one = Toy(3, 40, 8, seed=4)
+    a, gap = prompt_step(one, prompts)
+    truth, decided = [[t] for t in a.last.tolist()], [None] * 3
+    for _ in range(want_n):
+        a, gap = one.step(ints([1, 1, 1]), ints([t[-1] for t in truth]), ints([-1, -1, -1]), None)
+        for b, t in enumerate(a.last.tolist()):
+            if float(gap[b]) < 0.02 and decided[b] is None:
+                decided[b] = len(truth[b])
+            truth[b].append(t)
+    toy = Toy(3, 40, 8, seed=4)
+    a, _ = prompt_step(toy, prompts)
+    got, steps = [[t] for t in a.last.tolist()], 0
+    while min(len(t) for t in got) < want_n:
+        new, tokens, parents = [], [], []
+        for b, t in enumerate(got):
+            n = rng.choice([1, 4, 9, 20])
+            tree = D.random_tree(n, rng, chain=0.6, root=0.0)
+            node = [t[-1]]
+            depth = [0]
+            for i in range(1, n):  # what would really come, or anything
+                depth.append(depth[tree[i]] + 1)
+                at = len(t) - 1 + depth[i]
+                node.append(truth[b][at] if at < len(truth[b]) and rng.random() < 0.8 else rng.randrange(40))
+            new.append(n)
+            tokens += node
+            parents += tree
+        a, _ = toy.step(ints(new), ints(tokens), ints(parents), None)
+        said, at = a.tokens.tolist(), 0
+        for b, n in enumerate(new):
+            out = [x for x in said[at: at + n] if x >= 0]
+            assert len(out) == a.counts[b] and out[-1] == a.last[b]
+            got[b] += out
+            at += n
+        steps += 1
+        held = int(((toy.lens + 15) // 16).sum())
+        assert int(toy.n_free) + held == 40
+        assert toy.lens.tolist() == [len(p) + len(t) - 1 for p, t in zip(prompts, got)]
+    decided = [want_n if n is None else min(n, want_n) for n in decided]
+    assert sum(decided) >= 60
+    for b, n in enumerate(decided):
+        assert got[b][:n] == truth[b][:n]
+    assert steps < 30  # several tokens a step
+
+
+def test_drafted_step_captured_and_replayed():
+    rng = random.Random(3)
+    prompts = [[rng.randrange(40) for _ in range(n)] for n in (20, 7)]
+    drafts = [[rng.randrange(40) for _ in range(12)] for _ in range(4)]
+    parents, new = ints([-1, 0, 0, 1, 1, 2, -1, 0, 1, 1, 3, 0]), ints([6, 6])
+    results = []
+    for captured in (False, True):
+        toy = Toy(2, 20, 8, seed=9)
+        prompt_step(toy, prompts)
+        tokens = torch.zeros(12, dtype=torch.int32, device=DEV)
+        if captured:
+            state = [x.clone() for x in (toy.table, toy.lens, toy.free, toy.n_free, toy.cache.k.view(torch.uint8), toy.cache.v.view(torch.uint8), toy.cache.k_scale, toy.cache.v_scale)]
+            toy.step(new, tokens, parents, None)
+            for x, y in zip((toy.table, toy.lens, toy.free, toy.n_free, toy.cache.k.view(torch.uint8), toy.cache.v.view(torch.uint8), toy.cache.k_scale, toy.cache.v_scale), state):
+                x.copy_(y)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                a, _ = toy.step(new, tokens, parents, None)
+        out = []
+        for d in drafts:
+            tokens.copy_(ints(d))
+            if captured:
+                graph.replay()
+            else:
+                a, _ = toy.step(new, tokens, parents, None)
+            out += [x.clone() for x in (a.path, a.tokens, a.counts, a.lens, a.last, toy.lens, toy.n_free, toy.free, toy.table, toy.cache.k.view(torch.uint8), toy.cache.v_scale)]
+        results.append(out)
+    for x, y in zip(*results):
+        assert torch.equal(x, y)
+
+
+def test_samples_of_a_prompt_share_its_blocks():
+    """Samples that fork a prompt go on as rows that have it for themselves; their blocks all come back."""
+    rng = random.Random(5)
+    prompt = [rng.randrange(40) for _ in range(37)]
+    toys = [Toy(4, 30, 8, seed=2) for _ in range(2)]
+    first = [[rng.randrange(40) for _ in range(4)] for _ in range(6)]
+    shares = torch.zeros(30, dtype=torch.int32, device=DEV)
+    shared, alone = toys
+    prompt_step(shared, [prompt, [], [], []])
+    f = lb.fork_blocks(shared.table, shared.lens, ints([0, 0, 0]), ints([1, 2, 3]), shares, shared.free, shared.n_free, 16, upto=ints([37, 37, 32]),
+                       lens_out=shared.lens, n_free_out=shared.n_free)
+    lb.copy_blocks(shared.cache, f.copies)
+    assert f.granted.tolist() == [37, 37, 32] and shared.n_free.tolist() == [30 - 3 - 2] and int(shares.sum()) == 6
+    prompt_step(alone, [prompt, prompt, prompt, prompt[:32]])
+    for tokens in first:
+        outs = []
+        for toy in toys:
+            plan = lb.plan_blocks(toy.table, toy.lens, ints([1] * 4), toy.free, toy.n_free, 16, 4, lens_out=toy.lens, n_free_out=toy.n_free)
+            x = toy.embed[torch.tensor(tokens, device=DEV)]
+            q, k, v = (y.unflatten(1, (-1, 64)) for y in x.split((256, 128, 128), 1))
+            lb.append_kv(toy.cache, k, v, toy.table, plan)
+            outs.append(lb.attend(q, toy.cache, toy.table, plan))
+        assert torch.equal(*outs)
+    lb.release_blocks(shared.table, shared.lens, ints([1, 0, 1, 0]), shared.free, shared.n_free, 16, lens_out=shared.lens, n_free_out=shared.n_free, shares=shares)
+    assert int(shares.sum()) == 2
+    lb.release_blocks(shared.table, shared.lens, ints([0, 1, 0, 1]), shared.free, shared.n_free, 16, lens_out=shared.lens, n_free_out=shared.n_free, shares=shares)
+    assert int(shares.sum()) == 0 and shared.n_free.tolist() == [30] and sorted(shared.free.tolist()) == list(range(30)) and shared.lens.tolist() == [0] * 4
+
+
+def test_two_streams_and_another_order():
+    """Calls on two streams at once, each with what it works on."""
+    rows, parents = tree_rows([3000, 900, 10], [40, 64, 9], 16, 3)
+    cache = lb.KVCache8(*U.random_cache(rows[-1], 8, 16, 128))
+    plan = lb.StepPlan(*rows[2:5])
+    q = [torch.randn(113, 32, 128, generator=gen(i), device=DEV).bfloat16() for i in range(2)]
+    tree = lb.plan_tree(plan, ints(parents))
+    pos = ints(list(range(113)))
+    freqs = torch.rand(64, generator=gen(1), device=DEV)
+    want = [(lb.attend(x, cache, rows[1], plan, tree=tree), *lb.norm_rotate(x, x[:, :8], pos, freqs)) for x in q]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [[], []]
+    for _ in range(4):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append((lb.attend(q[i], cache, rows[1], plan, tree=tree), *lb.norm_rotate(q[i], q[i][:, :8], pos, freqs)))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for g in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(g, want[i]))
