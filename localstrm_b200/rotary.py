@@ -36,7 +36,7 @@ def norm_rotate(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, freqs
     f16, both of one type), then the first ``2 * len(freqs)`` values are turned in pairs by ``positions[t] * freqs[i]``
     (``positions`` int32 ``[T]``, ``StepPlan.positions`` or ``TreePlan.positions``; ``freqs`` float32): value i with value
     ``i + len(freqs)``, or value 2 i with 2 i + 1 where ``interleaved``.  Computed in f32 (the angle is reduced in f64: far positions keep
-    their fraction), rounded once.  ``q_out`` / ``k_out`` may be ``q`` and ``k`` themselves; results that overlap the inputs
+    their fraction), rounded once; squares of the values have to lie within f32.  ``q_out`` / ``k_out`` may be ``q`` and ``k`` themselves; results that overlap the inputs
     in another way, or each other, are refused."""
     _require_cuda(q)
     dev, dtype, shape, k_shape = q.get_device(), q.dtype, q.shape, k.shape
