@@ -31,6 +31,11 @@ template <> struct AtCfg<256, 2, 1> { static constexpr int NW = 8, ST = 3; };
 // Floats of one piece in the workspace: m, l, W of its rows, then the sums.
 __host__ __device__ constexpr int at_piece(int D, int NQ) { return 8 * NQ * (3 + D); }
 
+// From this many tokens on, rows of fewer queries pay for the start and end of a group in tensor memory, and those of 16 queries more
+// (launch_attend_rows).
+static constexpr int AT_LONG = 2560;
+__host__ __device__ constexpr int at_long_more(int D) { return D == 128 ? 640 : 1024; }
+
 struct AttendArgs {
   const void* q;
   int64_t q_st, q_sh;  // strides in elements: token, head
@@ -52,7 +57,10 @@ struct AttendArgs {
   int B, T;
   float scale;         // softmax scale times log2(e)
   int aligned;         // q and out rows start on 16-byte boundaries
-  int rows_lo, rows_hi;  // rows of the batch with rows_lo <= query rows per key head < rows_hi are this launch's
+  // Which rows of the batch are this launch's: all, those for tensor memory, or the others.  For tensor memory are rows of
+  // rows_any query rows per key head and more, and long ones from rows_long on.
+  int side;  // 0, 1, 2
+  int rows_any, rows_long, long_more;
   int fused;           // the grid is one cluster, which joins its own pieces
   int4* meta;          // [workers]: row, group, pieces (0: nothing to join)
   float* part;         // [workers][2][at_piece]: a warp's first piece, its last one
@@ -125,7 +133,9 @@ __device__ __forceinline__ AtRow at_row(const AttendArgs& a, int r) {
   w.len = a.lens[r];
   const int s = a.starts[r];
   const bool ok = w.n > 0 && w.n <= w.len && w.len <= ((int64_t)a.width << a.bs_shift) && s >= 0 && (int64_t)s + w.n <= a.T;
-  if (!ok || (int64_t)w.n * a.per < a.rows_lo || (int64_t)w.n * a.per >= a.rows_hi) w.n = 0;
+  const int64_t rows = (int64_t)w.n * a.per;
+  const bool tensor = rows >= a.rows_any || (rows >= a.rows_long && w.len >= (rows < a.rows_long + 16 ? AT_LONG : a.long_more));
+  if (!ok || (a.side && tensor != (a.side == 1))) w.n = 0;
   w.nt = w.n > 0 ? (w.len + 15) >> 4 : 0;
   w.mt = w.n > 0 ? (int)(((int64_t)w.n * a.per + 8 * NQ - 1) / (8 * NQ)) : 0;
   return w;

@@ -82,37 +82,42 @@ static inline cudaError_t launch_attend_few(const AttendArgs& a, int64_t rows, v
 
 // A step of single tokens has `per` query rows per key head and row; else the average decides.  A step with more
 // tokens than rows, and enough of them to fill the SMs, may mix prompt chunks, rows of a few tokens and single
-// tokens, and only the device knows which is which: rows of pa_from query rows and more go to the tensor-memory
-// kernel (which would widen the codes for 256 rows of which `per` are there), the others to the one for few rows, one
-// launch after the other on the same workspace.  Its group is that of a single token, or of 16 rows where the average
-// row is a short one.  Measured at 64 rows over 50 to 16,000 tokens, 8 key heads of 4 queries of 128 (in groups of 8 for comparison):
-// 5 tokens each 512 us (606), 8 tokens 532 (813), 9 tokens 750 (977); tensor memory from 41 rows on, 12 tokens 944 (1,190); single tokens
-// beside one chunk of 449 pay for it, 244 (219).  At D = 64 and with more heads per key head the tensor-memory kernel
-// is slower than groups of 16 up to 63 rows (9 tokens of D = 64: 668 us, 435).  Steps of chunks alone pay 10 us for the
-// second one's empty launches (220 -> 232 us for four chunks of 300 to 400 tokens); 60 single tokens over 6,000 beside two
-// chunks of 2,048 take 420 us.
+// tokens, and only the device knows which is which: rows of enough query rows go to the tensor-memory kernel, the others to the
+// one for few rows, one launch after the other on the same workspace.  Its group is that of a single token, or of 16 rows where the average
+// row is a short one (trees: always).  In tensor memory a row costs about the same up to 128 query rows, but more for its start and end; for few
+// rows it costs once more for every 16.  Measured with 8 key heads of 4 queries, us in tensor memory (in groups of 16):
+//   D = 128, 17 to 32 query rows: 64 rows over 1,000 tokens 115 (109-115), 2,000 170 (164-170), 4,000 243 (268-274); 512 over 300 455 (264)
+//   33 to 48: 64 rows over 1,000 121 (133), 2,000 178 (219), 4,000 250 (375); 512 over 100 344 (156), 300 436 (373), 600 516-547 (524-537)
+//   D = 64, 33 to 48: 64 rows over 1,000 94 (94), 2,000 143 (131), 4,000 203 (211); 512 over 300 356 (209)
+//   49 to 63: 64 rows over 2,000 147 (166), 4,000 215 (270); 512 over 300 379 (270), 1,000 520-553 (563)
+//   rows over 50 to 16,000, D = 128, all by these borders: 5, 8, 9, 12, 16 tokens 455, 459, 451, 453, 432
+// so that lengths from AT_LONG and at_long_more on decide below rows_any.  Causal steps of more than 8 heads per key head have one border, above a
+// single token's rows.  Single tokens beside one chunk of 449 pay for the second launch (10 us).
 // A step of no more tokens than rows counts as one of single tokens: a chunk among idle rows is right, but goes in
 // their groups (200 tokens over 8,000 beside 255 idle rows 213 us, alone 201; 500 beside 511 507 us, alone 171), as the
 // launches for chunks would cost every step of single tokens 8 to 10 us.
-// Trees: the rows of a batch are mostly alike, a few tokens to some dozens each, and the tensor-memory kernel is the faster one from 17
-// query rows on (D = 64: from 33), also where a single row has tokens enough for the SMs (48 rows over 4,000 tokens, 8
-// key heads of 4 queries of 128, in groups of 16 for comparison: 4 tokens each 161 us, 6 tokens 202 (243), 8 tokens 202 (314), 30 tokens
-// 212 (980); D = 64: 6 tokens 161, 10 tokens 177 (196); 64 tokens of 8 heads per key head over 20,000 alone 120 (300)).
+// Trees: the rows of a batch are mostly alike, a few tokens to some dozens each, so that a single row may have tokens enough for the SMs too
+// (64 tokens of 8 heads per key head over 20,000 alone 119 us, 300 in groups of 16), and in a batch of large ones the small ones
+// go along (48 of 8 to 32 tokens over 50 to 8,000: 206 us, 222 with a second launch for a few rows).
 template <int D, int DT, bool TREE>
 static inline cudaError_t launch_attend_rows(AttendArgs a, void* ws, cudaStream_t st) {
   const int64_t average = (int64_t)a.per * ((a.T + (int64_t)a.B - 1) / a.B);
-  a.rows_lo = 0;
-  a.rows_hi = INT32_MAX;
+  a.side = 0;
   if constexpr (D < 256) {
-    const int sms = sm_count(device_index()), pa_from = TREE ? (D == 128 ? 17 : 33) : D == 128 && a.per <= 8 ? 41 : 64;
+    const int sms = sm_count(device_index());
+    const bool low = TREE || a.per <= 8;
+    a.rows_any = low && D == 128 ? 49 : 64;
+    a.long_more = at_long_more(D);
+    a.rows_long = low ? (D == 128 ? 17 : 33) : 64;
+    if (TREE && average >= a.rows_any) a.rows_any = a.rows_long;
+    const int usual = ((int64_t)a.width << a.bs_shift) >= AT_LONG ? a.rows_long : a.rows_any;
     const int64_t tiles = ((((int64_t)a.width << a.bs_shift) + PA_KT - 1) / PA_KT) * a.heads * a.B;
-    if (a.T > a.B && ((int64_t)a.heads * a.per * a.T >= (int64_t)PA_ROWS * sms / 4 || (TREE && average >= pa_from && tiles >= sms))) {
-      a.rows_lo = pa_from;
+    if (a.T > a.B && ((int64_t)a.heads * a.per * a.T >= (int64_t)PA_ROWS * sms / 4 || (TREE && average >= usual && tiles >= sms))) {
+      a.side = 1;
       const cudaError_t e = launch_attend_tc<D, DT, TREE>(a, ws, st);
       if (e != cudaSuccess) return e;
-      a.rows_lo = 0;
-      a.rows_hi = pa_from;
-      return launch_attend_few<D, DT, TREE>(a, average < pa_from ? std::max((int64_t)a.per, std::min(average, (int64_t)16)) : a.per, ws, st);
+      a.side = 2;
+      return launch_attend_few<D, DT, TREE>(a, TREE || average < 64 ? std::max((int64_t)a.per, std::min(average, (int64_t)16)) : a.per, ws, st);
     }
   }
   return launch_attend_few<D, DT, TREE>(a, average, ws, st);

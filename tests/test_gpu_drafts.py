@@ -316,6 +316,24 @@ def test_attend_tree_layouts_and_refusals():
 
 
 # --------------------------------------------------------------------------- accepted tokens move up
+@pytest.mark.parametrize("per,dim", [(4, 128), (4, 64), (16, 128)])
+def test_attend_rows_between_the_kernels(per, dim):
+    """Rows on both sides of every border between the kernels in one step: 16 to 64 query rows, lengths around 640, 1,024 and 2,560, and short ones."""
+    new = [(4, 5, 8, 9, 12, 13, 15, 16)[i % 8] * 4 // per or 1 for i in range(72)]
+    ctx = [(2559, 2560, 2561, 1023, 1024, 639, 640, 17, 0)[i // 8] - (n if i // 8 < 7 else 0) for i, n in enumerate(new)]
+    rows, parents = tree_rows(ctx, new, 16, per)
+    cache = lb.KVCache8(*U.random_cache(rows[-1], 8, 16, dim, seed=per))
+    q = torch.randn(sum(new) + 1, 8 * per, dim, generator=gen(dim), device=DEV).bfloat16()
+    y, lse = check_attend_tree(q, cache, rows, parents + [-1])
+    assert bool(y[: sum(new)].isfinite().all())
+    chains = [i - 1 for n in new for i in range(n)]
+    check_attend_tree(q, cache, rows, chains + [-1])
+    got = lb.attend(q[: sum(new)], cache, rows[1], lb.StepPlan(*rows[2:5]))
+    want, mag, _ = U.attend_reference(q[: sum(new)], cache.k, cache.v, cache.k_scale, cache.v_scale, rows[0], *(x.tolist() for x in rows[2:5]), dim ** -0.5)
+    tol = 1.25 * 2.0 ** -11 * mag + torch.finfo(q.dtype).eps / 2 * want.abs() + 2.0 ** -24
+    assert bool(((got.double() - want).abs() <= tol).all())
+
+
 def check_compact(rows, heads, bs, dim, path, counts, seed, scales=None, nan=False):
     table, t, starts, granted, lens, blocks = rows
     k, v, ks, vs = U.random_cache(blocks, heads, bs, dim, seed=seed)
