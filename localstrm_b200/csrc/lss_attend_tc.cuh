@@ -103,6 +103,13 @@ __device__ __forceinline__ uint32_t pa_place(int r, int q) {
 // The warps go through the groups on their own, held together by the barriers of what they pass on alone: copies and
 // widening run ahead into the next group while the softmax finishes one and fetches its queries.  A stage of widened
 // keys or values belongs to steps of one parity, so that a stream that takes every other step sees all of its phases.
+// A wait knows a phase by its parity, so nobody may be two phases behind a barrier or miss one:
+//   qready[q]  a phase per wide group, waited on in every one by the stream's products alone;
+//   nready     a phase per narrow group: both softmax warpgroups arrive (the second one's word that it has left the group before: where
+//              it has no step, its products would end this group at once, and ofull[1] be two phases on) and the products
+//              of both and the second softmax wait, in every one;
+//   ofull[q]   a phase per group, seen by the stream's own softmax in every one, and by the second softmax for stream 0 behind nready,
+//              so that at most the last phase is under way.
 struct PaGroup {  // a group of query rows, and the tiles of it that a CTA takes
   int row, head, mt, tile0, tile1, nt;
   int start, ctx, n, rows, see_last, see_all, i0, i1;  // steps [i0, i1)
@@ -164,7 +171,7 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
   constexpr int NN = 4;                    // the widening is two steps, so two groups at most, ahead of the softmax
   static_assert(OP % 2 == 0, "a stage belongs to one stream");
   extern __shared__ __align__(1024) unsigned char pa_dyn[];
-  __shared__ __align__(8) uint64_t rfull[2][RS], rempty[2][RS], kfull[OP], kempty[OP], vfull[OP], vempty[OP], sfull[2][2], pready[2][2], pvdone[2], ofull[2], qready[2];
+  __shared__ __align__(8) uint64_t rfull[2][RS], rempty[2][RS], kfull[OP], kempty[OP], vfull[OP], vempty[OP], sfull[2][2], pready[2][2], pvdone[2], ofull[2], qready[2], nready;
   __shared__ uint32_t tmem_base;
   __shared__ int failed;
   __shared__ __align__(16) float2 sscale[PA_SC][4];  // scales of the step's 16-token parts: of K (< 0: not seen), log2 of that of V
@@ -205,6 +212,7 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
       mbar_init(&ofull[i], 1);
       mbar_init(&qready[i], 4);
     }
+    mbar_init(&nready, 8);
     fence_barrier_init();
   }
 
@@ -347,9 +355,11 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
         if (narrow) row_factor[r] = fq;
         fence_proxy_async();
         __syncwarp();
-        if (lane == 0) mbar_arrive_local(&qready[q]);
+        if (lane == 0) mbar_arrive_local(narrow ? &nready : &qready[q]);
       } else {  // the same rows
-        tc_wait(&qready[0], walk.groups & 1, &failed);
+        __syncwarp();
+        if (lane == 0) mbar_arrive_local(&nready);
+        tc_wait(&nready, (walk.groups - walk.wides) & 1, &failed);
         fq = row_factor[r];
       }
 
@@ -685,8 +695,8 @@ __global__ void __launch_bounds__(PA_NT, 1) lss_attend_tc_kernel(AttendArgs a) {
         const bool narrow = g.narrow;
         const int first = narrow ? g.i0 + ((walk.steps ^ q) & 1) : g.i0, by = narrow ? 2 : 1;
         const uint32_t q0 = tc_desc_lo(saddr(qs + (narrow ? 0 : q) * OPB));
-        if (narrow || q == 0) tc_wait(&qready[0], walk.groups & 1, &failed);
-        else tc_wait(&qready[1], walk.wides & 1, &failed);
+        if (narrow) tc_wait(&nready, (walk.groups - walk.wides) & 1, &failed);
+        else tc_wait(&qready[q], walk.wides & 1, &failed);
         auto score = [&](int i, uint32_t turn) {
           const uint32_t n = walk.steps + i - g.i0, st = n % OP, half = turn & 1;
           const bool ok = tc_wait(&kfull[st], (n / OP) & 1, &failed);

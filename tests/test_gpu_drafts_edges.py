@@ -1,0 +1,67 @@
+"""Operators around drafted tokens and shared blocks on the GPU: orders of work, layouts and states beside those of
+test_gpu_drafts.py."""
+import random
+
+import pytest
+import torch
+
+import localstrm_b200 as lb
+from tests import decode_util as U
+from tests import drafts_util as D
+from tests.test_gpu_drafts import DEV, check_attend_tree, gen, ints
+
+pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not torch.cuda.is_available(), reason="needs a CUDA device")]
+
+
+# --------------------------------------------------------------------------------------- attention
+def lagging(rows, new, heads, per, dim, seed):
+    """A cache and queries with which the two halves of a group of 256 query rows take different times: the scores of the
+    first half grow by some 12 (powers of two) every 64 tokens, so that its sums are rescaled at every step, those of the
+    second half hardly differ.  The largest scores are about 60: f32 holds them, and the sums of 16 products at a time that
+    lead to them, to 2^-18, a 2^-18 of the weight, well below the quarter of 2^-11 left for it."""
+    table, _, _, _, lens, blocks = rows
+    bs = 16
+    k, v, ks, vs = U.random_cache(blocks, heads, bs, dim, seed=seed)
+    ks.fill_(2.0 ** -7)
+    for line, ln in zip(table, lens.tolist()):
+        pages = torch.tensor(line[: -(-ln // bs)], device=DEV)
+        grow = (torch.arange(len(pages) * bs, device=DEV).view(-1, bs) * (448 / 320)).clamp(max=448).to(U.E4M3)
+        k.view(torch.uint8)[pages, :, :, 0] = grow.view(torch.uint8)[:, None]
+    q = torch.randn(sum(new), heads * per, dim, generator=gen(seed), device=DEV)
+    at = torch.cat([torch.arange(n * per, device=DEV) for n in new]).view(-1, per)  # row of the queries of one key head
+    big = 12 / 64 * 320 / 448 * 2 ** 7 / 1.4427 * dim ** 0.5
+    q.view(-1, heads, per, dim)[..., 0] = torch.where(at % 256 < 128, big, 0.0)[:, None]
+    return lb.KVCache8(k, v, ks, vs), q.bfloat16()
+
+
+MIXED = {
+    "prompts of 200 tokens": ([0] * 40, [200] * 40),
+    "prompts of 90 and 150": ([0] * 60, [90, 150] * 30),
+    "chunks of one step beside small trees": ([0, 3] * 60, [33 + i % 32 if i % 2 == 0 else 8 + i % 25 for i in range(120)]),
+    "all lengths": ([0] * 70, [33 + (i * 97) % 268 if i % 3 else 8 + i % 25 for i in range(70)]),
+}
+
+
+@pytest.mark.parametrize("dim", [128, 64])
+@pytest.mark.parametrize("name", MIXED)
+def test_attend_small_groups_between_whole_ones(name, dim):
+    """Groups of up to 128 query rows, for which the two streams of the tensor-memory kernel work together, between
+    groups of 256 of one and two steps, which they take on their own: neither may run into the other's queries."""
+    ctx, new = MIXED[name]
+    heads, per = 8, 4
+    rows = U.make_rows(ctx, new, 16, seed=dim)
+    cache, q = lagging(rows, new, heads, per, dim, seed=len(new))
+    parents = [p for i, n in enumerate(new) for p in D.random_tree(n, random.Random(i), root=0.0)]
+    plan = lb.StepPlan(*rows[2:5])
+    y, lse = check_attend_tree(q, cache, rows, parents)
+    tree = lb.plan_tree(plan, ints(parents))
+    want, mag, _ = U.attend_reference(q, cache.k, cache.v, cache.k_scale, cache.v_scale, rows[0], *(x.tolist() for x in rows[2:5]), dim ** -0.5)
+    causal = lb.attend(q, cache, rows[1], plan)
+    assert bool(((causal.double() - want).abs() <= 1.25 * 2.0 ** -11 * mag + 2.0 ** -8 * want.abs()).all())
+    busy, side = torch.zeros(1 << 24, device=DEV), torch.cuda.Stream()
+    for i in range(12):  # the same in every bit, with other work beside it too
+        if i % 2:
+            with torch.cuda.stream(side):
+                busy.add_(1)
+        assert torch.equal(lb.attend(q, cache, rows[1], plan, tree=tree), y) and torch.equal(lb.attend(q, cache, rows[1], plan), causal)
+    torch.cuda.synchronize()
