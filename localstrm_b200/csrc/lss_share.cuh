@@ -209,6 +209,8 @@ static __global__ void __launch_bounds__(BL_NT) lss_give_kernel(GiveArgs a) {
     }, nothing);
     __threadfence();
     cl.sync();
+  } else {
+    cl.sync();  // every CTA runs: its shared memory may be written
   }
   // Blocks that do not go back with this row are turned to their complement.
   auto choose = [&](int r, int j0, int (&id)[8]) {

@@ -8,7 +8,7 @@ import torch
 import localstrm_b200 as lb
 from tests import decode_util as U
 from tests import drafts_util as D
-from tests.test_gpu_drafts import DEV, check_attend_tree, gen, ints
+from tests.test_gpu_drafts import DEV, check_attend_tree, gen, ints, make_table
 
 pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not torch.cuda.is_available(), reason="needs a CUDA device")]
 
@@ -65,3 +65,40 @@ def test_attend_small_groups_between_whole_ones(name, dim):
                 busy.add_(1)
         assert torch.equal(lb.attend(q, cache, rows[1], plan, tree=tree), y) and torch.equal(lb.attend(q, cache, rows[1], plan), causal)
     torch.cuda.synchronize()
+
+
+# ---------------------------------------------------------------------------------- shared blocks
+@pytest.mark.parametrize("rows,hi", [(33, 200), (64, 4000), (511, 900), (512, 9000), (5000, 60), (16384, 20)])
+def test_release_kept_without_shares(rows, hi):
+    """Blocks of rejected tokens where no block is shared: clusters of 2 to 16 CTAs that write to each other's shared memory
+    from their first pass on, with other work on the SMs, so that they do not all begin at once; captured too."""
+    rng = random.Random(rows)
+    bs = 16
+    lens = [rng.randrange(hi + 1) for _ in range(rows)]
+    blocks = sum(-(-ln // bs) for ln in lens) + 7
+    table, left = make_table(lens, bs, blocks, rng)
+    free = left + [0] * (blocks - len(left))
+    codes = [int(rng.random() < 0.3) for _ in lens]
+    keep = [max(0, ln - rng.randrange(40)) for ln in lens]
+    want = D.give_reference(table, lens, codes, keep, None, free, len(left), bs)
+    line, ln, cd, kp, fr0, nf = ints(table), ints(lens), ints(codes), ints(keep), ints(free), ints([len(left)])
+    x, side = torch.randn(2048, 2048, device=DEV), torch.cuda.Stream()
+
+    def give():
+        fr = fr0.clone()
+        return (*lb.release_blocks(line, ln, cd, fr, nf, bs, keep=kp), fr)
+
+    got = [give()]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        with torch.cuda.stream(side):
+            x @ x
+        got.append(give())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        again = give()
+    for _ in range(3):
+        graph.replay()
+    for lens_out, n_free, fr in got + [again]:
+        assert lens_out.tolist() == want[0] and n_free.tolist() == want[1] and fr.tolist() == want[2]
