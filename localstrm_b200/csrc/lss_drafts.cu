@@ -6,11 +6,16 @@
 #include "lss_share.cuh"
 #include "lss_tree.cuh"
 
-// Extents of a token's heads: two arrays of T tokens (start, bytes between tokens, between heads, heads) of which
-// some token's part lies over one of the other's.
+// Two arrays of T tokens (start, bytes between tokens, between heads, heads) of which some head lies over one of the
+// other's.  With equal strides exactly, so that heads of the two may take turns; else by the extents of their tokens' heads.
 static bool tokens_overlap(const void* x, int64_t x_st, int64_t x_sh, int x_heads, const void* y, int64_t y_st, int64_t y_sh, int y_heads,
                            int T, int64_t n) {
-  return rows_overlap(x, x_st, (x_heads - 1) * x_sh + n, y, y_st, (y_heads - 1) * y_sh + n, T);
+  if (!rows_overlap(x, x_st, (x_heads - 1) * x_sh + n, y, y_st, (y_heads - 1) * y_sh + n, T)) return false;
+  if (T == 1) x_st = y_st = 0;  // one token, one head: the stride says nothing
+  if (x_heads == 1) x_sh = y_sh;
+  if (y_heads == 1) y_sh = x_sh;
+  if (x_st != y_st || x_sh != y_sh) return true;
+  return rows_meet((int64_t)(reinterpret_cast<intptr_t>(y) - reinterpret_cast<intptr_t>(x)), x_st, x_sh, T, T, x_heads, y_heads, n);
 }
 
 template <int DT, int N, int L, bool PAIRS>

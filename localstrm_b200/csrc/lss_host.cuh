@@ -90,6 +90,21 @@ static inline bool rows_overlap(const void* x, int64_t x_pitch, int64_t x_row, c
   const int64_t at = (d % x_pitch + x_pitch) % x_pitch;  // where y's rows start in x's pitch
   return at < x_row || at + y_row > x_pitch;
 }
+// Two arrays of rows of n bytes with equal strides st and sh, the second one d bytes behind the first, of which two rows share
+// memory: rows i and j strides apart begin d + i st + j sh bytes apart, i among Tx and Ty, j among Hx and Hy of them.
+static inline bool rows_meet(int64_t d, int64_t st, int64_t sh, int64_t Tx, int64_t Ty, int64_t Hx, int64_t Hy, int64_t n) {
+  if (Tx + Ty < Hx + Hy) {  // the walk is over the shorter side
+    std::swap(Tx, Hx);
+    std::swap(Ty, Hy);
+    std::swap(st, sh);
+  }
+  for (int64_t j = 1 - Hx; j < Hy; ++j) {
+    const int64_t r = d + j * sh, i0 = st > 0 ? (r >= 0 ? -((r + st - 1) / st) : -r / st) : 0;  // r + i0 st <= 0 < r + (i0 + 1) st
+    for (int64_t i = i0; i <= i0 + 1; ++i)  // the nearest ones that there are
+      if (std::abs(r + std::min(std::max(i, 1 - Tx), Ty - 1) * st) < n) return true;
+  }
+  return false;
+}
 // Two arrays of T x H rows of n bytes (start, bytes between tokens and between heads) that share memory without
 // being the same rows: a result would be written where another CTA still reads its query.  With equal strides
 // exactly, else wherever the extents meet.
@@ -99,17 +114,7 @@ static inline bool rows_shifted(const void* x, int64_t x_st, int64_t x_sh, const
   const int64_t d = (int64_t)(reinterpret_cast<intptr_t>(y) - reinterpret_cast<intptr_t>(x));
   if (d >= (T - 1) * x_st + (H - 1) * x_sh + n || -d >= (T - 1) * y_st + (H - 1) * y_sh + n) return false;
   if (x_st != y_st || x_sh != y_sh) return true;
-  if (d == 0) return false;
-  if (T < H) {  // the walk below is over the shorter side
-    std::swap(T, H);
-    std::swap(x_st, x_sh);
-  }
-  for (int64_t j = 1 - H; j < H; ++j) {  // rows i tokens and j heads apart begin d - i st - j sh bytes apart
-    const int64_t r = d - j * x_sh, i0 = x_st > 0 ? (r >= 0 ? r / x_st : -((-r + x_st - 1) / x_st)) : 0;
-    for (int64_t i = i0; i <= i0 + 1; ++i)
-      if (i > -T && i < T && std::abs(r - i * x_st) < n) return true;
-  }
-  return false;
+  return d != 0 && rows_meet(d, x_st, x_sh, T, T, H, H, n);
 }
 // Arrays of n entries of which one begins inside the other.
 static inline bool cut(const int32_t* x, const int32_t* y, int64_t n) { return x != y && x < y + n && y < x + n; }

@@ -8,9 +8,46 @@ import torch
 import localstrm_b200 as lb
 from tests import decode_util as U
 from tests import drafts_util as D
-from tests.test_gpu_drafts import DEV, check_attend_tree, gen, ints, make_table
+from tests.test_gpu_drafts import DEV, check_attend_tree, check_rotate, gen, ints, make_table, rotate_case
 
 pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not torch.cuda.is_available(), reason="needs a CUDA device")]
+
+
+# ------------------------------------------------------------------------------ norms and rotation
+@pytest.mark.parametrize("T,heads,dim,off", [(1, 3, 64, 0), (37, 6, 128, 0), (37, 6, 128, 1), (200, 1, 80, 0), (5, 64, 66, 0)])
+def test_rotate_heads_in_turn(T, heads, dim, off):
+    """Queries, keys and values of each head beside each other, token by token and head by head: in place, and from two of
+    the places into two others; what lies between stays."""
+    _, _, pos, freqs, qw, kw = rotate_case(T, 1, 1, dim, dim - dim % 4, torch.bfloat16, T)
+    n = T * heads * 4 * dim
+    for order in (lambda x: x.view(T, heads, 4, dim), lambda x: x.view(heads, 4, T, dim).permute(2, 0, 1, 3)):
+        flat = torch.randn(off + n + 3, generator=gen(dim), device=DEV).bfloat16()
+        four = order(flat[off: off + n])
+        want = check_rotate(four[:, :, 0], four[:, :, 1], pos, freqs, qw, kw, False)
+        before = flat.clone()
+        lb.norm_rotate(four[:, :, 0], four[:, :, 1], pos, freqs, qw, kw, q_out=four[:, :, 2], k_out=four[:, :, 3])
+        expect = before.clone()
+        order(expect[off: off + n])[:, :, 2], order(expect[off: off + n])[:, :, 3] = want
+        assert torch.equal(flat, expect)
+        lb.norm_rotate(four[:, :, 0], four[:, :, 1], pos, freqs, qw, kw, q_out=four[:, :, 0], k_out=four[:, :, 1])
+        order(expect[off: off + n])[:, :, 0], order(expect[off: off + n])[:, :, 1] = want
+        assert torch.equal(flat, expect)
+        for bad in (dict(q_out=four[:, :, 1]), dict(k_out=four[:, :, 0]), dict(q_out=four[:, :, 2], k_out=four[:, :, 2])):
+            with pytest.raises(lb.SamplerError):
+                lb.norm_rotate(four[:, :, 0], four[:, :, 1], pos, freqs, **bad)
+        assert torch.equal(flat, expect)
+
+
+def test_rotate_in_place_leaves_what_lies_around():
+    """Slices of a fused projection that do not begin on 16 bytes: what lies in front of the queries and behind the keys."""
+    T, hq, hk, dim = 37, 6, 2, 128
+    _, _, pos, freqs, qw, kw = rotate_case(T, hq, hk, dim, dim, torch.bfloat16, 5)
+    for off in (0, 1, 5):
+        fused = torch.randn(T, 1400, generator=gen(6), device=DEV).bfloat16()
+        before, end = fused.clone(), off + (hq + hk) * dim
+        q, k = fused[:, off: off + hq * dim].view(T, hq, dim), fused[:, off + hq * dim: end].view(T, hk, dim)
+        check_rotate(q, k, pos, freqs, qw, kw, False, q_out=q, k_out=k)
+        assert torch.equal(fused[:, :off], before[:, :off]) and torch.equal(fused[:, end:], before[:, end:])
 
 
 # --------------------------------------------------------------------------------------- attention
