@@ -112,7 +112,8 @@ static __global__ void __launch_bounds__(MV_NT) lss_compact_kernel(CompactArgs a
             off = t;
           }
           const int64_t ph = (int64_t)from * a.heads + head;
-          f[k] = __fdiv_rn(from == page ? was : scales[ph], top);
+          const float own = from == page ? was : scales[ph];
+          f[k] = own == top ? 1.0f : __fdiv_rn(own, top);  // all scales 0, in a caller's own cache: the codes as they are
           hold[k] = *reinterpret_cast<const uint2*>(codes + ((ph << sh) + off) * D + c * 8);
         }
       }

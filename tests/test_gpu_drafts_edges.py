@@ -139,3 +139,28 @@ def test_release_kept_without_shares(rows, hi):
         graph.replay()
     for lens_out, n_free, fr in got + [again]:
         assert lens_out.tolist() == want[0] and n_free.tolist() == want[1] and fr.tolist() == want[2]
+
+
+# --------------------------------------------------------------------------- accepted tokens move up
+@pytest.mark.parametrize("zeros", ["all", "some"])
+def test_compact_scales_of_zero(zeros):
+    """A caller's own cache may hold blocks whose scales are 0: codes move as they are where all of a block's tokens come
+    from such ones, and become 0 beside others."""
+    rows = U.make_rows([20, 7, 3], [40, 30, 9], 16, seed=5)
+    table, t, starts, granted, lens, blocks = rows
+    k, v, ks, vs = U.random_cache(blocks, 2, 16, 64, seed=1)
+    for s in (ks, vs):
+        s[torch.rand(s.shape, generator=gen(2), device=DEV) < (2.0 if zeros == "all" else 0.4)] = 0.0
+    cache = lb.KVCache8(k.clone(), v.clone(), ks.clone(), vs.clone())
+    path, counts = [], []
+    for n in (40, 30, 9):
+        kept = sorted({0, *random.Random(n).sample(range(n), n // 2)})
+        path += kept + [-1] * (n - len(kept))
+        counts.append(len(kept))
+    lb.compact_kv(cache, t, lb.StepPlan(starts, granted, lens), ints(path), ints(counts))
+    for was, scale, now, scale_now in ((k, ks, cache.k, cache.k_scale), (v, vs, cache.v, cache.v_scale)):
+        one = torch.where(scale == 0, 2.0 ** -200, scale.double()).cpu()  # so far below the others that codes beside them become 0
+        values, s = was.cpu().double(), one.clone()
+        D.compact_reference(values, s, table, starts.tolist(), granted.tolist(), lens.tolist(), path, counts)
+        assert torch.equal(now.cpu().double(), values)
+        assert torch.equal(scale_now.cpu().double(), torch.where(s == 2.0 ** -200, 0.0, s))
