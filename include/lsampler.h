@@ -415,7 +415,9 @@ int lss_kv_compact(uint8_t* k_cache, uint8_t* v_cache, float* k_scale, float* v_
  *
  * lss_block_give is lss_block_release for such blocks, and for rows that keep a part of theirs: a row with a code (NULL:
  * none has) gives all of its blocks back, any other those behind its first keep[b] tokens (NULL: it keeps all), which
- * become its length.  A block returns to the free list with the last of its holders, in row and block order of these;
+ * become its length.  keep[b] must not end inside a block that another row holds (it is then the row's block that is
+ * written next): such a row is forked onto an idle one, upto[i] tokens of it, and gives all of its blocks back.
+ * A block returns to the free list with the last of its holders, in row and block order of these;
  * shares NULL: no block is shared.  Entries outside [0, num_blocks) are passed over.  B * width at most 2^30. */
 int lss_block_fork(int32_t* table, int64_t table_stride, int width, const int32_t* lens, int B, int block_size,
                    const int32_t* src_rows, const int32_t* dst_rows, const int32_t* upto, int n, int32_t* shares,

@@ -175,7 +175,9 @@ def release_blocks(block_table: torch.Tensor, lens: torch.Tensor, codes: torch.T
 
     With ``keep [B]`` the other rows give back what lies behind their first ``keep[b]`` tokens, which become their length
     (``Accepted.lens``).  With ``shares [num_blocks]`` (as ``fork_blocks`` keeps them) a block goes back with the last of its
-    holders, in the order of these; without, blocks that rows share must be released once."""
+    holders, in the order of these; without, blocks that rows share must be released once.  ``keep`` must not end inside a block
+    that another row holds, which nothing here can tell (``Accepted.lens`` never does): the row's next tokens would be written
+    over the other's.  To cut a row there, fork it onto an idle row with ``upto`` and release it."""
     dev, B, width, stride = _table(block_table)
     lens_at, codes_at = _ints("lens", lens, B, dev), _ints("codes", codes, B, dev)
     blocks = free_blocks.numel()

@@ -141,6 +141,29 @@ def test_release_kept_without_shares(rows, hi):
         assert lens_out.tolist() == want[0] and n_free.tolist() == want[1] and fr.tolist() == want[2]
 
 
+def test_rows_cut_inside_shared_blocks():
+    """A row that is to go on from the middle of a block that another one holds is forked and released: what it writes then
+    is its own, and the other's block stays as it is in every bit."""
+    heads, bs, dim = 2, 16, 64
+    cache = lb.KVCache8(*U.random_cache(12, heads, bs, dim))
+    table, lens = ints([[3, 5, 7], [-1] * 3, [-1] * 3]), ints([40, 0, 0])
+    free, n_free, shares = ints([8, 9, 10, 11, 0, 1, 2, 4, 6, 0, 0, 0]), ints([9]), ints([0] * 12)
+    fork = lambda src, dst, upto: lb.fork_blocks(table, lens, ints([src]), ints([dst]), shares, free, n_free, bs, upto=ints([upto]), lens_out=lens, n_free_out=n_free)
+    lb.copy_blocks(cache, fork(0, 1, 40).copies)
+    lb.copy_blocks(cache, fork(1, 2, 20).copies)  # row 1 cut to 20 tokens: inside block 5, which row 0 holds
+    lb.release_blocks(table, lens, ints([0, 1, 0]), free, n_free, bs, lens_out=lens, n_free_out=n_free, shares=shares)
+    assert lens.tolist() == [40, 0, 20] and shares.tolist() == [0, 0, 0, 1] + [0] * 8 and n_free.tolist() == [8]
+    before = [x[[3, 5, 7]].clone() for x in (cache.k.view(torch.uint8), cache.v.view(torch.uint8), cache.k_scale, cache.v_scale)]
+    assert torch.equal(cache.k.view(torch.uint8)[table[2, 1].item()], cache.k.view(torch.uint8)[5])
+    plan = lb.plan_blocks(table, lens, ints([0, 0, 5]), free, n_free, bs, 5, lens_out=lens, n_free_out=n_free)
+    x = 1e4 * torch.randn(5, heads, dim, generator=gen(1), device=DEV)
+    lb.append_kv(cache, x, x, table, plan)
+    for was, now in zip(before, (cache.k.view(torch.uint8), cache.v.view(torch.uint8), cache.k_scale, cache.v_scale)):
+        assert torch.equal(was, now[[3, 5, 7]])
+    lb.release_blocks(table, lens, ints([1, 0, 1]), free, n_free, bs, lens_out=lens, n_free_out=n_free, shares=shares)
+    assert n_free.tolist() == [12] and sorted(free.tolist()) == list(range(12)) and shares.tolist() == [0] * 12
+
+
 # --------------------------------------------------------------------------- accepted tokens move up
 @pytest.mark.parametrize("zeros", ["all", "some"])
 def test_compact_scales_of_zero(zeros):
