@@ -390,7 +390,8 @@ int lss_attend_tree(const void* q, int64_t q_token_stride, int64_t q_head_stride
 /* What an accepted branch leaves in the cache: the keys and values of new token path[starts[b] + i] of row b become those
  * of its new token i, for i < counts[b] (lss_tree_accept's; path[i] >= i, other entries stay where they are).  `lens` are
  * those with all new tokens.  A block that takes in tokens gets the largest of the scales of the blocks that its tokens
- * come from (its own among them where tokens stay in it), and codes of other scales are rounded again, to nearest even.
+ * come from (its own among them where tokens stay in it), and codes of other scales are rounded again, to nearest even.  A
+ * scale that lss_kv_append widened for a token that is not accepted stays, and the context's codes as it rounded them.
  * What lies behind the accepted tokens is left as it was.  Blocks of one row only, as for lss_kv_append. */
 int lss_kv_compact(uint8_t* k_cache, uint8_t* v_cache, float* k_scale, float* v_scale, int num_blocks, int heads, int block_size,
                    int dim, const int32_t* table, int64_t table_stride, int width, const int32_t* starts, const int32_t* granted,

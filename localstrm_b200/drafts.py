@@ -72,8 +72,14 @@ def accept_drafts(plan: StepPlan, tree: TreePlan, tokens: torch.Tensor, targets:
     ``codes`` int32 ``[T]``: ``check_stop_batch``'s of the targets.  The first ``given[b]`` tokens of row b (default 1: the
     one sampled last) are accepted as they are; from the last of them the walk goes to the first child that is the sampled
     token, until there is none or the sampled token has a code.  So the request's new tokens are those that
-    sampling one by one would have given, whatever was drafted.  A row with a prompt chunk has all of it given; where the
+    sampling one by one gives with the same logits, whatever was drafted.  A row with a prompt chunk has all of it given; where the
     prompt goes on its new token means nothing (``plan.stops(accepted.codes, prompt_lens)`` drops its code).
+
+    The logits are those of the 8-bit cache as the step left it:
+    a drafted token of large values in the context's last block widens that block's scale, the context's values in it are
+    rounded again to the larger step (below 2^-6 of the scale they lose bits), and stay so when the token is rejected.  Where two
+    logits are nearly equal that can decide otherwise than a run without drafts.
+
     ``lens_out`` may be ``plan.lens`` (which ``compact_kv`` and ``plan.stops`` still need as it is)."""
     dev = _device(plan)
     B, T = plan.granted.numel(), tree.parents.numel()
@@ -97,7 +103,8 @@ def compact_kv(cache: KVCache8, block_table: torch.Tensor, plan: StepPlan, path:
     behind the context, in one layer's cache.  ``plan.lens`` are the lengths with all new tokens.
 
     A block that takes in tokens gets the largest of the scales that they, and the tokens that stay in it, had; codes of
-    a smaller scale are rounded again.  What lies behind the accepted tokens is left as it was."""
+    a smaller scale are rounded again.  A scale that a rejected token widened stays.  What lies behind the accepted tokens is
+    left as it was."""
     dev, B, width, stride = _table(block_table)
     blocks, heads, bs, dim = cache.check(dev)
     T = path.numel()
