@@ -4,7 +4,8 @@ A step with drafts runs ``plan_blocks`` for all drafted tokens, ``plan_tree`` on
 ``TreePlan.positions``), ``append_kv`` and ``attend`` (with ``tree=``).  After sampling a token behind every drafted one,
 ``accept_drafts`` follows the sampled tokens through the trees, ``compact_kv`` moves the accepted tokens' keys and
 values up in each layer's cache, and ``release_blocks`` (with ``keep=``) takes the rejected tokens' blocks back.  As
-with the other operators everything stays on the device.  LocalStrm decodes token by token and has no counterpart.
+with the other operators everything stays on the device; what the sampler takes as Python lists (histories of penalties, stop
+ids) does not, see ``accept_drafts``.  LocalStrm decodes token by token and has no counterpart.
 """
 from __future__ import annotations
 
@@ -75,12 +76,13 @@ def accept_drafts(plan: StepPlan, tree: TreePlan, tokens: torch.Tensor, targets:
     sampling one by one gives with the same logits, whatever was drafted.  A row with a prompt chunk has all of it given; where the
     prompt goes on its new token means nothing (``plan.stops(accepted.codes, prompt_lens)`` drops its code).
 
-    The logits are those of the 8-bit cache as the step left it:
+    Each target is sampled as if its token were the request's last: with penalties its history holds the drafted tokens
+    from the row's first to it, its ancestors, and not the other branches.  The logits are those of the 8-bit cache as the step left it:
     a drafted token of large values in the context's last block widens that block's scale, the context's values in it are
     rounded again to the larger step (below 2^-6 of the scale they lose bits), and stay so when the token is rejected.  Where two
     logits are nearly equal that can decide otherwise than a run without drafts.
 
-    ``lens_out`` may be ``plan.lens`` (which ``compact_kv`` and ``plan.stops`` still need as it is)."""
+    ``lens_out`` may be ``plan.lens``, which ``compact_kv``, ``plan.stops`` and ``release_blocks(keep=)`` still need as it is."""
     dev = _device(plan)
     B, T = plan.granted.numel(), tree.parents.numel()
     starts_at = _ints("plan.starts", plan.starts, B + 1, dev)

@@ -187,3 +187,99 @@ def test_compact_scales_of_zero(zeros):
         D.compact_reference(values, s, table, starts.tolist(), granted.tolist(), lens.tolist(), path, counts)
         assert torch.equal(now.cpu().double(), values)
         assert torch.equal(scale_now.cpu().double(), torch.where(s == 2.0 ** -200, 0.0, s))
+
+
+# ------------------------------------------------------------------------- drafted tokens and the sampler
+def node_histories(histories, new, tokens, parents):
+    out, first = [], 0
+    for history, n in zip(histories, new):
+        line = []
+        for i in range(n):
+            p = parents[first + i]
+            line.append((line[p] if p >= 0 else list(history)) + [tokens[first + i]])
+        out += line
+        first += n
+    return out
+
+
+def test_drafts_sampled_with_penalties():
+    """Each drafted token's target with the history of its own branch, by the framework's sampler: the tokens are those of
+    sampling one by one, with the same logits behind the same tokens and the same random number at the same place."""
+    vocab, rows, steps = 300, 4, 30
+    logits = 2 * torch.randn(vocab, vocab, generator=gen(1), device=DEV)  # behind each token
+    uniforms = torch.rand(rows, 200, generator=gen(2), device=DEV)
+    params = [lb.SamplingParams(temperature=t, top_k=k, top_p=0.95, repetition_penalty=r, frequency_penalty=f, presence_penalty=p)
+              for t, k, r, f, p in ((0.8, 20, 1.3, 0.0, 0.0), (0.0, -1, 1.5, 0.2, 0.1), (1.1, 5, 1.0, 0.5, 0.3), (0.7, 40, 1.2, 0.1, 0.0))]
+    rng = random.Random(3)
+    prompts = [[rng.randrange(vocab) for _ in range(n)] for n in (3, 9, 1, 20)]
+    truth = [list(p) for p in prompts]
+    for i in range(steps + 40):
+        tok = lb.sample_batch(logits[[t[-1] for t in truth]], params, truth, uniforms[:, i].contiguous()).tolist()
+        for t, x in zip(truth, tok):
+            t.append(x)
+    said, lens, drafted = [list(p) for p in prompts], [len(p) - 1 for p in prompts], 0
+    while min(len(s) - len(p) for s, p in zip(said, prompts)) < steps:
+        new, tokens, parents, place = [], [], [], []
+        for b, s in enumerate(said):
+            n = rng.choice([1, 3, 8, 14])
+            tree, depth = D.random_tree(n, rng, chain=0.6, root=0.0), [0]
+            node = [s[-1]]
+            for i in range(1, n):  # what will really come, or anything
+                depth.append(depth[tree[i]] + 1)
+                node.append(truth[b][len(s) - 1 + depth[i]] if rng.random() < 0.8 else rng.randrange(vocab))
+            new.append(n)
+            tokens += node
+            parents += tree
+            place += [(b, len(s) - len(prompts[b]) + d) for d in depth]
+        B = [b for b, n in enumerate(new) for _ in range(n)]
+        targets = lb.sample_batch(logits[tokens], [params[b] for b in B], node_histories([s[:-1] for s in said], new, tokens, parents),
+                                  torch.stack([uniforms[at] for at in place]))
+        starts = [sum(new[:i]) for i in range(rows + 1)]
+        plan = lb.StepPlan(ints(starts), ints(new), ints([ln + n for ln, n in zip(lens, new)]))
+        a = lb.accept_drafts(plan, lb.plan_tree(plan, ints(parents)), ints(tokens), targets)
+        got, lens = a.tokens.tolist(), a.lens.tolist()
+        for b, s in enumerate(said):
+            s += [x for x in got[starts[b]: starts[b + 1]] if x >= 0]
+            assert s == truth[b][: len(s)] and lens[b] == len(s) - 1
+        drafted += 1
+    assert drafted < steps  # several tokens a step
+
+
+def test_drafts_sampled_in_a_captured_step():
+    """Sampler with penalties from device arrays, and the acceptance, in one graph: other logits, random numbers, drafts and
+    histories with each replay."""
+    from localstrm_b200.sampling import build_history_csr
+    vocab, new, rng = 500, [5, 1, 9], random.Random(2)
+    T = sum(new)
+    parents = [p for n in new for p in D.random_tree(n, rng, root=0.0)]
+    rp = lb.RowParams.from_params([lb.SamplingParams(temperature=0.9, top_k=30, repetition_penalty=1.4)] * T, DEV)
+    plan = lb.StepPlan(ints([0, 5, 6, 15]), ints(new), ints([25, 8, 10]))
+    sampler = lb.BatchSampler(DEV)
+
+    def inputs(seed):
+        tokens = [random.Random(seed + i).randrange(4) for i in range(T)]  # few, so that branches are followed
+        offs, ids = build_history_csr(node_histories([[seed % vocab] * 6, [1, 2], [7]], new, tokens, parents), T, vocab)
+        logits = torch.randn(T, vocab, generator=gen(seed), device=DEV)
+        logits[:, :4] += 6
+        return logits, torch.rand(T, generator=gen(seed), device=DEV), ints(tokens), ints(offs.tolist()), ints(ids.tolist())
+
+    def step(logits, u, tokens, offs, ids):
+        tok = sampler.sample(logits, rp, offs, ids, u)
+        return tok, lb.accept_drafts(plan, lb.plan_tree(plan, ints_of), tokens, tok)
+
+    ints_of = ints(parents)
+    buffers = [x.clone() for x in inputs(0)]
+    step(*buffers)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        tok, a = step(*buffers)
+    for seed in range(1, 5):
+        fresh = inputs(seed)
+        for x, y in zip(buffers, fresh):
+            x.copy_(y)
+        graph.replay()
+        got = [x.clone() for x in (tok, a.path, a.tokens, a.counts, a.lens, a.last)]
+        want_tok, b = step(*fresh)
+        for x, y in zip(got, (want_tok, b.path, b.tokens, b.counts, b.lens, b.last)):
+            assert torch.equal(x, y)
+        assert D.accept_reference(parents, fresh[2].tolist(), want_tok.tolist(), None, None, [0, 5, 6, 15], new, [25, 8, 10], T)[2] == b.counts.tolist()
