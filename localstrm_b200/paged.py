@@ -80,7 +80,7 @@ class Forks:
 @dataclass
 class KVCache8:
     """Keys and values in 8 bits: ``k``, ``v`` float8_e4m3fn ``[num_blocks, heads, block_size, dim]``,
-    ``k_scale``, ``v_scale`` float32 ``[num_blocks, heads]``; a value is ``code * scale``."""
+    ``k_scale``, ``v_scale`` float32 ``[num_blocks, heads]``, positive and finite; a value is ``code * scale``."""
     k: torch.Tensor
     v: torch.Tensor
     k_scale: torch.Tensor
