@@ -283,3 +283,51 @@ def test_drafts_sampled_in_a_captured_step():
         for x, y in zip(got, (want_tok, b.path, b.tokens, b.counts, b.lens, b.last)):
             assert torch.equal(x, y)
         assert D.accept_reference(parents, fresh[2].tolist(), want_tok.tolist(), None, None, [0, 5, 6, 15], new, [25, 8, 10], T)[2] == b.counts.tolist()
+
+
+# --------------------------------------------------------------------------- shared blocks in one graph
+def test_fork_copy_and_release_captured():
+    """Forks, the copies of their last blocks and the release of all of them in one graph, replayed from other states, on
+    another stream than the one it was captured on."""
+    heads, bs, dim, B, blocks = 2, 16, 64, 6, 40
+    cache = lb.KVCache8(*U.random_cache(blocks, heads, bs, dim))
+    table, lens, n_free, shares = (torch.zeros(s, dtype=torch.int32, device=DEV) for s in ((B, 5), (B,), (1,), (blocks,)))
+    free, src, dst, upto, codes = (torch.zeros(s, dtype=torch.int32, device=DEV) for s in (blocks, 3, 3, 3, B))
+
+    def run():
+        f = lb.fork_blocks(table, lens, src, dst, shares, free, n_free, bs, upto=upto, lens_out=lens, n_free_out=n_free)
+        lb.copy_blocks(cache, f.copies)
+        after = [x.clone() for x in (lens, n_free, shares, table, f.granted, f.copies, cache.k.view(torch.uint8), cache.v_scale)]
+        lb.release_blocks(table, lens, codes, free, n_free, bs, lens_out=lens, n_free_out=n_free, shares=shares)
+        return after + [x.clone() for x in (lens, n_free, free, shares)]
+
+    def start(seed):
+        rng = random.Random(seed)
+        ids = rng.sample(range(blocks), blocks)
+        ln = [rng.randrange(1, 81), rng.randrange(1, 81), rng.randrange(1, 81), 0, 0, 0]
+        rows = [[ids.pop() for _ in range(-(-n // bs))] for n in ln]
+        left = rng.choice([1, 2, len(ids)])
+        for t, v in ((table, [r + [-1] * (5 - len(r)) for r in rows]), (lens, ln), (n_free, [left]), (shares, [0] * blocks), (free, ids[:left] + [0] * (blocks - left)),
+                     (src, [rng.randrange(3) for _ in range(3)]), (dst, rng.sample([3, 4, 5], 3)), (upto, [rng.randrange(1, 90) for _ in range(3)]),
+                     (codes, [rng.randrange(2) for _ in range(B)])):
+            t.copy_(ints(v))
+        for x, y in zip((cache.k.view(torch.uint8), cache.v.view(torch.uint8), cache.k_scale, cache.v_scale), U.random_cache(blocks, heads, bs, dim, seed=seed)):
+            x.copy_(y.view(torch.uint8) if y.dtype == U.E4M3 else y)
+
+    start(0)
+    run()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph):
+        kept = run()
+    for seed in range(1, 9):
+        start(seed)
+        line, ln, left, fr = table.tolist(), lens.tolist(), int(n_free), free.tolist()
+        want = [x.clone() for x in run()]
+        f, line2, sh2 = D.fork_reference(line, ln, src.tolist(), dst.tolist(), upto.tolist(), [0] * blocks, fr, left, bs)
+        assert want[0].tolist() == f["lens"] and want[1].tolist() == f["n_free"] and want[2].tolist() == sh2 and want[3].tolist() == line2
+        start(seed)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            graph.replay()
+        torch.cuda.current_stream().wait_stream(side)
+        assert all(torch.equal(x, y) for x, y in zip(kept, want))
