@@ -331,3 +331,60 @@ def test_fork_copy_and_release_captured():
             graph.replay()
         torch.cuda.current_stream().wait_stream(side)
         assert all(torch.equal(x, y) for x, y in zip(kept, want))
+
+
+# ------------------------------------------------------------------------------ prompts, and long caches
+@pytest.mark.parametrize("heads,per,dim", [(8, 4, 128), (2, 7, 64), (2, 3, 256)])
+def test_attend_prompt_chunks_beside_trees(heads, per, dim):
+    """A chunk of more than 1,024 new tokens is a chain whatever its parents say; trees, a single token, an idle row and a
+    refused one in the same step."""
+    ctx, new = [3, 700, 2600, 0, 40, 90, 1500], [1100, 20, 9, 1, 0, 33, 300]
+    rng = random.Random(dim)
+    rows = list(U.make_rows(ctx, new, 16, seed=dim))
+    parents = [p for n in new for p in D.random_tree(n, rng)]
+    granted, lens = rows[3].clone(), rows[4].clone()
+    granted[5], lens[5] = 0, 90  # refused: its tokens stay as they are
+    rows[3], rows[4] = granted, lens
+    cache = lb.KVCache8(*U.random_cache(rows[-1], heads, 16, dim, seed=per))
+    q = torch.randn(sum(new) + 3, heads * per, dim, generator=gen(dim), device=DEV).bfloat16()
+    y, _ = check_attend_tree(q, cache, tuple(rows), parents + [-1] * 3)
+    at = int(rows[2][5])
+    assert bool((y[at: at + 33] == 77).all()) and bool((y[sum(new):] == 77).all()) and bool(y[:at].isfinite().all())
+    plan = lb.StepPlan(*rows[2:5])
+    tree = lb.plan_tree(plan, ints(parents + [-1] * 3))
+    assert tree.positions[:1100].tolist() == list(range(3, 1103)) and tree.positions[at: at + 33].tolist() == [0] * 33
+
+
+def test_blocks_behind_four_gigabytes():
+    """Blocks whose places pass 32 bits: attention, accepted tokens, copies and appended tokens as in a small cache."""
+    heads, bs, dim, far = 8, 16, 128, 280_000  # 16 KB a block: 4.6 GB of keys, and of values
+    new, ctx = [20, 9, 40, 1], [100, 3000, 35, 17]
+    table, t, starts, granted, lens, blocks = U.make_rows(ctx, new, bs, seed=1)
+    small = lb.KVCache8(*U.random_cache(blocks, heads, bs, dim, seed=2))
+    big = lb.KVCache8(*(torch.empty(far, heads, bs, dim, dtype=torch.uint8, device=DEV).view(U.E4M3) for _ in range(2)),
+                      *(torch.ones(far, heads, device=DEV) for _ in range(2)))
+    ends = (0, far - blocks)  # low blocks are other ones, so that a place that lost its upper bits shows
+    parts = lambda c: (c.k.view(torch.uint8), c.v.view(torch.uint8), c.k_scale, c.v_scale)
+    for b, s in zip(parts(big), parts(small)):
+        b[: blocks] = s.flip(0)
+        b[far - blocks:] = s
+    assert (far - blocks) * heads * bs * dim > 2 ** 32
+    up = torch.where(t >= 0, t + ends[1], t)
+    plan, rng = lb.StepPlan(starts, granted, lens), random.Random(4)
+    tree = lb.plan_tree(plan, ints([p for n in new for p in D.random_tree(n, rng)]))
+    q = torch.randn(sum(new), 32, dim, generator=gen(3), device=DEV).bfloat16()
+    kv = torch.randn(2, sum(new), heads, dim, generator=gen(4), device=DEV)
+    path, counts = [], []
+    for n in new:
+        kept = sorted({0, *rng.sample(range(n), n // 2)})
+        path += kept + [-1] * (n - len(kept))
+        counts.append(len(kept))
+    out = []
+    for cache, tab, off in ((small, t, 0), (big, up.contiguous(), ends[1])):
+        lb.append_kv(cache, kv[0], kv[1], tab, plan)
+        o = [lb.attend(q, cache, tab, plan, tree=tree), lb.attend(q, cache, tab, plan)]
+        lb.compact_kv(cache, tab, plan, ints(path), ints(counts))
+        lb.copy_blocks(cache, ints([[table[1][0] + off, table[2][1] + off], [table[1][5] + off, blocks - 1 + off]]))
+        out.append(o + [x[off: off + blocks].clone() for x in parts(cache)])
+    assert all(torch.equal(x, y) for x, y in zip(*out))
+    assert torch.equal(big.k.view(torch.uint8)[:blocks], U.random_cache(blocks, heads, bs, dim, seed=2)[0].view(torch.uint8).flip(0))
