@@ -90,7 +90,7 @@ static inline cudaError_t launch_attend_few(const AttendArgs& a, int64_t rows, v
 //   33 to 48: 64 rows over 1,000 121 (133), 2,000 178 (219), 4,000 250 (375); 512 over 100 344 (156), 300 436 (373), 600 516-547 (524-537)
 //   D = 64, 33 to 48: 64 rows over 1,000 94 (94), 2,000 143 (131), 4,000 203 (211); 512 over 300 356 (209)
 //   49 to 63: 64 rows over 2,000 147 (166), 4,000 215 (270); 512 over 300 379 (270), 1,000 520-553 (563)
-//   rows over 50 to 16,000, D = 128, all by these borders: 5, 8, 9, 12, 16 tokens 455, 459, 451, 453, 432
+//   rows over 50 to 16,000, D = 128, all by these borders: 5, 8, 9, 12, 16 tokens 477, 483, 491, 481, 463
 // so that lengths from AT_LONG and at_long_more on decide below rows_any.  Causal steps of more than 8 heads per key head have one border, above a
 // single token's rows.  Single tokens beside one chunk of 449 pay for the second launch (10 us).
 // A step of no more tokens than rows counts as one of single tokens: a chunk among idle rows is right, but goes in
@@ -98,7 +98,7 @@ static inline cudaError_t launch_attend_few(const AttendArgs& a, int64_t rows, v
 // launches for chunks would cost every step of single tokens 8 to 10 us.
 // Trees: the rows of a batch are mostly alike, a few tokens to some dozens each, so that a single row may have tokens enough for the SMs too
 // (64 tokens of 8 heads per key head over 20,000 alone 119 us, 300 in groups of 16), and in a batch of large ones the small ones
-// go along (48 of 8 to 32 tokens over 50 to 8,000: 206 us, 222 with a second launch for a few rows).
+// go along (48 of 8 to 32 tokens over 50 to 8,000: 206 us, in the same run 222 with a second launch for a few rows).
 template <int D, int DT, bool TREE>
 static inline cudaError_t launch_attend_rows(AttendArgs a, void* ws, cudaStream_t st) {
   const int64_t average = (int64_t)a.per * ((a.T + (int64_t)a.B - 1) / a.B);

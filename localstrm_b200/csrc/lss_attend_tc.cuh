@@ -90,8 +90,8 @@ __device__ __forceinline__ uint32_t pa_place(int r, int q) {
 // group are added up by lss_attend_tc_join_kernel.
 // Measured (8 key heads of 128): four chunks of 296 to 416 tokens of 32 heads behind 1,000 to 6,000 others 192 us (one warp issuing for both
 // streams, codes widened from registers: 222 to 240), D = 64 160; three trees of 64 tokens of 64 heads over 60,000 to 100,000
-// 605 to 625 us, 610 to 640 one after the other, when the power cap takes the clock down (0.87 to 0.92 PFLOP/s); 48 trees of 8 to 32 tokens of 32 heads
-// over 50 to 8,000 206 us.  A step of a stream takes about 2,200 cycles: the exponentials of both streams 1,088 (16 per cycle and SM), products 615 a
+// 605 to 680 us (0.82 to 0.92 PFLOP/s; the upper end one after the other, when the power cap takes the clock down); 48 trees of 8 to 32 tokens of 32 heads
+// over 50 to 8,000 206 to 219 us (the upper end alone with cold caches).  A step of a stream takes about 2,200 cycles: the exponentials of both streams 1,088 (16 per cycle and SM), products 615 a
 // stream (48 cycles for 128 x 64 x 16 from shared memory, 64 for 128 x 128 x 16 with the weights in tensor memory), the rest is
 // the way of scores and weights through tensor memory and barriers.  A quarter of the exponentials as polynomials:
 // 3 % less, groups of 128 rows 1 % more; scores fetched before the weights of the step before are stored: 5 % more.

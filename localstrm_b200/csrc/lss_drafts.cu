@@ -22,7 +22,7 @@ template <int DT, int N, int L, bool PAIRS>
 static cudaError_t launch_rotate(const RotateArgs& a, cudaStream_t st) {
   const int teams = RO_NT / L, sms = sm_count(device_index());
   // Tokens per CTA, a power of two.  A wave of three CTAs per SM takes about as long as its teams' heads and four more
-  // (start, weights, sines): 1,000 tokens of 32 + 8 heads of 128 one by one 22 us, four by four 14; 8,192 by 8 or 32 39 us, by 16 45.
+  // (start, weights, sines): 1,000 tokens of 32 + 8 heads of 128 one by one 22 us, four by four 14; 8,192 by 8 or 32 39 us, by 16 45 (alone, cold caches).
   int tk = 1;
   int64_t best = INT64_MAX;
   for (int t = 1; t <= teams; t *= 2) {

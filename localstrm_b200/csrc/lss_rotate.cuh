@@ -94,10 +94,14 @@ __device__ __forceinline__ float ro_weight(const void* w, int dtype, int i) {
 // holds 2 N values that turn with each other, so that no value moves between lanes but for the sum of squares, and for
 // all of its team's heads, the queries' and then the keys', keeps the factors of a value and of its partner, w cos
 // and +-w sin, in registers.
-// Measured (cold caches, launch included): 8,192 tokens of 32 + 8 heads of 128 in bf16, 168 MB, 39 us (4.3 TB/s, 0.66 of the copy
-// rate), 4,096 in f32 35 us, one token of 16 heads of 64 3.8 us.  HBM bounds it, then the instructions (some 190 per
-// warp and four heads, 19 million in the first case) and the start of each CTA (weights, sines: about four heads' time), which
-// three CTAs per SM hide from each other.  One token per CTA with weights and sines in shared memory: 57 us.
+// Measured: 8,192 tokens of 32 + 8 heads of 128 in bf16, 168 MB: alone with cold caches and launch 39 us, one call behind the
+// other 34 to 36 (4.7 to 5.0 TB/s of its own bytes, 0.71 to 0.76 of the copy rate; counters see 3.5 TB/s of DRAM traffic, 0.53,
+// as not all results have left the L2 cache when it ends); 4,096 in f32 37 and 30 us, one token of 16 heads of 64 8 and 4 us.
+// Not HBM bounds it but the instructions (some 190 per warp and four heads, 19 million in the first case, 54 % of the issue
+// slots), their waits for shared memory and fixed latencies, and the start of each CTA (weights, sines: about four heads' time),
+// which three CTAs per SM hide from each other.  With half the bytes per head the starts weigh twice: 40 heads of 64 25 and
+// 17 us (floor 12.8); rows that are not on 16 bytes go value by value: 1,000 tokens of 40 heads of 66 37 and 24 us (1.6).
+// One token per CTA with weights and sines in shared memory: 57 us.
 template <int DT, int N, int L, bool PAIRS>  // PAIRS: interleaved
 __global__ void __launch_bounds__(RO_NT, N > 1 ? 3 : 2) lss_rotate_kernel(RotateArgs a, int tk) {
   constexpr int NU = N > 1 ? 1 : 8;   // units of 2 N values that a lane holds: dim <= 2 N L NU

@@ -133,7 +133,8 @@ constexpr int GV_MARK = -(1 << 30) - 1;  // less the place of a block's last hol
 // the count itself.  Then one pass counts per row, and one writes the list and zeroes the counts.  One cluster, a warp
 // per row, a cluster barrier between the passes; the rows' numbers of blocks go to all CTAs' shared memory, and the
 // entries stay in that of their warp, as far as it goes, so that a pass is one dependent load and not two.  Latency bounds
-// it: 512 rows of up to 8,600 tokens in blocks of 16, a third of them stopped: 23 us (on eight SMs 37, and with the table read in every pass 41).
+// it: 512 rows of up to 8,600 tokens in blocks of 16, a third of them stopped: 23 us (on eight SMs 37, and with the table read in every pass 41;
+// a quarter of the issue slots, warps wait for fences, cluster barriers and the scattered accesses alike).  Without shares 9 us.
 static __global__ void __launch_bounds__(BL_NT) lss_give_kernel(GiveArgs a) {
   extern __shared__ __align__(16) int32_t bl_sm[];
   __shared__ int64_t scr[32];
